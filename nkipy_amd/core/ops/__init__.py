@@ -22,6 +22,7 @@ from nkipy_amd.core.ops.nn import rms_norm, softmax, topk
 from nkipy_amd.core.ops.reduce import (
     all, any, argmax, argmin, count_nonzero, cumsum, max, mean, min, prod, std, sum, var,
 )
+from nkipy_amd.core.ops.serving import paged_attention, rotary_append, sample, window_attention
 from nkipy_amd.core.ops.transform import (
     astype, broadcast_to, concatenate, copy, copyto, diff, expand_dims, flip, pad, repeat,
     reshape, roll, split, squeeze, stack, swapaxes, tile, transpose,

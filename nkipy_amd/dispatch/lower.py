@@ -275,7 +275,7 @@ class Lowering:
         G.fuse_swiglu_planes(plan)
         return plan
 
-    _INPLACE_OPS = ("dynamic_update_slice", "scatter_along_axis", "put_along_axis", "scatter_strided")
+    _INPLACE_OPS = ("dynamic_update_slice", "scatter_along_axis", "put_along_axis", "scatter_strided", "paged_write")
 
     def _reads_done_before(self, p: Value, prod: Node, order: Dict[int, int]) -> bool:
         """True when every read of parameter ``p`` happens in a step that runs

@@ -496,12 +496,13 @@ def _build_default_patterns():
     )
     from nkipy_amd.dispatch.patterns_gemm import GemmPattern, SwigluPattern
     from nkipy_amd.dispatch.patterns_linattn import LinearAttentionPattern
+    from nkipy_amd.dispatch.serving import AppendPattern, ServingPattern
 
     # larger structures first: they contain matmuls / softmaxes that smaller
     # patterns would claim; GEMMs before RMSNorm so that a residual add
     # after a projection goes into the GEMM epilogue; the RoPE of q / k then
     # folds into its QKV projection
-    return [LinearAttentionPattern(), DecodeAttentionPattern(), AttentionPattern(), RopePattern(), HeadRopePattern(),
-            SwigluPattern(), GemmPattern(), SoftmaxPattern(), RmsNormPattern(), QkvRopeFusion(),
-            ProjectionPlanesFusion()]
+    return [AppendPattern(), ServingPattern(), LinearAttentionPattern(), DecodeAttentionPattern(), AttentionPattern(),
+            RopePattern(), HeadRopePattern(), SwigluPattern(), GemmPattern(), SoftmaxPattern(), RmsNormPattern(),
+            QkvRopeFusion(), ProjectionPlanesFusion()]
 
