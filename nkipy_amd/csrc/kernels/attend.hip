@@ -34,3 +34,538 @@ __device__ __forceinline__ void attend_rows_body(const AttendArgs &a) {
 extern "C" __global__ __launch_bounds__(256) void nk_attend_rows_bf16(AttendArgs a) { attend_rows_body<bf16>(a); }
 extern "C" __global__ __launch_bounds__(256) void nk_attend_rows_f16(AttendArgs a) { attend_rows_body<f16>(a); }
 extern "C" __global__ __launch_bounds__(256) void nk_attend_rows_f32(AttendArgs a) { attend_rows_body<float>(a); }
+
+// ---------------------------------------------------------------------------
+// The tiled form: 16-bit operands, head dim 64 or 128, 16-byte aligned rows.
+//
+// One workgroup of four waves per (tile of 128 rows, KV head, split); a wave
+// owns 32 rows.  S^T = K Q^T and O^T = V^T P^T by 32x32x16 matrix
+// instructions, so that a lane owns one row: its softmax offset and sum stay
+// in its own registers (the two lanes that hold a row meet at the end), and the
+// weights leave the first product in the order the second one takes them.
+//
+// Keys move in blocks of 32 through rings of four LDS slots each for K and V,
+// by loads straight into LDS; iteration j has the scores of block j + 1, the
+// values of block j - 1 and the softmax of block j in one basic block, and
+// moves K of block j + 4 and V of block j + 2 into the slots freed before it: one
+// barrier per block, three iterations for a move to land.  A key's row is
+// looked up once per workgroup: the rows of 32 blocks ahead stand in LDS, -1
+// where no query of the tile sees the key or it has no page.  Those rows come
+// from a row of zeros, so nothing of them enters a product; a value that is
+// not finite and seen by some rows of a tile only would still meet the others'
+// weights of 0, and the rows it spoils are computed again one by one.
+//
+// Blocks that every row sees in full take the loop body without mask; the
+// masked one serves the edges (the diagonal, the window's end, the sinks'
+// last block, missing pages).
+//
+// Softmax: p = 2^(s c - m), c = scale log2(e), with an offset m per row that
+// starts TOP below the first block's largest score and is raised (sums
+// rescaled, block recomputed) when a lane's 16 weights of a block exceed LIMIT:
+// the common block takes no maximum.  m divides out.  Sums are fp32; weights
+// enter the second product rounded to the operands' type, the one rounding
+// beside the result's own.  f16 weights start at 2^10 and stay below 2^14,
+// which leaves 2^34 between the largest and the least one that is kept.
+// ---------------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <typename T> struct Mat;
+template <> struct Mat<bf16> {
+  typedef __bf16 E;
+  typedef __bf16 V __attribute__((ext_vector_type(8)));
+  static constexpr float LIMIT = 65536.f, TOP = 0.f;
+  static NK_DEVICE f32x16 mul(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<f16> {
+  typedef _Float16 E;
+  typedef _Float16 V __attribute__((ext_vector_type(8)));
+  static constexpr float LIMIT = 16384.f, TOP = 10.f;
+  static NK_DEVICE f32x16 mul(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <bool B> struct Flag {
+  static constexpr bool value = B;
+};
+template <int N> struct Slot {
+  static constexpr int value = N;
+};
+
+// lane l of the wave fills LDS bytes lds + 16 l (lds uniform) from p; waits
+// for these moves are explicit
+NK_DEVICE void move16(const void *p, uint32_t lds) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :: "v"((uint64_t)p), "s"(m) : "memory", "m0");
+}
+
+#define ATT_AHEAD 32  // blocks whose rows are looked up at once
+
+// rows outside every sequence: zeros, shared out over the grid
+template <typename T>
+NK_DEVICE void att_zero_rest(const AttendArgs &a, int wg, int nwg) {
+  const int s0 = min(max(a.starts[0], 0), a.N), s1 = min(max(a.starts[a.B], s0), a.N);
+  const int n = a.Hq * a.D;
+  for (int x = wg; x < s0 + a.N - s1; x += nwg) {
+    T *o = (T *)a.o + (int64_t)(x < s0 ? x : x - s0 + s1) * n;
+    for (int e = threadIdx.x; e < n; e += 256) o[e] = T{};
+  }
+}
+
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
+  typedef typename Mat<T>::V V8;
+  constexpr int RB = D * 2, TB = ATT_KEYS * RB;  // bytes of a row, of a block
+  constexpr int LPR = RB / 16, RPM = 64 / LPR;   // lanes per row, rows per move
+  constexpr int NM = ATT_KEYS / RPM / 4;         // moves per wave and block
+  __shared__ __attribute__((aligned(1024))) uint8_t KR[4 * TB];
+  __shared__ __attribute__((aligned(1024))) uint8_t VR[4 * TB];
+  __shared__ __attribute__((aligned(16))) int32_t ent[PAGED ? 2 * ATT_AHEAD * ATT_KEYS : 4];
+  __shared__ int32_t lost[8];  // per half of ent and wave: some key has no page
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, lhi = lane >> 5;
+  const int rep = a.Hq / a.Hkv;
+
+  // Workgroups run round-robin over the eight XCDs: with the KV head fastest,
+  // the tiles of one head (eight heads, or a multiple) share an XCD's cache.
+  // The last tiles of a sequence, the longest without a window, go first.
+  int w = blockIdx.x;
+  if (PAGED && a.starts) att_zero_rest<T>(a, w, a.tiles * a.Hkv * a.nsplit);
+  const int g = w % a.Hkv;
+  w /= a.Hkv;
+  const int split = w % a.nsplit, t = a.tiles - 1 - w / a.nsplit;
+  int b, tile;
+  if (PAGED && a.starts) {
+    b = att_find(a.B, t, [&](int x) { return att_tile0(a, x); });
+    if (b < 0) return;
+    tile = t - att_tile0(a, b);
+  } else {
+    const int per = (a.S * rep + ATT_ROWS - 1) / ATT_ROWS;
+    b = t / per, tile = t % per;
+  }
+  const AttSeq sq = att_seq(a, b);
+  if ((int64_t)tile * ATT_ROWS >= (int64_t)sq.n * rep) return;
+  const AttSpan sp = att_span(a, sq, tile);
+  int j0, j1;
+  const int pieces = att_split(a, sp.nb, split, j0, j1);
+  if (split >= pieces) return;
+  const int n = j1 - j0;  // blocks of this workgroup
+
+  // this lane's row
+  const int row0 = tile * ATT_ROWS + wave * 32, rows = sq.n * rep;
+  const bool active = row0 < rows;
+  V8 qf[D / 16];
+  int p, klim;  // its position and last key
+  {
+    const int rld = min(row0 + l32, rows - 1), qi = rld / rep, h = g * rep + rld % rep;
+    p = sq.p0 + qi;
+    klim = row0 + l32 < rows && p >= 0 && p < sq.len ? min(p, sq.cap - 1) : -1;
+    const uint16_t *q = (const uint16_t *)a.q + (PAGED ? (int64_t)(sq.lo + qi) * a.q_ss : (int64_t)b * a.q_sb + (int64_t)qi * a.q_ss)
+                        + (int64_t)h * a.q_sh;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) qf[kk] = *reinterpret_cast<const V8 *>(q + kk * 16 + lhi * 8);
+  }
+  const uint16_t *kp = (const uint16_t *)a.k + (PAGED ? 0 : (int64_t)b * a.k_sb) + (int64_t)g * a.k_sh;
+  const uint16_t *vp = (const uint16_t *)a.v + (PAGED ? 0 : (int64_t)b * a.v_sb) + (int64_t)g * a.v_sh;
+
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int t2 = 0; t2 < D / 32; ++t2)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t2][r] = 0.f;
+  float m_run = -1e30f, l_run = 0.f;  // (finite: a masked score gives p = 0)
+  const float sl2 = a.scale * 1.44269504088896340736f;
+
+  // swizzles: 16-byte chunk c of row r stands at chunk c ^ kswz / vswz, so that
+  // 16 rows of a K fragment, and the four rows of a transposing V read, cover
+  // all banks
+  auto kswz = [](int r) __attribute__((always_inline)) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+  auto vswz = [](int r) __attribute__((always_inline)) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; };
+
+  // look up the rows of blocks 32 c .. 32 c + 31 of this workgroup
+  auto look_up = [&](int c) __attribute__((always_inline)) {
+    if constexpr (PAGED) {
+      bool miss = false;
+#pragma unroll 1
+      for (int x = tid; x < ATT_AHEAD * ATT_KEYS; x += 256) {
+        const int j = j0 + c * ATT_AHEAD + x / ATT_KEYS;
+        const int key = sp.kb(j) * ATT_KEYS + x % ATT_KEYS;
+        int at = -1;
+        if (j < j1 && key < sp.hi && (key >= sp.lo || key < a.sinks)) {
+          at = att_place(a, b, key);
+          miss |= at < 0;
+        }
+        ent[(c & 1) * ATT_AHEAD * ATT_KEYS + x] = at;
+      }
+      const bool any = __ballot(miss) != 0;
+      if (lane == 0) lost[(c & 1) * 4 + wave] = any;
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    }
+  };
+  // address of 16 bytes of row r (chunk c) of block j0 + jr, zeros where it has
+  // no use
+  auto source = [&](const uint16_t *base, int64_t ss, int jr, int r, int c) __attribute__((always_inline)) -> const void * {
+    int at = -1;
+    if constexpr (PAGED) {
+      if (jr < n) at = ent[(jr & (2 * ATT_AHEAD - 1)) * ATT_KEYS + r];
+    } else {
+      const int key = sp.kb(j0 + jr) * ATT_KEYS + r;
+      if (jr < n && key < sp.hi && (key >= sp.lo || key < a.sinks)) at = key;
+    }
+    asm volatile("" : "+v"(c));  // (sums with the bases would be kept in registers for every row)
+    const uint8_t *p = at < 0 ? (const uint8_t *)a.zeros : (const uint8_t *)(base + (int64_t)at * ss);
+    return p + c * 16;
+  };
+  const uint32_t k_lds = lds_addr(KR) + wave * 1024, v_lds = lds_addr(VR) + wave * 1024;
+  auto load_k = [&](auto sl, int jr) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const int r = (i * 4 + wave) * RPM + lane / LPR;
+      move16(source(kp, a.k_ss, jr, r, (lane % LPR) ^ kswz(r)), k_lds + (decltype(sl)::value & 3) * TB + i * 4096);
+    }
+  };
+  auto load_v = [&](auto sl, int jr) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const int r = (i * 4 + wave) * RPM + lane / LPR;
+      move16(source(vp, a.v_ss, jr, r, (lane % LPR) ^ vswz(r)), v_lds + (decltype(sl)::value & 3) * TB + i * 4096);
+    }
+  };
+  // an iteration leaves the moves of the last two outstanding
+  auto wait_moves = [&](auto count) __attribute__((always_inline)) {
+    static_assert(decltype(count)::value < 16, "vmcnt field");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | decltype(count)::value);
+  };
+
+  // K fragment kk: row l32, chunk 2 kk + lhi
+  const int kbase = l32 * RB + ((lhi ^ (kswz(l32) & 1)) << 4), kx = (kswz(l32) & ~1) << 4;
+  auto qk = [&](const uint8_t *K, f32x16 &s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+      s = Mat<T>::mul(*reinterpret_cast<const V8 *>(K + kbase + ((kk << 5) ^ kx)), qf[kk], s);
+  };
+  // transposing V read (group lane / 16, i = lane % 16): row 16 j + 8 si + 4 (group / 2) + i / 4,
+  // columns 32 dt + 16 (group % 2) + 4 (i % 4)
+  int vbase, vx;
+  {
+    const int grp = lane >> 4, gi = lane & 15, r = 4 * (grp >> 1) + (gi >> 2);
+    vbase = r * RB + (((grp & 1) * 2 + ((gi & 3) >> 1)) << 4) + (gi & 1) * 8;
+    vx = vswz(r) << 4;
+  }
+  auto pv = [&](const uint8_t *Vt, const V8 (&pf)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        s16x4 v[2];
+#pragma unroll
+        for (int si = 0; si < 2; ++si)
+          v[si] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4 *)(Vt + (16 * j + 8 * si) * RB + vbase + ((dt << 6) ^ vx)));
+        const s16x8 vf = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[dt] = Mat<T>::mul(__builtin_bit_cast(V8, vf), pf[j], acc[dt]);
+      }
+  };
+  auto expblock = [&](const f32x16 &s, V8 (&pf)[2]) __attribute__((always_inline)) {
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * j + e], sl2, -m_run));
+        if (e & 1) s1 += x; else s0 += x;
+        pf[j][e] = (typename Mat<T>::E)x;
+      }
+    return s0 + s1;
+  };
+  int missing = 0;  // the blocks being worked on have keys without a page
+  // element r of a lane's scores is key 32 kb + 8 (r / 4) + 4 lhi + r % 4
+  auto softmax = [&](f32x16 &s, V8 (&pf)[2], int jr, auto masked) __attribute__((always_inline)) {
+    if constexpr (decltype(masked)::value) {
+      const int k0 = sp.kb(j0 + jr) * ATT_KEYS + lhi * 4;
+      const int t0 = klim - k0, w0 = p - a.window - k0, s0 = a.sinks - k0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int x = (r >> 2) * 8 + (r & 3);
+        s[r] = x > t0 || (x <= w0 && x >= s0) ? -INFINITY : s[r];
+      }
+      if (PAGED && missing) {
+        const int32_t *en = ent + (jr & (2 * ATT_AHEAD - 1)) * ATT_KEYS + lhi * 4;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const int4 e = *reinterpret_cast<const int4 *>(en + r * 2);
+          asm volatile("" ::: "memory");  // (one at a time: registers)
+          s[r] = e.x < 0 ? -INFINITY : s[r];
+          s[r + 1] = e.y < 0 ? -INFINITY : s[r + 1];
+          s[r + 2] = e.z < 0 ? -INFINITY : s[r + 2];
+          s[r + 3] = e.w < 0 ? -INFINITY : s[r + 3];
+        }
+      }
+    }
+    float ls = expblock(s, pf);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= Mat<T>::LIMIT)) != 0, 0)) {
+      float bm = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
+      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+      const float m_new = fmaxf(m_run, bm * sl2 - Mat<T>::TOP);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+#pragma unroll
+      for (int t2 = 0; t2 < D / 32; ++t2)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t2][r] *= alpha;
+      l_run *= alpha;
+      ls = expblock(s, pf);
+    }
+    l_run += ls;
+  };
+
+  auto whole = [&](int jr) __attribute__((always_inline)) {  // every row sees the whole block
+    const int k0 = sp.kb(j0 + jr) * ATT_KEYS;
+    return k0 + ATT_KEYS - 1 <= sp.pa && k0 + ATT_KEYS <= sp.hi && (k0 > sp.pb - a.window || k0 + ATT_KEYS <= a.sinks) && !missing;
+  };
+
+  f32x16 sA, sB;
+  V8 pA[2], pB[2];
+  // the end of an iteration: the next moves, behind its matrix instructions
+  auto move_on = [&](auto sl, int jr) __attribute__((always_inline)) {
+    if (jr < n) {
+      load_k(sl, jr + 4);
+      load_v(Slot<decltype(sl)::value + 2>{}, jr + 2);
+    }
+    wait_moves(Slot<4 * NM>{});
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // a whole block between others
+  auto inner = [&](auto sl, int jr, f32x16 &cur, f32x16 &nxt, V8 (&prev)[2], V8 (&now)[2]) __attribute__((always_inline)) {
+    constexpr int SL = decltype(sl)::value;
+    pv(VR + ((SL + 3) & 3) * TB, prev);
+    qk(KR + ((SL + 1) & 3) * TB, nxt);
+    softmax(cur, now, jr, Flag<false>{});
+    // every LDS read first, then matrix instructions with the softmax between them
+    __builtin_amdgcn_sched_group_barrier(0x100, 3 * D / 16, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 3 * 128 / D, 0);
+    }
+    move_on(sl, jr);
+  };
+  // the first and last blocks and those with a mask; iteration n has the last values
+  auto edge = [&](auto sl, int jr, f32x16 &cur, f32x16 &nxt, V8 (&prev)[2], V8 (&now)[2]) __attribute__((always_inline)) {
+    constexpr int SL = decltype(sl)::value;
+    if (jr > n) return;
+    if (jr + 1 < n) qk(KR + ((SL + 1) & 3) * TB, nxt);
+    if (jr > 0) pv(VR + ((SL + 3) & 3) * TB, prev);
+    if (jr < n) softmax(cur, now, jr, Flag<true>{});
+    move_on(sl, jr);
+  };
+
+  if (n > 0) {
+    look_up(0);
+    __syncthreads();
+    load_k(Slot<0>{}, 0);
+    load_k(Slot<1>{}, 1);
+    load_k(Slot<2>{}, 2);
+    load_v(Slot<0>{}, 0);
+    load_k(Slot<3>{}, 3);
+    load_v(Slot<1>{}, 1);
+    wait_moves(Slot<4 * NM>{});
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (active) qk(KR, sA);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): block 0 is read before its slot is refilled
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    auto ahead = [&](int jr) __attribute__((always_inline)) {
+      if (PAGED && jr % ATT_AHEAD == 0) {
+        const int32_t *f = lost + (jr / ATT_AHEAD & 1) * 4;
+        missing = __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]);
+        // (the other half was last read an iteration, and a barrier, ago)
+        if (jr + ATT_AHEAD < n) look_up(jr / ATT_AHEAD + 1);
+      }
+    };
+    if (active) {
+      int jr = 0;
+      ahead(0);
+      while (true) {
+        edge(Slot<0>{}, jr, sA, sB, pB, pA);
+        edge(Slot<1>{}, jr + 1, sB, sA, pA, pB);
+        edge(Slot<2>{}, jr + 2, sA, sB, pB, pA);
+        edge(Slot<3>{}, jr + 3, sB, sA, pA, pB);
+        jr += 4;
+        if (jr > n) break;
+        ahead(jr);
+        while (jr + 4 < n && whole(jr) && whole(jr + 1) && whole(jr + 2) && whole(jr + 3)) {
+          inner(Slot<0>{}, jr, sA, sB, pB, pA);
+          inner(Slot<1>{}, jr + 1, sB, sA, pA, pB);
+          inner(Slot<2>{}, jr + 2, sA, sB, pB, pA);
+          inner(Slot<3>{}, jr + 3, sB, sA, pA, pB);
+          jr += 4;
+          ahead(jr);
+        }
+      }
+    } else {  // rows past the sequence's: the moves only
+      for (int jr = 0; jr <= n; jr += 4) {
+        ahead(jr);
+        move_on(Slot<0>{}, jr);
+        if (jr + 1 <= n) move_on(Slot<1>{}, jr + 1);
+        if (jr + 2 <= n) move_on(Slot<2>{}, jr + 2);
+        if (jr + 3 <= n) move_on(Slot<3>{}, jr + 3);
+      }
+    }
+    wait_moves(Slot<0>{});  // no move outlives the workgroup
+  }
+
+  // (the row's place is found again: kept through the loop it costs registers)
+  int again = l32;
+  asm volatile("" : "+v"(again));
+  const int row = row0 + again, rld = min(row, rows - 1), qi = rld / rep, h = g * rep + rld % rep;
+  const bool ok = klim >= 0;
+  l_run += __shfl_xor(l_run, 32, 64);
+  const int64_t nr = (int64_t)a.N * a.Hq;
+  const int64_t orow = ((int64_t)(PAGED ? sq.lo + qi : b * a.S + qi)) * a.Hq + h;
+  float *wo = a.ws + (split * nr + orow) * D, *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + orow) * 2;
+  uint16_t *o = (uint16_t *)a.o + orow * D;
+
+  // rows that a value which is not finite may have spoiled
+  float z = l_run * 0.f;
+#pragma unroll
+  for (int t2 = 0; t2 < D / 32; ++t2)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z = __builtin_fmaf(acc[t2][r], 0.f, z);
+  uint64_t spoiled = __ballot(ok && z != 0.f);
+  spoiled = (spoiled | spoiled >> 32) & 0xffffffffull;
+  const bool mine = spoiled >> l32 & 1;
+  const bool put = row < rows && !mine;
+  if (put && pieces == 1) {
+    const float inv = ok && l_run != 0.f ? 1.0f / l_run : 0.f;
+#pragma unroll
+    for (int t2 = 0; t2 < D / 32; ++t2)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = inv == 0.f ? 0.f : acc[t2][gq * 4 + e] * inv;
+        T y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Elt<T>::store(y, e, x[e]);
+        uint2 u;
+        __builtin_memcpy(&u, y, 8);
+        *reinterpret_cast<uint2 *>(o + t2 * 32 + gq * 8 + lhi * 4) = u;
+      }
+  } else if (put) {
+#pragma unroll
+    for (int t2 = 0; t2 < D / 32; ++t2)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        float4 x;
+        x.x = ok ? acc[t2][gq * 4] : 0.f;
+        x.y = ok ? acc[t2][gq * 4 + 1] : 0.f;
+        x.z = ok ? acc[t2][gq * 4 + 2] : 0.f;
+        x.w = ok ? acc[t2][gq * 4 + 3] : 0.f;
+        *reinterpret_cast<float4 *>(wo + t2 * 32 + gq * 8 + lhi * 4) = x;
+      }
+    if (lhi == 0) wm[0] = ok ? m_run : -1e30f, wm[1] = ok ? l_run : 0.f;
+  }
+  // these again, reading only what they see
+  while (spoiled) {
+    const int src = __builtin_ctzll(spoiled);
+    spoiled &= spoiled - 1;
+    float m, l, x[4];
+    att_row<T>(a, sq, sp, b, __shfl(qi, src, 64), __shfl(h, src, 64), j0, j1, m, l, x);
+    const int64_t at = __shfl((int)orow, src, 64);  // (rows are below 2^31)
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      if (pieces == 1) {
+        Elt<T>::store((T *)a.o + at * D, lane + 64 * e, l == 0.f ? 0.f : x[e] / l);
+      } else {
+        a.ws[(split * nr + at) * D + lane + 64 * e] = x[e];
+      }
+    }
+    if (pieces > 1 && lane == 0) {
+      float *q = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + at) * 2;
+      q[0] = l == 0.f ? -1e30f : m * 1.44269504088896340736f;
+      q[1] = l;
+    }
+  }
+}
+
+#define NK_TILE(T, name, D)                                                                                  \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_paged_##name##_d##D(AttendArgs a) {    \
+    attend_tile_body<T, D, true>(a);                                                                         \
+  }                                                                                                          \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_plain_##name##_d##D(AttendArgs a) {    \
+    attend_tile_body<T, D, false>(a);                                                                        \
+  }
+NK_TILE(bf16, bf16, 128)
+NK_TILE(f16, f16, 128)
+NK_TILE(bf16, bf16, 64)
+NK_TILE(f16, f16, 64)
+
+// ---------------------------------------------------------------------------
+// The splits of a row joined, in their order: o = sum 2^(m_s - M) o_s / sum
+// 2^(m_s - M) l_s.  One wave per row; up to 64 splits, a lane each for their
+// offsets.  Rows that one split had are written already.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+__device__ __forceinline__ void attend_join_body(const AttendArgs &a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nr = (int64_t)a.N * a.Hq;
+  if (r >= nr) return;
+  const int t = (int)(r / a.Hq), h = (int)(r % a.Hq), rep = a.Hq / a.Hkv;
+  const int b = a.starts ? att_find(a.B, t, [&](int x) { return a.starts[x]; }) : t / a.S;
+  if (b < 0) return;
+  const AttSeq sq = att_seq(a, b);
+  const int i = t - sq.lo;
+  if (i >= sq.n) return;
+  int j0, j1;
+  const int pieces = att_split(a, att_span(a, sq, (i * rep + h % rep) / ATT_ROWS).nb, 0, j0, j1);
+  if (pieces == 1) return;
+  const float *wm = a.ws + (int64_t)a.nsplit * nr * D;
+  float m = -1e30f, l = 0.f;
+  if (lane < pieces) {
+    const float2 v = *reinterpret_cast<const float2 *>(wm + (lane * nr + r) * 2);
+    m = v.x, l = v.y;
+  }
+  const float w = __builtin_amdgcn_exp2f(m - wave_max(m));
+  const float total = wave_sum(lane < pieces ? w * l : 0.f);
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  float acc[D / 64];
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) acc[e] = 0.f;
+  for (int s0 = 0; s0 < pieces; s0 += 8) {
+    float x[8][D / 64];
+#pragma unroll
+    for (int s = 0; s < 8; ++s)  // (past the last piece: the last again, unused)
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) x[s][e] = a.ws[((int64_t)min(s0 + s, pieces - 1) * nr + r) * D + lane + 64 * e];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if (s0 + s >= pieces) break;
+      const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + s));
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(ws, x[s][e], acc[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) Elt<T>::store((T *)a.o + r * D, lane + 64 * e, total == 0.f ? 0.f : acc[e] * inv);
+}
+#define NK_JOIN(T, name, D)                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void nk_attend_join_##name##_d##D(AttendArgs a) { \
+    attend_join_body<T, D>(a);                                                                    \
+  }
+NK_JOIN(bf16, bf16, 128)
+NK_JOIN(f16, f16, 128)
+NK_JOIN(bf16, bf16, 64)
+NK_JOIN(f16, f16, 64)

@@ -20,6 +20,7 @@ from nkipy_amd.core.backend.ir import Node, Value
 from nkipy_amd.dispatch import generic as G
 from nkipy_amd.dispatch.launchers import Launch, LaunchError, dtype_tag
 from nkipy_amd.dispatch.patterns import LaunchStep, Match
+from nkipy_amd.dispatch.plan import Slot
 from nkipy_amd.dispatch.views import View, resolve
 
 NO_WINDOW = 2**30
@@ -80,12 +81,34 @@ def rotary_append(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q=0, 
                   bytes=nbytes)
 
 
+ATT_ROWS, ATT_KEYS = 128, 32  # rows of a tile, keys of a block (attend.h)
+ATT_SLOTS = 512               # workgroups of the tiled form that run at once: two per CU
+ATT_MIN_BLOCKS = 4            # blocks a split has at least
+ATT_MAX_SPLIT = 64            # a lane of the joining wave for each
+
+
+def attend_tiled(dtype, D) -> bool:
+    """Whether the tiled kernels have this type and head dim."""
+    return dt.canonical(dtype) in (dt.bfloat16, dt.float16) and D in (64, 128)
+
+
+def attend_splits(B, S, N, Hq, Hkv, keys, window=0, sinks=0, starts=False) -> Tuple[int, int]:
+    """(tiles per KV head, splits of a tile's keys): splits where the tiles
+    leave CUs idle, for the longest sequence that the tensors can hold."""
+    rep = Hq // Hkv
+    tiles = N * rep // ATT_ROWS + B if starts else B * -(-S * rep // ATT_ROWS)
+    seen = min(keys, window + sinks + -(-ATT_ROWS // rep) + ATT_KEYS) if window else keys
+    most = max(1, -(-seen // (ATT_KEYS * ATT_MIN_BLOCKS)))
+    return tiles, max(1, min(ATT_SLOTS // (tiles * Hkv), most, ATT_MAX_SPLIT))
+
+
 def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S=1, T=0, tables=0, lens=0, starts=0, first=0,
-           page=1, pages=0, width=0, pitch=0, window=0, sinks=0) -> List[Launch]:
+           page=1, pages=0, width=0, pitch=0, window=0, sinks=0, ws=0, zeros=0) -> List[Launch]:
     """Attention over a paged cache (``tables``; strides of q are (0, row,
     head), of the cache (0, row, head) with ``pitch`` rows from page to page)
     or plain tensors (B sequences of S queries and T keys; strides (sequence,
-    row, head))."""
+    row, head)).  ``zeros``: D zeros of the operands' type, for the tiled form;
+    ``ws``: 4 splits N Hq (D + 2) bytes where ``attend_splits`` splits."""
     if N < 1 or B < 1 or N * Hq >= 2**31:
         raise LaunchError(f"attention of {N} queries of {B} sequences and {Hq} heads")
     if Hkv < 1 or Hq % Hkv or not 1 <= D <= 256:
@@ -98,8 +121,24 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     a = _fields(AttendArgs(), q=q, k=k, v=v, o=o, tables=tables, lens=lens, starts=starts, first=first,
                 q_sb=q_str[0], q_ss=q_str[1], q_sh=q_str[2], k_sb=k_str[0], k_ss=k_str[1], k_sh=k_str[2],
                 v_sb=v_str[0], v_ss=v_str[1], v_sh=v_str[2], B=B, S=S, N=N, T=T, Hq=Hq, Hkv=Hkv, D=D, page=page, pages=pages,
-                width=width, pitch=pitch, window=window or NO_WINDOW, sinks=sinks, nsplit=1, min_blocks=1, scale=scale)
-    return [Launch("attend", f"nk_attend_rows_{dtype_tag(dtype)}", (-(-N * Hq // 4), 1, 1), (256, 1, 1), a)]
+                width=width, pitch=pitch, window=window or NO_WINDOW, sinks=sinks, nsplit=1, min_blocks=1, scale=scale,
+                ws=ws, zeros=zeros)
+    tag = dtype_tag(dtype)
+    tiled = attend_tiled(dtype, D) and zeros and not any(x % 16 for x in (q, k, v, o, zeros, ws)) \
+        and not any(x % 8 for x in (*q_str, *k_str, *v_str))
+    if not tiled:
+        return [Launch("attend", f"nk_attend_rows_{tag}", (-(-N * Hq // 4), 1, 1), (256, 1, 1), a)]
+    a.tiles, a.nsplit = attend_splits(B, S, N, Hq, Hkv, width * page if tables else T, window, sinks, bool(starts))
+    a.min_blocks = ATT_MIN_BLOCKS
+    if a.nsplit > 1 and not ws:
+        raise LaunchError(f"attention of {a.nsplit} splits needs a workspace")
+    if a.tiles * Hkv * a.nsplit >= 2**31 or Hq // Hkv * S >= 2**31:
+        raise LaunchError("attention: too many tiles for one launch")
+    kind = "paged" if tables else "plain"
+    out = [Launch("attend", f"nk_attend_tile_{kind}_{tag}_d{D}", (a.tiles * Hkv * a.nsplit, 1, 1), (256, 1, 1), a)]
+    if a.nsplit > 1:
+        out.append(Launch("attend", f"nk_attend_join_{tag}_d{D}", (-(-N * Hq // 4), 1, 1), (256, 1, 1), a))
+    return out
 
 
 def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_p) -> Launch:
@@ -294,10 +333,18 @@ class AttendMatch(Match):
                 more["first"] = rest.pop(0)
         if not q.size:
             return []
+        tmp = {}
+        if attend_tiled(q.dtype, kw["D"]):
+            keys = tables.shape[1] * k.shape[1] if self.paged else k.shape[1]
+            splits = attend_splits(kw["B"], kw.get("S", 1), kw["N"], kw["Hq"], kw["Hkv"], keys, kw["window"], kw["sinks"],
+                                   "starts" in more)[1]
+            tmp["zeros"] = Slot(plan.add_buffer(2 * kw["D"], "const", "attend.zeros", np.zeros(kw["D"], np.uint16)))
+            if splits > 1:
+                tmp["ws"] = Slot(plan.add_buffer(4 * splits * kw["N"] * kw["Hq"] * (kw["D"] + 2), "temp", "attend.splits"))
 
         def make(addr):
             return attend(q.dtype, _at(addr, self.q), _at(addr, self.k), _at(addr, self.v), addr(n.out),
-                          **kw, **{x: addr(y) for x, y in more.items()})
+                          **kw, **{x: addr(y) for x, y in {**more, **tmp}.items()})
 
         desc = (f"{'paged' if self.paged else 'window'} attention N={kw['N']} B={kw['B']} Hq={kw['Hq']} Hkv={kw['Hkv']} "
                 f"D={kw['D']} window={at['window']} sinks={at['sinks']}")
