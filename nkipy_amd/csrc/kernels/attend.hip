@@ -113,6 +113,30 @@ NK_DEVICE void att_zero_rest(const AttendArgs &a, int wg, int nwg) {
   }
 }
 
+// Workgroups run round-robin over the eight XCDs: with the KV head fastest, the
+// tiles of one head (eight heads, or a multiple) share an XCD's cache.  The last
+// tiles of a sequence, the longest without a window, go first.
+struct AttWork {
+  int g, split, b, tile;  // b < 0: nothing to do
+};
+template <bool PAGED>
+NK_DEVICE AttWork att_work(const AttendArgs &a, int w) {
+  AttWork k;
+  const int rep = a.Hq / a.Hkv;
+  k.g = w % a.Hkv;
+  w /= a.Hkv;
+  k.split = w % a.nsplit;
+  const int t = a.tiles - 1 - w / a.nsplit;
+  if (PAGED && a.starts) {
+    k.b = att_find(a.B, t, [&](int x) { return att_tile0(a, x); });
+    k.tile = k.b < 0 ? 0 : t - att_tile0(a, k.b);
+  } else {
+    const int per = (a.S * rep + ATT_ROWS - 1) / ATT_ROWS;
+    k.b = t / per, k.tile = t % per;
+  }
+  return k;
+}
+
 template <typename T, int D, bool PAGED>
 __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   typedef typename Mat<T>::V V8;
@@ -129,23 +153,10 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   const int l32 = lane & 31, lhi = lane >> 5;
   const int rep = a.Hq / a.Hkv;
 
-  // Workgroups run round-robin over the eight XCDs: with the KV head fastest,
-  // the tiles of one head (eight heads, or a multiple) share an XCD's cache.
-  // The last tiles of a sequence, the longest without a window, go first.
-  int w = blockIdx.x;
-  if (PAGED && a.starts) att_zero_rest<T>(a, w, a.tiles * a.Hkv * a.nsplit);
-  const int g = w % a.Hkv;
-  w /= a.Hkv;
-  const int split = w % a.nsplit, t = a.tiles - 1 - w / a.nsplit;
-  int b, tile;
-  if (PAGED && a.starts) {
-    b = att_find(a.B, t, [&](int x) { return att_tile0(a, x); });
-    if (b < 0) return;
-    tile = t - att_tile0(a, b);
-  } else {
-    const int per = (a.S * rep + ATT_ROWS - 1) / ATT_ROWS;
-    b = t / per, tile = t % per;
-  }
+  if (PAGED && a.starts) att_zero_rest<T>(a, blockIdx.x, a.tiles * a.Hkv * a.nsplit);
+  const AttWork wk = att_work<PAGED>(a, blockIdx.x);
+  const int g = wk.g, split = wk.split, b = wk.b, tile = wk.tile;
+  if (b < 0) return;
   const AttSeq sq = att_seq(a, b);
   if ((int64_t)tile * ATT_ROWS >= (int64_t)sq.n * rep) return;
   const AttSpan sp = att_span(a, sq, tile);
@@ -245,9 +256,11 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   auto qk = [&](const uint8_t *K, f32x16 &s) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    int x = kx;
+    asm volatile("" : "+v"(x));  // (eight sums kept through the loop would cost as many registers)
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
-      s = Mat<T>::mul(*reinterpret_cast<const V8 *>(K + kbase + ((kk << 5) ^ kx)), qf[kk], s);
+      s = Mat<T>::mul(*reinterpret_cast<const V8 *>(K + kbase + ((kk << 5) ^ x)), qf[kk], s);
   };
   // transposing V read (group lane / 16, i = lane % 16): row 16 j + 8 si + 4 (group / 2) + i / 4,
   // columns 32 dt + 16 (group % 2) + 4 (i % 4)
@@ -347,8 +360,8 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   // a whole block between others
   auto inner = [&](auto sl, int jr, f32x16 &cur, f32x16 &nxt, V8 (&prev)[2], V8 (&now)[2]) __attribute__((always_inline)) {
     constexpr int SL = decltype(sl)::value;
-    pv(VR + ((SL + 3) & 3) * TB, prev);
     qk(KR + ((SL + 1) & 3) * TB, nxt);
+    pv(VR + ((SL + 3) & 3) * TB, prev);
     softmax(cur, now, jr, Flag<false>{});
     // every LDS read first, then matrix instructions with the softmax between them
     __builtin_amdgcn_sched_group_barrier(0x100, 3 * D / 16, 0);
@@ -478,23 +491,34 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
       }
     if (lhi == 0) wm[0] = ok ? m_run : -1e30f, wm[1] = ok ? l_run : 0.f;
   }
-  // these again, reading only what they see
+  // These again, reading only what they see.  (The arguments are read anew, so
+  // that none of them takes a register through the loop above for this.)
   while (spoiled) {
+    typedef const __attribute__((address_space(4))) AttendArgs *Kernarg;
+    Kernarg args = (Kernarg)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    const AttendArgs &a2 = *(const AttendArgs *)args;
+    const AttWork wk2 = att_work<PAGED>(a2, blockIdx.x);
+    const AttSeq sq2 = att_seq(a2, wk2.b);
+    const AttSpan sp2 = att_span(a2, sq2, wk2.tile);
+    const int64_t nr2 = (int64_t)a2.N * a2.Hq;
+    int k0, k1;
+    const int pieces2 = att_split(a2, sp2.nb, wk2.split, k0, k1);
     const int src = __builtin_ctzll(spoiled);
     spoiled &= spoiled - 1;
     float m, l, x[4];
-    att_row<T>(a, sq, sp, b, __shfl(qi, src, 64), __shfl(h, src, 64), j0, j1, m, l, x);
+    att_row<T>(a2, sq2, sp2, wk2.b, __shfl(qi, src, 64), __shfl(h, src, 64), k0, k1, m, l, x);
     const int64_t at = __shfl((int)orow, src, 64);  // (rows are below 2^31)
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
-      if (pieces == 1) {
-        Elt<T>::store((T *)a.o + at * D, lane + 64 * e, l == 0.f ? 0.f : x[e] / l);
+      if (pieces2 == 1) {
+        Elt<T>::store((T *)a2.o + at * D, lane + 64 * e, l == 0.f ? 0.f : x[e] / l);
       } else {
-        a.ws[(split * nr + at) * D + lane + 64 * e] = x[e];
+        a2.ws[(wk2.split * nr2 + at) * D + lane + 64 * e] = x[e];
       }
     }
-    if (pieces > 1 && lane == 0) {
-      float *q = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + at) * 2;
+    if (pieces2 > 1 && lane == 0) {
+      float *q = a2.ws + (int64_t)a2.nsplit * nr2 * D + (wk2.split * nr2 + at) * 2;
       q[0] = l == 0.f ? -1e30f : m * 1.44269504088896340736f;
       q[1] = l;
     }
