@@ -132,20 +132,33 @@ NK_APPEND(float, f32)
 // ---------------------------------------------------------------------------
 // The draw of a token.
 //
-// Weights w = exp((x - max) / T) are kept as whole numbers of 2^-40: sums of
-// them are exact in 64 bits, so no order of additions or atomics changes a
-// result, and what rounds to 0 (below 2^-41 of the largest, 4e-13) takes no
-// part.  All three filters keep a beginning of the order (value, then index),
-// so they come down to one border: a value, and how many of its ties stay,
-// lowest index first.  The border is found without sorting the row:
-//   1. the largest logit;
-//   2. a histogram of counts and weights over BINS equal steps of (x - max) / T;
-//   3. the bin in which the count (top_k) or the weight (top_p) is reached;
-//   4. that bin's few values ranked against each other in LDS; a bin of more
-//      than LIST values (many ties, a narrow spread) is first cut down by
-//      further histograms over its range of values.
-// Then the kept weights are summed over tiles of the row in index order, the
-// tile holding uniform x total is found, and the token in it.
+// Weights w = 2^t, t = (x - max) log2(e) / T, are kept as whole numbers of
+// 2^-40: sums of them are exact in 64 bits, so no order of additions or atomics
+// changes a result, and what rounds to 0 (below 2^-41 of the largest, 4e-13)
+// takes no part.  All three filters keep a beginning of the order (value
+// descending, then index), so they come down to one border, the last (value,
+// index) that stays, and the row is never sorted.
+//
+// Long rows take three launches, two of them over segments of the row, so that
+// a few rows fill the chip:
+//   top    each segment's largest value;
+//   hist   each segment's counts and weights over BINS equal steps of t;
+//   pick   one workgroup per row: the segments' histograms added, the bin in
+//          which the count (top_k) or the weight (top_p) is reached, and the
+//          values that matter listed in LDS: everything down to that bin, if
+//          that is up to LIST values, and the border and the draw are searched
+//          there; else that bin alone for the border, then the segment that holds
+//          uniform x the kept weight, by the segments' sums.
+// Rows of up to LIST tokens are one launch: the list is the row.
+//
+// A search (smp_select) finds where the running count or weight of a list in
+// descending order of a key reaches a goal: histograms of 1024 steps of what is
+// left of the keys' range, until a step is one key.  The key is the value for a
+// border, the index for ties and for the draw.  A bin of more than LIST values
+// (ties, a narrow spread) is searched in the row itself.
+//
+// Bound by one read of the logits and, in hist, by about 30 instructions per
+// logit; with few rows by the latency of its launches.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
   const void *x;
@@ -154,17 +167,21 @@ struct SampleArgs {
   const float *temp;     // per row; null: c_temp (likewise below)
   const int32_t *topk;
   const float *topp, *minp;
+  uint64_t *tops;        // (rows, nseg): largest key and the complement of its index
+  uint64_t *sums;        // (rows, nseg, BINS + 1): weights per bin, then their sum
+  uint32_t *cnts;        // (rows, nseg, BINS)
   int64_t ld;            // elements from row to row
-  int32_t rows, vocab;
+  int32_t rows, vocab, seg, nseg;  // seg: tokens of a segment
   float c_temp;
   int32_t c_topk;        // below 1: all
   float c_topp, c_minp;  // 1, 0: all
 };
 
 #define SMP_BLOCK 1024
-#define SMP_BINS 2048
-#define SMP_LIST 2048
-#define SMP_TILES 1024  // tiles of a row, at most
+#define SMP_SEG_BLOCK 256
+#define SMP_BINS 512
+#define SMP_LIST 8192
+#define SMP_STEPS 1024
 typedef unsigned long long u64;
 
 // order of the values as whole numbers; -0 and 0 tie
@@ -172,28 +189,151 @@ NK_DEVICE uint32_t smp_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+NK_DEVICE float smp_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
 struct SmpRow {
-  float best, temp;
-  // (x - best) / temp; the largest is 0 also where it is infinite
-  NK_DEVICE float depth(float x) const { return x == best ? 0.f : (x - best) / temp; }
+  float best, c;  // largest logit, log2(e) / T
+  NK_DEVICE void set(float b, float temp) {
+    best = b;
+    c = fminf(1.44269504088896340736f / temp, 3.4e38f);
+  }
+  // log2 of the weight; the largest logit has 0 also where it is infinite
+  NK_DEVICE float depth(float x) const { return x == best ? 0.f : (x - best) * c; }
 };
-// weight in steps of 2^-40; 0 for NaN
-NK_DEVICE u64 smp_weight(float d) {
-  if (!(d > -29.f)) return 0;
-  const float w = exp_acc(d) * 0x1p40f;  // at most 2^40 and a few ulp
+// weight in steps of 2^-40; 0 for NaN.  The hardware's 2^t is within an ulp, 1e-7
+// of the weight.
+NK_DEVICE u64 smp_weight(float t) {
+  if (!(t > -42.f)) return 0;
+  const float w = __builtin_amdgcn_exp2f(t) * 0x1p40f;
   const uint32_t hi = (uint32_t)(w * 0x1p-16f);
-  const float rest = w - (float)hi * 0x1p16f;  // exact: below 2^16
+  const float rest = __builtin_fmaf((float)hi, -0x1p16f, w);  // exact: below 2^16
   return ((u64)hi << 16) + (u64)(uint32_t)__builtin_rintf(rest);
 }
-// the deepest weight above 0 is at 28.42: bin 2046
-NK_DEVICE int smp_bin(float d) { return min(SMP_BINS - 1, (int)(d * -72.f)); }
+// (a weight above 0 has t >= -41: bin 492 at most)
+NK_DEVICE int smp_bin(float t) { return min(SMP_BINS - 1, (int)(t * -12.f)); }
 
-template <typename V>
-NK_DEVICE V smp_shfl_up(V v, int n) {
-  return __shfl_up(v, n, 64);
+// Logits lo .. hi-1 of a row in pieces of 16 aligned bytes: f(index, value) by
+// THREADS threads.  The pieces at the ends are read element by element.
+template <typename T, int THREADS, typename F>
+NK_DEVICE void smp_each(const T *x, int lo, int hi, F f) {
+  constexpr int E = 16 / sizeof(T);
+  const int off = (int)(((uintptr_t)(x + lo) & 15) / sizeof(T));  // elements of the first piece before lo
+  for (int i = lo - off + threadIdx.x * E; i < hi; i += THREADS * E) {
+    if (i >= lo && i + E <= hi) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(x + i);
+      T v[E];
+      __builtin_memcpy(v, &u, 16);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f(i + e, Elt<T>::load(v, e));
+    } else {
+#pragma unroll 1
+      for (int e = max(0, lo - i); e < min(E, hi - i); ++e) f(i + e, Elt<T>::load(x, i + e));
+    }
+  }
 }
-// exclusive sums of c and w over the workgroup's threads, and the totals
-NK_DEVICE void smp_scan(uint32_t c, u64 w, uint32_t &ce, u64 &we, uint32_t &ct, u64 &wt, uint32_t *sc, u64 *sw) {
+
+template <int WAVES>
+NK_DEVICE u64 smp_max(u64 v, u64 *red) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = max(v, (u64)__shfl_xor(v, o, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) v = max(v, red[i]);
+  return v;
+}
+template <int WAVES>
+NK_DEVICE u64 smp_sum(u64 v, u64 *red) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += (u64)__shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) v += red[i];
+  return v;
+}
+// largest value of a stretch and its lowest index, as one number; 0 where all
+// are NaN or -inf
+template <typename T, int THREADS>
+NK_DEVICE u64 smp_top(const T *x, int lo, int hi, u64 *red) {
+  u64 top = 0;
+  smp_each<T, THREADS>(x, lo, hi, [&](int i, float v) {
+    if (v > -INFINITY) top = max(top, (u64)smp_key(v) << 32 | (uint32_t)~i);
+  });
+  return smp_max<THREADS / 64>(top, red);
+}
+
+template <typename T>
+__device__ __forceinline__ void sample_top_body(const SampleArgs &a) {
+  __shared__ u64 red[SMP_SEG_BLOCK / 64];
+  const int r = blockIdx.x / a.nseg, s = blockIdx.x % a.nseg;
+  const u64 top = smp_top<T, SMP_SEG_BLOCK>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), red);
+  if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
+}
+template <int THREADS>
+NK_DEVICE u64 smp_row_top(const SampleArgs &a, int r, u64 *red) {
+  u64 top = 0;
+  for (int i = threadIdx.x; i < a.nseg; i += THREADS) top = max(top, (u64)a.tops[(int64_t)r * a.nseg + i]);
+  return smp_max<THREADS / 64>(top, red);
+}
+// its settings; false where there is nothing to weigh: no logit to draw, or no
+// temperature
+NK_DEVICE bool smp_settings(const SampleArgs &a, int r, u64 top, SmpRow &row) {
+  const float temp = a.temp ? a.temp[r] : a.c_temp;
+  row.set(smp_value((uint32_t)(top >> 32)), temp);
+  return top && temp > 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
+  __shared__ u64 sum[SMP_BINS];
+  __shared__ uint32_t cnt[SMP_BINS];
+  __shared__ u64 red[SMP_SEG_BLOCK / 64];
+  const int r = blockIdx.x / a.nseg, s = blockIdx.x % a.nseg, tid = threadIdx.x;
+  for (int i = tid; i < SMP_BINS; i += SMP_SEG_BLOCK) sum[i] = 0, cnt[i] = 0;
+  SmpRow row;
+  if (!smp_settings(a, r, smp_row_top<SMP_SEG_BLOCK>(a, r, red), row)) return;
+  u64 all = 0;
+  const bool bins = a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f;
+  smp_each<T, SMP_SEG_BLOCK>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), [&](int, float v) {
+    const float t = row.depth(v);
+    const u64 w = smp_weight(t);
+    all += w;
+    if (bins && w) {
+      const int b = smp_bin(t);
+      atomicAdd(&cnt[b], 1u);
+      atomicAdd(&sum[b], w);
+    }
+  });
+  all = smp_sum<SMP_SEG_BLOCK / 64>(all, red);  // (and the histogram is whole)
+  uint64_t *so = a.sums + (int64_t)blockIdx.x * (SMP_BINS + 1);
+  uint32_t *co = a.cnts + (int64_t)blockIdx.x * SMP_BINS;
+  if (bins)
+    for (int i = tid; i < SMP_BINS; i += SMP_SEG_BLOCK) so[i] = sum[i], co[i] = cnt[i];
+  if (tid == 0) so[SMP_BINS] = all;
+}
+
+struct SmpShared {
+  u64 hsum[SMP_BINS];      // the row's histogram
+  u64 sum[SMP_STEPS];      // a search's
+  uint32_t hcnt[SMP_BINS];
+  uint32_t cnt[SMP_STEPS];
+  uint32_t key[SMP_LIST], idx[SMP_LIST];
+  u64 red[SMP_BLOCK / 64], sw[SMP_BLOCK / 64];
+  uint32_t sc[SMP_BLOCK / 64];
+  uint32_t n, kmin, kmax;
+  // where a running sum reached its goal: step, and count and weight before and with it
+  uint32_t bin, cb, ca;
+  u64 wb, wa;
+};
+
+// Running sums of one count and weight per thread, on top of cb and wb: the
+// first to reach `need` (COUNT) or `goal`.
+template <bool COUNT>
+NK_DEVICE void smp_search(SmpShared &s, uint32_t c, u64 w, uint32_t cb, u64 wb, uint32_t need, u64 goal) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   uint32_t ci = c;
   u64 wi = w;
@@ -204,294 +344,321 @@ NK_DEVICE void smp_scan(uint32_t c, u64 w, uint32_t &ce, u64 &we, uint32_t &ct, 
     if (lane >= o) ci += cu, wi += wu;
   }
   __syncthreads();
-  if (lane == 63) sc[wid] = ci, sw[wid] = wi;
+  if (lane == 63) s.sc[wid] = ci, s.sw[wid] = wi;
   __syncthreads();
-  ct = 0, wt = 0;
-  uint32_t cb = 0;
-  u64 wb = 0;
+  ci += cb, wi += wb;
 #pragma unroll
-  for (int i = 0; i < SMP_BLOCK / 64; ++i) {
-    if (i < wid) cb += sc[i], wb += sw[i];
-    ct += sc[i], wt += sw[i];
-  }
-  ce = cb + ci - c;
-  we = wb + wi - w;
-}
-
-struct SmpShared {
-  uint32_t cnt[2][SMP_BINS];
-  u64 sum[2][SMP_BINS];
-  uint32_t key[SMP_LIST], idx[SMP_LIST];
-  u64 w[SMP_LIST];
-  uint32_t skey[SMP_LIST];
-  uint32_t sc[SMP_BLOCK / 64];
-  u64 sw[SMP_BLOCK / 64];
-  u64 red[SMP_BLOCK / 64];
-  uint32_t n, kmin, kmax;
-  // what a search found
-  uint32_t bin, cb, key_at, ties;
-  u64 wb, upto;
-};
-
-// Where the running count reaches `need` (COUNT) or the running weight `goal`,
-// over the SMP_BINS entries of a histogram or the SMP_LIST of a ranked list
-// (two per thread); false where neither does.
-template <bool COUNT>
-NK_DEVICE bool smp_search(SmpShared &s, const uint32_t *cnt, const u64 *sum, uint32_t cb, u64 wb, uint32_t need, u64 goal) {
-  const int i = 2 * threadIdx.x;
-  const uint32_t c0 = cnt ? cnt[i] : 1, c1 = cnt ? cnt[i + 1] : 1;
-  const u64 w0 = sum[i], w1 = sum[i + 1];
-  uint32_t ce, ct;
-  u64 we, wt;
-  smp_scan(c0 + c1, w0 + w1, ce, we, ct, wt, s.sc, s.sw);
-  ce += cb, we += wb;
-  const bool before0 = COUNT ? ce < need : we < goal;
-  const bool in0 = COUNT ? ce + c0 >= need : we + w0 >= goal;
-  const bool in1 = COUNT ? ce + c0 + c1 >= need : we + w0 + w1 >= goal;
-  if (before0 && in1) {
-    s.bin = in0 ? i : i + 1;
-    s.cb = in0 ? ce : ce + c0;
-    s.wb = in0 ? we : we + w0;
-    s.upto = in0 ? we + w0 : we + w0 + w1;
-  }
+  for (int i = 0; i < SMP_BLOCK / 64; ++i)
+    if (i < wid) ci += s.sc[i], wi += s.sw[i];
+  if (COUNT ? ci - c < need && ci >= need : wi - w < goal && wi >= goal)
+    s.bin = threadIdx.x, s.cb = ci - c, s.ca = ci, s.wb = wi - w, s.wa = wi;
   __syncthreads();
-  return COUNT ? cb + ct >= need : wb + wt >= goal;
 }
 
-// The border in bin `s.bin` of the first histogram: the key of the last value
-// kept, how many of its ties are (s.key_at, s.ties), and the weight up to and
-// with it (s.upto).
-template <typename T, bool COUNT>
-NK_DEVICE void smp_border(SmpShared &s, const T *x, int vocab, const SmpRow &r, uint32_t need, u64 goal) {
+// where a search ended: the key, how many of its elements are in, and the weight
+// up to and with them
+struct SmpBorder {
+  uint32_t key, ties;
+  u64 upto;
+};
+// Of elements 0 .. n-1, f(i, key, weight) says which take part.  Those of one
+// key weigh the same.
+template <bool COUNT, typename F>
+NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, F f, uint32_t cb, u64 wb, uint32_t need, u64 goal) {
   const int tid = threadIdx.x;
-  const int bin = s.bin;
-  uint32_t cb = s.cb;
-  u64 wb = s.wb;
-  uint32_t klo = 0, khi = 0xffffffffu;  // the keys left
-  bool by_bin = true;
+  __syncthreads();
+  if (tid == 0) s.kmin = 0xffffffffu, s.kmax = 0;
+  __syncthreads();
+  uint32_t mn = 0xffffffffu, mx = 0, k;
+  u64 w;
+  for (int i = tid; i < n; i += SMP_BLOCK)
+    if (f(i, k, w)) mn = min(mn, k), mx = max(mx, k);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) mn = min(mn, (uint32_t)__shfl_xor(mn, o, 64)), mx = max(mx, (uint32_t)__shfl_xor(mx, o, 64));
+  if ((tid & 63) == 0) atomicMin(&s.kmin, mn), atomicMax(&s.kmax, mx);
+  __syncthreads();
+  uint32_t klo = s.kmin, khi = s.kmax;
+  SmpBorder b;
   while (true) {
+    const uint32_t range = max(khi, klo) - klo;
+    const int shift = range < SMP_STEPS ? 0 : 22 - __builtin_clz(range);
+    s.cnt[tid] = 0, s.sum[tid] = 0;
     __syncthreads();
-    if (tid == 0) s.n = 0, s.kmin = 0xffffffffu, s.kmax = 0;
-    __syncthreads();
-    uint32_t mn = 0xffffffffu, mx = 0;
-    for (int i = tid; i < vocab; i += SMP_BLOCK) {
-      const float v = Elt<T>::load(x, i);
-      const float d = r.depth(v);
-      const uint32_t k = smp_key(v);
-      if (!(d > -29.f) || (by_bin ? smp_bin(d) != bin : k < klo || k > khi)) continue;
-      const u64 w = smp_weight(d);
-      if (!w) continue;
-      mn = min(mn, k), mx = max(mx, k);
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < SMP_LIST) s.key[at] = k, s.idx[at] = i, s.w[at] = w;
-    }
-    atomicMin(&s.kmin, mn);
-    atomicMax(&s.kmax, mx);
-    __syncthreads();
-    const uint32_t n = s.n;
-    klo = s.kmin, khi = s.kmax;
-    if (n <= SMP_LIST) break;
-    // too many: a histogram of their range of keys, one key a bin once it is
-    // narrow enough
-    by_bin = false;
-    int shift = 0;
-    while (((khi - klo) >> shift) >= SMP_BINS) ++shift;
-    for (int i = tid; i < SMP_BINS; i += SMP_BLOCK) s.cnt[1][i] = 0, s.sum[1][i] = 0;
-    __syncthreads();
-    for (int i = tid; i < vocab; i += SMP_BLOCK) {
-      const float v = Elt<T>::load(x, i);
-      const float d = r.depth(v);
-      const uint32_t k = smp_key(v);
-      if (!(d > -29.f) || k < klo || k > khi) continue;
-      const u64 w = smp_weight(d);
-      if (!w) continue;
-      atomicAdd(&s.cnt[1][(khi - k) >> shift], 1u);
-      atomicAdd(&s.sum[1][(khi - k) >> shift], w);
-    }
-    __syncthreads();
-    smp_search<COUNT>(s, s.cnt[1], s.sum[1], cb, wb, need, goal);
-    const uint32_t sub = s.bin;
-    cb = s.cb, wb = s.wb;
-    if (shift == 0) {  // one key: its ties share a weight
-      if (tid == 0) {
-        const u64 w = s.sum[1][sub] / s.cnt[1][sub];
-        s.key_at = khi - sub;
-        s.ties = COUNT ? need - cb : (uint32_t)((goal - wb + w - 1) / w);
-        s.upto = wb + s.ties * w;
+    for (int i = tid; i < n; i += SMP_BLOCK)
+      if (f(i, k, w) && k >= klo && k <= khi) {
+        atomicAdd(&s.cnt[(khi - k) >> shift], 1u);
+        atomicAdd(&s.sum[(khi - k) >> shift], w);
       }
-      __syncthreads();
-      return;
+    __syncthreads();
+    smp_search<COUNT>(s, s.cnt[tid], s.sum[tid], cb, wb, need, goal);
+    const uint32_t at = s.bin;
+    cb = s.cb, wb = s.wb;
+    if (shift == 0) {
+      const u64 each = (s.wa - wb) / max(s.ca - cb, 1u);
+      b.key = khi - at;
+      b.ties = COUNT ? need - cb : (uint32_t)((goal - wb + each - 1) / max(each, (u64)1));
+      b.upto = wb + b.ties * each;
+      return b;
     }
-    const uint32_t top = khi - (sub << shift), low = top - ((1u << shift) - 1);
-    klo = low > top ? klo : max(klo, low);
+    const uint32_t top = khi - (at << shift);
+    klo = top - klo < (1u << shift) ? klo : top - (1u << shift) + 1;
     khi = top;
   }
-  // rank the list: larger keys first, then lower indices
-  const uint32_t n = s.n;
-  uint32_t myk[SMP_LIST / SMP_BLOCK], rank[SMP_LIST / SMP_BLOCK];
-  u64 myw[SMP_LIST / SMP_BLOCK];
-#pragma unroll
-  for (int e = 0; e < SMP_LIST / SMP_BLOCK; ++e) {
-    const uint32_t i = tid + e * SMP_BLOCK;
-    rank[e] = i;
-    myk[e] = 0, myw[e] = 0;
-    if (i < n) {
-      const uint32_t k = s.key[i], ix = s.idx[i];
-      uint32_t c = 0;
-      for (uint32_t j = 0; j < n; ++j) c += s.key[j] > k || (s.key[j] == k && s.idx[j] < ix);
-      rank[e] = c;
-      myk[e] = k, myw[e] = s.w[i];
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < SMP_LIST / SMP_BLOCK; ++e) s.skey[rank[e]] = myk[e], s.w[rank[e]] = myw[e];
-  __syncthreads();
-  smp_search<COUNT>(s, nullptr, s.w, cb, wb, need, goal);
-  if (tid == 0) {
-    const uint32_t at = min(s.bin, n - 1), k = s.skey[at];
-    uint32_t ties = 1;
-    while (ties <= at && s.skey[at - ties] == k) ++ties;
-    s.key_at = k;
-    s.ties = ties;
-  }
-  __syncthreads();
 }
 
-template <typename T>
-__device__ __forceinline__ void sample_body(const SampleArgs &a) {
-  __shared__ SmpShared s;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r = blockIdx.x;
-  const T *x = (const T *)a.x + (int64_t)r * a.ld;
-  SmpRow row;
-  row.temp = a.temp ? a.temp[r] : a.c_temp;
-  // 1. the largest logit and its lowest index
-  u64 top = 0;
-  for (int i = tid; i < a.vocab; i += SMP_BLOCK) {
-    const float v = Elt<T>::load(x, i);
-    if (v > -INFINITY) top = max(top, (u64)smp_key(v) << 32 | (uint32_t)~i);
-  }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) top = max(top, (u64)__shfl_xor(top, o, 64));
-  if (lane == 0) s.red[wid] = top;
+// the elements of a stretch for which f holds, into the list
+template <typename T, typename F>
+NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, F f) {
   __syncthreads();
-  for (int i = 0; i < SMP_BLOCK / 64; ++i) top = max(top, s.red[i]);
-  const int32_t first = top ? (int32_t)~(uint32_t)top : -1;
-  if (first < 0 || !(row.temp > 0.f)) {
-    if (tid == 0) a.out[r] = first;
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  smp_each<T, SMP_BLOCK>(x, lo, hi, [&](int i, float v) {
+    if (f(i, v)) {
+      const uint32_t at = atomicAdd(&s.n, 1u);
+      if (at < SMP_LIST) s.key[at] = smp_key(v), s.idx[at] = i;
+    }
+  });
+  __syncthreads();
+  return s.n;
+}
+
+template <bool B> struct SmpFlag {
+  static constexpr bool value = B;
+};
+// SMALL: the row is one segment of up to LIST tokens, and this its only launch
+template <typename T, bool SMALL>
+__device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
+  __shared__ SmpShared s;
+  const int tid = threadIdx.x, r = blockIdx.x;
+  const T *x = (const T *)a.x + r * a.ld;
+  const u64 top = SMALL ? smp_top<T, SMP_BLOCK>(x, 0, a.vocab, s.red) : smp_row_top<SMP_BLOCK>(a, r, s.red);
+  SmpRow row;
+  if (!smp_settings(a, r, top, row)) {
+    if (tid == 0) a.out[r] = top ? (int32_t)~(uint32_t)top : -1;
     return;
   }
-  row.best = Elt<T>::load(x, first);
   const int topk = a.topk ? a.topk[r] : a.c_topk;
   const float topp = a.topp ? a.topp[r] : a.c_topp, minp = a.minp ? a.minp[r] : a.c_minp;
-  const bool by_k = topk > 0 && topk < a.vocab, by_p = topp < 1.f;
-  uint32_t border = 0, ties = 0xffffffffu;
-  if (by_k || by_p) {
-    // 2. the histogram
-    for (int i = tid; i < SMP_BINS; i += SMP_BLOCK) s.cnt[0][i] = 0, s.sum[0][i] = 0;
-    __syncthreads();
-    u64 all = 0;
-    for (int i = tid; i < a.vocab; i += SMP_BLOCK) {
-      const float d = row.depth(Elt<T>::load(x, i));
-      const u64 w = smp_weight(d);
-      if (!w) continue;
-      const int b = smp_bin(d);
-      all += w;
-      atomicAdd(&s.cnt[0][b], 1u);
-      atomicAdd(&s.sum[0][b], w);
-    }
-    // 3. and 4., first by the count, then by the weight of what it left
-    uint32_t ce, ct;
-    u64 we, total;
-    smp_scan(0, all, ce, we, ct, total, s.sc, s.sw);
-    if (by_k && smp_search<true>(s, s.cnt[0], s.sum[0], 0, 0, topk, 0)) {
-      smp_border<T, true>(s, x, a.vocab, row, topk, 0);
-      border = s.key_at, ties = s.ties, total = s.upto;
-    }
-    if (by_p) {
-      // whole steps: at least topp of the total, at least one
-      const double g = ceil((double)fmaxf(topp, 0.f) * (double)total);
-      const u64 goal = min(max((u64)g, (u64)1), total);
-      __syncthreads();
-      smp_search<false>(s, s.cnt[0], s.sum[0], 0, 0, 0, goal);
-      smp_border<T, false>(s, x, a.vocab, row, 0, goal);
-      border = s.key_at, ties = s.ties;
-    }
-  }
-  // the kept weights of each tile, in index order; ties of the border apart,
-  // as how many of them stay depends on the tiles before
-  const int tile = max(256, (a.vocab + SMP_TILES * 256 - 1) / (SMP_TILES * 256) * 256);
-  const int tiles = (a.vocab + tile - 1) / tile;
-  const float floor_w = fminf(minp, 1.f);
-  u64 *tw = s.sum[1];
-  uint32_t *tt = s.cnt[1];
-  auto weigh = [&](int i, uint32_t &tie) -> u64 {
-    const float v = Elt<T>::load(x, i);
-    const float d = row.depth(v);
-    const u64 w = smp_weight(d);
-    const uint32_t k = smp_key(v);
-    tie = 0;
-    if (!w || k < border || (floor_w > 0.f && !(exp_acc(d) >= floor_w))) return 0;
-    if (k == border) {
-      tie = 1;
-      return 0;
-    }
-    return w;
+  const bool by_k = topk > 0 && topk < a.vocab, by_p = topp < 1.f, by_m = minp > 0.f;
+  const float tmin = by_m ? log2f(fminf(minp, 1.f)) : -INFINITY;  // the least depth that min_p keeps
+
+  // a listed or stored element's weight
+  auto listed = [&](int i, uint32_t &k, u64 &w) {
+    k = s.key[i];
+    w = smp_weight(row.depth(smp_value(k)));
+    return true;
   };
-  // (a border of 0, the whole row, is no value's key)
-  const float best_border = border ? __uint_as_float(border & 0x80000000u ? border & 0x7fffffffu : ~border) : 0.f;
-  u64 tie_w = border ? smp_weight(row.depth(best_border)) : 0;
-  __syncthreads();
-  for (int t = wid; t < tiles; t += SMP_BLOCK / 64) {
-    u64 w = 0;
+  auto stored = [&](int i, uint32_t &k, u64 &w) {
+    const float v = Elt<T>::load(x, i);
+    k = smp_key(v);
+    w = smp_weight(row.depth(v));
+    return w != 0;
+  };
+  const uint64_t *sums = a.sums + (int64_t)r * a.nseg * (SMP_BINS + 1);
+  const uint32_t *cnts = a.cnts + (int64_t)r * a.nseg * SMP_BINS;
+  bool whole = SMALL;      // the list holds all that is kept
+  u64 total = 0;           // weight of the row
+  int n = 0;
+  uint32_t cbin = 0;       // the border's bin, count and weight before it (not whole)
+  int last = SMP_BINS - 1; // bins up to here can be kept
+  if (SMALL) {
+    n = smp_gather(s, x, 0, a.vocab, [&](int, float v) { return smp_weight(row.depth(v)) != 0; });
+    if (by_p && !(by_k && n >= topk)) {
+      for (int i = tid; i < n; i += SMP_BLOCK) {
+        uint32_t k;
+        u64 w;
+        listed(i, k, w);
+        total += w;
+      }
+      total = smp_sum<SMP_BLOCK / 64>(total, s.red);
+    }
+  } else if (by_k || by_p || by_m) {
     uint32_t c = 0;
-    for (int i = t * tile + lane; i < min(a.vocab, (t + 1) * tile); i += 64) {
-      uint32_t tie;
-      w += weigh(i, tie);
-      c += tie;
+    u64 w = 0;
+    const int bin = tid % SMP_BINS;
+    for (int i = tid / SMP_BINS; i < a.nseg; i += SMP_BLOCK / SMP_BINS) {
+      c += cnts[(int64_t)i * SMP_BINS + bin];
+      w += sums[(int64_t)i * (SMP_BINS + 1) + bin];
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) w += (u64)__shfl_xor(w, o, 64), c += __shfl_xor(c, o, 64);
-    if (lane == 0) tw[t] = w, tt[t] = c;
+    if (tid < SMP_BINS) s.hcnt[bin] = c, s.hsum[bin] = w;
+    __syncthreads();
+    if (tid >= SMP_BINS) s.hcnt[bin] += c, s.hsum[bin] += w;
+    total = smp_sum<SMP_BLOCK / 64>(w, s.red);  // (and the histogram is whole)
   }
-  __syncthreads();
-  uint32_t c = tid < tiles ? tt[tid] : 0, ce, ct;
-  u64 w = tid < tiles ? tw[tid] : 0, we, wt;
-  smp_scan(c, w, ce, we, ct, wt, s.sc, s.sw);
-  // weights with the ties that stay
-  we += min(ce, ties) * tie_w;
-  w += (min(ce + c, ties) - min(ce, ties)) * tie_w;
-  wt += min(ct, ties) * tie_w;
+  auto bin_of_row = [&](bool count, uint32_t need, u64 goal) {
+    const uint32_t c = tid < SMP_BINS ? s.hcnt[tid] : 0;
+    const u64 w = tid < SMP_BINS ? s.hsum[tid] : 0;
+    __syncthreads();
+    if (tid == 0) s.bin = SMP_BINS, s.cb = 0, s.ca = 0, s.wb = 0, s.wa = 0;
+    if (count) smp_search<true>(s, c, w, 0, 0, need, goal);
+    else smp_search<false>(s, c, w, 0, 0, need, goal);
+  };
+  auto share = [&](u64 of) {  // whole steps: at least topp of it, at least one
+    return min(max((u64)ceil((double)fmaxf(topp, 0.f) * (double)of), (u64)1), of);
+  };
+  bool k_cuts = by_k, p_cuts = by_p;
+  if (SMALL) {
+    k_cuts = by_k && n >= topk;
+  } else if (by_k || by_p || by_m) {
+    // the bin that holds the first border; a top_k past the row's weights cuts nothing
+    if (by_k) {
+      bin_of_row(true, topk, 0);
+      k_cuts = s.bin < SMP_BINS;
+    }
+    if (!k_cuts && by_p) bin_of_row(false, 0, share(total));
+    if (k_cuts || by_p) last = s.bin;
+    if (by_m && !(k_cuts && by_p) && smp_bin(tmin) < last) {
+      last = smp_bin(tmin);  // min_p ends before either: their border is of no use
+      k_cuts = p_cuts = false;
+    }
+    // everything down to there, where the list can hold it
+    const uint32_t upto = (uint32_t)smp_sum<SMP_BLOCK / 64>(tid <= last ? s.hcnt[tid] : 0, s.red);
+    if (upto <= SMP_LIST) {
+      const float least = -((float)last + 1.01f) / 12.f;
+      n = smp_gather(s, x, 0, a.vocab, [&](int, float v) {
+        const float t = row.depth(v);
+        return t > least && smp_bin(t) <= last && smp_weight(t) != 0;
+      });
+      whole = true;
+    }
+  }
+
+  // the border: the last (value, index) kept
+  uint32_t bkey = 0, bidx = 0xffffffffu;
+  auto tie_break = [&](const SmpBorder &b, int len, auto each, auto index) {
+    bkey = b.key;
+    // the highest index of its ties that stays: by count, lowest first
+    bidx = ~smp_select<true>(s, len, [&](int i, uint32_t &k, u64 &w) {
+      const bool in = each(i, k, w) && k == b.key;
+      k = ~index(i);
+      return in;
+    }, 0, 0, b.ties, 0).key;
+  };
+  int held = -1;  // the bin that the list holds
+  auto in_list = [&](int i) { return s.idx[i]; };
+  auto in_row = [&](int i) { return (uint32_t)i; };
+  if (whole) {
+    if (k_cuts || p_cuts) {
+      SmpBorder b;
+      if (k_cuts) b = smp_select<true>(s, n, listed, 0, 0, topk, 0);
+      if (p_cuts) b = smp_select<false>(s, n, listed, 0, 0, 0, share(k_cuts ? b.upto : total));
+      tie_break(b, n, listed, in_list);
+    }
+  } else if (k_cuts || p_cuts) {
+    SmpBorder b;
+    // the values of one bin, from the list or, too many, from the row
+    bool fits = false;
+    auto find = [&](auto count, uint32_t need, u64 goal) {
+      const int bin = s.bin;
+      const uint32_t cb = s.cb;
+      const u64 wb = s.wb;
+      cbin = bin;
+      auto of_bin = [&](int i, uint32_t &k, u64 &w) { return stored(i, k, w) && smp_bin(row.depth(smp_value(k))) == bin; };
+      if (bin != held) {
+        fits = s.ca - cb <= SMP_LIST;
+        if (fits) n = smp_gather(s, x, 0, a.vocab, [&](int, float v) {
+          const float t = row.depth(v);
+          return smp_bin(t) == bin && smp_weight(t) != 0;
+        });
+        held = fits ? bin : -1;
+      }
+      constexpr bool COUNT = decltype(count)::value;
+      b = fits ? smp_select<COUNT>(s, n, listed, cb, wb, need, goal) : smp_select<COUNT>(s, a.vocab, of_bin, cb, wb, need, goal);
+    };
+    if (k_cuts) find(SmpFlag<true>{}, topk, 0);
+    if (p_cuts) {
+      const u64 goal = share(k_cuts ? b.upto : total);
+      bin_of_row(false, 0, goal);
+      find(SmpFlag<false>{}, 0, goal);
+    }
+    if (fits) tie_break(b, n, listed, in_list);
+    else tie_break(b, a.vocab, stored, in_row);
+  }
+  auto kept = [&](uint32_t k, uint32_t i, float t) { return (k > bkey || (k == bkey && i <= bidx)) && t >= tmin; };
+
+  // the draw: the first kept index up to and with which the weights exceed
+  // uniform x their sum, that is, reach the whole number behind it
   const float uni = a.u[r];
-  u64 goal = uni > 0.f ? (u64)(fmin((double)uni, 1.) * (double)wt) : 0;
-  if (!(uni < 1.f) || goal >= wt) goal = wt - 1;  // (NaN too: the last kept)
-  if (we <= goal && goal < we + w) s.bin = tid, s.cb = ce, s.wb = we;
-  __syncthreads();
-  if (wid) return;
-  const int t0 = s.bin * tile, t1 = min(a.vocab, t0 + tile);
-  uint32_t cb = s.cb;
-  u64 wb = s.wb;
-  for (int i0 = t0; i0 < t1; i0 += 64) {
-    uint32_t tie = 0;
-    u64 mine = i0 + lane < t1 ? weigh(i0 + lane, tie) : 0;
-    const u64 tied = __ballot(tie);
-    const uint32_t before = cb + __popcll(tied & ((1ull << lane) - 1));
-    if (tie && before < ties) mine = tie_w;
-    u64 run = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const u64 up = __shfl_up(run, o, 64);
-      if (lane >= o) run += up;
+  auto goal_of = [&](u64 all) {
+    const u64 g = uni > 0.f ? (u64)(fmin((double)uni, 1.) * (double)all) : 0;
+    return !(uni < 1.f) || g >= all ? all : g + 1;  // (NaN too: the last kept)
+  };
+  auto draw = [&](u64 goal, u64 before) {
+    const uint32_t at = ~smp_select<false>(s, n, [&](int i, uint32_t &k, u64 &w) {
+      listed(i, k, w);
+      const bool in = kept(k, s.idx[i], row.depth(smp_value(k)));
+      k = ~s.idx[i];
+      return in;
+    }, 0, before, 0, goal).key;
+    if (tid == 0) a.out[r] = at;
+  };
+  if (whole) {
+    u64 all = 0;
+    for (int i = tid; i < n; i += SMP_BLOCK) {
+      uint32_t k;
+      u64 w;
+      listed(i, k, w);
+      if (kept(k, s.idx[i], row.depth(smp_value(k)))) all += w;
     }
-    const u64 hit = __ballot(wb + run > goal);
-    if (hit) {
-      if (lane == 0) a.out[r] = i0 + __builtin_ctzll(hit);
-      return;
-    }
-    cb += __popcll(tied);
-    wb += (u64)__shfl(run, 63, 64);
+    draw(goal_of(smp_sum<SMP_BLOCK / 64>(all, s.red)), 0);
+    return;
   }
+  // by segments: bins before the border's are kept whole; of the one it is in,
+  // what is kept is added value by value
+  const int edge = min(k_cuts || p_cuts ? (int)cbin : SMP_BINS, by_m ? smp_bin(tmin) : SMP_BINS);
+  u64 *seg = s.sum;  // (up to STEPS segments)
+  __syncthreads();
+  seg[tid] = 0;
+  __syncthreads();
+  if (edge == SMP_BINS) {
+    for (int i = tid; i < a.nseg; i += SMP_BLOCK) seg[i] = sums[(int64_t)i * (SMP_BINS + 1) + SMP_BINS];
+  } else {
+    for (int i = tid >> 6; i < a.nseg; i += SMP_BLOCK / 64) {  // a wave for each
+      u64 w = 0;
+      for (int b = tid & 63; b < edge; b += 64) w += sums[(int64_t)i * (SMP_BINS + 1) + b];
+#pragma unroll
+      for (int o = 32; o; o >>= 1) w += (u64)__shfl_xor(w, o, 64);
+      if ((tid & 63) == 0) atomicAdd(&seg[i], w);
+    }
+    if (held == edge) {
+      for (int i = tid; i < n; i += SMP_BLOCK) {
+        const float t = row.depth(smp_value(s.key[i]));
+        if (kept(s.key[i], s.idx[i], t)) atomicAdd(&seg[s.idx[i] / a.seg], smp_weight(t));
+      }
+    } else {
+      smp_each<T, SMP_BLOCK>(x, 0, a.vocab, [&](int i, float v) {
+        const float t = row.depth(v);
+        if (!(t > -42.f) || smp_bin(t) != edge) return;
+        const u64 w = smp_weight(t);
+        if (w && kept(smp_key(v), i, t)) atomicAdd(&seg[i / a.seg], w);
+      });
+    }
+  }
+  __syncthreads();
+  const u64 mine = tid < a.nseg ? seg[tid] : 0;
+  const u64 goal = goal_of(smp_sum<SMP_BLOCK / 64>(mine, s.red));
+  smp_search<false>(s, 0, mine, 0, 0, 0, goal);
+  const int at = s.bin;
+  const u64 before = s.wb;
+  n = smp_gather(s, x, at * a.seg, min(a.vocab, (at + 1) * a.seg), [&](int i, float v) {
+    const float t = row.depth(v);
+    return smp_weight(t) != 0 && kept(smp_key(v), i, t);
+  });
+  draw(goal, before);
 }
-extern "C" __global__ __launch_bounds__(SMP_BLOCK) void nk_sample_bf16(SampleArgs a) { sample_body<bf16>(a); }
-extern "C" __global__ __launch_bounds__(SMP_BLOCK) void nk_sample_f16(SampleArgs a) { sample_body<f16>(a); }
-extern "C" __global__ __launch_bounds__(SMP_BLOCK) void nk_sample_f32(SampleArgs a) { sample_body<float>(a); }
+#define NK_SAMPLE(T, name)                                                                          \
+  extern "C" __global__ __launch_bounds__(SMP_SEG_BLOCK) void nk_sample_top_##name(SampleArgs a) {  \
+    sample_top_body<T>(a);                                                                          \
+  }                                                                                                 \
+  extern "C" __global__ __launch_bounds__(SMP_SEG_BLOCK) void nk_sample_hist_##name(SampleArgs a) { \
+    sample_hist_body<T>(a);                                                                         \
+  }                                                                                                 \
+  extern "C" __global__ __launch_bounds__(SMP_BLOCK) void nk_sample_pick_##name(SampleArgs a) {     \
+    sample_pick_body<T, false>(a);                                                                  \
+  }                                                                                                 \
+  extern "C" __global__ __launch_bounds__(SMP_BLOCK) void nk_sample_row_##name(SampleArgs a) {      \
+    sample_pick_body<T, true>(a);                                                                   \
+  }
+NK_SAMPLE(bf16, bf16)
+NK_SAMPLE(f16, f16)
+NK_SAMPLE(float, f32)

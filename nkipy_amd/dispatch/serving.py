@@ -45,9 +45,9 @@ class AttendArgs(ctypes.Structure):
 
 
 class SampleArgs(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp")]
-                + [("ld", ctypes.c_int64), ("rows", ctypes.c_int32), ("vocab", ctypes.c_int32),
-                   ("c_temp", ctypes.c_float), ("c_topk", ctypes.c_int32), ("c_topp", ctypes.c_float),
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp", "tops", "sums", "cnts")]
+                + [("ld", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("rows", "vocab", "seg", "nseg")]
+                + [("c_temp", ctypes.c_float), ("c_topk", ctypes.c_int32), ("c_topp", ctypes.c_float),
                    ("c_minp", ctypes.c_float)])
 
 
@@ -141,15 +141,46 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     return out
 
 
-def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_p) -> Launch:
+SMP_LIST, SMP_BINS = 8192, 512  # tokens of a row in one launch, bins of a histogram (serving.hip)
+
+
+def sample_segments(rows: int, vocab: int) -> Tuple[int, int]:
+    """(tokens of a segment, segments of a row): as long as the segments still
+    fill the CUs, since the last launch adds a histogram for each."""
+    for seg in (8192, 4096, 2048):
+        if seg == 2048 or rows * -(-vocab // seg) >= 512:
+            break
+    while -(-vocab // seg) > 1024:
+        seg *= 2
+    return seg, -(-vocab // seg)
+
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    if vocab <= SMP_LIST:
+        return 0
+    return rows * sample_segments(rows, vocab)[1] * (8 + 8 * (SMP_BINS + 1) + 4 * SMP_BINS)
+
+
+def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_p, ws=0) -> List[Launch]:
     """One token per row of logits; each filter is (address of one value per
-    row or 0, number)."""
+    row or 0, number).  ``ws``: ``sample_workspace_bytes``."""
     if rows < 1 or not 1 <= vocab <= 2**22:
         raise LaunchError(f"sample: {rows} rows of {vocab}")
     a = _fields(SampleArgs(), x=x, u=u, out=out, ld=ld, rows=rows, vocab=vocab, temp=temperature[0], c_temp=temperature[1],
                 topk=top_k[0], c_topk=top_k[1], topp=top_p[0], c_topp=top_p[1], minp=min_p[0], c_minp=min_p[1])
-    return Launch("serving", f"nk_sample_{dtype_tag(dtype)}", (rows, 1, 1), (1024, 1, 1), a,
-                  bytes=rows * (vocab * dt.itemsize(dtype) + 8))
+    tag, nbytes = dtype_tag(dtype), rows * (vocab * dt.itemsize(dtype) + 8)
+    if vocab <= SMP_LIST:
+        return [Launch("serving", f"nk_sample_row_{tag}", (rows, 1, 1), (1024, 1, 1), a, bytes=nbytes)]
+    a.seg, a.nseg = sample_segments(rows, vocab)
+    if not ws or ws % 8:
+        raise LaunchError("sample: long rows need a workspace")
+    n = rows * a.nseg
+    if n >= 2**31:
+        raise LaunchError("sample: too many rows for one launch")
+    _fields(a, tops=ws, sums=ws + 8 * n, cnts=ws + 8 * n * (SMP_BINS + 2))
+    return [Launch("serving", f"nk_sample_top_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
+            Launch("serving", f"nk_sample_hist_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
+            Launch("serving", f"nk_sample_pick_{tag}", (rows, 1, 1), (1024, 1, 1), a)]
 
 
 # ---------------------------------------------------------------------------
@@ -371,9 +402,13 @@ class SampleMatch(Match):
             x = n.attrs.get(name)
             given[name] = (rest.pop(0), none) if x == "rows" else (None, none if x is None else x)
 
+        need = sample_workspace_bytes(rows, vocab)
+        ws = Slot(plan.add_buffer(need, "temp", "sample.segments")) if need else None
+
         def make(addr):
             f = {name: (addr(v) if v is not None else 0, c) for name, (v, c) in given.items()}
-            return sample(n.inputs[0].dtype, _at(addr, self.x), addr(n.inputs[1]), addr(n.out), rows, vocab, self.ld, **f)
+            return sample(n.inputs[0].dtype, _at(addr, self.x), addr(n.inputs[1]), addr(n.out), rows, vocab, self.ld,
+                          ws=addr(ws) if ws is not None else 0, **f)
 
         return [LaunchStep("sample", f"sample {rows}x{vocab}", self.inputs, self.outputs, make)]
 
