@@ -133,8 +133,8 @@ NK_APPEND(float, f32)
 // The draw of a token.
 //
 // Weights w = 2^t, t = (x - max) log2(e) / T, are kept as whole numbers of
-// 2^-40: sums of them are exact in 64 bits, so no order of additions or atomics
-// changes a result, and what rounds to 0 (below 2^-41 of the largest, 4e-13)
+// 2^-36: sums of them are exact in 64 bits, so no order of additions or atomics
+// changes a result, and what rounds to 0 (below 2^-37 of the largest, 7e-12)
 // takes no part.  All three filters keep a beginning of the order (value
 // descending, then index), so they come down to one border, the last (value,
 // index) that stays, and the row is never sorted.
@@ -142,7 +142,9 @@ NK_APPEND(float, f32)
 // Long rows take three launches, two of them over segments of the row, so that
 // a few rows fill the chip:
 //   top    each segment's largest value;
-//   hist   each segment's counts and weights over BINS equal steps of t;
+//   hist   each segment's counts and weights over BINS equal steps of t, a bin's
+//          both in one word (14 bits count up to 8192 tokens, 50 the weight), so
+//          that a logit costs one LDS atomic;
 //   pick   one workgroup per row: the segments' histograms added, the bin in
 //          which the count (top_k) or the weight (top_p) is reached, and the
 //          values that matter listed in LDS: everything down to that bin, if
@@ -151,11 +153,12 @@ NK_APPEND(float, f32)
 //          uniform x the kept weight, by the segments' sums.
 // Rows of up to LIST tokens are one launch: the list is the row.
 //
-// A search (smp_select) finds where the running count or weight of a list in
-// descending order of a key reaches a goal: histograms of 1024 steps of what is
-// left of the keys' range, until a step is one key.  The key is the value for a
-// border, the index for ties and for the draw.  A bin of more than LIST values
-// (ties, a narrow spread) is searched in the row itself.
+// A list of up to FEW is ranked value against value.  Else a search (smp_select)
+// finds where the running count or weight, in descending order of a key, reaches
+// a goal: histograms of 1024 steps of what is left of the keys' range, until a
+// step has up to a wave's elements, which it ranks, or is one key.  The key is
+// the value for a border, the index for ties and for the draw.  A bin of more
+// than LIST values (ties, a narrow spread) is searched in the row itself.
 //
 // Bound by one read of the logits and, in hist, by about 30 instructions per
 // logit; with few rows by the latency of its launches.
@@ -168,8 +171,7 @@ struct SampleArgs {
   const int32_t *topk;
   const float *topp, *minp;
   uint64_t *tops;        // (rows, nseg): largest key and the complement of its index
-  uint64_t *sums;        // (rows, nseg, BINS + 1): weights per bin, then their sum
-  uint32_t *cnts;        // (rows, nseg, BINS)
+  uint64_t *hist;        // (rows, nseg, BINS + 1): weight and count per bin, then the weight in all
   int64_t ld;            // elements from row to row
   int32_t rows, vocab, seg, nseg;  // seg: tokens of a segment
   float c_temp;
@@ -182,14 +184,33 @@ struct SampleArgs {
 #define SMP_BINS 512
 #define SMP_LIST 8192
 #define SMP_STEPS 1024
+#define SMP_FEW 256
 typedef unsigned long long u64;
 
-// order of the values as whole numbers; -0 and 0 tie
-NK_DEVICE uint32_t smp_key(float x) {
-  const uint32_t u = __float_as_uint(x + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-NK_DEVICE float smp_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+// order of the values as whole numbers, of 16 bits for the 16-bit types; -0 and
+// 0 tie
+template <typename T> struct SmpKey {
+  static NK_DEVICE uint32_t of(float x) {
+    uint16_t h;
+    T v;
+    Elt<T>::store(&v, 0, x + 0.f);  // (exact: x is such a value)
+    __builtin_memcpy(&h, &v, 2);
+    return h & 0x8000u ? (uint16_t)~h : h | 0x8000u;
+  }
+  static NK_DEVICE float value(uint32_t k) {
+    const uint16_t h = k & 0x8000u ? k & 0x7fffu : (uint16_t)~k;
+    T v;
+    __builtin_memcpy(&v, &h, 2);
+    return Elt<T>::load(&v, 0);
+  }
+};
+template <> struct SmpKey<float> {
+  static NK_DEVICE uint32_t of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+  }
+  static NK_DEVICE float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+};
 
 struct SmpRow {
   float best, c;  // largest logit, log2(e) / T
@@ -200,36 +221,78 @@ struct SmpRow {
   // log2 of the weight; the largest logit has 0 also where it is infinite
   NK_DEVICE float depth(float x) const { return x == best ? 0.f : (x - best) * c; }
 };
-// weight in steps of 2^-40; 0 for NaN.  The hardware's 2^t is within an ulp, 1e-7
-// of the weight.
-NK_DEVICE u64 smp_weight(float t) {
-  if (!(t > -42.f)) return 0;
-  const float w = __builtin_amdgcn_exp2f(t) * 0x1p40f;
-  const uint32_t hi = (uint32_t)(w * 0x1p-16f);
-  const float rest = __builtin_fmaf((float)hi, -0x1p16f, w);  // exact: below 2^16
-  return ((u64)hi << 16) + (u64)(uint32_t)__builtin_rintf(rest);
-}
-// (a weight above 0 has t >= -41: bin 492 at most)
-NK_DEVICE int smp_bin(float t) { return min(SMP_BINS - 1, (int)(t * -12.f)); }
+// Weight in steps of 2^-36, as hi 2^18 + lo; 0 for NaN.  The hardware's 2^t is
+// within an ulp, 1e-7 of the weight.
+struct SmpWeight {
+  uint32_t hi, lo;
+  NK_DEVICE SmpWeight(float t) {
+    const float p = t > -38.f ? __builtin_amdgcn_exp2f(t) * 0x1p18f : 0.f;
+    hi = (uint32_t)p;
+    lo = min((uint32_t)__builtin_fmaf(p - (float)hi, 0x1p18f, 0.5f), 0x3ffffu);  // (the difference is exact)
+  }
+  NK_DEVICE u64 sum() const { return ((u64)hi << 18) + lo; }
+  NK_DEVICE u64 counted() const { return (u64)hi << 32 | lo << 14 | 1; }  // sum() 2^14 + 1
+};
+NK_DEVICE u64 smp_weight(float t) { return SmpWeight(t).sum(); }
+// (a weight above 0 has t >= -37: bin 481 at most)
+#define SMP_RATE 13.f  // bins per unit of t
+NK_DEVICE int smp_bin(float t) { return min(SMP_BINS - 1, (int)(t * -SMP_RATE)); }
 
-// Logits lo .. hi-1 of a row in pieces of 16 aligned bytes: f(index, value) by
-// THREADS threads.  The pieces at the ends are read element by element.
-template <typename T, int THREADS, typename F>
+// Logits lo .. hi-1 of a row in pieces of 16 aligned bytes, U of a thread in
+// flight at once: f(index, value) by THREADS threads.  The pieces at the ends
+// are read element by element.
+template <typename T, int THREADS, int U, typename F>
 NK_DEVICE void smp_each(const T *x, int lo, int hi, F f) {
   constexpr int E = 16 / sizeof(T);
   const int off = (int)(((uintptr_t)(x + lo) & 15) / sizeof(T));  // elements of the first piece before lo
-  for (int i = lo - off + threadIdx.x * E; i < hi; i += THREADS * E) {
-    if (i >= lo && i + E <= hi) {
-      const uint4 u = *reinterpret_cast<const uint4 *>(x + i);
-      T v[E];
-      __builtin_memcpy(v, &u, 16);
+  for (int i0 = lo - off + threadIdx.x * E; i0 < hi; i0 += U * THREADS * E) {
+    uint4 w[U];
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(i + e, Elt<T>::load(v, e));
-    } else {
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * THREADS * E;
+      if (i >= lo && i + E <= hi) w[u] = *reinterpret_cast<const uint4 *>(x + i);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * THREADS * E;
+      if (i >= lo && i + E <= hi) {
+        T v[E];
+        __builtin_memcpy(v, &w[u], 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f(i + e, Elt<T>::load(v, e));
+      } else {
 #pragma unroll 1
-      for (int e = max(0, lo - i); e < min(E, hi - i); ++e) f(i + e, Elt<T>::load(x, i + e));
+        for (int e = max(0, lo - i); e < min(E, hi - i); ++e) f(i + e, Elt<T>::load(x, i + e));
+      }
     }
   }
+}
+
+// running sum over the lanes of a wave, this one's included: row shifts of 1, 2,
+// 4, 8 lanes, then the rows' ends broadcast
+template <int CTRL, int ROWS>
+NK_DEVICE u64 smp_dpp(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+  return (u64)hi << 32 | lo;
+}
+NK_DEVICE u64 smp_running(u64 v) {
+  v += smp_dpp<0x111, 0xF>(v);
+  v += smp_dpp<0x112, 0xF>(v);
+  v += smp_dpp<0x114, 0xF>(v);
+  v += smp_dpp<0x118, 0xF>(v);
+  v += smp_dpp<0x142, 0xA>(v);
+  v += smp_dpp<0x143, 0xC>(v);
+  return v;
+}
+NK_DEVICE uint32_t smp_running(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+  return v;
 }
 
 template <int WAVES>
@@ -245,10 +308,9 @@ NK_DEVICE u64 smp_max(u64 v, u64 *red) {
 }
 template <int WAVES>
 NK_DEVICE u64 smp_sum(u64 v, u64 *red) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += (u64)__shfl_xor(v, o, 64);
+  v = smp_running(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0;
 #pragma unroll
@@ -259,10 +321,12 @@ NK_DEVICE u64 smp_sum(u64 v, u64 *red) {
 // are NaN or -inf
 template <typename T, int THREADS>
 NK_DEVICE u64 smp_top(const T *x, int lo, int hi, u64 *red) {
-  u64 top = 0;
-  smp_each<T, THREADS>(x, lo, hi, [&](int i, float v) {
-    if (v > -INFINITY) top = max(top, (u64)smp_key(v) << 32 | (uint32_t)~i);
+  float best = -INFINITY;
+  int at = -1;
+  smp_each<T, THREADS, 4>(x, lo, hi, [&](int i, float v) {  // (a thread's indices rise)
+    if (v > best) best = v, at = i;
   });
+  const u64 top = at < 0 ? 0 : (u64)SmpKey<T>::of(best) << 32 | (uint32_t)~at;
   return smp_max<THREADS / 64>(top, red);
 }
 
@@ -281,39 +345,40 @@ NK_DEVICE u64 smp_row_top(const SampleArgs &a, int r, u64 *red) {
 }
 // its settings; false where there is nothing to weigh: no logit to draw, or no
 // temperature
+template <typename T>
 NK_DEVICE bool smp_settings(const SampleArgs &a, int r, u64 top, SmpRow &row) {
   const float temp = a.temp ? a.temp[r] : a.c_temp;
-  row.set(smp_value((uint32_t)(top >> 32)), temp);
+  row.set(SmpKey<T>::value((uint32_t)(top >> 32)), temp);
   return top && temp > 0.f;
 }
 
 template <typename T>
 __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
-  __shared__ u64 sum[SMP_BINS];
-  __shared__ uint32_t cnt[SMP_BINS];
+  __shared__ u64 bins[SMP_BINS][4];  // (four of each: lanes of one wave meet less often)
   __shared__ u64 red[SMP_SEG_BLOCK / 64];
   const int r = blockIdx.x / a.nseg, s = blockIdx.x % a.nseg, tid = threadIdx.x;
-  for (int i = tid; i < SMP_BINS; i += SMP_SEG_BLOCK) sum[i] = 0, cnt[i] = 0;
+  for (int i = tid; i < SMP_BINS * 4; i += SMP_SEG_BLOCK) bins[i >> 2][i & 3] = 0;
   SmpRow row;
-  if (!smp_settings(a, r, smp_row_top<SMP_SEG_BLOCK>(a, r, red), row)) return;
+  if (!smp_settings<T>(a, r, smp_row_top<SMP_SEG_BLOCK>(a, r, red), row)) return;
   u64 all = 0;
-  const bool bins = a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f;
-  smp_each<T, SMP_SEG_BLOCK>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), [&](int, float v) {
+  const bool cuts = a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f;
+  smp_each<T, SMP_SEG_BLOCK, 4>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), [&](int, float v) {
     const float t = row.depth(v);
-    const u64 w = smp_weight(t);
-    all += w;
-    if (bins && w) {
-      const int b = smp_bin(t);
-      atomicAdd(&cnt[b], 1u);
-      atomicAdd(&sum[b], w);
-    }
+    const SmpWeight w(t);
+    if (!cuts) all += w.sum();
+    else if (w.hi | w.lo) atomicAdd(&bins[smp_bin(t)][tid & 3], w.counted());
   });
-  all = smp_sum<SMP_SEG_BLOCK / 64>(all, red);  // (and the histogram is whole)
-  uint64_t *so = a.sums + (int64_t)blockIdx.x * (SMP_BINS + 1);
-  uint32_t *co = a.cnts + (int64_t)blockIdx.x * SMP_BINS;
-  if (bins)
-    for (int i = tid; i < SMP_BINS; i += SMP_SEG_BLOCK) so[i] = sum[i], co[i] = cnt[i];
-  if (tid == 0) so[SMP_BINS] = all;
+  uint64_t *ho = a.hist + (int64_t)blockIdx.x * (SMP_BINS + 1);
+  __syncthreads();
+  if (cuts) {
+    for (int i = tid; i < SMP_BINS; i += SMP_SEG_BLOCK) {
+      const u64 h = bins[i][0] + bins[i][1] + bins[i][2] + bins[i][3];
+      all += h >> 14;
+      ho[i] = h;
+    }
+  }
+  all = smp_sum<SMP_SEG_BLOCK / 64>(all, red);
+  if (tid == 0) ho[SMP_BINS] = all;
 }
 
 struct SmpShared {
@@ -324,7 +389,11 @@ struct SmpShared {
   uint32_t key[SMP_LIST], idx[SMP_LIST];
   u64 red[SMP_BLOCK / 64], sw[SMP_BLOCK / 64];
   uint32_t sc[SMP_BLOCK / 64];
-  uint32_t n, kmin, kmax;
+  u64 cw[64];              // a search's last elements
+  uint32_t ck[64];
+  uint32_t n, few;
+  uint32_t rkey, rties, rof;
+  u64 rupto;
   // where a running sum reached its goal: step, and count and weight before and with it
   uint32_t bin, cb, ca;
   u64 wb, wa;
@@ -335,14 +404,8 @@ struct SmpShared {
 template <bool COUNT>
 NK_DEVICE void smp_search(SmpShared &s, uint32_t c, u64 w, uint32_t cb, u64 wb, uint32_t need, u64 goal) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  uint32_t ci = c;
-  u64 wi = w;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t cu = __shfl_up(ci, o, 64);
-    const u64 wu = __shfl_up(wi, o, 64);
-    if (lane >= o) ci += cu, wi += wu;
-  }
+  uint32_t ci = smp_running(c);
+  u64 wi = smp_running(w);
   __syncthreads();
   if (lane == 63) s.sc[wid] = ci, s.sw[wid] = wi;
   __syncthreads();
@@ -355,46 +418,42 @@ NK_DEVICE void smp_search(SmpShared &s, uint32_t c, u64 w, uint32_t cb, u64 wb, 
   __syncthreads();
 }
 
-// where a search ended: the key, how many of its elements are in, and the weight
-// up to and with them
+// where a search ended: the key, how many of its elements are in, how many there
+// are, and the weight up to and with those in
 struct SmpBorder {
-  uint32_t key, ties;
+  uint32_t key, ties, of;
   u64 upto;
 };
-// Of elements 0 .. n-1, f(i, key, weight) says which take part.  Those of one
-// key weigh the same.
-template <bool COUNT, typename F>
-NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, F f, uint32_t cb, u64 wb, uint32_t need, u64 goal) {
-  const int tid = threadIdx.x;
-  __syncthreads();
-  if (tid == 0) s.kmin = 0xffffffffu, s.kmax = 0;
-  __syncthreads();
-  uint32_t mn = 0xffffffffu, mx = 0, k;
-  u64 w;
-  for (int i = tid; i < n; i += SMP_BLOCK)
-    if (f(i, k, w)) mn = min(mn, k), mx = max(mx, k);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) mn = min(mn, (uint32_t)__shfl_xor(mn, o, 64)), mx = max(mx, (uint32_t)__shfl_xor(mx, o, 64));
-  if ((tid & 63) == 0) atomicMin(&s.kmin, mn), atomicMax(&s.kmax, mx);
-  __syncthreads();
-  uint32_t klo = s.kmin, khi = s.kmax;
+// Of elements 0 .. n-1, key(i, k) says which take part, if weight(i) is not 0;
+// their keys are in klo .. khi.  Those of one key weigh the same.
+template <bool COUNT, typename K, typename W>
+NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, K key, W weight, uint32_t klo, uint32_t khi, uint32_t cb, u64 wb,
+                               uint32_t need, u64 goal) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint32_t k;
   SmpBorder b;
   while (true) {
-    const uint32_t range = max(khi, klo) - klo;
+    const uint32_t range = khi - klo;
     const int shift = range < SMP_STEPS ? 0 : 22 - __builtin_clz(range);
+    __syncthreads();
     s.cnt[tid] = 0, s.sum[tid] = 0;
+    if (tid == 0) s.few = 0;
     __syncthreads();
     for (int i = tid; i < n; i += SMP_BLOCK)
-      if (f(i, k, w) && k >= klo && k <= khi) {
-        atomicAdd(&s.cnt[(khi - k) >> shift], 1u);
-        atomicAdd(&s.sum[(khi - k) >> shift], w);
+      if (key(i, k) && k >= klo && k <= khi) {
+        const u64 w = weight(i);
+        if (w) {
+          atomicAdd(&s.cnt[(khi - k) >> shift], 1u);
+          atomicAdd(&s.sum[(khi - k) >> shift], w);
+        }
       }
     __syncthreads();
     smp_search<COUNT>(s, s.cnt[tid], s.sum[tid], cb, wb, need, goal);
-    const uint32_t at = s.bin;
+    const uint32_t at = s.bin, left = s.ca - s.cb;
     cb = s.cb, wb = s.wb;
     if (shift == 0) {
-      const u64 each = (s.wa - wb) / max(s.ca - cb, 1u);
+      b.of = max(left, 1u);
+      const u64 each = (s.wa - wb) / b.of;
       b.key = khi - at;
       b.ties = COUNT ? need - cb : (uint32_t)((goal - wb + each - 1) / max(each, (u64)1));
       b.upto = wb + b.ties * each;
@@ -403,21 +462,99 @@ NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, F f, uint32_t cb, u64 wb, ui
     const uint32_t top = khi - (at << shift);
     klo = top - klo < (1u << shift) ? klo : top - (1u << shift) + 1;
     khi = top;
+    if (left > 64) continue;
+    // the rest by one wave
+    for (int i = tid; i < n; i += SMP_BLOCK)
+      if (key(i, k) && k >= klo && k <= khi) {
+        const u64 w = weight(i);
+        if (w) {
+          const uint32_t to = atomicAdd(&s.few, 1u);
+          if (to < 64) s.ck[to] = k, s.cw[to] = w;
+        }
+      }
+    __syncthreads();
+    if (tid < 64) {
+      const bool in = lane < left;
+      const uint32_t mk = in ? s.ck[lane] : 0;
+      const u64 mw = in ? s.cw[lane] : 0;
+      uint32_t c = cb, of = 0;
+      u64 w = wb;
+      for (int j = 0; j < left; ++j) {
+        const uint32_t kj = __builtin_amdgcn_readlane(mk, j);
+        if (kj > mk) ++c, w += s.cw[j];
+        of += kj == mk;
+      }
+      if (in && (COUNT ? c < need && c + of >= need : w < goal && w + of * mw >= goal)) {  // (its ties agree)
+        s.rkey = mk, s.rof = of;
+        s.rties = COUNT ? need - c : (uint32_t)((goal - w + mw - 1) / mw);
+        s.rupto = w + s.rties * mw;
+      }
+    }
+    __syncthreads();
+    b.key = s.rkey, b.ties = s.rties, b.of = s.rof, b.upto = s.rupto;
+    return b;
   }
 }
 
-// the elements of a stretch for which f holds, into the list
+// The elements low <= v <= top of a stretch for which f holds, into the list
+// (s.n of them, those past LIST left out).  The two comparisons are all that most
+// elements cost: one CU reads the row.  A wave takes places for a few pieces of
+// all its threads at once.
 template <typename T, typename F>
-NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, F f) {
+NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, float top, F f) {
+  constexpr int E = 16 / sizeof(T), U = 4;
+  const int lane = threadIdx.x & 63;
+  const int off = (int)(((uintptr_t)(x + lo) & 15) / sizeof(T));
   __syncthreads();
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
-  smp_each<T, SMP_BLOCK>(x, lo, hi, [&](int i, float v) {
-    if (f(i, v)) {
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < SMP_LIST) s.key[at] = smp_key(v), s.idx[at] = i;
+  // (every lane of a wave takes part in every round)
+  for (int w0 = lo - off + (threadIdx.x - lane) * E; w0 < hi; w0 += U * SMP_BLOCK * E) {
+    const int i0 = w0 + lane * E;
+    uint4 w[U];
+    uint32_t in = 0;  // a bit for each of U E elements
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * SMP_BLOCK * E;
+      if (i >= lo && i + E <= hi) w[u] = *reinterpret_cast<const uint4 *>(x + i);
     }
-  });
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * SMP_BLOCK * E;
+      if (i >= lo && i + E <= hi) {
+        T v[E];
+        __builtin_memcpy(v, &w[u], 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float y = Elt<T>::load(v, e);
+          in |= (y >= low && y <= top ? 1u : 0u) << (u * E + e);
+        }
+      } else {  // the ends, element by element
+#pragma unroll 1
+        for (int e = max(0, lo - i); e < min(E, hi - i); ++e) {
+          const float y = Elt<T>::load(x, i + e);
+          in |= (y >= low && y <= top ? 1u : 0u) << (u * E + e);
+        }
+      }
+    }
+    if (!__any(in != 0)) continue;
+    auto place = [&](uint32_t bits) {
+      const int bit = __builtin_ctz(bits);
+      return i0 + bit / E * SMP_BLOCK * E + bit % E;
+    };
+    for (uint32_t m = in; m; m &= m - 1) {  // (few: read again)
+      const int i = place(m);
+      if (!f(i, Elt<T>::load(x, i))) in &= ~(m & -m);
+    }
+    const uint32_t c = __popc(in), run = smp_running(c);
+    uint32_t at = 0;
+    if (lane == 63) at = atomicAdd(&s.n, run);
+    at = __builtin_amdgcn_readlane(at, 63) + run - c;
+    for (; in; in &= in - 1, ++at) {
+      const int i = place(in);
+      if (at < SMP_LIST) s.key[at] = SmpKey<T>::of(Elt<T>::load(x, i)), s.idx[at] = i;
+    }
+  }
   __syncthreads();
   return s.n;
 }
@@ -433,7 +570,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   const T *x = (const T *)a.x + r * a.ld;
   const u64 top = SMALL ? smp_top<T, SMP_BLOCK>(x, 0, a.vocab, s.red) : smp_row_top<SMP_BLOCK>(a, r, s.red);
   SmpRow row;
-  if (!smp_settings(a, r, top, row)) {
+  if (!smp_settings<T>(a, r, top, row)) {
     if (tid == 0) a.out[r] = top ? (int32_t)~(uint32_t)top : -1;
     return;
   }
@@ -442,54 +579,60 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   const bool by_k = topk > 0 && topk < a.vocab, by_p = topp < 1.f, by_m = minp > 0.f;
   const float tmin = by_m ? log2f(fminf(minp, 1.f)) : -INFINITY;  // the least depth that min_p keeps
 
-  // a listed or stored element's weight
-  auto listed = [&](int i, uint32_t &k, u64 &w) {
-    k = s.key[i];
-    w = smp_weight(row.depth(smp_value(k)));
-    return true;
+  const uint64_t *hist = a.hist + (int64_t)r * a.nseg * (SMP_BINS + 1);
+  // values that the values of a bin lie below and above, by a margin of a
+  // fiftieth of it and a step of the type
+  const float step = 1.f / (SMP_RATE * row.c);
+  auto over = [&](int bin) -> float {
+    const float v = row.best - (bin - 0.02f) * step;
+    return step > 0.f && v < row.best ? SmpKey<float>::value(SmpKey<float>::of(v) + 1) : row.best;
   };
-  auto stored = [&](int i, uint32_t &k, u64 &w) {
-    const float v = Elt<T>::load(x, i);
-    k = smp_key(v);
-    w = smp_weight(row.depth(v));
-    return w != 0;
+  auto under = [&](int bin) -> float {
+    const float v = row.best - (bin + 1.02f) * step;
+    return step > 0.f && v > -3e38f ? SmpKey<float>::value(SmpKey<float>::of(v) - 1) : -INFINITY;
   };
-  const uint64_t *sums = a.sums + (int64_t)r * a.nseg * (SMP_BINS + 1);
-  const uint32_t *cnts = a.cnts + (int64_t)r * a.nseg * SMP_BINS;
-  bool whole = SMALL;      // the list holds all that is kept
-  u64 total = 0;           // weight of the row
+  const bool cuts = by_k || by_p || by_m;
+  bool whole = SMALL;  // the list holds all that may be kept
+  u64 total = 0;       // weight of the row
   int n = 0;
-  uint32_t cbin = 0;       // the border's bin, count and weight before it (not whole)
-  int last = SMP_BINS - 1; // bins up to here can be kept
   if (SMALL) {
-    n = smp_gather(s, x, 0, a.vocab, [&](int, float v) { return smp_weight(row.depth(v)) != 0; });
-    if (by_p && !(by_k && n >= topk)) {
+    n = smp_gather(s, x, 0, a.vocab, -INFINITY, INFINITY, [&](int, float v) { return smp_weight(row.depth(v)) != 0; });
+    if (cuts) {
+      if (tid < SMP_BINS) s.hcnt[tid] = 0, s.hsum[tid] = 0;
+      __syncthreads();
       for (int i = tid; i < n; i += SMP_BLOCK) {
-        uint32_t k;
-        u64 w;
-        listed(i, k, w);
+        const float t = row.depth(SmpKey<T>::value(s.key[i]));
+        const u64 w = smp_weight(t);
         total += w;
+        atomicAdd(&s.hcnt[smp_bin(t)], 1u);
+        atomicAdd(&s.hsum[smp_bin(t)], w);
       }
-      total = smp_sum<SMP_BLOCK / 64>(total, s.red);
+      total = smp_sum<SMP_BLOCK / 64>(total, s.red);  // (and the histogram is whole)
     }
-  } else if (by_k || by_p || by_m) {
+  } else if (cuts) {
     uint32_t c = 0;
     u64 w = 0;
     const int bin = tid % SMP_BINS;
-    for (int i = tid / SMP_BINS; i < a.nseg; i += SMP_BLOCK / SMP_BINS) {
-      c += cnts[(int64_t)i * SMP_BINS + bin];
-      w += sums[(int64_t)i * (SMP_BINS + 1) + bin];
+    for (int i0 = tid / SMP_BINS; i0 < a.nseg; i0 += 16) {  // (eight segments' loads at once)
+      u64 h[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        h[j] = hist[(int64_t)min(i0 + j * (SMP_BLOCK / SMP_BINS), a.nseg - 1) * (SMP_BINS + 1) + bin];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j * (SMP_BLOCK / SMP_BINS) < a.nseg) c += (uint32_t)h[j] & 0x3fff, w += h[j] >> 14;
     }
     if (tid < SMP_BINS) s.hcnt[bin] = c, s.hsum[bin] = w;
     __syncthreads();
     if (tid >= SMP_BINS) s.hcnt[bin] += c, s.hsum[bin] += w;
     total = smp_sum<SMP_BLOCK / 64>(w, s.red);  // (and the histogram is whole)
   }
+  // the bin where the row's running count or weight gets there (s.bin; BINS: in none)
   auto bin_of_row = [&](bool count, uint32_t need, u64 goal) {
     const uint32_t c = tid < SMP_BINS ? s.hcnt[tid] : 0;
     const u64 w = tid < SMP_BINS ? s.hsum[tid] : 0;
     __syncthreads();
-    if (tid == 0) s.bin = SMP_BINS, s.cb = 0, s.ca = 0, s.wb = 0, s.wa = 0;
+    if (tid == 0) s.bin = SMP_BINS;
     if (count) smp_search<true>(s, c, w, 0, 0, need, goal);
     else smp_search<false>(s, c, w, 0, 0, need, goal);
   };
@@ -497,10 +640,9 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     return min(max((u64)ceil((double)fmaxf(topp, 0.f) * (double)of), (u64)1), of);
   };
   bool k_cuts = by_k, p_cuts = by_p;
-  if (SMALL) {
-    k_cuts = by_k && n >= topk;
-  } else if (by_k || by_p || by_m) {
-    // the bin that holds the first border; a top_k past the row's weights cuts nothing
+  if (cuts) {
+    int last = SMP_BINS - 1;  // bins up to here may be kept
+    // the first border's bin; a top_k past the row's weights cuts nothing
     if (by_k) {
       bin_of_row(true, topk, 0);
       k_cuts = s.bin < SMP_BINS;
@@ -512,70 +654,14 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
       k_cuts = p_cuts = false;
     }
     // everything down to there, where the list can hold it
-    const uint32_t upto = (uint32_t)smp_sum<SMP_BLOCK / 64>(tid <= last ? s.hcnt[tid] : 0, s.red);
-    if (upto <= SMP_LIST) {
-      const float least = -((float)last + 1.01f) / 12.f;
-      n = smp_gather(s, x, 0, a.vocab, [&](int, float v) {
+    if (!SMALL && smp_sum<SMP_BLOCK / 64>(tid <= last ? s.hcnt[tid % SMP_BINS] : 0, s.red) <= SMP_LIST) {
+      n = smp_gather(s, x, 0, a.vocab, under(last), row.best, [&](int, float v) {
         const float t = row.depth(v);
-        return t > least && smp_bin(t) <= last && smp_weight(t) != 0;
+        return smp_bin(t) <= last && smp_weight(t) != 0;
       });
       whole = true;
     }
   }
-
-  // the border: the last (value, index) kept
-  uint32_t bkey = 0, bidx = 0xffffffffu;
-  auto tie_break = [&](const SmpBorder &b, int len, auto each, auto index) {
-    bkey = b.key;
-    // the highest index of its ties that stays: by count, lowest first
-    bidx = ~smp_select<true>(s, len, [&](int i, uint32_t &k, u64 &w) {
-      const bool in = each(i, k, w) && k == b.key;
-      k = ~index(i);
-      return in;
-    }, 0, 0, b.ties, 0).key;
-  };
-  int held = -1;  // the bin that the list holds
-  auto in_list = [&](int i) { return s.idx[i]; };
-  auto in_row = [&](int i) { return (uint32_t)i; };
-  if (whole) {
-    if (k_cuts || p_cuts) {
-      SmpBorder b;
-      if (k_cuts) b = smp_select<true>(s, n, listed, 0, 0, topk, 0);
-      if (p_cuts) b = smp_select<false>(s, n, listed, 0, 0, 0, share(k_cuts ? b.upto : total));
-      tie_break(b, n, listed, in_list);
-    }
-  } else if (k_cuts || p_cuts) {
-    SmpBorder b;
-    // the values of one bin, from the list or, too many, from the row
-    bool fits = false;
-    auto find = [&](auto count, uint32_t need, u64 goal) {
-      const int bin = s.bin;
-      const uint32_t cb = s.cb;
-      const u64 wb = s.wb;
-      cbin = bin;
-      auto of_bin = [&](int i, uint32_t &k, u64 &w) { return stored(i, k, w) && smp_bin(row.depth(smp_value(k))) == bin; };
-      if (bin != held) {
-        fits = s.ca - cb <= SMP_LIST;
-        if (fits) n = smp_gather(s, x, 0, a.vocab, [&](int, float v) {
-          const float t = row.depth(v);
-          return smp_bin(t) == bin && smp_weight(t) != 0;
-        });
-        held = fits ? bin : -1;
-      }
-      constexpr bool COUNT = decltype(count)::value;
-      b = fits ? smp_select<COUNT>(s, n, listed, cb, wb, need, goal) : smp_select<COUNT>(s, a.vocab, of_bin, cb, wb, need, goal);
-    };
-    if (k_cuts) find(SmpFlag<true>{}, topk, 0);
-    if (p_cuts) {
-      const u64 goal = share(k_cuts ? b.upto : total);
-      bin_of_row(false, 0, goal);
-      find(SmpFlag<false>{}, 0, goal);
-    }
-    if (fits) tie_break(b, n, listed, in_list);
-    else tie_break(b, a.vocab, stored, in_row);
-  }
-  auto kept = [&](uint32_t k, uint32_t i, float t) { return (k > bkey || (k == bkey && i <= bidx)) && t >= tmin; };
-
   // the draw: the first kept index up to and with which the weights exceed
   // uniform x their sum, that is, reach the whole number behind it
   const float uni = a.u[r];
@@ -583,54 +669,153 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     const u64 g = uni > 0.f ? (u64)(fmin((double)uni, 1.) * (double)all) : 0;
     return !(uni < 1.f) || g >= all ? all : g + 1;  // (NaN too: the last kept)
   };
-  auto draw = [&](u64 goal, u64 before) {
-    const uint32_t at = ~smp_select<false>(s, n, [&](int i, uint32_t &k, u64 &w) {
-      listed(i, k, w);
-      const bool in = kept(k, s.idx[i], row.depth(smp_value(k)));
+
+  // A few values: ranked against each other, everything else is in their order.
+  if (whole && n <= SMP_FEW) {
+    const bool in = tid < n;
+    const u64 mine = in ? (u64)s.key[tid] << 32 | (uint32_t)~s.idx[tid] : 0;
+    if (in) s.sum[tid] = mine;
+    __syncthreads();
+    uint32_t rank = 0;
+    if (in)
+      for (int j = 0; j < n; ++j) rank += s.sum[j] > mine;
+    __syncthreads();
+    if (in) s.sum[rank] = mine;
+    __syncthreads();
+    const u64 it = in ? s.sum[tid] : 0;
+    const float t = in ? row.depth(SmpKey<T>::value((uint32_t)(it >> 32))) : 0.f;
+    const u64 w = in ? smp_weight(t) : 0;
+    u64 run = smp_running(w);
+    if ((tid & 63) == 63) s.sw[tid >> 6] = run;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SMP_FEW / 64; ++i)
+      if (i < tid >> 6) run += s.sw[i];
+    uint32_t keep = k_cuts ? min(topk, n) : n;
+    if (in) s.hsum[tid] = run;
+    __syncthreads();
+    if (p_cuts) {
+      const u64 goal = share(k_cuts ? s.hsum[keep - 1] : total);
+      keep = min(keep, 1 + (uint32_t)smp_sum<SMP_BLOCK / 64>(in && run < goal, s.red));
+    }
+    if (by_m) keep = min(keep, (uint32_t)smp_sum<SMP_BLOCK / 64>(in && t >= tmin, s.red));
+    const u64 goal = goal_of(s.hsum[keep - 1]);
+    __syncthreads();
+    if (in) s.hsum[tid] = w;
+    __syncthreads();
+    if (tid < keep) {
+      u64 upto = 0;  // the weight of indices up to this one's (complements order them backwards)
+      for (int j = 0; j < keep; ++j) upto += (uint32_t)s.sum[j] >= (uint32_t)it ? s.hsum[j] : 0;
+      if (upto >= goal && upto - w < goal) a.out[r] = ~(uint32_t)it;
+    }
+    return;
+  }
+
+  // the border: the last (value, index) kept
+  uint32_t bkey = 0, bidx = 0xffffffffu;
+  int edge = SMP_BINS;  // its bin
+  int held = -1;        // the bin whose values the list holds
+  if (k_cuts || p_cuts) {
+    SmpBorder b;
+    // the values of the bin found last: from the list, or too many for it, from the row
+    bool listing = whole;
+    auto find = [&](auto count, uint32_t need, u64 goal) {
+      constexpr bool COUNT = decltype(count)::value;
+      const uint32_t cb = s.cb, many = s.ca - s.cb;
+      const u64 wb = s.wb;
+      edge = s.bin;
+      if (!whole && edge != held) {
+        listing = many <= SMP_LIST;
+        held = listing ? edge : -1;
+        if (listing) n = smp_gather(s, x, 0, a.vocab, under(edge), over(edge), [&](int, float v) {
+          const float t = row.depth(v);
+          return smp_bin(t) == edge && smp_weight(t) != 0;
+        });
+      }
+      const uint32_t klo = max(SmpKey<T>::of(under(edge)), 1u) - 1, khi = SmpKey<T>::of(over(edge));
+      if (listing) {
+        b = smp_select<COUNT>(s, n, [&](int i, uint32_t &k) {
+          k = s.key[i];
+          return smp_bin(row.depth(SmpKey<T>::value(k))) == edge;
+        }, [&](int i) { return smp_weight(row.depth(SmpKey<T>::value(s.key[i]))); }, klo, khi, cb, wb, need, goal);
+      } else {
+        b = smp_select<COUNT>(s, a.vocab, [&](int i, uint32_t &k) {
+          const float v = Elt<T>::load(x, i);
+          k = SmpKey<T>::of(v);
+          return smp_bin(row.depth(v)) == edge;
+        }, [&](int i) { return smp_weight(row.depth(Elt<T>::load(x, i))); }, klo, khi, cb, wb, need, goal);
+      }
+    };
+    if (k_cuts) find(SmpFlag<true>{}, topk, 0);
+    if (p_cuts) {
+      const u64 goal = share(k_cuts ? b.upto : total);
+      bin_of_row(false, 0, goal);
+      find(SmpFlag<false>{}, 0, goal);
+    }
+    bkey = b.key;
+    // the highest index of its ties that stays: by count, lowest first
+    if (b.ties < b.of) {
+      const uint32_t klo = ~(uint32_t)(a.vocab - 1);
+      auto one = [](int) -> u64 { return 1; };
+      if (listing) {
+        bidx = ~smp_select<true>(s, n, [&](int i, uint32_t &k) {
+          k = ~s.idx[i];
+          return s.key[i] == bkey;
+        }, one, klo, ~0u, 0, 0, b.ties, 0).key;
+      } else {
+        bidx = ~smp_select<true>(s, a.vocab, [&](int i, uint32_t &k) {
+          k = ~i;
+          const float v = Elt<T>::load(x, i);
+          return v == v && SmpKey<T>::of(v) == bkey;
+        }, one, klo, ~0u, 0, 0, b.ties, 0).key;
+      }
+    }
+  }
+  auto kept = [&](uint32_t k, uint32_t i, float t) { return (k > bkey || (k == bkey && i <= bidx)) && t >= tmin; };
+
+  // a listed element's weight, 0 where it is not kept
+  auto weigh = [&](int i) -> u64 {
+    const float t = row.depth(SmpKey<T>::value(s.key[i]));
+    return kept(s.key[i], s.idx[i], t) ? smp_weight(t) : 0;
+  };
+  auto draw = [&](u64 goal, u64 before, int lo, int hi) {
+    const uint32_t at = ~smp_select<false>(s, n, [&](int i, uint32_t &k) {
       k = ~s.idx[i];
-      return in;
-    }, 0, before, 0, goal).key;
+      return true;
+    }, weigh, ~(uint32_t)(hi - 1), ~(uint32_t)lo, 0, before, 0, goal).key;
     if (tid == 0) a.out[r] = at;
   };
   if (whole) {
     u64 all = 0;
-    for (int i = tid; i < n; i += SMP_BLOCK) {
-      uint32_t k;
-      u64 w;
-      listed(i, k, w);
-      if (kept(k, s.idx[i], row.depth(smp_value(k)))) all += w;
-    }
-    draw(goal_of(smp_sum<SMP_BLOCK / 64>(all, s.red)), 0);
+    for (int i = tid; i < n; i += SMP_BLOCK) all += weigh(i);
+    draw(goal_of(smp_sum<SMP_BLOCK / 64>(all, s.red)), 0, 0, a.vocab);
     return;
   }
   // by segments: bins before the border's are kept whole; of the one it is in,
   // what is kept is added value by value
-  const int edge = min(k_cuts || p_cuts ? (int)cbin : SMP_BINS, by_m ? smp_bin(tmin) : SMP_BINS);
+  if (by_m) edge = min(edge, smp_bin(tmin));
   u64 *seg = s.sum;  // (up to STEPS segments)
   __syncthreads();
   seg[tid] = 0;
   __syncthreads();
   if (edge == SMP_BINS) {
-    for (int i = tid; i < a.nseg; i += SMP_BLOCK) seg[i] = sums[(int64_t)i * (SMP_BINS + 1) + SMP_BINS];
+    for (int i = tid; i < a.nseg; i += SMP_BLOCK) seg[i] = hist[(int64_t)i * (SMP_BINS + 1) + SMP_BINS];
   } else {
     for (int i = tid >> 6; i < a.nseg; i += SMP_BLOCK / 64) {  // a wave for each
       u64 w = 0;
-      for (int b = tid & 63; b < edge; b += 64) w += sums[(int64_t)i * (SMP_BINS + 1) + b];
+      for (int b = tid & 63; b < edge; b += 64) w += hist[(int64_t)i * (SMP_BINS + 1) + b] >> 14;
 #pragma unroll
       for (int o = 32; o; o >>= 1) w += (u64)__shfl_xor(w, o, 64);
       if ((tid & 63) == 0) atomicAdd(&seg[i], w);
     }
     if (held == edge) {
-      for (int i = tid; i < n; i += SMP_BLOCK) {
-        const float t = row.depth(smp_value(s.key[i]));
-        if (kept(s.key[i], s.idx[i], t)) atomicAdd(&seg[s.idx[i] / a.seg], smp_weight(t));
-      }
+      for (int i = tid; i < n; i += SMP_BLOCK) atomicAdd(&seg[s.idx[i] / a.seg], weigh(i));
     } else {
-      smp_each<T, SMP_BLOCK>(x, 0, a.vocab, [&](int i, float v) {
+      smp_each<T, SMP_BLOCK, 4>(x, 0, a.vocab, [&](int i, float v) {
         const float t = row.depth(v);
-        if (!(t > -42.f) || smp_bin(t) != edge) return;
+        if (!(t > -38.f) || smp_bin(t) != edge) return;
         const u64 w = smp_weight(t);
-        if (w && kept(smp_key(v), i, t)) atomicAdd(&seg[i / a.seg], w);
+        if (w && kept(SmpKey<T>::of(v), i, t)) atomicAdd(&seg[i / a.seg], w);
       });
     }
   }
@@ -640,11 +825,11 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   smp_search<false>(s, 0, mine, 0, 0, 0, goal);
   const int at = s.bin;
   const u64 before = s.wb;
-  n = smp_gather(s, x, at * a.seg, min(a.vocab, (at + 1) * a.seg), [&](int i, float v) {
+  n = smp_gather(s, x, at * a.seg, min(a.vocab, (at + 1) * a.seg), bkey ? SmpKey<T>::value(bkey) : -INFINITY, INFINITY, [&](int i, float v) {
     const float t = row.depth(v);
-    return smp_weight(t) != 0 && kept(smp_key(v), i, t);
+    return smp_weight(t) != 0 && kept(SmpKey<T>::of(v), i, t);
   });
-  draw(goal, before);
+  draw(goal, before, at * a.seg, min(a.vocab, (at + 1) * a.seg));
 }
 #define NK_SAMPLE(T, name)                                                                          \
   extern "C" __global__ __launch_bounds__(SMP_SEG_BLOCK) void nk_sample_top_##name(SampleArgs a) {  \

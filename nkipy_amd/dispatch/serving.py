@@ -45,7 +45,7 @@ class AttendArgs(ctypes.Structure):
 
 
 class SampleArgs(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp", "tops", "sums", "cnts")]
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp", "tops", "hist")]
                 + [("ld", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("rows", "vocab", "seg", "nseg")]
                 + [("c_temp", ctypes.c_float), ("c_topk", ctypes.c_int32), ("c_topp", ctypes.c_float),
                    ("c_minp", ctypes.c_float)])
@@ -158,7 +158,7 @@ def sample_segments(rows: int, vocab: int) -> Tuple[int, int]:
 def sample_workspace_bytes(rows: int, vocab: int) -> int:
     if vocab <= SMP_LIST:
         return 0
-    return rows * sample_segments(rows, vocab)[1] * (8 + 8 * (SMP_BINS + 1) + 4 * SMP_BINS)
+    return 8 * rows * sample_segments(rows, vocab)[1] * (SMP_BINS + 2)
 
 
 def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_p, ws=0) -> List[Launch]:
@@ -177,7 +177,7 @@ def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_
     n = rows * a.nseg
     if n >= 2**31:
         raise LaunchError("sample: too many rows for one launch")
-    _fields(a, tops=ws, sums=ws + 8 * n, cnts=ws + 8 * n * (SMP_BINS + 2))
+    _fields(a, tops=ws, hist=ws + 8 * n)
     return [Launch("serving", f"nk_sample_top_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_hist_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_pick_{tag}", (rows, 1, 1), (1024, 1, 1), a)]
