@@ -330,12 +330,22 @@ NK_DEVICE u64 smp_top(const T *x, int lo, int hi, u64 *red) {
   return smp_max<THREADS / 64>(top, red);
 }
 
+// Workgroup i runs on XCD i % 8: a row's segments go where the workgroup of its
+// last launch reads the row again, so that it finds it in that XCD's cache.
+// Grid: 8 nseg ceil(rows / 8).
+NK_DEVICE void smp_place(const SampleArgs &a, int &r, int &s) {
+  const int i = blockIdx.x >> 3;
+  r = (i / a.nseg << 3) + (blockIdx.x & 7);
+  s = i % a.nseg;
+}
 template <typename T>
 __device__ __forceinline__ void sample_top_body(const SampleArgs &a) {
   __shared__ u64 red[SMP_SEG_BLOCK / 64];
-  const int r = blockIdx.x / a.nseg, s = blockIdx.x % a.nseg;
+  int r, s;
+  smp_place(a, r, s);
+  if (r >= a.rows) return;
   const u64 top = smp_top<T, SMP_SEG_BLOCK>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), red);
-  if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
+  if (threadIdx.x == 0) a.tops[(int64_t)r * a.nseg + s] = top;
 }
 template <int THREADS>
 NK_DEVICE u64 smp_row_top(const SampleArgs &a, int r, u64 *red) {
@@ -356,7 +366,10 @@ template <typename T>
 __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
   __shared__ u64 bins[SMP_BINS][4];  // (four of each: lanes of one wave meet less often)
   __shared__ u64 red[SMP_SEG_BLOCK / 64];
-  const int r = blockIdx.x / a.nseg, s = blockIdx.x % a.nseg, tid = threadIdx.x;
+  const int tid = threadIdx.x;
+  int r, s;
+  smp_place(a, r, s);
+  if (r >= a.rows) return;
   for (int i = tid; i < SMP_BINS * 4; i += SMP_SEG_BLOCK) bins[i >> 2][i & 3] = 0;
   SmpRow row;
   if (!smp_settings<T>(a, r, smp_row_top<SMP_SEG_BLOCK>(a, r, red), row)) return;
@@ -368,7 +381,7 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
     if (!cuts) all += w.sum();
     else if (w.hi | w.lo) atomicAdd(&bins[smp_bin(t)][tid & 3], w.counted());
   });
-  uint64_t *ho = a.hist + (int64_t)blockIdx.x * (SMP_BINS + 1);
+  uint64_t *ho = a.hist + ((int64_t)r * a.nseg + s) * (SMP_BINS + 1);
   __syncthreads();
   if (cuts) {
     for (int i = tid; i < SMP_BINS; i += SMP_SEG_BLOCK) {
@@ -386,6 +399,7 @@ struct SmpShared {
   u64 sum[SMP_STEPS];      // a search's
   uint32_t hcnt[SMP_BINS];
   uint32_t cnt[SMP_STEPS];
+  u64 w[SMP_LIST];         // the list: weights, keys, indices
   uint32_t key[SMP_LIST], idx[SMP_LIST];
   u64 red[SMP_BLOCK / 64], sw[SMP_BLOCK / 64];
   uint32_t sc[SMP_BLOCK / 64];
@@ -430,6 +444,10 @@ template <bool COUNT, typename K, typename W>
 NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, K key, W weight, uint32_t klo, uint32_t khi, uint32_t cb, u64 wb,
                                uint32_t need, u64 goal) {
   const int tid = threadIdx.x, lane = tid & 63;
+  // a list stands nearly in the order of indices: neighbouring lanes take
+  // elements apart, or they would meet in one step
+  const int per = n <= SMP_LIST ? (n + SMP_BLOCK - 1) / SMP_BLOCK | 1 : 1, begin = tid * per;  // (odd: the lanes' banks)
+  const int step = n <= SMP_LIST ? 1 : SMP_BLOCK, end = n <= SMP_LIST ? min(n, begin + per) : n;
   uint32_t k;
   SmpBorder b;
   while (true) {
@@ -439,7 +457,7 @@ NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, K key, W weight, uint32_t kl
     s.cnt[tid] = 0, s.sum[tid] = 0;
     if (tid == 0) s.few = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += SMP_BLOCK)
+    for (int i = begin; i < end; i += step)
       if (key(i, k) && k >= klo && k <= khi) {
         const u64 w = weight(i);
         if (w) {
@@ -464,7 +482,7 @@ NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, K key, W weight, uint32_t kl
     khi = top;
     if (left > 64) continue;
     // the rest by one wave
-    for (int i = tid; i < n; i += SMP_BLOCK)
+    for (int i = begin; i < end; i += step)
       if (key(i, k) && k >= klo && k <= khi) {
         const u64 w = weight(i);
         if (w) {
@@ -496,28 +514,57 @@ NK_DEVICE SmpBorder smp_select(SmpShared &s, int n, K key, W weight, uint32_t kl
   }
 }
 
-// The elements low <= v <= top of a stretch for which f holds, into the list
-// (s.n of them, those past LIST left out).  The two comparisons are all that most
-// elements cost: one CU reads the row.  A wave takes places for a few pieces of
-// all its threads at once.
-template <typename T, typename F>
-NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, float top, F f) {
+// The least key of a float for which f holds, if it holds for `top` and for every
+// key above one it holds for; it should be above `out` and not above `in`.  Each
+// lane of a wave tries a key of its own.
+template <typename F>
+NK_DEVICE uint32_t smp_least(uint32_t out, uint32_t in, uint32_t top, F f) {
+  const int lane = threadIdx.x & 63;
+  const u64 guess = __ballot(f(lane ? in : out));
+  if (guess & 1 || out >= in) out = 0;
+  if (!(guess & 2) || in > top) in = top;
+  while (in - out > 1) {
+    const uint32_t step = max((in - out) / 64, 1u), k = out + (lane + 1) * step;
+    const u64 hit = __ballot(k < in && f(k));
+    const uint32_t at = hit ? __builtin_ctzll(hit) : min(64u, (in - out - 1) / step);  // (lanes below `in`)
+    if (hit) in = out + (at + 1) * step;
+    out += at * step;
+  }
+  return in;
+}
+// the largest float below that of a key
+NK_DEVICE float smp_below(uint32_t k) { return SmpKey<float>::value(k == 0x80000000u ? 0x7ffffffeu : k - 1); }
+
+// The elements low <= v <= top of a stretch, into the list (s.n of them, those
+// past LIST left out).  The two comparisons are all that an element costs: one CU
+// reads the row.  A wave takes places for a few pieces of all its threads at
+// once; keys and weights are filled in afterwards, all reads in flight.
+template <typename T>
+NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, float top, const SmpRow &row) {
   constexpr int E = 16 / sizeof(T), U = 4;
   const int lane = threadIdx.x & 63;
   const int off = (int)(((uintptr_t)(x + lo) & 15) / sizeof(T));
   __syncthreads();
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
-  // (every lane of a wave takes part in every round)
-  for (int w0 = lo - off + (threadIdx.x - lane) * E; w0 < hi; w0 += U * SMP_BLOCK * E) {
-    const int i0 = w0 + lane * E;
-    uint4 w[U];
-    uint32_t in = 0;  // a bit for each of U E elements
+  auto fetch = [&](uint4 (&w)[U], int i0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * SMP_BLOCK * E;
       if (i >= lo && i + E <= hi) w[u] = *reinterpret_cast<const uint4 *>(x + i);
     }
+  };
+  const int first = lo - off + (threadIdx.x - lane) * E;
+  uint4 next[U];
+  fetch(next, first + lane * E);
+  // (every lane of a wave takes part in every round)
+  for (int w0 = first; w0 < hi; w0 += U * SMP_BLOCK * E) {
+    const int i0 = w0 + lane * E;
+    uint4 w[U];
+    uint32_t in = 0;  // a bit for each of U E elements
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = next[u];
+    fetch(next, i0 + U * SMP_BLOCK * E);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * SMP_BLOCK * E;
@@ -538,25 +585,28 @@ NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, fl
       }
     }
     if (!__any(in != 0)) continue;
-    auto place = [&](uint32_t bits) {
-      const int bit = __builtin_ctz(bits);
-      return i0 + bit / E * SMP_BLOCK * E + bit % E;
-    };
-    for (uint32_t m = in; m; m &= m - 1) {  // (few: read again)
-      const int i = place(m);
-      if (!f(i, Elt<T>::load(x, i))) in &= ~(m & -m);
-    }
     const uint32_t c = __popc(in), run = smp_running(c);
     uint32_t at = 0;
     if (lane == 63) at = atomicAdd(&s.n, run);
     at = __builtin_amdgcn_readlane(at, 63) + run - c;
     for (; in; in &= in - 1, ++at) {
-      const int i = place(in);
-      if (at < SMP_LIST) s.key[at] = SmpKey<T>::of(Elt<T>::load(x, i)), s.idx[at] = i;
+      const int bit = __builtin_ctz(in);
+      if (at < SMP_LIST) s.idx[at] = i0 + bit / E * SMP_BLOCK * E + bit % E;
     }
   }
   __syncthreads();
-  return s.n;
+  const int n = s.n;
+#pragma unroll
+  for (int j = 0; j < SMP_LIST / SMP_BLOCK; ++j) {
+    const int i = j * SMP_BLOCK + threadIdx.x;
+    if (i < n) {
+      const float v = Elt<T>::load(x, s.idx[i]);
+      s.key[i] = SmpKey<T>::of(v);
+      s.w[i] = smp_weight(row.depth(v));
+    }
+  }
+  __syncthreads();
+  return n;
 }
 
 template <bool B> struct SmpFlag {
@@ -580,32 +630,35 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   const float tmin = by_m ? log2f(fminf(minp, 1.f)) : -INFINITY;  // the least depth that min_p keeps
 
   const uint64_t *hist = a.hist + (int64_t)r * a.nseg * (SMP_BINS + 1);
-  // values that the values of a bin lie below and above, by a margin of a
-  // fiftieth of it and a step of the type
-  const float step = 1.f / (SMP_RATE * row.c);
-  auto over = [&](int bin) -> float {
-    const float v = row.best - (bin - 0.02f) * step;
-    return step > 0.f && v < row.best ? SmpKey<float>::value(SmpKey<float>::of(v) + 1) : row.best;
+  // a value `at` bins below the largest, as a key: near there, and past every
+  // value of a bin with a fiftieth of a bin to spare and a key on either side
+  auto near = [&](float at) -> uint32_t {
+    const float v = row.best - at / (SMP_RATE * row.c);
+    return v > -3e38f ? SmpKey<float>::of(fminf(v, row.best)) : 0;
   };
-  auto under = [&](int bin) -> float {
-    const float v = row.best - (bin + 1.02f) * step;
-    return step > 0.f && v > -3e38f ? SmpKey<float>::value(SmpKey<float>::of(v) - 1) : -INFINITY;
+  // the least float of bins up to `bin` that weighs anything, as its key: as the
+  // arithmetic of the bins has it
+  auto least = [&](int bin) -> uint32_t {
+    return smp_least(near(bin + 1.02f), near(bin + 0.98f), SmpKey<float>::of(row.best), [&](uint32_t k) {
+      const float t = row.depth(SmpKey<float>::value(k));
+      const SmpWeight w(t);
+      return (w.hi | w.lo) && smp_bin(t) <= bin;
+    });
   };
   const bool cuts = by_k || by_p || by_m;
   bool whole = SMALL;  // the list holds all that may be kept
   u64 total = 0;       // weight of the row
   int n = 0;
   if (SMALL) {
-    n = smp_gather(s, x, 0, a.vocab, -INFINITY, INFINITY, [&](int, float v) { return smp_weight(row.depth(v)) != 0; });
+    n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(SMP_BINS - 1)), row.best, row);
     if (cuts) {
       if (tid < SMP_BINS) s.hcnt[tid] = 0, s.hsum[tid] = 0;
       __syncthreads();
       for (int i = tid; i < n; i += SMP_BLOCK) {
-        const float t = row.depth(SmpKey<T>::value(s.key[i]));
-        const u64 w = smp_weight(t);
-        total += w;
-        atomicAdd(&s.hcnt[smp_bin(t)], 1u);
-        atomicAdd(&s.hsum[smp_bin(t)], w);
+        const int bin = smp_bin(row.depth(SmpKey<T>::value(s.key[i])));
+        total += s.w[i];
+        atomicAdd(&s.hcnt[bin], 1u);
+        atomicAdd(&s.hsum[bin], s.w[i]);
       }
       total = smp_sum<SMP_BLOCK / 64>(total, s.red);  // (and the histogram is whole)
     }
@@ -655,10 +708,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     }
     // everything down to there, where the list can hold it
     if (!SMALL && smp_sum<SMP_BLOCK / 64>(tid <= last ? s.hcnt[tid % SMP_BINS] : 0, s.red) <= SMP_LIST) {
-      n = smp_gather(s, x, 0, a.vocab, under(last), row.best, [&](int, float v) {
-        const float t = row.depth(v);
-        return smp_bin(t) <= last && smp_weight(t) != 0;
-      });
+      n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(last)), row.best, row);
       whole = true;
     }
   }
@@ -727,17 +777,17 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
       if (!whole && edge != held) {
         listing = many <= SMP_LIST;
         held = listing ? edge : -1;
-        if (listing) n = smp_gather(s, x, 0, a.vocab, under(edge), over(edge), [&](int, float v) {
-          const float t = row.depth(v);
-          return smp_bin(t) == edge && smp_weight(t) != 0;
-        });
+        if (listing) n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(edge)),
+                                    edge ? smp_below(least(edge - 1)) : row.best, row);
       }
-      const uint32_t klo = max(SmpKey<T>::of(under(edge)), 1u) - 1, khi = SmpKey<T>::of(over(edge));
+      const uint32_t low = near(edge + 1.02f), top = near(edge - 0.02f);
+      const uint32_t klo = low ? max(SmpKey<T>::of(SmpKey<float>::value(low)), 1u) - 1 : 0;
+      const uint32_t khi = SmpKey<T>::of(top ? SmpKey<float>::value(top) : row.best) + 1;
       if (listing) {
         b = smp_select<COUNT>(s, n, [&](int i, uint32_t &k) {
           k = s.key[i];
           return smp_bin(row.depth(SmpKey<T>::value(k))) == edge;
-        }, [&](int i) { return smp_weight(row.depth(SmpKey<T>::value(s.key[i]))); }, klo, khi, cb, wb, need, goal);
+        }, [&](int i) { return s.w[i]; }, klo, khi, cb, wb, need, goal);
       } else {
         b = smp_select<COUNT>(s, a.vocab, [&](int i, uint32_t &k) {
           const float v = Elt<T>::load(x, i);
@@ -775,8 +825,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
 
   // a listed element's weight, 0 where it is not kept
   auto weigh = [&](int i) -> u64 {
-    const float t = row.depth(SmpKey<T>::value(s.key[i]));
-    return kept(s.key[i], s.idx[i], t) ? smp_weight(t) : 0;
+    return kept(s.key[i], s.idx[i], row.depth(SmpKey<T>::value(s.key[i]))) ? s.w[i] : 0;
   };
   auto draw = [&](u64 goal, u64 before, int lo, int hi) {
     const uint32_t at = ~smp_select<false>(s, n, [&](int i, uint32_t &k) {
@@ -825,10 +874,8 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   smp_search<false>(s, 0, mine, 0, 0, 0, goal);
   const int at = s.bin;
   const u64 before = s.wb;
-  n = smp_gather(s, x, at * a.seg, min(a.vocab, (at + 1) * a.seg), bkey ? SmpKey<T>::value(bkey) : -INFINITY, INFINITY, [&](int i, float v) {
-    const float t = row.depth(v);
-    return smp_weight(t) != 0 && kept(SmpKey<T>::of(v), i, t);
-  });
+  n = smp_gather(s, x, at * a.seg, min(a.vocab, (at + 1) * a.seg),
+                 bkey ? SmpKey<T>::value(bkey) : SmpKey<float>::value(least(SMP_BINS - 1)), row.best, row);
   draw(goal, before, at * a.seg, min(a.vocab, (at + 1) * a.seg));
 }
 #define NK_SAMPLE(T, name)                                                                          \

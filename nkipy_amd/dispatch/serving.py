@@ -174,10 +174,10 @@ def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_
     a.seg, a.nseg = sample_segments(rows, vocab)
     if not ws or ws % 8:
         raise LaunchError("sample: long rows need a workspace")
-    n = rows * a.nseg
+    n = -(-rows // 8) * 8 * a.nseg
     if n >= 2**31:
         raise LaunchError("sample: too many rows for one launch")
-    _fields(a, tops=ws, hist=ws + 8 * n)
+    _fields(a, tops=ws, hist=ws + 8 * rows * a.nseg)
     return [Launch("serving", f"nk_sample_top_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_hist_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_pick_{tag}", (rows, 1, 1), (1024, 1, 1), a)]
