@@ -561,10 +561,12 @@ NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, fl
   for (int w0 = first; w0 < hi; w0 += U * SMP_BLOCK * E) {
     const int i0 = w0 + lane * E;
     uint4 w[U];
-    uint32_t in = 0;  // a bit for each of U E elements
+    uint32_t in = 0;  // a bit for each of U E elements, the first the highest
 #pragma unroll
     for (int u = 0; u < U; ++u) w[u] = next[u];
     fetch(next, i0 + U * SMP_BLOCK * E);
+    // (the middle of the three is y itself within the bounds, and not for NaN)
+    auto inside = [&](float y) { return __builtin_amdgcn_fmed3f(y, low, top) == y; };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * SMP_BLOCK * E;
@@ -572,16 +574,11 @@ NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, fl
         T v[E];
         __builtin_memcpy(v, &w[u], 16);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float y = Elt<T>::load(v, e);
-          in |= (y >= low && y <= top ? 1u : 0u) << (u * E + e);
-        }
+        for (int e = 0; e < E; ++e) in += in + (inside(Elt<T>::load(v, e)) ? 1 : 0);
       } else {  // the ends, element by element
 #pragma unroll 1
-        for (int e = max(0, lo - i); e < min(E, hi - i); ++e) {
-          const float y = Elt<T>::load(x, i + e);
-          in |= (y >= low && y <= top ? 1u : 0u) << (u * E + e);
-        }
+        for (int e = 0; e < E; ++e)
+          in += in + (i + e >= lo && i + e < hi && inside(Elt<T>::load(x, max(lo, min(i + e, hi - 1)))) ? 1 : 0);
       }
     }
     if (!__any(in != 0)) continue;
@@ -590,7 +587,7 @@ NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, fl
     if (lane == 63) at = atomicAdd(&s.n, run);
     at = __builtin_amdgcn_readlane(at, 63) + run - c;
     for (; in; in &= in - 1, ++at) {
-      const int bit = __builtin_ctz(in);
+      const int bit = U * E - 1 - __builtin_ctz(in);
       if (at < SMP_LIST) s.idx[at] = i0 + bit / E * SMP_BLOCK * E + bit % E;
     }
   }
