@@ -117,10 +117,10 @@ NK_DEVICE AttSpan att_span(const AttendArgs &a, const AttSeq &s, int tile) {
   return t;
 }
 
-// the part of a tile's blocks that split s takes: at least min_blocks, so few
+// the part of a tile's blocks that split s takes: a multiple of min_blocks, so few
 // splits of a short sequence have any; returns their number
 NK_DEVICE int att_split(const AttendArgs &a, int nb, int s, int &j0, int &j1) {
-  const int per = max((nb + a.nsplit - 1) / a.nsplit, a.min_blocks);
+  const int per = max((nb + a.nsplit * a.min_blocks - 1) / (a.nsplit * a.min_blocks), 1) * a.min_blocks;
   j0 = min(s * per, nb);
   j1 = min(j0 + per, nb);
   return max(1, (nb + per - 1) / per);

@@ -538,14 +538,210 @@ NK_TILE(bf16, bf16, 64)
 NK_TILE(f16, f16, 64)
 
 // ---------------------------------------------------------------------------
-// The splits of a row joined, in their order: o = sum 2^(m_s - M) o_s / sum
-// 2^(m_s - M) l_s.  One wave per row; up to 64 splits, a lane each for their
-// offsets.  Rows that one split had are written already.
+// One new token per sequence (16-bit operands, head dim 64 or 128): bound by the
+// read of the keys and values, so the waves of a workgroup take blocks of 32 keys
+// of their own, no barrier between them, and meet at the end.
+//
+// A wave has up to 16 heads of the group as the columns of 16x16x32 products,
+// S^T = K Q^T and O^T = V^T P^T.  K fragments come straight from memory (16 bytes
+// of a row per lane); V goes to an LDS slot of the wave's own, from which
+// transposing reads take four keys of a column.  Every head sees the same keys.
 // ---------------------------------------------------------------------------
-template <typename T, int D>
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+NK_DEVICE f32x4 mul16(Mat<bf16>::V a, Mat<bf16>::V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+NK_DEVICE f32x4 mul16(Mat<f16>::V a, Mat<f16>::V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
+  typedef typename Mat<T>::V V8;
+  constexpr int RB = D * 2, TB = ATT_KEYS * RB, LPR = RB / 16, RPM = 64 / LPR, NM = ATT_KEYS / RPM;
+  constexpr int NW = 4;
+  constexpr int SUM = NW * 16 * (D + 2) * 4;  // the waves' sums
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * TB > SUM ? NW * TB : SUM];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, grp = lane >> 4;
+  const int rep = a.Hq / a.Hkv, per = (rep + 15) / 16;
+  int w = blockIdx.x;
+  const int g = w % a.Hkv;
+  w /= a.Hkv;
+  const int split = w % a.nsplit;
+  w /= a.nsplit;
+  const int h0 = w % per * 16, b = w / per;  // first head of the group's
+  const AttSeq sq = att_seq(a, b);
+  const AttSpan sp = att_span(a, sq, 0);
+  int j0, j1;
+  const int pieces = att_split(a, sp.nb, split, j0, j1);
+  if (split >= pieces) return;
+  const int p = sq.p0, klim = min(p, sq.cap - 1);
+
+  const bool head = h0 + l16 < rep;
+  V8 qf[D / 32];
+  {
+    const uint16_t *q = (const uint16_t *)a.q + (PAGED ? (int64_t)b * a.q_ss : (int64_t)b * a.q_sb) +
+                        (int64_t)(g * rep + min(h0 + l16, rep - 1)) * a.q_sh;
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) qf[kk] = *reinterpret_cast<const V8 *>(q + kk * 32 + grp * 8);
+  }
+  const uint16_t *kp = (const uint16_t *)a.k + (PAGED ? 0 : (int64_t)b * a.k_sb) + (int64_t)g * a.k_sh;
+  const uint16_t *vp = (const uint16_t *)a.v + (PAGED ? 0 : (int64_t)b * a.v_sb) + (int64_t)g * a.v_sh;
+  const uint8_t *zeros = (const uint8_t *)a.zeros;
+
+  f32x4 acc[D / 16];
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -1e30f, l_run = 0.f;
+  const float sl2 = a.scale * 1.44269504088896340736f;
+
+  // 16 rows of a transposing read, two chunks each, cover all banks
+  auto swz = [](int r) __attribute__((always_inline)) { return D == 128 ? (r & 7) << 1 : ((r >> 1) & 3) << 1; };
+  uint8_t *const slot = lds + wave * TB;
+  const uint32_t slot_lds = lds_addr(lds) + wave * TB;
+  // lane l looks up key l % 32 of a block: its row, -1 where it is not seen
+  auto place = [&](int j) __attribute__((always_inline)) {
+    const int key = sp.kb(j) * ATT_KEYS + (lane & 31);
+    return j < j1 && key <= klim && (key > p - a.window || key < a.sinks) ? att_place(a, b, key) : -1;
+  };
+
+  int ent = place(j0 + wave);
+  for (int j = j0 + wave; j < j1; j += NW) {
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const int r = i * RPM + lane / LPR, c = ((lane % LPR) ^ swz(r)) * 16;
+      const int at = __shfl(ent, r, 64);
+      move16((at < 0 ? zeros : (const uint8_t *)(vp + (int64_t)at * a.v_ss)) + c, slot_lds + i * 1024);
+    }
+    V8 kf[2][D / 32];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int at = __shfl(ent, kt * 16 + l16, 64);
+      const uint16_t *k = at < 0 ? (const uint16_t *)zeros : kp + (int64_t)at * a.k_ss;
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk) kf[kt][kk] = *reinterpret_cast<const V8 *>(k + kk * 32 + grp * 8);
+    }
+    const uint32_t seen = (uint32_t)__ballot(ent >= 0);
+    ent = place(j + NW);  // (on its way while this block is worked on)
+    f32x4 s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk) s[kt] = mul16(kf[kt][kk], qf[kk], s[kt]);
+    }
+    // element r of tile kt is key 16 kt + 4 grp + r
+    const uint32_t mine = seen >> (grp * 4);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[kt][r] = mine >> (kt * 16 + r) & 1 ? s[kt][r] : -INFINITY;
+    V8 pf;
+    auto weigh = [&]() __attribute__((always_inline)) {
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], sl2, -m_run));
+        sum += x;
+        pf[e] = (typename Mat<T>::E)x;
+      }
+      return sum;
+    };
+    float ls = weigh();
+    if (__builtin_amdgcn_ballot_w64(!(ls <= Mat<T>::LIMIT)) != 0) {
+      float bm = s[0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) bm = fmaxf(bm, s[e >> 2][e & 3]);
+      bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+      const float m_new = fmaxf(m_run, bm * sl2 - Mat<T>::TOP);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[t][r] *= alpha;
+      l_run *= alpha;
+      ls = weigh();
+    }
+    l_run += ls;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): V is there
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      s16x4 v[2];
+#pragma unroll
+      for (int si = 0; si < 2; ++si) {
+        const int r = 16 * si + 4 * grp + (l16 >> 2);
+        const int c = (t * 2 + ((l16 & 3) >> 1)) ^ swz(r);
+        v[si] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(slot + r * RB + c * 16 + (l16 & 1) * 8));
+      }
+      const s16x8 vf = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      acc[t] = mul16(__builtin_bit_cast(V8, vf), pf, acc[t]);
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the slot is read before it is refilled
+    asm volatile("" ::: "memory");
+  }
+
+  // The waves' sums: their offsets meet, then each row's sums are added in the
+  // waves' order.
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  float *so = reinterpret_cast<float *>(lds), *sm = so + NW * 16 * D;  // (NW, 16, D) sums; (NW, 16) weights, (16) in all
+  __syncthreads();
+  if (grp == 0) so[wave * 16 + l16] = m_run;
+  __syncthreads();
+  const float m = fmaxf(fmaxf(so[l16], so[16 + l16]), fmaxf(so[32 + l16], so[48 + l16]));
+  __syncthreads();
+  // (an infinite score's offset is infinite: its sums are NaN already)
+  const float f = m_run == m ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+    *reinterpret_cast<float4 *>(so + (wave * 16 + l16) * D + t * 16 + grp * 4) =
+        make_float4(acc[t][0] * f, acc[t][1] * f, acc[t][2] * f, acc[t][3] * f);
+  if (grp == 0) sm[wave * 16 + l16] = l_run * f;
+  __syncthreads();
+  const int64_t nr = (int64_t)a.N * a.Hq, r0 = (int64_t)b * a.Hq + g * rep + h0;
+#pragma unroll
+  for (int x = 0; x < 16 * D / 256; ++x) {
+    const int e = x * 256 + tid, r = e / D;
+    if (h0 + r >= rep) break;  // (rows rise)
+    const float o = (so[e] + so[16 * D + e]) + (so[2 * 16 * D + e] + so[3 * 16 * D + e]);
+    const float l = (sm[r] + sm[16 + r]) + (sm[32 + r] + sm[48 + r]);
+    if (pieces == 1) {
+      Elt<T>::store((T *)a.o + r0 * D, e, l == 0.f ? 0.f : o / l);
+    } else {
+      a.ws[(split * nr + r0) * D + e] = o;
+    }
+  }
+  if (pieces > 1 && wave == 0 && grp == 0 && h0 + l16 < rep) {
+    float *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + r0 + l16) * 2;
+    wm[0] = m, wm[1] = (sm[l16] + sm[16 + l16]) + (sm[32 + l16] + sm[48 + l16]);
+  }
+}
+#define NK_STEP(T, name, D)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_step_paged_##name##_d##D(AttendArgs a) {   \
+    attend_step_body<T, D, true>(a);                                                                        \
+  }                                                                                                         \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_step_plain_##name##_d##D(AttendArgs a) {   \
+    attend_step_body<T, D, false>(a);                                                                       \
+  }
+NK_STEP(bf16, bf16, 128)
+NK_STEP(f16, f16, 128)
+NK_STEP(bf16, bf16, 64)
+NK_STEP(f16, f16, 64)
+
+// ---------------------------------------------------------------------------
+// The splits of a row joined, in their order: o = sum 2^(m_s - M) o_s / sum
+// 2^(m_s - M) l_s.  Up to 64 splits, a lane each for their offsets; bound by the
+// latency of its reads.  One wave per row, or (W = 4) a workgroup, each wave a
+// quarter of the splits, all of its reads in flight at once.  Rows that one split
+// had are written already.
+// ---------------------------------------------------------------------------
+template <typename T, int D, int W>
 __device__ __forceinline__ void attend_join_body(const AttendArgs &a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nr = (int64_t)a.N * a.Hq;
+  __shared__ float part[W == 1 ? 1 : W][D];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t r = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x, nr = (int64_t)a.N * a.Hq;
   if (r >= nr) return;
   const int t = (int)(r / a.Hq), h = (int)(r % a.Hq), rep = a.Hq / a.Hkv;
   const int b = a.starts ? att_find(a.B, t, [&](int x) { return a.starts[x]; }) : t / a.S;
@@ -557,6 +753,17 @@ __device__ __forceinline__ void attend_join_body(const AttendArgs &a) {
   const int pieces = att_split(a, att_span(a, sq, (i * rep + h % rep) / ATT_ROWS).nb, 0, j0, j1);
   if (pieces == 1) return;
   const float *wm = a.ws + (int64_t)a.nsplit * nr * D;
+  const int w0 = W == 1 ? 0 : wave;  // this wave's splits: w0, w0 + W, ...
+  constexpr int U = W == 1 ? 4 : 16;
+  float acc[D / 64], x[U][D / 64];
+  auto fetch = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < U; ++s)  // (past the last piece: the last again, unused)
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e)
+        x[s][e] = a.ws[((int64_t)min(s0 + s * W, pieces - 1) * nr + r) * D + lane + 64 * e];
+  };
+  fetch(w0);
   float m = -1e30f, l = 0.f;
   if (lane < pieces) {
     const float2 v = *reinterpret_cast<const float2 *>(wm + (lane * nr + r) * 2);
@@ -565,29 +772,38 @@ __device__ __forceinline__ void attend_join_body(const AttendArgs &a) {
   const float w = __builtin_amdgcn_exp2f(m - wave_max(m));
   const float total = wave_sum(lane < pieces ? w * l : 0.f);
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  float acc[D / 64];
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) acc[e] = 0.f;
-  for (int s0 = 0; s0 < pieces; s0 += 8) {
-    float x[8][D / 64];
+  for (int s0 = w0; s0 < pieces; s0 += U * W) {
+    if (s0 != w0) fetch(s0);
 #pragma unroll
-    for (int s = 0; s < 8; ++s)  // (past the last piece: the last again, unused)
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) x[s][e] = a.ws[((int64_t)min(s0 + s, pieces - 1) * nr + r) * D + lane + 64 * e];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      if (s0 + s >= pieces) break;
-      const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + s));
+    for (int s = 0; s < U; ++s) {
+      if (s0 + s * W >= pieces) break;
+      const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + s * W));
 #pragma unroll
       for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(ws, x[s][e], acc[e]);
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) part[wave][lane + 64 * e] = acc[e];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      const int d = lane + 64 * e;
+      acc[e] = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
     }
   }
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) Elt<T>::store((T *)a.o + r * D, lane + 64 * e, total == 0.f ? 0.f : acc[e] * inv);
 }
-#define NK_JOIN(T, name, D)                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void nk_attend_join_##name##_d##D(AttendArgs a) { \
-    attend_join_body<T, D>(a);                                                                    \
+#define NK_JOIN(T, name, D)                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void nk_attend_join_##name##_d##D(AttendArgs a) {     \
+    attend_join_body<T, D, 1>(a);                                                                    \
+  }                                                                                                  \
+  extern "C" __global__ __launch_bounds__(256) void nk_attend_join4_##name##_d##D(AttendArgs a) {    \
+    attend_join_body<T, D, 4>(a);                                                                    \
   }
 NK_JOIN(bf16, bf16, 128)
 NK_JOIN(f16, f16, 128)
