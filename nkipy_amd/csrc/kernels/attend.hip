@@ -101,6 +101,9 @@ NK_DEVICE void move16(const void *p, uint32_t lds) {
 }
 
 #define ATT_AHEAD 32  // blocks whose rows are looked up at once
+// offset of a row that is not there: past the end of any buffer resource, also
+// with a place in a row added
+#define ATT_NOWHERE 0xfffff000u
 
 // rows outside every sequence: zeros, shared out over the grid
 template <typename T>
@@ -137,7 +140,10 @@ NK_DEVICE AttWork att_work(const AttendArgs &a, int w) {
   return k;
 }
 
-template <typename T, int D, bool PAGED>
+// FAR: keys or values over 4 GiB, or keys and values of different row strides in
+// one cache: 64-bit addresses, and a row of zeros for what has no use.  Else offsets
+// into a buffer resource, past whose end a move writes zeros.
+template <typename T, int D, bool PAGED, bool FAR>
 __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   typedef typename Mat<T>::V V8;
   constexpr int RB = D * 2, TB = ATT_KEYS * RB;  // bytes of a row, of a block
@@ -209,6 +215,7 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
           at = att_place(a, b, key);
           miss |= at < 0;
         }
+        if constexpr (!FAR) at = at < 0 ? (int)ATT_NOWHERE : (int)((uint32_t)at * (uint32_t)a.k_ss * 2);
         ent[(c & 1) * ATT_AHEAD * ATT_KEYS + x] = at;
       }
       const bool any = __ballot(miss) != 0;
@@ -216,33 +223,54 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     }
   };
-  // address of 16 bytes of row r (chunk c) of block j0 + jr, zeros where it has
-  // no use
-  auto source = [&](const uint16_t *base, int64_t ss, int jr, int r, int c) __attribute__((always_inline)) -> const void * {
-    int at = -1;
-    if constexpr (PAGED) {
-      if (jr < n) at = ent[(jr & (2 * ATT_AHEAD - 1)) * ATT_KEYS + r];
-    } else {
-      const int key = sp.kb(j0 + jr) * ATT_KEYS + r;
-      if (jr < n && key < sp.hi && (key >= sp.lo || key < a.sinks)) at = key;
-    }
-    asm volatile("" : "+v"(c));  // (sums with the bases would be kept in registers for every row)
-    const uint8_t *p = at < 0 ? (const uint8_t *)a.zeros : (const uint8_t *)(base + (int64_t)at * ss);
-    return p + c * 16;
-  };
   const uint32_t k_lds = lds_addr(KR) + wave * 1024, v_lds = lds_addr(VR) + wave * 1024;
+  const int64_t rows_there = PAGED ? (int64_t)a.pages * a.pitch : sp.hi;
+  const i32x4_t rk = rsrc_words(kp, (rows_there - 1) * a.k_ss * 2 + RB), rv = rsrc_words(vp, (rows_there - 1) * a.v_ss * 2 + RB);
+  const int r0 = wave * RPM + lane / LPR;
+  const uint32_t kown = r0 * (uint32_t)a.k_ss * 2 + (((lane % LPR) ^ kswz(r0)) << 4);
+  const uint32_t vown = r0 * (uint32_t)a.v_ss * 2 + (((lane % LPR) ^ vswz(r0)) << 4);
+  // move i of block j0 + jr: row r, 16-byte chunk c of this lane, which are `own`
+  // bytes into the block for i = 0
+  auto move = [&](const uint16_t *base, i32x4_t rsrc, int64_t ss, int jr, int i, int r, int c, uint32_t own, uint32_t lds)
+      __attribute__((always_inline)) {
+    const int k0 = sp.kb(j0 + jr) * ATT_KEYS;
+    if constexpr (!FAR) {
+      uint32_t off;
+      if constexpr (PAGED) {
+        off = jr < n ? (uint32_t)ent[(jr & (2 * ATT_AHEAD - 1)) * ATT_KEYS + r] : ATT_NOWHERE;
+      } else {
+        // (the block's part is uniform; past the last key the resource ends)
+        off = own + (uint32_t)(k0 + i * 4 * RPM) * (uint32_t)ss * 2;
+        rsrc[2] = jr < n ? rsrc[2] : 0;
+        if (k0 < sp.lo && k0 + ATT_KEYS > a.sinks) off = k0 + r < sp.lo && k0 + r >= a.sinks ? ATT_NOWHERE : off;
+      }
+      dma16_asm(rsrc, lds, PAGED ? off + c * 16 : off);
+    } else {
+      int at = -1;
+      if constexpr (PAGED) {
+        if (jr < n) at = ent[(jr & (2 * ATT_AHEAD - 1)) * ATT_KEYS + r];
+      } else {
+        if (jr < n && k0 + r < sp.hi && (k0 + r >= sp.lo || k0 + r < a.sinks)) at = k0 + r;
+      }
+      move16((at < 0 ? (const uint8_t *)a.zeros : (const uint8_t *)(base + (int64_t)at * ss)) + c * 16, lds);
+    }
+  };
   auto load_k = [&](auto sl, int jr) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
-      const int r = (i * 4 + wave) * RPM + lane / LPR;
-      move16(source(kp, a.k_ss, jr, r, (lane % LPR) ^ kswz(r)), k_lds + (decltype(sl)::value & 3) * TB + i * 4096);
+      int l = lane;
+      if constexpr (PAGED && FAR) asm volatile("" : "+v"(l));  // (registers: found again every time)
+      const int r = (i * 4 + wave) * RPM + l / LPR;
+      move(kp, rk, a.k_ss, jr, i, r, (l % LPR) ^ kswz(r), kown, k_lds + (decltype(sl)::value & 3) * TB + i * 4096);
     }
   };
   auto load_v = [&](auto sl, int jr) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
-      const int r = (i * 4 + wave) * RPM + lane / LPR;
-      move16(source(vp, a.v_ss, jr, r, (lane % LPR) ^ vswz(r)), v_lds + (decltype(sl)::value & 3) * TB + i * 4096);
+      int l = lane;
+      if constexpr (PAGED && FAR) asm volatile("" : "+v"(l));  // (registers: found again every time)
+      const int r = (i * 4 + wave) * RPM + l / LPR;
+      move(vp, rv, a.v_ss, jr, i, r, (l % LPR) ^ vswz(r), vown, v_lds + (decltype(sl)::value & 3) * TB + i * 4096);
     }
   };
   // an iteration leaves the moves of the last two outstanding
@@ -313,10 +341,11 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
         for (int r = 0; r < 16; r += 4) {
           const int4 e = *reinterpret_cast<const int4 *>(en + r * 2);
           asm volatile("" ::: "memory");  // (one at a time: registers)
-          s[r] = e.x < 0 ? -INFINITY : s[r];
-          s[r + 1] = e.y < 0 ? -INFINITY : s[r + 1];
-          s[r + 2] = e.z < 0 ? -INFINITY : s[r + 2];
-          s[r + 3] = e.w < 0 ? -INFINITY : s[r + 3];
+          auto gone = [](int x) { return FAR ? x < 0 : (uint32_t)x >= ATT_NOWHERE; };
+          s[r] = gone(e.x) ? -INFINITY : s[r];
+          s[r + 1] = gone(e.y) ? -INFINITY : s[r + 1];
+          s[r + 2] = gone(e.z) ? -INFINITY : s[r + 2];
+          s[r + 3] = gone(e.w) ? -INFINITY : s[r + 3];
         }
       }
     }
@@ -525,12 +554,18 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   }
 }
 
-#define NK_TILE(T, name, D)                                                                                  \
-  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_paged_##name##_d##D(AttendArgs a) {    \
-    attend_tile_body<T, D, true>(a);                                                                         \
-  }                                                                                                          \
-  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_plain_##name##_d##D(AttendArgs a) {    \
-    attend_tile_body<T, D, false>(a);                                                                        \
+#define NK_TILE(T, name, D)                                                                                      \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_paged_##name##_d##D(AttendArgs a) {        \
+    attend_tile_body<T, D, true, false>(a);                                                                      \
+  }                                                                                                              \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_plain_##name##_d##D(AttendArgs a) {        \
+    attend_tile_body<T, D, false, false>(a);                                                                     \
+  }                                                                                                              \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_paged_far_##name##_d##D(AttendArgs a) {    \
+    attend_tile_body<T, D, true, true>(a);                                                                       \
+  }                                                                                                              \
+  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_plain_far_##name##_d##D(AttendArgs a) {    \
+    attend_tile_body<T, D, false, true>(a);                                                                      \
   }
 NK_TILE(bf16, bf16, 128)
 NK_TILE(f16, f16, 128)

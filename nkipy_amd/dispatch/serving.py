@@ -150,7 +150,10 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
         raise LaunchError(f"attention of {a.nsplit} splits needs a workspace")
     if a.tiles * Hkv * a.nsplit >= 2**31 or Hq // Hkv * S >= 2**31:
         raise LaunchError("attention: too many tiles for one launch")
-    kind = f"{'step' if step else 'tile'}_{'paged' if tables else 'plain'}"
+    # tiles address a sequence's rows by 32-bit offsets where those reach
+    reach = 2 * max(k_str[1], v_str[1]) * (pages * pitch if tables else T + 64)
+    far = not step and (reach >= 2**32 - 4096 or (tables and k_str[1] != v_str[1]))
+    kind = f"{'step' if step else 'tile'}_{'paged' if tables else 'plain'}{'_far' if far else ''}"
     out = [Launch("attend", f"nk_attend_{kind}_{tag}_d{D}", (a.tiles * Hkv * a.nsplit, 1, 1), (256, 1, 1), a)]
     if a.nsplit > ATT_JOIN_WIDE:
         out.append(Launch("attend", f"nk_attend_join4_{tag}_d{D}", (N * Hq, 1, 1), (256, 1, 1), a))
