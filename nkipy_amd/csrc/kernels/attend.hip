@@ -55,9 +55,9 @@ extern "C" __global__ __launch_bounds__(256) void nk_attend_rows_f32(AttendArgs 
 // not finite and seen by some rows of a tile only would still meet the others'
 // weights of 0, and the rows it spoils are computed again one by one.
 //
-// Blocks that every row sees in full take the loop body without mask; the
-// masked one serves the edges (the diagonal, the window's end, the sinks'
-// last block, missing pages).
+// Scores of blocks that some row does not see in full (the diagonal, the window's
+// end, the sinks' last block, missing pages) are masked ahead of that body, which
+// is one for all blocks.
 //
 // Softmax: p = 2^(s c - m), c = scale log2(e), with an offset m per row that
 // starts TOP below the first block's largest score and is raised (sums
@@ -118,7 +118,10 @@ NK_DEVICE void att_zero_rest(const AttendArgs &a, int wg, int nwg) {
 
 // Workgroups run round-robin over the eight XCDs: with the KV head fastest, the
 // tiles of one head (eight heads, or a multiple) share an XCD's cache.  The last
-// tiles of a sequence, the longest without a window, go first.
+// tiles of a sequence, the longest without a window, go first; splits that only
+// the longest sequences have come last, and so leave no CU with two workgroups
+// while others have none (256 tokens behind 4000: 70 us with the splits of a tile
+// side by side, 48 so).
 struct AttWork {
   int g, split, b, tile;  // b < 0: nothing to do
 };
@@ -128,8 +131,8 @@ NK_DEVICE AttWork att_work(const AttendArgs &a, int w) {
   const int rep = a.Hq / a.Hkv;
   k.g = w % a.Hkv;
   w /= a.Hkv;
-  k.split = w % a.nsplit;
-  const int t = a.tiles - 1 - w / a.nsplit;
+  const int t = a.tiles - 1 - w % a.tiles;
+  k.split = w / a.tiles;
   if (PAGED && a.starts) {
     k.b = att_find(a.B, t, [&](int x) { return att_tile0(a, x); });
     k.tile = k.b < 0 ? 0 : t - att_tile0(a, k.b);
@@ -325,30 +328,31 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
     return s0 + s1;
   };
   int missing = 0;  // the blocks being worked on have keys without a page
-  // element r of a lane's scores is key 32 kb + 8 (r / 4) + 4 lhi + r % 4
-  auto softmax = [&](f32x16 &s, V8 (&pf)[2], int jr, auto masked) __attribute__((always_inline)) {
-    if constexpr (decltype(masked)::value) {
-      const int k0 = sp.kb(j0 + jr) * ATT_KEYS + lhi * 4;
-      const int t0 = klim - k0, w0 = p - a.window - k0, s0 = a.sinks - k0;
+  // What no row sees of block jr out of its scores; past the last block, all of it.
+  // Element r of a lane is key 32 kb + 8 (r / 4) + 4 lhi + r % 4.
+  auto mask = [&](f32x16 &s, int jr) __attribute__((always_inline)) {
+    const int k0 = sp.kb(j0 + jr) * ATT_KEYS + lhi * 4;
+    const int t0 = jr < n ? klim - k0 : -1, w0 = p - a.window - k0, s0 = a.sinks - k0;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int x = (r >> 2) * 8 + (r & 3);
-        s[r] = x > t0 || (x <= w0 && x >= s0) ? -INFINITY : s[r];
-      }
-      if (PAGED && missing) {
-        const int32_t *en = ent + (jr & (2 * ATT_AHEAD - 1)) * ATT_KEYS + lhi * 4;
+    for (int r = 0; r < 16; ++r) {
+      const int x = (r >> 2) * 8 + (r & 3);
+      s[r] = x > t0 || (x <= w0 && x >= s0) ? -INFINITY : s[r];
+    }
+    if (PAGED && missing) {
+      const int32_t *en = ent + (jr & (2 * ATT_AHEAD - 1)) * ATT_KEYS + lhi * 4;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const int4 e = *reinterpret_cast<const int4 *>(en + r * 2);
-          asm volatile("" ::: "memory");  // (one at a time: registers)
-          auto gone = [](int x) { return FAR ? x < 0 : (uint32_t)x >= ATT_NOWHERE; };
-          s[r] = gone(e.x) ? -INFINITY : s[r];
-          s[r + 1] = gone(e.y) ? -INFINITY : s[r + 1];
-          s[r + 2] = gone(e.z) ? -INFINITY : s[r + 2];
-          s[r + 3] = gone(e.w) ? -INFINITY : s[r + 3];
-        }
+      for (int r = 0; r < 16; r += 4) {
+        const int4 e = *reinterpret_cast<const int4 *>(en + r * 2);
+        asm volatile("" ::: "memory");  // (one at a time: registers)
+        auto gone = [](int x) { return FAR ? x < 0 : (uint32_t)x >= ATT_NOWHERE; };
+        s[r] = gone(e.x) ? -INFINITY : s[r];
+        s[r + 1] = gone(e.y) ? -INFINITY : s[r + 1];
+        s[r + 2] = gone(e.z) ? -INFINITY : s[r + 2];
+        s[r + 3] = gone(e.w) ? -INFINITY : s[r + 3];
       }
     }
+  };
+  auto softmax = [&](f32x16 &s, V8 (&pf)[2]) __attribute__((always_inline)) {
     float ls = expblock(s, pf);
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= Mat<T>::LIMIT)) != 0, 0)) {
       float bm = s[0];
@@ -370,28 +374,33 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
 
   auto whole = [&](int jr) __attribute__((always_inline)) {  // every row sees the whole block
     const int k0 = sp.kb(j0 + jr) * ATT_KEYS;
-    return k0 + ATT_KEYS - 1 <= sp.pa && k0 + ATT_KEYS <= sp.hi && (k0 > sp.pb - a.window || k0 + ATT_KEYS <= a.sinks) && !missing;
+    return jr < n && k0 + ATT_KEYS - 1 <= sp.pa && k0 + ATT_KEYS <= sp.hi && (k0 > sp.pb - a.window || k0 + ATT_KEYS <= a.sinks) && !missing;
   };
 
   f32x16 sA, sB;
   V8 pA[2], pB[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pB[j][e] = (typename Mat<T>::E)0.f;
   // the end of an iteration: the next moves, behind its matrix instructions
   auto move_on = [&](auto sl, int jr) __attribute__((always_inline)) {
-    if (jr < n) {
-      load_k(sl, jr + 4);
-      load_v(Slot<decltype(sl)::value + 2>{}, jr + 2);
-    }
+    load_k(sl, jr + 4);
+    load_v(Slot<decltype(sl)::value + 2>{}, jr + 2);
     wait_moves(Slot<4 * NM>{});
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  // a whole block between others
-  auto inner = [&](auto sl, int jr, f32x16 &cur, f32x16 &nxt, V8 (&prev)[2], V8 (&now)[2]) __attribute__((always_inline)) {
+  // Iteration jr, one body for all: the values of the block before (of zeros
+  // before the first), the scores of the one behind (of zeros past the last), the
+  // softmax of this one.  The last, jr = n, adds the last block's values.
+  auto step = [&](auto sl, int jr, f32x16 &cur, f32x16 &nxt, V8 (&prev)[2], V8 (&now)[2]) __attribute__((always_inline)) {
     constexpr int SL = decltype(sl)::value;
+    if (!whole(jr)) mask(cur, jr);
     qk(KR + ((SL + 1) & 3) * TB, nxt);
     pv(VR + ((SL + 3) & 3) * TB, prev);
-    softmax(cur, now, jr, Flag<false>{});
+    softmax(cur, now);
     // every LDS read first, then matrix instructions with the softmax between them
     __builtin_amdgcn_sched_group_barrier(0x100, 3 * D / 16, 0);
     __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
@@ -402,19 +411,11 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
     }
     move_on(sl, jr);
   };
-  // the first and last blocks and those with a mask; iteration n has the last values
-  auto edge = [&](auto sl, int jr, f32x16 &cur, f32x16 &nxt, V8 (&prev)[2], V8 (&now)[2]) __attribute__((always_inline)) {
-    constexpr int SL = decltype(sl)::value;
-    if (jr > n) return;
-    if (jr + 1 < n) qk(KR + ((SL + 1) & 3) * TB, nxt);
-    if (jr > 0) pv(VR + ((SL + 3) & 3) * TB, prev);
-    if (jr < n) softmax(cur, now, jr, Flag<true>{});
-    move_on(sl, jr);
-  };
 
   if (n > 0) {
     look_up(0);
     __syncthreads();
+    load_v(Slot<3>{}, n);  // (zeros)
     load_k(Slot<0>{}, 0);
     load_k(Slot<1>{}, 1);
     load_k(Slot<2>{}, 2);
@@ -438,24 +439,16 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
       }
     };
     if (active) {
-      int jr = 0;
-      ahead(0);
-      while (true) {
-        edge(Slot<0>{}, jr, sA, sB, pB, pA);
-        edge(Slot<1>{}, jr + 1, sB, sA, pA, pB);
-        edge(Slot<2>{}, jr + 2, sA, sB, pB, pA);
-        edge(Slot<3>{}, jr + 3, sB, sA, pA, pB);
-        jr += 4;
-        if (jr > n) break;
+      for (int jr = 0;; jr += 4) {
         ahead(jr);
-        while (jr + 4 < n && whole(jr) && whole(jr + 1) && whole(jr + 2) && whole(jr + 3)) {
-          inner(Slot<0>{}, jr, sA, sB, pB, pA);
-          inner(Slot<1>{}, jr + 1, sB, sA, pA, pB);
-          inner(Slot<2>{}, jr + 2, sA, sB, pB, pA);
-          inner(Slot<3>{}, jr + 3, sB, sA, pA, pB);
-          jr += 4;
-          ahead(jr);
-        }
+        step(Slot<0>{}, jr, sA, sB, pB, pA);
+        if (jr + 1 > n) break;
+        step(Slot<1>{}, jr + 1, sB, sA, pA, pB);
+        if (jr + 2 > n) break;
+        step(Slot<2>{}, jr + 2, sA, sB, pB, pA);
+        if (jr + 3 > n) break;
+        step(Slot<3>{}, jr + 3, sB, sA, pA, pB);
+        if (jr + 4 > n) break;
       }
     } else {  // rows past the sequence's: the moves only
       for (int jr = 0; jr <= n; jr += 4) {
@@ -554,23 +547,24 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   }
 }
 
-#define NK_TILE(T, name, D)                                                                                      \
-  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_paged_##name##_d##D(AttendArgs a) {        \
+#define NK_TILE(T, name, D, OCC)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256, OCC) void nk_attend_tile_paged_##name##_d##D(AttendArgs a) {        \
     attend_tile_body<T, D, true, false>(a);                                                                      \
   }                                                                                                              \
-  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_plain_##name##_d##D(AttendArgs a) {        \
+  extern "C" __global__ __launch_bounds__(256, OCC) void nk_attend_tile_plain_##name##_d##D(AttendArgs a) {        \
     attend_tile_body<T, D, false, false>(a);                                                                     \
   }                                                                                                              \
-  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_paged_far_##name##_d##D(AttendArgs a) {    \
+  extern "C" __global__ __launch_bounds__(256, OCC) void nk_attend_tile_paged_far_##name##_d##D(AttendArgs a) {    \
     attend_tile_body<T, D, true, true>(a);                                                                       \
   }                                                                                                              \
-  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend_tile_plain_far_##name##_d##D(AttendArgs a) {    \
+  extern "C" __global__ __launch_bounds__(256, OCC) void nk_attend_tile_plain_far_##name##_d##D(AttendArgs a) {    \
     attend_tile_body<T, D, false, true>(a);                                                                      \
   }
-NK_TILE(bf16, bf16, 128)
-NK_TILE(f16, f16, 128)
-NK_TILE(bf16, bf16, 64)
-NK_TILE(f16, f16, 64)
+// (workgroups per CU: three of head dim 64 fit)
+NK_TILE(bf16, bf16, 128, 2)
+NK_TILE(f16, f16, 128, 2)
+NK_TILE(bf16, bf16, 64, 3)
+NK_TILE(f16, f16, 64, 3)
 
 // ---------------------------------------------------------------------------
 // One new token per sequence (16-bit operands, head dim 64 or 128): bound by the
@@ -601,9 +595,7 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   int w = blockIdx.x;
   const int g = w % a.Hkv;
   w /= a.Hkv;
-  const int split = w % a.nsplit;
-  w /= a.nsplit;
-  const int h0 = w % per * 16, b = w / per;  // first head of the group's
+  const int split = w / a.tiles, h0 = w % a.tiles % per * 16, b = w % a.tiles / per;  // (h0: first head of the group's)
   const AttSeq sq = att_seq(a, b);
   const AttSpan sp = att_span(a, sq, 0);
   int j0, j1;

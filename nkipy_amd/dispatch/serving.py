@@ -86,6 +86,8 @@ ATT_SLOTS = 512               # workgroups that fill the chip: two per CU
 ATT_STEP_GRID = 2048          # workgroups of a step, to even out lengths
 ATT_STEP_BLOCKS = 32          # blocks that a split of a step has at least past ATT_SLOTS
 ATT_MIN_BLOCKS = 4            # blocks that any split has at least
+ATT_TILE_BLOCKS = int(__import__('os').environ.get('ATB', '4'))
+ATT_SLOTS_T = int(__import__('os').environ.get('AST', '512'))
 ATT_MAX_SPLIT = 64            # a lane of the joining wave for each
 ATT_JOIN_WIDE = 4             # splits past which a workgroup joins a row
 ATT_STEP_HEADS = 16           # heads of a group in one workgroup of a step
@@ -111,10 +113,10 @@ def attend_work(B, S, N, Hq, Hkv, keys, window=0, sinks=0, starts=False) -> Tupl
         units = N * rep // ATT_ROWS + B if starts else B * -(-S * rep // ATT_ROWS)
         tokens = -(-ATT_ROWS // rep)
     seen = min(keys, window + sinks + tokens + ATT_KEYS) if window else keys
-    splits = ATT_SLOTS // (units * Hkv)
+    splits = (ATT_SLOTS if step else ATT_SLOTS_T) // (units * Hkv)
     if step:
         splits = max(splits, min(ATT_STEP_GRID // (units * Hkv), seen // (ATT_KEYS * ATT_STEP_BLOCKS)))
-    most = max(1, -(-seen // (ATT_KEYS * ATT_MIN_BLOCKS)))
+    most = max(1, -(-seen // (ATT_KEYS * (ATT_MIN_BLOCKS if step else ATT_TILE_BLOCKS))))
     return step, units, max(1, min(splits, most, ATT_MAX_SPLIT))
 
 
@@ -145,7 +147,7 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     if not tiled:
         return [Launch("attend", f"nk_attend_rows_{tag}", (-(-N * Hq // 4), 1, 1), (256, 1, 1), a)]
     step, a.tiles, a.nsplit = attend_work(B, S, N, Hq, Hkv, width * page if tables else T, window, sinks, bool(starts))
-    a.min_blocks = ATT_MIN_BLOCKS
+    a.min_blocks = ATT_MIN_BLOCKS if step else ATT_TILE_BLOCKS
     if a.nsplit > 1 and not ws:
         raise LaunchError(f"attention of {a.nsplit} splits needs a workspace")
     if a.tiles * Hkv * a.nsplit >= 2**31 or Hq // Hkv * S >= 2**31:
