@@ -82,12 +82,11 @@ def rotary_append(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q=0, 
 
 
 ATT_ROWS, ATT_KEYS = 128, 32  # rows of a tile, keys of a block (attend.h)
-ATT_SLOTS = 512               # workgroups that fill the chip: two per CU
+ATT_CUS, ATT_SLOTS = 256, 512  # CUs; workgroups that fill them, two each
 ATT_STEP_GRID = 2048          # workgroups of a step, to even out lengths
 ATT_STEP_BLOCKS = 32          # blocks that a split of a step has at least past ATT_SLOTS
-ATT_MIN_BLOCKS = 4            # blocks that any split has at least
-ATT_TILE_BLOCKS = int(__import__('os').environ.get('ATB', '4'))
-ATT_SLOTS_T = int(__import__('os').environ.get('AST', '512'))
+ATT_MIN_BLOCKS = 4            # blocks that any split of a step has at least
+ATT_TILE_BLOCKS = 8           # blocks that a tile's split has at least
 ATT_MAX_SPLIT = 64            # a lane of the joining wave for each
 ATT_JOIN_WIDE = 4             # splits past which a workgroup joins a row
 ATT_STEP_HEADS = 16           # heads of a group in one workgroup of a step
@@ -98,13 +97,22 @@ def attend_tiled(dtype, D) -> bool:
     return dt.canonical(dtype) in (dt.bfloat16, dt.float16) and D in (64, 128)
 
 
-def attend_work(B, S, N, Hq, Hkv, keys, window=0, sinks=0, starts=False) -> Tuple[bool, int, int]:
+def attend_work(B, S, N, Hq, Hkv, D, keys, window=0, sinks=0, starts=False) -> Tuple[bool, int, int]:
     """(whether this is a step, workgroups of a KV head and split, splits of the
-    keys): one new token per sequence is a step.  Keys are split where the rest
-    leaves CUs idle, for the longest sequence that the tensors can hold; a step's
-    long ones further, so that sequences of many lengths end together (64 of up
-    to 8192 keys: 260 us with one split, 238 with four; 64 with a window of 500:
-    27 us with one, 45 with four)."""
+    keys): one new token per sequence is a step.  Splits are for the longest
+    sequence that the tensors can hold; the kernels give a shorter one fewer.
+
+    A step's keys are split where the rest leaves CUs idle, and long ones
+    further, so that sequences of many lengths end together (64 of up to 8192
+    keys: 260 us with one split, 238 with four; 64 with a window of 500: 27 us
+    with one, 45 with four).
+
+    Tiles take the splits of the least estimated time, in us: a block of keys is
+    0.75 for a CU's only workgroup and 0.52 for each of more; the sums of every
+    split are written and read at 4.5 TB/s, by a launch of 5.  (Measured: 1000
+    tokens of one prompt 27 us with one split, 42 with eight; 256 tokens behind
+    3744 cached 44 with four, 56 with seven, 104 with one; 40 tokens of eight
+    sequences of 8000 43 with seven, 60 with three.)"""
     rep = Hq // Hkv
     step = not starts and S == 1
     if step:
@@ -113,11 +121,17 @@ def attend_work(B, S, N, Hq, Hkv, keys, window=0, sinks=0, starts=False) -> Tupl
         units = N * rep // ATT_ROWS + B if starts else B * -(-S * rep // ATT_ROWS)
         tokens = -(-ATT_ROWS // rep)
     seen = min(keys, window + sinks + tokens + ATT_KEYS) if window else keys
-    splits = (ATT_SLOTS if step else ATT_SLOTS_T) // (units * Hkv)
+    blocks = -(-seen // ATT_KEYS)
     if step:
+        splits = ATT_SLOTS // (units * Hkv)
         splits = max(splits, min(ATT_STEP_GRID // (units * Hkv), seen // (ATT_KEYS * ATT_STEP_BLOCKS)))
-    most = max(1, -(-seen // (ATT_KEYS * (ATT_MIN_BLOCKS if step else ATT_TILE_BLOCKS))))
-    return step, units, max(1, min(splits, most, ATT_MAX_SPLIT))
+        splits = min(splits, -(-blocks // ATT_MIN_BLOCKS))
+    else:
+        def cost(s):
+            join = 5 + s * N * Hq * (D + 2) * 8 / 4.5e6 if s > 1 else 0
+            return -(-blocks // s) * max(0.75, 0.52 * -(-units * Hkv * s // ATT_CUS)) + join
+        splits = min(range(1, min(ATT_MAX_SPLIT, max(1, blocks // ATT_TILE_BLOCKS)) + 1), key=cost)
+    return step, units, max(1, min(splits, ATT_MAX_SPLIT))
 
 
 def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S=1, T=0, tables=0, lens=0, starts=0, first=0,
@@ -146,7 +160,7 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
         and not any(x % 8 for x in (*q_str, *k_str, *v_str))
     if not tiled:
         return [Launch("attend", f"nk_attend_rows_{tag}", (-(-N * Hq // 4), 1, 1), (256, 1, 1), a)]
-    step, a.tiles, a.nsplit = attend_work(B, S, N, Hq, Hkv, width * page if tables else T, window, sinks, bool(starts))
+    step, a.tiles, a.nsplit = attend_work(B, S, N, Hq, Hkv, D, width * page if tables else T, window, sinks, bool(starts))
     a.min_blocks = ATT_MIN_BLOCKS if step else ATT_TILE_BLOCKS
     if a.nsplit > 1 and not ws:
         raise LaunchError(f"attention of {a.nsplit} splits needs a workspace")
@@ -390,7 +404,7 @@ class AttendMatch(Match):
         tmp = {}
         if attend_tiled(q.dtype, kw["D"]):
             keys = tables.shape[1] * k.shape[1] if self.paged else k.shape[1]
-            splits = attend_work(kw["B"], kw.get("S", 1), kw["N"], kw["Hq"], kw["Hkv"], keys, kw["window"], kw["sinks"],
+            splits = attend_work(kw["B"], kw.get("S", 1), kw["N"], kw["Hq"], kw["Hkv"], kw["D"], keys, kw["window"], kw["sinks"],
                                  "starts" in more)[2]
             tmp["zeros"] = Slot(plan.add_buffer(2 * kw["D"], "const", "attend.zeros", np.zeros(kw["D"], np.uint16)))
             if splits > 1:
