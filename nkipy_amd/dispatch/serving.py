@@ -88,7 +88,8 @@ ATT_STEP_BLOCKS = 32          # blocks that a split of a step has at least past 
 ATT_MIN_BLOCKS = 4            # blocks that any split of a step has at least
 ATT_TILE_BLOCKS = 8           # blocks that a tile's split has at least
 ATT_MAX_SPLIT = 64            # a lane of the joining wave for each
-ATT_JOIN_WIDE = 4             # splits past which a workgroup joins a row
+ATT_JOIN_WIDE = 4             # splits past which a workgroup joins a row of fewer
+ATT_JOIN_ROWS = 1024          # than this; a wave does it where waves fill the chip
 ATT_STEP_HEADS = 16           # heads of a group in one workgroup of a step
 
 
@@ -111,7 +112,7 @@ def attend_work(B, S, N, Hq, Hkv, D, keys, window=0, sinks=0, starts=False) -> T
     0.75 for a CU's only workgroup and 0.52 for each of more; the sums of every
     split are written and read at 4.5 TB/s, by a launch of 5.  (Measured: 1000
     tokens of one prompt 27 us with one split, 42 with eight; 256 tokens behind
-    3744 cached 44 with four, 56 with seven, 104 with one; 40 tokens of eight
+    3744 cached 42 with seven, 44 with four, 104 with one; 40 tokens of eight
     sequences of 8000 43 with seven, 60 with three.)"""
     rep = Hq // Hkv
     step = not starts and S == 1
@@ -171,7 +172,9 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     far = not step and (reach >= 2**32 - 4096 or (tables and k_str[1] != v_str[1]))
     kind = f"{'step' if step else 'tile'}_{'paged' if tables else 'plain'}{'_far' if far else ''}"
     out = [Launch("attend", f"nk_attend_{kind}_{tag}_d{D}", (a.tiles * Hkv * a.nsplit, 1, 1), (256, 1, 1), a)]
-    if a.nsplit > ATT_JOIN_WIDE:
+    # a workgroup a row, then a wave, us: 32 rows of 63 splits 14 and 29, 256 of 19
+    # 94 and 99, 1024 of 8 46.3 and 45.7, 8192 of 7 58 and 42
+    if a.nsplit > ATT_JOIN_WIDE and N * Hq < ATT_JOIN_ROWS:
         out.append(Launch("attend", f"nk_attend_join4_{tag}_d{D}", (N * Hq, 1, 1), (256, 1, 1), a))
     elif a.nsplit > 1:
         out.append(Launch("attend", f"nk_attend_join_{tag}_d{D}", (-(-N * Hq // 4), 1, 1), (256, 1, 1), a))
