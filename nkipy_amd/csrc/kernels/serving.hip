@@ -172,8 +172,11 @@ struct SampleArgs {
   const float *topp, *minp;
   uint64_t *tops;        // (rows, nseg): largest key and the complement of its index
   uint64_t *hist;        // (rows, nseg, BINS + 1): weight and count per bin, then the weight in all
+  uint64_t *lists;       // (rows, nseg, SEG_LIST): keys and indices of a segment's largest values
+  uint32_t *counts;      // (rows, nseg): how many, up to 0xffff, and 2^16 (the last whole bin listed + 1)
+  uint16_t *subs;        // (rows, nseg, sub): high halves of the keys of parts' largest values
   int64_t ld;            // elements from row to row
-  int32_t rows, vocab, seg, nseg;  // seg: tokens of a segment
+  int32_t rows, vocab, seg, nseg, sub;  // seg: tokens of a segment; sub: parts of one, at most 64
   float c_temp;
   int32_t c_topk;        // below 1: all
   float c_topp, c_minp;  // 1, 0: all
@@ -185,6 +188,8 @@ struct SampleArgs {
 #define SMP_LIST 8192
 #define SMP_STEPS 1024
 #define SMP_FEW 256
+#define SMP_SEG_LIST 512
+#define SMP_SUBS 1024  // parts of a row at most
 typedef unsigned long long u64;
 
 // order of the values as whole numbers, of 16 bits for the 16-bit types; -0 and
@@ -203,6 +208,8 @@ template <typename T> struct SmpKey {
     __builtin_memcpy(&v, &h, 2);
     return Elt<T>::load(&v, 0);
   }
+  static NK_DEVICE uint32_t high(uint32_t k) { return k; }
+  static NK_DEVICE uint32_t from_high(uint32_t k) { return k; }
 };
 template <> struct SmpKey<float> {
   static NK_DEVICE uint32_t of(float x) {
@@ -210,6 +217,8 @@ template <> struct SmpKey<float> {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
   }
   static NK_DEVICE float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+  static NK_DEVICE uint32_t high(uint32_t k) { return k >> 16; }
+  static NK_DEVICE uint32_t from_high(uint32_t k) { return k << 16; }
 };
 
 struct SmpRow {
@@ -318,16 +327,77 @@ NK_DEVICE u64 smp_sum(u64 v, u64 *red) {
   return v;
 }
 // largest value of a stretch and its lowest index, as one number; 0 where all
-// are NaN or -inf
-template <typename T, int THREADS>
-NK_DEVICE u64 smp_top(const T *x, int lo, int hi, u64 *red) {
+// are NaN or -inf; own(a thread's largest key)
+template <typename T, int THREADS, typename F>
+NK_DEVICE u64 smp_top(const T *x, int lo, int hi, u64 *red, F own) {
   float best = -INFINITY;
   int at = -1;
   smp_each<T, THREADS, 4>(x, lo, hi, [&](int i, float v) {  // (a thread's indices rise)
     if (v > best) best = v, at = i;
   });
   const u64 top = at < 0 ? 0 : (u64)SmpKey<T>::of(best) << 32 | (uint32_t)~at;
+  own((uint32_t)(top >> 32));
   return smp_max<THREADS / 64>(top, red);
+}
+
+// The elements low <= v <= top of a stretch: their indices, those past LIMIT left
+// out, and how many they are.  The two comparisons are all that an element costs.  A
+// wave takes places for a few pieces of all its threads at once, with all reads in
+// flight.
+template <typename T, int THREADS, int LIMIT>
+NK_DEVICE int smp_list(uint32_t *count, uint32_t *idx, const T *x, int lo, int hi, float low, float top) {
+  constexpr int E = 16 / sizeof(T), U = 4;
+  const int lane = threadIdx.x & 63;
+  const int off = (int)(((uintptr_t)(x + lo) & 15) / sizeof(T));
+  __syncthreads();
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  auto fetch = [&](uint4 (&w)[U], int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * THREADS * E;
+      if (i >= lo && i + E <= hi) w[u] = *reinterpret_cast<const uint4 *>(x + i);
+    }
+  };
+  const int first = lo - off + (threadIdx.x - lane) * E;
+  uint4 next[U];
+  fetch(next, first + lane * E);
+  // (every lane of a wave takes part in every round)
+  for (int w0 = first; w0 < hi; w0 += U * THREADS * E) {
+    const int i0 = w0 + lane * E;
+    uint4 w[U];
+    uint32_t in = 0;  // a bit for each of U E elements, the first the highest
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = next[u];
+    fetch(next, i0 + U * THREADS * E);
+    // (the middle of the three is y itself within the bounds, and not for NaN)
+    auto inside = [&](float y) { return __builtin_amdgcn_fmed3f(y, low, top) == y; };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * THREADS * E;
+      if (i >= lo && i + E <= hi) {
+        T v[E];
+        __builtin_memcpy(v, &w[u], 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) in += in + (inside(Elt<T>::load(v, e)) ? 1 : 0);
+      } else {  // the ends, element by element
+#pragma unroll 1
+        for (int e = 0; e < E; ++e)
+          in += in + (i + e >= lo && i + e < hi && inside(Elt<T>::load(x, max(lo, min(i + e, hi - 1)))) ? 1 : 0);
+      }
+    }
+    if (!__any(in != 0)) continue;
+    const uint32_t c = __popc(in), run = smp_running(c);
+    uint32_t at = 0;
+    if (lane == 63) at = atomicAdd(count, run);
+    at = __builtin_amdgcn_readlane(at, 63) + run - c;
+    for (; in; in &= in - 1, ++at) {
+      const int bit = U * E - 1 - __builtin_ctz(in);
+      if (at < LIMIT) idx[at] = i0 + bit / E * THREADS * E + bit % E;
+    }
+  }
+  __syncthreads();
+  return *count;
 }
 
 // Workgroup i runs on XCD i % 8: a row's segments go where the workgroup of its
@@ -344,7 +414,13 @@ __device__ __forceinline__ void sample_top_body(const SampleArgs &a) {
   int r, s;
   smp_place(a, r, s);
   if (r >= a.rows) return;
-  const u64 top = smp_top<T, SMP_SEG_BLOCK>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), red);
+  const u64 top = smp_top<T, SMP_SEG_BLOCK>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), red,
+                                            [&](uint32_t k) {
+    k = SmpKey<T>::high(k);
+    const int lanes = SMP_SEG_BLOCK / max(a.sub, SMP_SEG_BLOCK / 64);  // of a part
+    for (int o = 1; o < lanes; o <<= 1) k = max(k, (uint32_t)__shfl_xor(k, o, 64));
+    if (a.sub && threadIdx.x % lanes == 0) a.subs[((int64_t)r * a.nseg + s) * a.sub + threadIdx.x / lanes] = k;
+  });
   if (threadIdx.x == 0) a.tops[(int64_t)r * a.nseg + s] = top;
 }
 template <int THREADS>
@@ -362,36 +438,110 @@ NK_DEVICE bool smp_settings(const SampleArgs &a, int r, u64 top, SmpRow &row) {
   return top && temp > 0.f;
 }
 
+// The least key's high half that `need` parts of a row reach: as many values are
+// not below it.  A wave's work; the keys in its lanes' registers.
+NK_DEVICE uint32_t smp_reached(const SampleArgs &a, int r, int need) {
+  const int lane = threadIdx.x & 63, n = a.nseg * a.sub;
+  const uint16_t *p = a.subs + (int64_t)r * n;
+  uint32_t k[SMP_SUBS / 64];
+#pragma unroll
+  for (int j = 0; j < SMP_SUBS / 64; ++j) k[j] = j * 64 + lane < n ? p[j * 64 + lane] : 0;
+  uint32_t at = 0;
+#pragma unroll 1
+  for (uint32_t bit = 0x8000; bit; bit >>= 1) {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < SMP_SUBS / 64; ++j) c += __popcll(__ballot(k[j] >= (at | bit)));
+    if (c >= need) at |= bit;
+  }
+  return at;
+}
+// Whether a row's top_k values are listed without a histogram: the parts' largest
+// values bound them from below, closely while k is not near the parts' number.
+NK_DEVICE bool smp_by_parts(const SampleArgs &a, int topk) {
+  return topk > 0 && topk < a.vocab && topk <= a.nseg * a.sub * 3 / 4;
+}
+NK_DEVICE int smp_topk(const SampleArgs &a, int r) { return a.topk ? a.topk[r] : a.c_topk; }
+
+// A segment's histogram to ho (CUTS: some filter is on; else its weight alone)
+template <typename T, int THREADS, bool CUTS>
+NK_DEVICE void smp_segment(u64 (*bins)[4], u64 *red, const T *x, int lo, int hi, const SmpRow &row, uint64_t *ho) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; CUTS && i < SMP_BINS * 4; i += THREADS) bins[i >> 2][i & 3] = 0;
+  __syncthreads();
+  u64 all = 0;
+  smp_each<T, THREADS, 4>(x, lo, hi, [&](int, float v) {
+    const float t = row.depth(v);
+    const SmpWeight w(t);
+    if (!CUTS) all += w.sum();
+    else if (w.hi | w.lo) atomicAdd(&bins[smp_bin(t)][tid & 3], w.counted());
+  });
+  __syncthreads();
+  for (int i = tid; CUTS && i < SMP_BINS; i += THREADS) {
+    const u64 h = bins[i][0] + bins[i][1] + bins[i][2] + bins[i][3];
+    all += h >> 14;
+    ho[i] = h;
+  }
+  all = smp_sum<THREADS / 64>(all, red);
+  if (tid == 0) ho[SMP_BINS] = all;
+}
+
 template <typename T>
 __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
   __shared__ u64 bins[SMP_BINS][4];  // (four of each: lanes of one wave meet less often)
   __shared__ u64 red[SMP_SEG_BLOCK / 64];
+  __shared__ uint32_t idx[SMP_SEG_LIST], count, reach;
   const int tid = threadIdx.x;
   int r, s;
   smp_place(a, r, s);
   if (r >= a.rows) return;
-  for (int i = tid; i < SMP_BINS * 4; i += SMP_SEG_BLOCK) bins[i >> 2][i & 3] = 0;
   SmpRow row;
   if (!smp_settings<T>(a, r, smp_row_top<SMP_SEG_BLOCK>(a, r, red), row)) return;
-  u64 all = 0;
-  const bool cuts = a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f;
-  smp_each<T, SMP_SEG_BLOCK, 4>((const T *)a.x + r * a.ld, s * a.seg, min(a.vocab, (s + 1) * a.seg), [&](int, float v) {
-    const float t = row.depth(v);
-    const SmpWeight w(t);
-    if (!cuts) all += w.sum();
-    else if (w.hi | w.lo) atomicAdd(&bins[smp_bin(t)][tid & 3], w.counted());
-  });
-  uint64_t *ho = a.hist + ((int64_t)r * a.nseg + s) * (SMP_BINS + 1);
-  __syncthreads();
-  if (cuts) {
-    for (int i = tid; i < SMP_BINS; i += SMP_SEG_BLOCK) {
-      const u64 h = bins[i][0] + bins[i][1] + bins[i][2] + bins[i][3];
-      all += h >> 14;
-      ho[i] = h;
+  const T *x = (const T *)a.x + r * a.ld;
+  const int lo = s * a.seg, hi = min(a.vocab, (s + 1) * a.seg), topk = smp_topk(a, r);
+  const int64_t at = (int64_t)r * a.nseg + s;
+  uint64_t *ho = a.hist + at * (SMP_BINS + 1);
+  // what is below this weighs nothing
+  float low = fmaxf(row.best - 38.5f / row.c, -3.40282347e38f);
+  int whole = SMP_BINS;
+  if (smp_by_parts(a, topk)) {
+    if (tid < 64) {
+      const uint32_t k = smp_reached(a, r, topk);
+      if (tid == 0) reach = k;
     }
+    __syncthreads();
+    low = fmaxf(low, SmpKey<T>::value(SmpKey<T>::from_high(reach)));  // (a key past -inf's is NaN)
+  } else if (a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f) {
+    smp_segment<T, SMP_SEG_BLOCK, true>(bins, red, x, lo, hi, row, ho);
+    // the bins that a list holds, down to the middle of the last
+    if (tid == 0) reach = SMP_BINS;
+    auto count_of = [&](int i) { return (uint32_t)(bins[i][0] + bins[i][1] + bins[i][2] + bins[i][3]) & 0x3fff; };
+    const uint32_t c0 = count_of(2 * tid), c = c0 + count_of(2 * tid + 1);
+    uint32_t run = smp_running(c);
+    __syncthreads();
+    if ((tid & 63) == 63) red[tid >> 6] = run;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SMP_SEG_BLOCK / 64; ++i)
+      if (i < tid >> 6) run += (uint32_t)red[i];
+    if (run > SMP_SEG_LIST && run - c <= SMP_SEG_LIST) reach = 2 * tid + (run - c + c0 <= SMP_SEG_LIST);
+    __syncthreads();
+    whole = reach;  // (the first bin that does not fit)
+    if (whole < SMP_BINS) {
+      // a value in the middle of the last bin: not below any of the bins before it
+      low = fmaxf(low, row.best - ((float)whole - 0.5f) / (SMP_RATE * row.c));
+      whole = max(whole - 1, 0);
+      if (!whole) low = INFINITY;
+    }
+  } else {
+    smp_segment<T, SMP_SEG_BLOCK, false>(bins, red, x, lo, hi, row, ho);
+    return;
   }
-  all = smp_sum<SMP_SEG_BLOCK / 64>(all, red);
-  if (tid == 0) ho[SMP_BINS] = all;
+  const int n = smp_list<T, SMP_SEG_BLOCK, SMP_SEG_LIST>(&count, idx, x, lo, hi, low, row.best);
+  for (int i = tid; i < min(n, SMP_SEG_LIST); i += SMP_SEG_BLOCK)
+    a.lists[at * SMP_SEG_LIST + i] = (u64)SmpKey<T>::of(Elt<T>::load(x, idx[i])) << 32 | idx[i];
+  if (tid == 0) a.counts[at] = (uint32_t)whole << 16 | min(n, 0xffff);
 }
 
 struct SmpShared {
@@ -535,64 +685,10 @@ NK_DEVICE uint32_t smp_least(uint32_t out, uint32_t in, uint32_t top, F f) {
 // the largest float below that of a key
 NK_DEVICE float smp_below(uint32_t k) { return SmpKey<float>::value(k == 0x80000000u ? 0x7ffffffeu : k - 1); }
 
-// The elements low <= v <= top of a stretch, into the list (s.n of them, those
-// past LIST left out).  The two comparisons are all that an element costs: one CU
-// reads the row.  A wave takes places for a few pieces of all its threads at
-// once; keys and weights are filled in afterwards, all reads in flight.
+// those of a stretch with low <= v <= top, with keys and weights
 template <typename T>
 NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, float top, const SmpRow &row) {
-  constexpr int E = 16 / sizeof(T), U = 4;
-  const int lane = threadIdx.x & 63;
-  const int off = (int)(((uintptr_t)(x + lo) & 15) / sizeof(T));
-  __syncthreads();
-  if (threadIdx.x == 0) s.n = 0;
-  __syncthreads();
-  auto fetch = [&](uint4 (&w)[U], int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * SMP_BLOCK * E;
-      if (i >= lo && i + E <= hi) w[u] = *reinterpret_cast<const uint4 *>(x + i);
-    }
-  };
-  const int first = lo - off + (threadIdx.x - lane) * E;
-  uint4 next[U];
-  fetch(next, first + lane * E);
-  // (every lane of a wave takes part in every round)
-  for (int w0 = first; w0 < hi; w0 += U * SMP_BLOCK * E) {
-    const int i0 = w0 + lane * E;
-    uint4 w[U];
-    uint32_t in = 0;  // a bit for each of U E elements, the first the highest
-#pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = next[u];
-    fetch(next, i0 + U * SMP_BLOCK * E);
-    // (the middle of the three is y itself within the bounds, and not for NaN)
-    auto inside = [&](float y) { return __builtin_amdgcn_fmed3f(y, low, top) == y; };
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * SMP_BLOCK * E;
-      if (i >= lo && i + E <= hi) {
-        T v[E];
-        __builtin_memcpy(v, &w[u], 16);
-#pragma unroll
-        for (int e = 0; e < E; ++e) in += in + (inside(Elt<T>::load(v, e)) ? 1 : 0);
-      } else {  // the ends, element by element
-#pragma unroll 1
-        for (int e = 0; e < E; ++e)
-          in += in + (i + e >= lo && i + e < hi && inside(Elt<T>::load(x, max(lo, min(i + e, hi - 1)))) ? 1 : 0);
-      }
-    }
-    if (!__any(in != 0)) continue;
-    const uint32_t c = __popc(in), run = smp_running(c);
-    uint32_t at = 0;
-    if (lane == 63) at = atomicAdd(&s.n, run);
-    at = __builtin_amdgcn_readlane(at, 63) + run - c;
-    for (; in; in &= in - 1, ++at) {
-      const int bit = U * E - 1 - __builtin_ctz(in);
-      if (at < SMP_LIST) s.idx[at] = i0 + bit / E * SMP_BLOCK * E + bit % E;
-    }
-  }
-  __syncthreads();
-  const int n = s.n;
+  const int n = smp_list<T, SMP_BLOCK, SMP_LIST>(&s.n, s.idx, x, lo, hi, low, top);
 #pragma unroll
   for (int j = 0; j < SMP_LIST / SMP_BLOCK; ++j) {
     const int i = j * SMP_BLOCK + threadIdx.x;
@@ -615,18 +711,18 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   __shared__ SmpShared s;
   const int tid = threadIdx.x, r = blockIdx.x;
   const T *x = (const T *)a.x + r * a.ld;
-  const u64 top = SMALL ? smp_top<T, SMP_BLOCK>(x, 0, a.vocab, s.red) : smp_row_top<SMP_BLOCK>(a, r, s.red);
+  const u64 top = SMALL ? smp_top<T, SMP_BLOCK>(x, 0, a.vocab, s.red, [](uint32_t) {}) : smp_row_top<SMP_BLOCK>(a, r, s.red);
   SmpRow row;
   if (!smp_settings<T>(a, r, top, row)) {
     if (tid == 0) a.out[r] = top ? (int32_t)~(uint32_t)top : -1;
     return;
   }
-  const int topk = a.topk ? a.topk[r] : a.c_topk;
+  const int topk = smp_topk(a, r);
   const float topp = a.topp ? a.topp[r] : a.c_topp, minp = a.minp ? a.minp[r] : a.c_minp;
   const bool by_k = topk > 0 && topk < a.vocab, by_p = topp < 1.f, by_m = minp > 0.f;
   const float tmin = by_m ? log2f(fminf(minp, 1.f)) : -INFINITY;  // the least depth that min_p keeps
 
-  const uint64_t *hist = a.hist + (int64_t)r * a.nseg * (SMP_BINS + 1);
+  uint64_t *hist = a.hist + (int64_t)r * a.nseg * (SMP_BINS + 1);
   // a value `at` bins below the largest, as a key: near there, and past every
   // value of a bin with a fiftieth of a bin to spare and a key on either side
   auto near = [&](float at) -> uint32_t {
@@ -646,8 +742,56 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   bool whole = SMALL;  // the list holds all that may be kept
   u64 total = 0;       // weight of the row
   int n = 0;
-  if (SMALL) {
-    n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(SMP_BINS - 1)), row.best, row);
+  // The segments' lists, their bins up to `last`, if those are whole and together
+  // up to LIST: a wave for each 64 places, eight reads in flight.
+  auto join = [&](int last) {
+    const uint32_t mine = tid < a.nseg ? a.counts[(int64_t)r * a.nseg + tid] : SMP_BINS << 16;
+    const uint32_t c = mine & 0xffff;
+    if (tid < a.nseg) s.cnt[tid] = c;
+    if (tid == 0) s.n = 0;
+    const bool lost = c > SMP_SEG_LIST || (int)(mine >> 16) <= min(last, SMP_BINS - 1);
+    const u64 all = smp_sum<SMP_BLOCK / 64>((u64)lost << 32 | c, s.red);
+    if (all >> 32 || (last == SMP_BINS && (uint32_t)all > SMP_LIST)) return false;
+    const uint64_t *lists = a.lists + (int64_t)r * a.nseg * SMP_SEG_LIST;
+    const int lane = tid & 63, parts = a.nseg * (SMP_SEG_LIST / 64);
+    for (int q0 = __builtin_amdgcn_readfirstlane(tid >> 6); q0 < parts; q0 += SMP_BLOCK / 8) {
+      u64 e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int q = q0 + j * (SMP_BLOCK / 64), seg = q % a.nseg, i = q / a.nseg * 64 + lane;
+        e[j] = ~0ull;  // (no index is so large)
+        if (q < parts && i < s.cnt[seg]) e[j] = lists[(int64_t)seg * SMP_SEG_LIST + i];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t k = (uint32_t)(e[j] >> 32);
+        const float t = row.depth(SmpKey<T>::value(k));
+        const u64 w = smp_weight(t);
+        const bool in = e[j] != ~0ull && w && smp_bin(t) <= last;
+        const u64 b = __ballot(in);
+        if (!b) continue;
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&s.n, (uint32_t)__popcll(b));
+        at = __builtin_amdgcn_readfirstlane(at) + __popcll(b & ((1ull << lane) - 1));
+        if (in && at < SMP_LIST) s.key[at] = k, s.idx[at] = (uint32_t)e[j], s.w[at] = w;
+      }
+    }
+    __syncthreads();
+    n = min((int)s.n, SMP_LIST);
+    return true;
+  };
+  const bool parts = !SMALL && smp_by_parts(a, topk);
+  if (parts) {
+    whole = join(SMP_BINS);
+    for (int i = 0; !whole && i < a.nseg; ++i)  // (many alike: the histograms after all)
+      smp_segment<T, SMP_BLOCK, true>((u64(*)[4])s.w, s.red, x, i * a.seg, min(a.vocab, (i + 1) * a.seg), row,
+                                      hist + (int64_t)i * (SMP_BINS + 1));
+    __syncthreads();
+  }
+  // (a few listed values are ranked below, and need no bins)
+  const bool ranked = parts && whole && n <= SMP_FEW;
+  if (SMALL) n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(SMP_BINS - 1)), row.best, row);
+  if (whole && !ranked) {
     if (cuts) {
       if (tid < SMP_BINS) s.hcnt[tid] = 0, s.hsum[tid] = 0;
       __syncthreads();
@@ -659,7 +803,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
       }
       total = smp_sum<SMP_BLOCK / 64>(total, s.red);  // (and the histogram is whole)
     }
-  } else if (cuts) {
+  } else if (cuts && !whole) {
     uint32_t c = 0;
     u64 w = 0;
     const int bin = tid % SMP_BINS;
@@ -690,7 +834,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     return min(max((u64)ceil((double)fmaxf(topp, 0.f) * (double)of), (u64)1), of);
   };
   bool k_cuts = by_k, p_cuts = by_p;
-  if (cuts) {
+  if (cuts && !ranked) {
     int last = SMP_BINS - 1;  // bins up to here may be kept
     // the first border's bin; a top_k past the row's weights cuts nothing
     if (by_k) {
@@ -704,8 +848,8 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
       k_cuts = p_cuts = false;
     }
     // everything down to there, where the list can hold it
-    if (!SMALL && smp_sum<SMP_BLOCK / 64>(tid <= last ? s.hcnt[tid % SMP_BINS] : 0, s.red) <= SMP_LIST) {
-      n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(last)), row.best, row);
+    if (!whole && smp_sum<SMP_BLOCK / 64>(tid <= last ? s.hcnt[tid % SMP_BINS] : 0, s.red) <= SMP_LIST) {
+      if (parts || !join(last)) n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(last)), row.best, row);
       whole = true;
     }
   }

@@ -45,8 +45,9 @@ class AttendArgs(ctypes.Structure):
 
 
 class SampleArgs(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp", "tops", "hist")]
-                + [("ld", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("rows", "vocab", "seg", "nseg")]
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp", "tops", "hist",
+                                                 "lists", "counts", "subs")]
+                + [("ld", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("rows", "vocab", "seg", "nseg", "sub")]
                 + [("c_temp", ctypes.c_float), ("c_topk", ctypes.c_int32), ("c_topp", ctypes.c_float),
                    ("c_minp", ctypes.c_float)])
 
@@ -181,7 +182,9 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     return out
 
 
-SMP_LIST, SMP_BINS = 8192, 512  # tokens of a row in one launch, bins of a histogram (serving.hip)
+# tokens of a row in one launch, bins of a histogram, values listed of a segment,
+# parts of a row (serving.hip)
+SMP_LIST, SMP_BINS, SMP_SEG_LIST, SMP_SUBS = 8192, 512, 512, 1024
 
 
 def sample_segments(rows: int, vocab: int) -> Tuple[int, int]:
@@ -195,10 +198,20 @@ def sample_segments(rows: int, vocab: int) -> Tuple[int, int]:
     return seg, -(-vocab // seg)
 
 
+def sample_parts(nseg: int) -> int:
+    """Parts of a segment whose largest values are kept: up to 64, of 4 to 64
+    lanes each, and up to SMP_SUBS in a row; 0 where there are more segments."""
+    sub = 64
+    while sub >= 4 and nseg * sub > SMP_SUBS:
+        sub //= 2
+    return sub if sub >= 4 else 0
+
+
 def sample_workspace_bytes(rows: int, vocab: int) -> int:
     if vocab <= SMP_LIST:
         return 0
-    return 8 * rows * sample_segments(rows, vocab)[1] * (SMP_BINS + 2)
+    nseg = sample_segments(rows, vocab)[1]
+    return rows * nseg * (8 * (SMP_BINS + 2 + SMP_SEG_LIST) + 4 + 2 * sample_parts(nseg))
 
 
 def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_p, ws=0) -> List[Launch]:
@@ -217,7 +230,9 @@ def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_
     n = -(-rows // 8) * 8 * a.nseg
     if n >= 2**31:
         raise LaunchError("sample: too many rows for one launch")
-    _fields(a, tops=ws, hist=ws + 8 * rows * a.nseg)
+    every = rows * a.nseg
+    _fields(a, sub=sample_parts(a.nseg), tops=ws, hist=ws + 8 * every, lists=ws + 8 * every * (SMP_BINS + 2),
+            counts=ws + 8 * every * (SMP_BINS + 2 + SMP_SEG_LIST), subs=ws + every * (8 * (SMP_BINS + 2 + SMP_SEG_LIST) + 4))
     return [Launch("serving", f"nk_sample_top_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_hist_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_pick_{tag}", (rows, 1, 1), (1024, 1, 1), a)]

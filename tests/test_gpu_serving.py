@@ -540,6 +540,89 @@ def test_sample_large_vocabulary():
     check_sample(rng, x, "f32", 1.0)
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("vocab", [8193, 40001, 131080])
+def test_sample_long_rows(t, vocab):
+    """Rows of several segments: few and many kept, past what the segments' lists
+    and the row's hold."""
+    rng = np.random.default_rng(58)
+    x = rng.standard_normal((3 if vocab < 100000 else 1, vocab)) * 3
+    for k in (1, 50, 257, 700, 6000, vocab - 1):
+        check_sample(rng, x, t, 0.8, top_k=k)
+    check_sample(rng, x, t, 0.8, top_k=300, top_p=0.9)
+    check_sample(rng, x, t, 0.8, top_k=300, min_p=0.05)
+    check_sample(rng, x, t, 0.8, min_p=0.01)
+    check_sample(rng, x, t, 0.8, top_k=5000, top_p=0.95, min_p=1e-6)
+    for p in (0.0, 0.3, 0.9, 0.999):
+        check_sample(rng, x, t, 1.0, top_p=p)
+        check_sample(rng, x, t, 6.0, top_p=p)
+    check_sample(rng, x, t, 0.05, top_k=200)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+@pytest.mark.parametrize("top_k,top_p", [(1, None), (5, 0.5), (300, None), (600, 0.613), (None, 0.613), (9000, 0.9)])
+def test_sample_long_ties(t, top_k, top_p):
+    """Whole rows of one value, of few, of two; all large values in one segment."""
+    rng = np.random.default_rng(59)
+    check_sample(rng, np.zeros((2, 20011)), t, 1.0, top_k, top_p)
+    check_sample(rng, np.round(rng.standard_normal((3, 20011)) * 2), t, 1.0, top_k, top_p)
+    check_sample(rng, np.repeat([[1.0, 9.0]], 10001, 1).reshape(1, -1), t, 1.0, top_k, top_p)
+    check_sample(rng, np.linspace(8, -8, 20011).reshape(1, -1), t, 1.0, top_k, top_p)
+    check_sample(rng, np.linspace(-8, 8, 20011).reshape(1, -1), t, 0.1, top_k, top_p)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+def test_sample_long_masked(t):
+    """A few tokens left of a long row, fewer than top_k; infinities and NaN."""
+    rng = np.random.default_rng(60)
+    low = {"bf16": -3.3895314e38, "f16": -65504.0, "f32": np.finfo(np.float32).min}[t]
+    for mask in (-np.inf, low, np.nan):
+        x = np.full((4, 30000), mask, np.float32)
+        for r, m in enumerate((1, 10, 60, 3000)):
+            x[r, rng.permutation(30000)[:m]] = rng.standard_normal(m) * 2
+        for k in (3, 40, 900):
+            check_sample(rng, x, t, top_k=k)
+            check_sample(rng, x, t, top_k=k, top_p=0.8, min_p=0.01)
+        check_sample(rng, x, t, top_p=0.9)
+    x = np.full((4, 30000), -np.inf, np.float32)
+    x[1] = np.nan
+    x[2, [777, 29999]] = np.inf
+    x[3] = low
+    u = np.array([0.3, 0.3, 0.7, 0.5], np.float32)
+    for kw in (dict(top_k=50), dict(top_p=0.9), dict(min_p=0.1)):
+        got = run(f_sample, P.cast(x, t), u, **kw)["output0"]
+        assert list(got[:3]) == [-1, -1, 29999]
+        assert got[3] == {"top_k": 25, "top_p": 13500, "min_p": 15000}[list(kw)[0]]
+
+
+def test_sample_long_rows_of_parameters():
+    rng = np.random.default_rng(62)
+    x = (rng.standard_normal((9, 17001)) * 3).astype(np.float32)
+    temp = np.array([1, 0, 0.5, np.inf, 1, 2, np.nan, 1e-30, 1], np.float32)
+    k = np.array([10, 5, 0, -3, 1, 17002, 7, 9, 500], np.int32)
+    p = np.array([0.9, 0.5, 2.0, 1.0, 0.1, 0.0, 0.3, np.nan, 0.99], np.float32)
+    m = np.array([0.1, 0, -1, 0, 0, 7.0, np.nan, np.nan, 1e-3], np.float32)
+    u = np.full(9, 0.4, np.float32)
+    got = run(f_sample, x, u, temp, k, p, m)["output0"]
+    assert (got == f_sample(x, u, temp, k, p, m)).all()
+    assert got[3] == int(0.4 * 17001)
+
+
+def test_sample_long_strided_rows():
+    """Odd rows that start off any alignment, drawn again and again from one load."""
+    rng = np.random.default_rng(63)
+    x = P.cast(rng.standard_normal((5, 2, 20003)) * 3, "bf16")
+    u = rng.random(5).astype(np.float32)
+    f = lambda x, u: T.sample(x[:, -1, 1:20000], u, top_k=50, top_p=0.9)  # noqa: E731
+    dk, ins, outs = load(f, x, u)
+    want = T.sample(np.ascontiguousarray(x[:, -1, 1:20000]), u, top_k=50, top_p=0.9)
+    for graph in (False, True, False, True):
+        for _ in range(3):
+            dk(ins, outs, sync=False, graph=graph)
+        dk(ins, outs, sync=True, graph=graph)
+        assert (outs["output0"].numpy() == want).all()
+
+
 # ---------------------------------------------------------------------------
 # Together
 # ---------------------------------------------------------------------------
