@@ -172,8 +172,8 @@ struct SampleArgs {
   const float *topp, *minp;
   uint64_t *tops;        // (rows, nseg): largest key and the complement of its index
   uint64_t *hist;        // (rows, nseg, BINS + 1): weight and count per bin, then the weight in all
-  uint64_t *lists;       // (rows, nseg, SEG_LIST): keys and indices of a segment's largest values
-  uint32_t *counts;      // (rows, nseg): how many, up to 0xffff, and 2^16 (the last whole bin listed + 1)
+  uint16_t *order;       // (rows, nseg, seg): a segment's tokens by bin, or a few of the largest
+  uint16_t *places;      // (rows, nseg, BINS + 2): where each bin's begin, and the last one's end; or how many
   uint16_t *subs;        // (rows, nseg, sub): high halves of the keys of parts' largest values
   int64_t ld;            // elements from row to row
   int32_t rows, vocab, seg, nseg, sub;  // seg: tokens of a segment; sub: parts of one, at most 64
@@ -187,7 +187,7 @@ struct SampleArgs {
 #define SMP_BINS 512
 #define SMP_LIST 8192
 #define SMP_STEPS 1024
-#define SMP_FEW 256
+#define SMP_FEW 512
 #define SMP_SEG_LIST 512
 #define SMP_SUBS 1024  // parts of a row at most
 typedef unsigned long long u64;
@@ -463,34 +463,107 @@ NK_DEVICE bool smp_by_parts(const SampleArgs &a, int topk) {
 }
 NK_DEVICE int smp_topk(const SampleArgs &a, int r) { return a.topk ? a.topk[r] : a.c_topk; }
 
-// A segment's histogram to ho (CUTS: some filter is on; else its weight alone)
-template <typename T, int THREADS, bool CUTS>
-NK_DEVICE void smp_segment(u64 (*bins)[4], u64 *red, const T *x, int lo, int hi, const SmpRow &row, uint64_t *ho) {
+// A segment's weights by bin (its histogram) to ho, its tokens in the order of
+// their bins to `order`, where each bin begins to `places`.  The histogram's
+// atomics return a token's place within its bin.
+template <typename T>
+NK_DEVICE void smp_segment(u64 (*bins)[4], uint16_t *ord, u64 *red, const T *x, int n, const SmpRow &row, uint64_t *ho,
+                           uint16_t *order, uint16_t *places) {
+  constexpr int THREADS = SMP_SEG_BLOCK;
+  static_assert(SMP_BINS == 2 * THREADS, "two bins of a thread");
+  constexpr int E = 16 / sizeof(T), U = (SMP_LIST + E + THREADS * E - 1) / (THREADS * E);
   const int tid = threadIdx.x;
   __syncthreads();
-  for (int i = tid; CUTS && i < SMP_BINS * 4; i += THREADS) bins[i >> 2][i & 3] = 0;
+  for (int i = tid; i < SMP_BINS * 4; i += THREADS) bins[i >> 2][i & 3] = 0;
   __syncthreads();
-  u64 all = 0;
-  smp_each<T, THREADS, 4>(x, lo, hi, [&](int, float v) {
-    const float t = row.depth(v);
-    const SmpWeight w(t);
-    if (!CUTS) all += w.sum();
-    else if (w.hi | w.lo) atomicAdd(&bins[smp_bin(t)][tid & 3], w.counted());
-  });
-  __syncthreads();
-  for (int i = tid; CUTS && i < SMP_BINS; i += THREADS) {
-    const u64 h = bins[i][0] + bins[i][1] + bins[i][2] + bins[i][3];
-    all += h >> 14;
-    ho[i] = h;
+  const int off = (int)(((uintptr_t)x & 15) / sizeof(T)), i0 = tid * E - off;  // (as in smp_each)
+  uint4 w[U];
+  uint32_t at[U * E];  // bin and place
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = i0 + u * THREADS * E;
+    if (i >= 0 && i + E <= n) {
+      w[u] = *reinterpret_cast<const uint4 *>(x + i);
+    } else if (i < n) {  // an end: element by element, -inf beyond
+      u64 p[2] = {0, 0};
+#pragma unroll 1
+      for (int e = 0; e < E; ++e) {
+        T v;
+        Elt<T>::store(&v, 0, -INFINITY);
+        if (i + e >= 0 && i + e < n) v = x[i + e];
+        u64 bits = 0;
+        __builtin_memcpy(&bits, &v, sizeof(T));
+        p[0] = p[0] >> (8 * sizeof(T)) | p[1] << (64 - 8 * sizeof(T));
+        p[1] = p[1] >> (8 * sizeof(T)) | bits << (64 - 8 * sizeof(T));
+      }
+      w[u] = make_uint4((uint32_t)p[0], (uint32_t)(p[0] >> 32), (uint32_t)p[1], (uint32_t)(p[1] >> 32));
+    }
   }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    T v[E];
+    __builtin_memcpy(v, &w[u], 16);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float t = row.depth(Elt<T>::load(v, e));
+      const SmpWeight y(t);
+      at[u * E + e] = ~0u;
+      if ((y.hi | y.lo) && i0 + u * THREADS * E < n) {
+        const int bin = smp_bin(t);
+        at[u * E + e] = bin << 16 | ((uint32_t)atomicAdd(&bins[bin][tid & 3], y.counted()) & 0x3fff);
+      }
+    }
+  }
+  __syncthreads();
+  // two bins of a thread: added up, then replaced by where their parts begin
+  u64 all = 0;
+  uint32_t c[8], mine = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    u64 h = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const u64 y = bins[2 * tid + j][q];
+      h += y;
+      c[4 * j + q] = mine;
+      mine += (uint32_t)y & 0x3fff;
+    }
+    all += h >> 14;
+    ho[2 * tid + j] = h;
+  }
+  uint32_t run = smp_running(mine);
   all = smp_sum<THREADS / 64>(all, red);
-  if (tid == 0) ho[SMP_BINS] = all;
+  __syncthreads();
+  if ((tid & 63) == 63) red[tid >> 6] = run;
+  __syncthreads();
+  run -= mine;
+  uint32_t total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) {
+    if (i < tid >> 6) run += (uint32_t)red[i];
+    total += (uint32_t)red[i];
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) bins[2 * tid + (q >> 2)][q & 3] = run + c[q];
+  places[2 * tid] = run, places[2 * tid + 1] = run + c[4];
+  if (tid == 0) ho[SMP_BINS] = all, places[SMP_BINS] = total;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t k = at[u * E + e];
+      if (k != ~0u) ord[(uint32_t)bins[k >> 16][tid & 3] + (k & 0xffff)] = i0 + u * THREADS * E + e;
+    }
+  __syncthreads();
+  for (int i = tid; i < (int)total; i += THREADS) order[i] = ord[i];
 }
 
 template <typename T>
 __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
   __shared__ u64 bins[SMP_BINS][4];  // (four of each: lanes of one wave meet less often)
   __shared__ u64 red[SMP_SEG_BLOCK / 64];
+  __shared__ uint16_t ord[SMP_LIST];
   __shared__ uint32_t idx[SMP_SEG_LIST], count, reach;
   const int tid = threadIdx.x;
   int r, s;
@@ -498,50 +571,31 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
   if (r >= a.rows) return;
   SmpRow row;
   if (!smp_settings<T>(a, r, smp_row_top<SMP_SEG_BLOCK>(a, r, red), row)) return;
-  const T *x = (const T *)a.x + r * a.ld;
-  const int lo = s * a.seg, hi = min(a.vocab, (s + 1) * a.seg), topk = smp_topk(a, r);
+  const int lo = s * a.seg, n = min(a.vocab - lo, a.seg), topk = smp_topk(a, r);
+  const T *x = (const T *)a.x + r * a.ld + lo;
   const int64_t at = (int64_t)r * a.nseg + s;
   uint64_t *ho = a.hist + at * (SMP_BINS + 1);
-  // what is below this weighs nothing
-  float low = fmaxf(row.best - 38.5f / row.c, -3.40282347e38f);
-  int whole = SMP_BINS;
+  uint16_t *order = a.order + at * a.seg, *places = a.places + at * (SMP_BINS + 2);
   if (smp_by_parts(a, topk)) {
     if (tid < 64) {
       const uint32_t k = smp_reached(a, r, topk);
       if (tid == 0) reach = k;
     }
     __syncthreads();
-    low = fmaxf(low, SmpKey<T>::value(SmpKey<T>::from_high(reach)));  // (a key past -inf's is NaN)
+    // (what is 38.5 below weighs nothing; a key past -inf's is a NaN, which fmaxf drops)
+    float low = fmaxf(row.best - 38.5f / row.c, -3.40282347e38f);
+    low = fmaxf(low, SmpKey<T>::value(SmpKey<T>::from_high(reach)));
+    const int c = smp_list<T, SMP_SEG_BLOCK, SMP_SEG_LIST>(&count, idx, x, 0, n, low, row.best);
+    for (int i = tid; i < min(c, SMP_SEG_LIST); i += SMP_SEG_BLOCK) order[i] = idx[i];
+    if (tid == 0) places[0] = c;
   } else if (a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f) {
-    smp_segment<T, SMP_SEG_BLOCK, true>(bins, red, x, lo, hi, row, ho);
-    // the bins that a list holds, down to the middle of the last
-    if (tid == 0) reach = SMP_BINS;
-    auto count_of = [&](int i) { return (uint32_t)(bins[i][0] + bins[i][1] + bins[i][2] + bins[i][3]) & 0x3fff; };
-    const uint32_t c0 = count_of(2 * tid), c = c0 + count_of(2 * tid + 1);
-    uint32_t run = smp_running(c);
-    __syncthreads();
-    if ((tid & 63) == 63) red[tid >> 6] = run;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < SMP_SEG_BLOCK / 64; ++i)
-      if (i < tid >> 6) run += (uint32_t)red[i];
-    if (run > SMP_SEG_LIST && run - c <= SMP_SEG_LIST) reach = 2 * tid + (run - c + c0 <= SMP_SEG_LIST);
-    __syncthreads();
-    whole = reach;  // (the first bin that does not fit)
-    if (whole < SMP_BINS) {
-      // a value in the middle of the last bin: not below any of the bins before it
-      low = fmaxf(low, row.best - ((float)whole - 0.5f) / (SMP_RATE * row.c));
-      whole = max(whole - 1, 0);
-      if (!whole) low = INFINITY;
-    }
+    smp_segment<T>(bins, ord, red, x, n, row, ho, order, places);
   } else {
-    smp_segment<T, SMP_SEG_BLOCK, false>(bins, red, x, lo, hi, row, ho);
-    return;
+    u64 all = 0;
+    smp_each<T, SMP_SEG_BLOCK, 4>(x, 0, n, [&](int, float v) { all += smp_weight(row.depth(v)); });
+    all = smp_sum<SMP_SEG_BLOCK / 64>(all, red);
+    if (tid == 0) ho[SMP_BINS] = all;
   }
-  const int n = smp_list<T, SMP_SEG_BLOCK, SMP_SEG_LIST>(&count, idx, x, lo, hi, low, row.best);
-  for (int i = tid; i < min(n, SMP_SEG_LIST); i += SMP_SEG_BLOCK)
-    a.lists[at * SMP_SEG_LIST + i] = (u64)SmpKey<T>::of(Elt<T>::load(x, idx[i])) << 32 | idx[i];
-  if (tid == 0) a.counts[at] = (uint32_t)whole << 16 | min(n, 0xffff);
 }
 
 struct SmpShared {
@@ -549,6 +603,7 @@ struct SmpShared {
   u64 sum[SMP_STEPS];      // a search's
   uint32_t hcnt[SMP_BINS];
   uint32_t cnt[SMP_STEPS];
+  uint32_t place[SMP_STEPS];
   u64 w[SMP_LIST];         // the list: weights, keys, indices
   uint32_t key[SMP_LIST], idx[SMP_LIST];
   u64 red[SMP_BLOCK / 64], sw[SMP_BLOCK / 64];
@@ -684,7 +739,6 @@ NK_DEVICE uint32_t smp_least(uint32_t out, uint32_t in, uint32_t top, F f) {
 }
 // the largest float below that of a key
 NK_DEVICE float smp_below(uint32_t k) { return SmpKey<float>::value(k == 0x80000000u ? 0x7ffffffeu : k - 1); }
-
 // those of a stretch with low <= v <= top, with keys and weights
 template <typename T>
 NK_DEVICE int smp_gather(SmpShared &s, const T *x, int lo, int hi, float low, float top, const SmpRow &row) {
@@ -722,7 +776,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   const bool by_k = topk > 0 && topk < a.vocab, by_p = topp < 1.f, by_m = minp > 0.f;
   const float tmin = by_m ? log2f(fminf(minp, 1.f)) : -INFINITY;  // the least depth that min_p keeps
 
-  uint64_t *hist = a.hist + (int64_t)r * a.nseg * (SMP_BINS + 1);
+  const uint64_t *hist = a.hist + (int64_t)r * a.nseg * (SMP_BINS + 1);
   // a value `at` bins below the largest, as a key: near there, and past every
   // value of a bin with a fiftieth of a bin to spare and a key on either side
   auto near = [&](float at) -> uint32_t {
@@ -742,68 +796,100 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   bool whole = SMALL;  // the list holds all that may be kept
   u64 total = 0;       // weight of the row
   int n = 0;
-  // The segments' lists, their bins up to `last`, if those are whole and together
-  // up to LIST: a wave for each 64 places, eight reads in flight.
-  auto join = [&](int last) {
-    const uint32_t mine = tid < a.nseg ? a.counts[(int64_t)r * a.nseg + tid] : SMP_BINS << 16;
-    const uint32_t c = mine & 0xffff;
-    if (tid < a.nseg) s.cnt[tid] = c;
-    if (tid == 0) s.n = 0;
-    const bool lost = c > SMP_SEG_LIST || (int)(mine >> 16) <= min(last, SMP_BINS - 1);
-    const u64 all = smp_sum<SMP_BLOCK / 64>((u64)lost << 32 | c, s.red);
-    if (all >> 32 || (last == SMP_BINS && (uint32_t)all > SMP_LIST)) return false;
-    const uint64_t *lists = a.lists + (int64_t)r * a.nseg * SMP_SEG_LIST;
-    const int lane = tid & 63, parts = a.nseg * (SMP_SEG_LIST / 64);
-    for (int q0 = __builtin_amdgcn_readfirstlane(tid >> 6); q0 < parts; q0 += SMP_BLOCK / 8) {
-      u64 e[8];
+  // Into the list: c tokens of segment `tid`, those from place `from` of its order on.
+  auto pull = [&](uint32_t from, uint32_t c) {
+    uint32_t run = smp_running(c);
+    __syncthreads();
+    if ((tid & 63) == 63) s.sc[tid >> 6] = run;
+    __syncthreads();
+    uint32_t all = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int q = q0 + j * (SMP_BLOCK / 64), seg = q % a.nseg, i = q / a.nseg * 64 + lane;
-        e[j] = ~0ull;  // (no index is so large)
-        if (q < parts && i < s.cnt[seg]) e[j] = lists[(int64_t)seg * SMP_SEG_LIST + i];
+    for (int i = 0; i < SMP_BLOCK / 64; ++i) {
+      if (i < tid >> 6) run += s.sc[i];
+      all += s.sc[i];
+    }
+    s.cnt[tid] = run - c;                      // its first place in the list
+    s.place[tid] = from;                       // and that in its order
+    __syncthreads();
+    n = min((int)all, SMP_LIST);
+    constexpr int U = 4;  // reads of a thread in flight
+#pragma unroll 1
+    for (int i0 = tid; i0 < n; i0 += U * SMP_BLOCK) {
+      uint32_t at[U];
+      T v[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * SMP_BLOCK;
+        if (i < n) {
+          int seg = 0;  // the last that begins by i
+          for (int step = SMP_STEPS / 2; step; step >>= 1)
+            if (seg + step < a.nseg && s.cnt[seg + step] <= (uint32_t)i) seg += step;
+          const uint32_t place = s.place[seg] + (i - s.cnt[seg]);
+          at[j] = seg * a.seg + a.order[((int64_t)r * a.nseg + seg) * a.seg + place];
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t k = (uint32_t)(e[j] >> 32);
-        const float t = row.depth(SmpKey<T>::value(k));
-        const u64 w = smp_weight(t);
-        const bool in = e[j] != ~0ull && w && smp_bin(t) <= last;
-        const u64 b = __ballot(in);
-        if (!b) continue;
-        uint32_t at = 0;
-        if (lane == 0) at = atomicAdd(&s.n, (uint32_t)__popcll(b));
-        at = __builtin_amdgcn_readfirstlane(at) + __popcll(b & ((1ull << lane) - 1));
-        if (in && at < SMP_LIST) s.key[at] = k, s.idx[at] = (uint32_t)e[j], s.w[at] = w;
+      for (int j = 0; j < U; ++j)
+        if (i0 + j * SMP_BLOCK < n) v[j] = x[at[j]];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * SMP_BLOCK;
+        if (i < n) {
+          const float f = Elt<T>::load(&v[j], 0);
+          s.key[i] = SmpKey<T>::of(f), s.idx[i] = at[j], s.w[i] = smp_weight(row.depth(f));
+        }
       }
     }
     __syncthreads();
-    n = min((int)s.n, SMP_LIST);
-    return true;
   };
+  const uint16_t *places = a.places + ((int64_t)r * a.nseg + tid) * (SMP_BINS + 2);  // (where tid < nseg)
   const bool parts = !SMALL && smp_by_parts(a, topk);
-  if (parts) {
-    whole = join(SMP_BINS);
-    for (int i = 0; !whole && i < a.nseg; ++i)  // (many alike: the histograms after all)
-      smp_segment<T, SMP_BLOCK, true>((u64(*)[4])s.w, s.red, x, i * a.seg, min(a.vocab, (i + 1) * a.seg), row,
-                                      hist + (int64_t)i * (SMP_BINS + 1));
+  // the tokens of bins b0 .. b1; from the row where its segments have no order
+  auto pull_bins = [&](int b0, int b1) {
+    if (parts) {
+      n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(b1)), b0 ? smp_below(least(b0 - 1)) : row.best, row);
+    } else {
+      const uint32_t from = tid < a.nseg ? places[b0] : 0;
+      pull(from, tid < a.nseg ? places[b1 + 1] - from : 0);
+    }
+  };
+  auto clear_bins = [&]() {
+    if (tid < SMP_BINS) s.hcnt[tid] = 0, s.hsum[tid] = 0;
     __syncthreads();
+  };
+  auto add_bin = [&](float t, u64 w) {
+    const int bin = smp_bin(t);
+    total += w;
+    atomicAdd(&s.hcnt[bin], 1u);
+    atomicAdd(&s.hsum[bin], w);
+  };
+  if (parts) {
+    const uint32_t c = tid < a.nseg ? places[0] : 0;
+    const u64 all = smp_sum<SMP_BLOCK / 64>((u64)(c > SMP_SEG_LIST) << 32 | c, s.red);
+    whole = all <= SMP_LIST;
+    if (whole) {
+      pull(0, c);
+    } else {  // many alike, or one segment has most: the row's histogram after all
+      clear_bins();
+      smp_each<T, SMP_BLOCK, 1>(x, 0, a.vocab, [&](int, float v) {
+        const float t = row.depth(v);
+        const u64 w = smp_weight(t);
+        if (w) add_bin(t, w);
+      });
+      total = smp_sum<SMP_BLOCK / 64>(total, s.red);
+    }
   }
   // (a few listed values are ranked below, and need no bins)
   const bool ranked = parts && whole && n <= SMP_FEW;
   if (SMALL) n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(SMP_BINS - 1)), row.best, row);
   if (whole && !ranked) {
     if (cuts) {
-      if (tid < SMP_BINS) s.hcnt[tid] = 0, s.hsum[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += SMP_BLOCK) {
-        const int bin = smp_bin(row.depth(SmpKey<T>::value(s.key[i])));
-        total += s.w[i];
-        atomicAdd(&s.hcnt[bin], 1u);
-        atomicAdd(&s.hsum[bin], s.w[i]);
-      }
+      clear_bins();
+      for (int i = tid; i < n; i += SMP_BLOCK)
+        if (s.w[i]) add_bin(row.depth(SmpKey<T>::value(s.key[i])), s.w[i]);
       total = smp_sum<SMP_BLOCK / 64>(total, s.red);  // (and the histogram is whole)
     }
-  } else if (cuts && !whole) {
+  } else if (cuts && !whole && !parts) {
     uint32_t c = 0;
     u64 w = 0;
     const int bin = tid % SMP_BINS;
@@ -849,7 +935,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     }
     // everything down to there, where the list can hold it
     if (!whole && smp_sum<SMP_BLOCK / 64>(tid <= last ? s.hcnt[tid % SMP_BINS] : 0, s.red) <= SMP_LIST) {
-      if (parts || !join(last)) n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(last)), row.best, row);
+      pull_bins(0, last);
       whole = true;
     }
   }
@@ -918,8 +1004,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
       if (!whole && edge != held) {
         listing = many <= SMP_LIST;
         held = listing ? edge : -1;
-        if (listing) n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(edge)),
-                                    edge ? smp_below(least(edge - 1)) : row.best, row);
+        if (listing) pull_bins(edge, edge);
       }
       const uint32_t low = near(edge + 1.02f), top = near(edge - 0.02f);
       const uint32_t klo = low ? max(SmpKey<T>::of(SmpKey<float>::value(low)), 1u) - 1 : 0;
@@ -988,22 +1073,22 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   __syncthreads();
   seg[tid] = 0;
   __syncthreads();
-  if (edge == SMP_BINS) {
+  if (edge == SMP_BINS && !parts) {
     for (int i = tid; i < a.nseg; i += SMP_BLOCK) seg[i] = hist[(int64_t)i * (SMP_BINS + 1) + SMP_BINS];
   } else {
-    for (int i = tid >> 6; i < a.nseg; i += SMP_BLOCK / 64) {  // a wave for each
+    for (int i = tid >> 6; !parts && i < a.nseg; i += SMP_BLOCK / 64) {  // a wave for each
       u64 w = 0;
       for (int b = tid & 63; b < edge; b += 64) w += hist[(int64_t)i * (SMP_BINS + 1) + b] >> 14;
 #pragma unroll
       for (int o = 32; o; o >>= 1) w += (u64)__shfl_xor(w, o, 64);
       if ((tid & 63) == 0) atomicAdd(&seg[i], w);
     }
-    if (held == edge) {
+    if (held == edge && !parts) {
       for (int i = tid; i < n; i += SMP_BLOCK) atomicAdd(&seg[s.idx[i] / a.seg], weigh(i));
     } else {
       smp_each<T, SMP_BLOCK, 4>(x, 0, a.vocab, [&](int i, float v) {
         const float t = row.depth(v);
-        if (!(t > -38.f) || smp_bin(t) != edge) return;
+        if (!(t > -38.f) || (!parts && smp_bin(t) != edge)) return;
         const u64 w = smp_weight(t);
         if (w && kept(SmpKey<T>::of(v), i, t)) atomicAdd(&seg[i / a.seg], w);
       });
@@ -1015,8 +1100,12 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   smp_search<false>(s, 0, mine, 0, 0, 0, goal);
   const int at = s.bin;
   const u64 before = s.wb;
-  n = smp_gather(s, x, at * a.seg, min(a.vocab, (at + 1) * a.seg),
-                 bkey ? SmpKey<T>::value(bkey) : SmpKey<float>::value(least(SMP_BINS - 1)), row.best, row);
+  n = min(a.vocab - at * a.seg, a.seg);  // the segment
+  for (int i = tid; i < n; i += SMP_BLOCK) {
+    const float f = Elt<T>::load(x, at * a.seg + i);
+    s.key[i] = SmpKey<T>::of(f), s.idx[i] = at * a.seg + i, s.w[i] = smp_weight(row.depth(f));
+  }
+  __syncthreads();
   draw(goal, before, at * a.seg, min(a.vocab, (at + 1) * a.seg));
 }
 #define NK_SAMPLE(T, name)                                                                          \

@@ -46,7 +46,7 @@ class AttendArgs(ctypes.Structure):
 
 class SampleArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp", "tops", "hist",
-                                                 "lists", "counts", "subs")]
+                                                 "order", "places", "subs")]
                 + [("ld", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("rows", "vocab", "seg", "nseg", "sub")]
                 + [("c_temp", ctypes.c_float), ("c_topk", ctypes.c_int32), ("c_topp", ctypes.c_float),
                    ("c_minp", ctypes.c_float)])
@@ -182,9 +182,8 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     return out
 
 
-# tokens of a row in one launch, bins of a histogram, values listed of a segment,
-# parts of a row (serving.hip)
-SMP_LIST, SMP_BINS, SMP_SEG_LIST, SMP_SUBS = 8192, 512, 512, 1024
+# tokens of a row in one launch, bins of a histogram, parts of a row (serving.hip)
+SMP_LIST, SMP_BINS, SMP_SUBS = 8192, 512, 1024
 
 
 def sample_segments(rows: int, vocab: int) -> Tuple[int, int]:
@@ -210,8 +209,8 @@ def sample_parts(nseg: int) -> int:
 def sample_workspace_bytes(rows: int, vocab: int) -> int:
     if vocab <= SMP_LIST:
         return 0
-    nseg = sample_segments(rows, vocab)[1]
-    return rows * nseg * (8 * (SMP_BINS + 2 + SMP_SEG_LIST) + 4 + 2 * sample_parts(nseg))
+    seg, nseg = sample_segments(rows, vocab)
+    return rows * nseg * (8 * (SMP_BINS + 2) + 2 * (seg + SMP_BINS + 2 + sample_parts(nseg)))
 
 
 def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_p, ws=0) -> List[Launch]:
@@ -231,8 +230,10 @@ def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_
     if n >= 2**31:
         raise LaunchError("sample: too many rows for one launch")
     every = rows * a.nseg
-    _fields(a, sub=sample_parts(a.nseg), tops=ws, hist=ws + 8 * every, lists=ws + 8 * every * (SMP_BINS + 2),
-            counts=ws + 8 * every * (SMP_BINS + 2 + SMP_SEG_LIST), subs=ws + every * (8 * (SMP_BINS + 2 + SMP_SEG_LIST) + 4))
+    order = ws + 8 * every * (SMP_BINS + 2)
+    places = order + 2 * every * a.seg
+    _fields(a, sub=sample_parts(a.nseg), tops=ws, hist=ws + 8 * every, order=order, places=places,
+            subs=places + 2 * every * (SMP_BINS + 2))
     return [Launch("serving", f"nk_sample_top_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_hist_{tag}", (n, 1, 1), (256, 1, 1), a, bytes=nbytes),
             Launch("serving", f"nk_sample_pick_{tag}", (rows, 1, 1), (1024, 1, 1), a)]
