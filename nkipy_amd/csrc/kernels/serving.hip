@@ -141,10 +141,13 @@ NK_APPEND(float, f32)
 //
 // Long rows take three launches, two of them over segments of the row, so that
 // a few rows fill the chip:
-//   top    each segment's largest value;
+//   top    each segment's largest value, and those of its parts, some lanes' each;
 //   hist   each segment's counts and weights over BINS equal steps of t, a bin's
 //          both in one word (14 bits count up to 8192 tokens, 50 the weight), so
-//          that a logit costs one LDS atomic;
+//          that a logit costs one LDS atomic, whose answer is its place among
+//          the tokens in the order of their bins, which are written too.  A row
+//          with top_k takes no histogram: the k-th of its parts' largest values
+//          is not above the k-th value, and the segments list what is not below;
 //   pick   one workgroup per row: the segments' histograms added, the bin in
 //          which the count (top_k) or the weight (top_p) is reached, and the
 //          values that matter listed in LDS: everything down to that bin, if
@@ -158,10 +161,13 @@ NK_APPEND(float, f32)
 // a goal: histograms of 1024 steps of what is left of the keys' range, until a
 // step has up to a wave's elements, which it ranks, or is one key.  The key is
 // the value for a border, the index for ties and for the draw.  A bin of more
-// than LIST values (ties, a narrow spread) is searched in the row itself.
+// than LIST values (ties, a narrow spread) is searched in the row itself, and a
+// top_k row whose lists overflow is read again by pick.
 //
-// Bound by one read of the logits and, in hist, by about 30 instructions per
-// logit; with few rows by the latency of its launches.
+// Bound by the latency of one CU's steps in pick, by about 30 instructions per
+// logit in hist, and by one read of the logits (top, hist, pick in us): 64 rows of
+// 151936 bf16 with every filter 6, 11, 21, by nucleus alone 7, 21, 42; 17 rows of
+// 128257 fp32 by nucleus 5, 12, 33; one row of 32000 with top_k 3, 8, 9.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
   const void *x;
@@ -189,6 +195,9 @@ struct SampleArgs {
 #define SMP_STEPS 1024
 #define SMP_FEW 512
 #define SMP_SEG_LIST 512
+// copies of a bin, so that lanes of one wave meet less often; with four, 33 KB of
+// LDS, one workgroup less fits a CU (64 rows of 151936: 27 us, 21 with two)
+#define SMP_COPIES 2
 #define SMP_SUBS 1024  // parts of a row at most
 typedef unsigned long long u64;
 
@@ -467,14 +476,14 @@ NK_DEVICE int smp_topk(const SampleArgs &a, int r) { return a.topk ? a.topk[r] :
 // their bins to `order`, where each bin begins to `places`.  The histogram's
 // atomics return a token's place within its bin.
 template <typename T>
-NK_DEVICE void smp_segment(u64 (*bins)[4], uint16_t *ord, u64 *red, const T *x, int n, const SmpRow &row, uint64_t *ho,
+NK_DEVICE void smp_segment(u64 (*bins)[SMP_COPIES], uint16_t *ord, u64 *red, const T *x, int n, const SmpRow &row, uint64_t *ho,
                            uint16_t *order, uint16_t *places) {
   constexpr int THREADS = SMP_SEG_BLOCK;
   static_assert(SMP_BINS == 2 * THREADS, "two bins of a thread");
   constexpr int E = 16 / sizeof(T), U = (SMP_LIST + E + THREADS * E - 1) / (THREADS * E);
   const int tid = threadIdx.x;
   __syncthreads();
-  for (int i = tid; i < SMP_BINS * 4; i += THREADS) bins[i >> 2][i & 3] = 0;
+  for (int i = tid; i < SMP_BINS * SMP_COPIES; i += THREADS) (&bins[0][0])[i] = 0;
   __syncthreads();
   const int off = (int)(((uintptr_t)x & 15) / sizeof(T)), i0 = tid * E - off;  // (as in smp_each)
   uint4 w[U];
@@ -510,22 +519,22 @@ NK_DEVICE void smp_segment(u64 (*bins)[4], uint16_t *ord, u64 *red, const T *x, 
       at[u * E + e] = ~0u;
       if ((y.hi | y.lo) && i0 + u * THREADS * E < n) {
         const int bin = smp_bin(t);
-        at[u * E + e] = bin << 16 | ((uint32_t)atomicAdd(&bins[bin][tid & 3], y.counted()) & 0x3fff);
+        at[u * E + e] = bin << 16 | ((uint32_t)atomicAdd(&bins[bin][tid % SMP_COPIES], y.counted()) & 0x3fff);
       }
     }
   }
   __syncthreads();
   // two bins of a thread: added up, then replaced by where their parts begin
   u64 all = 0;
-  uint32_t c[8], mine = 0;
+  uint32_t c[2 * SMP_COPIES], mine = 0;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     u64 h = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < SMP_COPIES; ++q) {
       const u64 y = bins[2 * tid + j][q];
       h += y;
-      c[4 * j + q] = mine;
+      c[SMP_COPIES * j + q] = mine;
       mine += (uint32_t)y & 0x3fff;
     }
     all += h >> 14;
@@ -544,8 +553,8 @@ NK_DEVICE void smp_segment(u64 (*bins)[4], uint16_t *ord, u64 *red, const T *x, 
     total += (uint32_t)red[i];
   }
 #pragma unroll
-  for (int q = 0; q < 8; ++q) bins[2 * tid + (q >> 2)][q & 3] = run + c[q];
-  places[2 * tid] = run, places[2 * tid + 1] = run + c[4];
+  for (int q = 0; q < 2 * SMP_COPIES; ++q) bins[2 * tid + q / SMP_COPIES][q % SMP_COPIES] = run + c[q];
+  places[2 * tid] = run, places[2 * tid + 1] = run + c[SMP_COPIES];
   if (tid == 0) ho[SMP_BINS] = all, places[SMP_BINS] = total;
   __syncthreads();
 #pragma unroll
@@ -553,7 +562,7 @@ NK_DEVICE void smp_segment(u64 (*bins)[4], uint16_t *ord, u64 *red, const T *x, 
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const uint32_t k = at[u * E + e];
-      if (k != ~0u) ord[(uint32_t)bins[k >> 16][tid & 3] + (k & 0xffff)] = i0 + u * THREADS * E + e;
+      if (k != ~0u) ord[(uint32_t)bins[k >> 16][tid % SMP_COPIES] + (k & 0xffff)] = i0 + u * THREADS * E + e;
     }
   __syncthreads();
   for (int i = tid; i < (int)total; i += THREADS) order[i] = ord[i];
@@ -561,10 +570,10 @@ NK_DEVICE void smp_segment(u64 (*bins)[4], uint16_t *ord, u64 *red, const T *x, 
 
 template <typename T>
 __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
-  __shared__ u64 bins[SMP_BINS][4];  // (four of each: lanes of one wave meet less often)
+  __shared__ u64 bins[SMP_BINS][SMP_COPIES];
   __shared__ u64 red[SMP_SEG_BLOCK / 64];
   __shared__ uint16_t ord[SMP_LIST];
-  __shared__ uint32_t idx[SMP_SEG_LIST], count, reach;
+  __shared__ uint32_t count, reach;
   const int tid = threadIdx.x;
   int r, s;
   smp_place(a, r, s);
@@ -585,8 +594,8 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
     // (what is 38.5 below weighs nothing; a key past -inf's is a NaN, which fmaxf drops)
     float low = fmaxf(row.best - 38.5f / row.c, -3.40282347e38f);
     low = fmaxf(low, SmpKey<T>::value(SmpKey<T>::from_high(reach)));
-    const int c = smp_list<T, SMP_SEG_BLOCK, SMP_SEG_LIST>(&count, idx, x, 0, n, low, row.best);
-    for (int i = tid; i < min(c, SMP_SEG_LIST); i += SMP_SEG_BLOCK) order[i] = idx[i];
+    const int c = smp_list<T, SMP_SEG_BLOCK, SMP_SEG_LIST>(&count, (uint32_t *)bins, x, 0, n, low, row.best);
+    for (int i = tid; i < min(c, SMP_SEG_LIST); i += SMP_SEG_BLOCK) order[i] = ((uint32_t *)bins)[i];
     if (tid == 0) places[0] = c;
   } else if (a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f) {
     smp_segment<T>(bins, ord, red, x, n, row, ho, order, places);
