@@ -10,9 +10,13 @@ runtime tensor), GQA by ``np.repeat``, scores over the whole cache
 rounded to bf16, the causal mask row(s) of the current positions (-1e5 above
 the diagonal), softmax, weighted values and the output projection.
 
+``qwen3_paged_attention_kernel`` is the same layer for a batch of sequences
+of their own lengths, packed without padding, over a paged cache: prompts,
+pieces of prompts and single tokens alike.
+
 ``greedy_sampling`` follows kernels/sampling.py:113-148 on one device: the
 final RMSNorm, logits of the last position and the index of the largest
-logit by ``topk(k=1)``.
+logit by ``topk(k=1)``.  ``sampling`` draws from the same logits instead.
 """
 
 import numpy as np
@@ -83,6 +87,30 @@ def qwen3_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, norm_eps
     return np.matmul(out, o_weight)
 
 
+def qwen3_paged_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, norm_eps, n_heads, head_dim, n_kv_heads,
+                                 key_cache, value_cache, block_tables, context_lens, query_starts, o_weight,
+                                 rope_base=1000000, window=None, sinks=0):
+    """x (tokens, hidden), the new tokens of all sequences one after another ->
+    (tokens, hidden); key_cache / value_cache (pages, page_size, n_kv_heads,
+    head_dim) take their keys and values in place.  Sequence b's tokens are
+    query_starts[b] .. query_starts[b + 1] - 1, the last of its
+    context_lens[b] (``query_starts=None``: one token each), on the pages of
+    block_tables[b]; a window with its sinks narrows what each sees."""
+    n = x.shape[0]
+    q_end = n_heads * head_dim
+    k_end = q_end + n_kv_heads * head_dim
+    xq, xk, xv = np.split(np.matmul(x, qkv_weight), [q_end, k_end], axis=1)
+    xq = rmsnorm_kernel(xq.reshape(n, n_heads, head_dim), q_norm_weight, norm_eps)
+    xk = rmsnorm_kernel(xk.reshape(n, n_kv_heads, head_dim), k_norm_weight, norm_eps)
+    xv = xv.reshape(n, n_kv_heads, head_dim)
+    cos, sin = compute_cos_sin_cache(head_dim, block_tables.shape[1] * key_cache.shape[1], base=rope_base)
+    xq = tensor_apis.rotary_append(xq, xk, xv, tensor_apis.constant(cos), tensor_apis.constant(sin), key_cache, value_cache,
+                                   block_tables, context_lens, query_starts)
+    out = tensor_apis.paged_attention(xq, key_cache, value_cache, block_tables, context_lens, query_starts,
+                                      window=window, sinks=sinks)
+    return np.matmul(out.reshape(n, q_end), o_weight)
+
+
 def cached_attention(xq, cache_k, cache_v, start_pos=None):
     """Attention of the queries xq (B, S, Hq, D) over the whole KV cache
     (B, MAXS, Hkv, D), as examples/models/qwen3/kernels/attention.py:107-143
@@ -121,3 +149,12 @@ def greedy_sampling(h, norm_weight, lm_head_weight, norm_eps):
     logits = h[:, -1, :] @ lm_head_weight
     _, next_id = tensor_apis.topk(logits, k=1, axis=1)
     return next_id
+
+
+def sampling(h, norm_weight, lm_head_weight, norm_eps, uniform, temperature=1.0, top_k=None, top_p=None, min_p=None):
+    """A token drawn for the last position of each row, by one uniform number
+    each: (B, S, H) -> (B,) int32.  Temperature and filters as
+    ``tensor_apis.sample`` takes them."""
+    h = rmsnorm_kernel(h, norm_weight, norm_eps)
+    logits = h[:, -1, :] @ lm_head_weight
+    return tensor_apis.sample(logits, uniform, temperature, top_k, top_p, min_p)
