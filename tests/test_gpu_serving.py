@@ -262,6 +262,25 @@ def test_paged_far_pages():
             assert (raw[0] == x[b].view(np.uint16)).all()
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(40, 2, 64), (17, 1, 128), (160, 1, 64), (256, 2, 128)])
+@pytest.mark.parametrize("new", [None, [1, 9, 2]])
+def test_paged_large_groups(hq, hkv, d, new):
+    """More heads of a group than a step's workgroup takes, and than a tile has rows."""
+    rng = np.random.default_rng(24)
+    check_paged(rng, "bf16", hq, hkv, d, 16, [70, 9, 300], new, 0, 0)
+    check_paged(rng, "f16", hq, hkv, d, 16, [70, 9, 300], new, 33, 2)
+
+
+@pytest.mark.parametrize("seqs,hq,hkv,length", [(1, 4, 2, 9000), (40, 32, 1, 2100), (3, 8, 1, 6000)])
+def test_paged_split_keys(seqs, hq, hkv, length):
+    """Splits joined by a workgroup for each row, and by a wave where rows are many;
+    short sequences beside the long one, which have no part in most splits."""
+    rng = np.random.default_rng(25)
+    lens = [length] + [int(x) for x in rng.integers(0, 400, seqs - 1)]
+    check_paged(rng, "bf16", hq, hkv, 64, 32, lens, None, 0, 0)
+    check_paged(rng, "bf16", hq, hkv, 64, 32, lens, [min(9, x) for x in lens], 0, 0)
+
+
 def test_paged_unordered_starts_stay_inside():
     """Starts and lengths that make no sense read and write nothing outside
     the tensors (the results are of no use)."""
@@ -336,6 +355,47 @@ def test_window_spoiled_keys_unseen():
     want = P.dense(q, k, v, lengths, None, 64, 0, "f16")
     k[1, 77:], v[1, 77:] = np.float16(np.nan), np.float16(np.inf)
     close(run(f_window, q, k, v, lengths, window=64)["output0"], *want)
+
+
+@pytest.mark.parametrize("t,d", [("bf16", 64), ("f16", 128), ("bf16", 128)])
+def test_window_single_tokens(t, d):
+    """One query of each sequence over plain keys of their own lengths."""
+    rng = np.random.default_rng(36)
+    q, k, v = (draw(rng, (4, s, h, d), t) for s, h in ((1, 6), (777, 2), (777, 2)))
+    lengths, positions = np.array([777, 0, 300, 5], np.int32), np.array([776, 3, 299, 900], np.int32)
+    for a, b in ((None, None), (lengths, positions), (None, positions), (lengths, None)):
+        for window, sinks in ((0, 0), (130, 7)):
+            got = run(f_window, q, k, v, a, b, window=window or None, sinks=sinks)["output0"]
+            close(got, *P.dense(q, k, v, a, None if b is None else b.astype(np.int64), window, sinks, t))
+
+
+@pytest.mark.parametrize("S", [1, 50])
+def test_window_broadcast_keys(S):
+    """Keys and values that all sequences share, and one row that is every key."""
+    rng = np.random.default_rng(37)
+    q, k, v, one = (draw(rng, (b, s, h, 64), "bf16") for b, s, h in ((3, S, 4), (1, 90, 2), (1, 90, 2), (1, 1, 2)))
+    f = lambda q, k, v: T.window_attention(q, np.broadcast_to(k, (3, 90, 2, 64)), np.broadcast_to(v, (3, 90, 2, 64)))  # noqa: E731
+    for a in (k, one):
+        keys, vals = (np.ascontiguousarray(np.broadcast_to(x, (3, 90, 2, 64))) for x in (a, v))
+        close(run(f, q, a, v)["output0"], *P.dense(q, keys, vals, None, None, 0, 0, "bf16"))
+        close(run(f, q, v, a)["output0"], *P.dense(q, vals, keys, None, None, 0, 0, "bf16"))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_window_far_rows(d):
+    """Keys 16 MB apart, so that the last lie past 2^32 bytes."""
+    rng = np.random.default_rng(38)
+    wide = 2**23 // d
+    kd, vd = (DeviceTensor.empty((1, 300, wide, d), dt.bfloat16, name=n) for n in ("k", "v"))
+    k, v = draw(rng, (1, 300, 2, d), "bf16"), draw(rng, (1, 300, 2, d), "bf16")
+    for x, dev in ((k, kd), (v, vd)):
+        for j in range(300):
+            raw = np.ascontiguousarray(x[0, j].view(np.uint16))
+            dev.tensor_ref.write(raw.ctypes.data, raw.nbytes, j * 2**24)
+    f = lambda q, k, v: T.window_attention(q, k[:, :, :2], v[:, :, :2], window=200, sinks=3)  # noqa: E731
+    for S in (1, 280):
+        q = draw(rng, (1, S, 4, d), "bf16")
+        close(run(f, q, kd, vd)["output0"], *P.dense(q, k, v, None, None, 200, 3, "bf16"))
 
 
 # ---------------------------------------------------------------------------
@@ -635,6 +695,39 @@ def _step(heads, kv):
         return o, logits, T.sample(logits, u, temperature=0.9, top_k=20, top_p=0.95), q
 
     return step
+
+
+def test_calls_queued_by_turns():
+    """Kernels with workspaces of their own, queued by turns without a wait, eager and
+    replayed."""
+    rng = np.random.default_rng(64)
+    tables, lens, _, pages = P.batch(rng, [5000, 40], None, 16)
+    kc, vc = draw(rng, (pages, 16, 2, 64), "bf16"), draw(rng, (pages, 16, 2, 64), "bf16")
+    x = P.cast(rng.standard_normal((2, 30000)) * 3, "f32")
+    work = []
+    for i in range(3):
+        q, u = draw(rng, (2, 4, 64), "bf16"), rng.random(2).astype(np.float32)
+        f = lambda q, kc, vc, tables, lens: T.paged_attention(q, kc, vc, tables, lens)  # noqa: E731
+        work.append((load(f, q, kc, vc, tables, lens), None if i else P.paged(q, kc, vc, tables, lens, None, 0, 0, "bf16")))
+        f = lambda x, u: T.sample(x, u, 0.9, 100, 0.9)  # noqa: E731
+        work.append((load(f, x, u), T.sample(x, u, 0.9, 100, 0.9)))
+    alone = []
+    for (dk, ins, outs), _ in work:
+        dk(ins, outs)
+        alone.append(outs["output0"].numpy())
+    for graph in (False, True, True):
+        for turn in range(4):
+            for (dk, ins, outs), _ in work:
+                dk(ins, outs, sync=False, graph=graph)
+        for (dk, ins, outs), _ in work:
+            dk(ins, outs, sync=True, graph=graph)
+        for (call, want), first in zip(work, alone):
+            got = call[2]["output0"].numpy()
+            assert (got == first).all()
+            if isinstance(want, tuple):
+                close(got, *want)
+            elif want is not None:
+                assert (got == want).all()
 
 
 def test_serving_step_together():
