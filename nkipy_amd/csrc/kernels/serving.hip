@@ -15,7 +15,8 @@ using namespace nk;
 // p % page of page tables[b][p / page].  Bound by memory: every element is
 // read and written once.  One workgroup per token: its sequence, position and
 // page are found once and its heads share the tables' row.  A thread moves E
-// elements of each half of a pair (16 bytes with E = 8).
+// elements of each half of a pair (16 bytes with E = 8).  8000 tokens of 32 / 8
+// heads of 128, bf16: 40 us, 4.9 TB/s.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   const void *q, *k, *v;
