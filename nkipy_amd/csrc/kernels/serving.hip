@@ -807,7 +807,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   u64 total = 0;       // weight of the row
   int n = 0;
   // Into the list: c tokens of segment `tid`, those from place `from` of its order on.
-  auto pull = [&](uint32_t from, uint32_t c) {
+  auto pull = [&](uint32_t from, uint32_t c) __attribute__((always_inline)) {
     uint32_t run = smp_running(c);
     __syncthreads();
     if ((tid & 63) == 63) s.sc[tid >> 6] = run;
@@ -822,32 +822,30 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     s.place[tid] = from;                       // and that in its order
     __syncthreads();
     n = min((int)all, SMP_LIST);
-    constexpr int U = 4;  // reads of a thread in flight
+    constexpr int U = SMP_LIST / SMP_BLOCK;  // all reads in flight
+    uint32_t at[U];
+    T v[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = j * SMP_BLOCK + tid;
+      if (i < n) {
+        int seg = 0;  // the last that begins by i
 #pragma unroll 1
-    for (int i0 = tid; i0 < n; i0 += U * SMP_BLOCK) {
-      uint32_t at[U];
-      T v[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = i0 + j * SMP_BLOCK;
-        if (i < n) {
-          int seg = 0;  // the last that begins by i
-          for (int step = SMP_STEPS / 2; step; step >>= 1)
-            if (seg + step < a.nseg && s.cnt[seg + step] <= (uint32_t)i) seg += step;
-          const uint32_t place = s.place[seg] + (i - s.cnt[seg]);
-          at[j] = seg * a.seg + a.order[((int64_t)r * a.nseg + seg) * a.seg + place];
-        }
+        for (int step = SMP_STEPS / 2; step; step >>= 1)
+          if (seg + step < a.nseg && s.cnt[seg + step] <= (uint32_t)i) seg += step;
+        const uint32_t place = s.place[seg] + (i - s.cnt[seg]);
+        at[j] = seg * a.seg + a.order[((int64_t)r * a.nseg + seg) * a.seg + place];
       }
+    }
 #pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (i0 + j * SMP_BLOCK < n) v[j] = x[at[j]];
+    for (int j = 0; j < U; ++j)
+      if (j * SMP_BLOCK + tid < n) v[j] = x[at[j]];
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = i0 + j * SMP_BLOCK;
-        if (i < n) {
-          const float f = Elt<T>::load(&v[j], 0);
-          s.key[i] = SmpKey<T>::of(f), s.idx[i] = at[j], s.w[i] = smp_weight(row.depth(f));
-        }
+    for (int j = 0; j < U; ++j) {
+      const int i = j * SMP_BLOCK + tid;
+      if (i < n) {
+        const float f = Elt<T>::load(&v[j], 0);
+        s.key[i] = SmpKey<T>::of(f), s.idx[i] = at[j], s.w[i] = smp_weight(row.depth(f));
       }
     }
     __syncthreads();
@@ -855,7 +853,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   const uint16_t *places = a.places + ((int64_t)r * a.nseg + tid) * (SMP_BINS + 2);  // (where tid < nseg)
   const bool parts = !SMALL && smp_by_parts(a, topk);
   // the tokens of bins b0 .. b1; from the row where its segments have no order
-  auto pull_bins = [&](int b0, int b1) {
+  auto pull_bins = [&](int b0, int b1) __attribute__((always_inline)) {
     if (parts) {
       n = smp_gather(s, x, 0, a.vocab, SmpKey<float>::value(least(b1)), b0 ? smp_below(least(b0 - 1)) : row.best, row);
     } else {
@@ -959,16 +957,21 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
 
   // A few values: ranked against each other, everything else is in their order.
   if (whole && n <= SMP_FEW) {
-    const bool in = tid < n;
-    const u64 mine = in ? (u64)s.key[tid] << 32 | (uint32_t)~s.idx[tid] : 0;
-    if (in) s.sum[tid] = mine;
+    static_assert(SMP_BLOCK == 2 * SMP_FEW, "two threads a value");
+    const int e = tid >> 1, half = tid & 1;  // each half of the others
+    const u64 mine = e < n ? (u64)s.key[e] << 32 | (uint32_t)~s.idx[e] : 0;
+    if (e < n) s.sum[e] = mine;
     __syncthreads();
     uint32_t rank = 0;
-    if (in)
-      for (int j = 0; j < n; ++j) rank += s.sum[j] > mine;
+    if (e < n) {
+#pragma unroll 8
+      for (int j = half; j < n; j += 2) rank += s.sum[j] > mine;
+    }
+    rank += __shfl_xor(rank, 1, 64);
     __syncthreads();
-    if (in) s.sum[rank] = mine;
+    if (e < n && !half) s.sum[rank] = mine;
     __syncthreads();
+    const bool in = tid < n;
     const u64 it = in ? s.sum[tid] : 0;
     const float t = in ? row.depth(SmpKey<T>::value((uint32_t)(it >> 32))) : 0.f;
     const u64 w = in ? smp_weight(t) : 0;
@@ -990,10 +993,13 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     __syncthreads();
     if (in) s.hsum[tid] = w;
     __syncthreads();
-    if (tid < keep) {
+    if (e < keep) {
+      const uint32_t at = (uint32_t)s.sum[e];
       u64 upto = 0;  // the weight of indices up to this one's (complements order them backwards)
-      for (int j = 0; j < keep; ++j) upto += (uint32_t)s.sum[j] >= (uint32_t)it ? s.hsum[j] : 0;
-      if (upto >= goal && upto - w < goal) a.out[r] = ~(uint32_t)it;
+#pragma unroll 8
+      for (int j = half; j < keep; j += 2) upto += (uint32_t)s.sum[j] >= at ? s.hsum[j] : 0;
+      upto += (u64)__shfl_xor(upto, 1, 64);
+      if (!half && upto >= goal && upto - s.hsum[e] < goal) a.out[r] = ~at;
     }
     return;
   }
