@@ -823,18 +823,26 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     __syncthreads();
     n = min((int)all, SMP_LIST);
     constexpr int U = SMP_LIST / SMP_BLOCK;  // all reads in flight
-    uint32_t at[U];
+    uint32_t at[U];  // a segment, the last that begins by this place; then the token
     T v[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) at[j] = 0;
+#pragma unroll 1
+    for (int step = SMP_STEPS / 2; step; step >>= 1) {
+      if (step >= a.nseg) continue;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (j * SMP_BLOCK >= n) continue;
+        const int to = min((int)at[j] + step, a.nseg - 1);  // (past the last segment: the last)
+        if (s.cnt[to] <= (uint32_t)(j * SMP_BLOCK + tid)) at[j] = to;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int i = j * SMP_BLOCK + tid;
       if (i < n) {
-        int seg = 0;  // the last that begins by i
-#pragma unroll 1
-        for (int step = SMP_STEPS / 2; step; step >>= 1)
-          if (seg + step < a.nseg && s.cnt[seg + step] <= (uint32_t)i) seg += step;
-        const uint32_t place = s.place[seg] + (i - s.cnt[seg]);
-        at[j] = seg * a.seg + a.order[((int64_t)r * a.nseg + seg) * a.seg + place];
+        const uint32_t place = s.place[at[j]] + (i - s.cnt[at[j]]);
+        at[j] = at[j] * a.seg + a.order[((int64_t)r * a.nseg + at[j]) * a.seg + place];
       }
     }
 #pragma unroll
