@@ -355,13 +355,22 @@ class AppendPattern:
                 group = []
 
     @staticmethod
-    def _key(n: Node):
-        k = 1 + n.attrs["starts"]
-        return tuple(v.id for v in n.inputs[-k:])  # lengths, starts
+    def _shared(n: Node):
+        """What the parts of one launch have in common, by name."""
+        where = n.inputs[-(1 + n.attrs["starts"]):]
+        rows = n.inputs[0 if n.op == "rotate_rows" else 1]
+        out = {"where": [v.id for v in where], "rows": (rows.shape[0], rows.shape[2], rows.dtype)}
+        if n.op == "rotate_rows" or n.attrs["rotary"]:
+            at = 1 if n.op == "rotate_rows" else 2
+            out["turn"] = [v.id for v in n.inputs[at:at + 2]]
+        if n.op == "paged_write":
+            out["cache"] = (n.inputs[0].shape, n.inputs[4 if n.attrs["rotary"] else 2].id)
+        return out
 
     def _joins(self, group, n):
         kind = lambda m: (m.op, m.attrs.get("rotary"))  # noqa: E731
-        return self._key(n) == self._key(group[0]) and all(kind(m) != kind(n) for m in group)
+        mine = self._shared(n)
+        return all(kind(m) != kind(n) and all(mine.get(x, y) == y for x, y in self._shared(m).items()) for m in group)
 
     @staticmethod
     def _claim(L, group):

@@ -244,3 +244,19 @@ def test_empty_batches_launch_nothing():
                      i(2, 2), i(2), i(3)).steps
     assert T.paged_attention(f(0, 2, 8), f(3, 4, 2, 8), f(3, 4, 2, 8), i(2, 2), i(2), i(3)).shape == (0, 2, 8)
     assert T.sample(f(0, 9), f(0)).shape == (0,)
+
+
+def test_two_appends_keep_their_own_tables():
+    """A call whose rotated q nobody reads, then one with other tables: the second's
+    q is not turned by the first's."""
+
+    def two(q, k, v, cos, sin, cos2, sin2, kc, vc, kc2, vc2, tables, lens):
+        T.rotary_append(q, k, v, cos, sin, kc, vc, tables, lens)
+        return T.rotary_append(q, k, v, cos2, sin2, kc2, vc2, tables, lens)
+
+    f = lambda *s: np.zeros(s, np.float32)  # noqa: E731
+    i = lambda *s: np.zeros(s, np.int32)  # noqa: E731
+    p = _plan(two, f(2, 2, 8), f(2, 2, 8), f(2, 2, 8), f(5, 4), f(5, 4), f(5, 2), f(5, 2), f(3, 2, 2, 8), f(3, 2, 2, 8),
+              f(4, 2, 2, 8), f(4, 2, 2, 8), i(2, 2), i(2))
+    assert p.kernel_kinds == ["rotary_append", "rotary_append"]
+    assert [sorted(s.desc.split(": ")[1].split(", ")) for s in p.steps] == [["k", "v"], ["k", "q", "v"]]
