@@ -357,6 +357,15 @@ def test_window_spoiled_keys_unseen():
     close(run(f_window, q, k, v, lengths, window=64)["output0"], *want)
 
 
+@pytest.mark.parametrize("t,d", [("bf16", 64), ("f16", 128), ("f32", 32)])
+def test_window_without_keys(t, d):
+    rng = np.random.default_rng(39)
+    for S in (1, 5, 200):
+        f = lambda q, k, v: T.window_attention(q, k[:, 3:3], v[:, 3:3])  # noqa: E731
+        q, k = draw(rng, (2, S, 4, d), t), draw(rng, (2, 7, 2, d), t)
+        assert (P.up(run(f, q, k, k)["output0"]) == 0).all()
+
+
 @pytest.mark.parametrize("t,d", [("bf16", 64), ("f16", 128), ("bf16", 128)])
 def test_window_single_tokens(t, d):
     """One query of each sequence over plain keys of their own lengths."""
@@ -442,6 +451,48 @@ def test_append_dropped_tokens():
     got = run(f_append, q, k, v, cos, sin, kc, vc, tables, lens, starts)
     for name, w, e in zip(("output0", "kc", "vc"), want, tol):
         close(got[name], w, e)
+
+
+def test_append_twice():
+    """Two calls of one kernel, other tables for the second: into caches of their
+    own, and into the same ones."""
+    rng = np.random.default_rng(46)
+    t, n = "f32", 6
+    tables, lens, starts, pages = P.batch(rng, [9, 30], [2, 4], 8)
+    x = [draw(rng, (n, h, 64), t) for h in (4, 2, 2, 4, 2, 2)]
+    ang = [np.outer(np.arange(40), b ** np.arange(m)).astype(np.float32) for b, m in ((0.6, 32), (0.3, 16))]
+    trig = [f(a) for a in ang for f in (np.cos, np.sin)]
+    caches = [draw(rng, (pages, 8, 2, 64), t) for _ in range(4)]
+
+    def apart(q, k, v, q2, k2, v2, cos, sin, cos2, sin2, kc, vc, kc2, vc2, tables, lens, starts):
+        T.rotary_append(q, k, v, cos, sin, kc, vc, tables, lens, starts)
+        return T.rotary_append(q2, k2, v2, cos2, sin2, kc2, vc2, tables, lens, starts)
+
+    got = run(apart, *x, *trig, *caches, tables, lens, starts)
+    one = P.append(*x[:3], *trig[:2], *caches[:2], tables, lens, starts, t)
+    two = P.append(*x[3:], *trig[2:], *caches[2:], tables, lens, starts, t)
+    for g, w, e in zip((got[k] for k in ("output0", "kc", "vc", "kc2", "vc2")), (two[0][0], *one[0][1:], *two[0][1:]),
+                       (two[1][0], *one[1][1:], *two[1][1:])):
+        close(g, w, e)
+
+    def same(q, k, v, q2, k2, v2, cos, sin, cos2, sin2, kc, vc, tables, lens, later, starts):
+        a = T.rotary_append(q, k, v, cos, sin, kc, vc, tables, lens, starts)
+        old = kc + 0.0
+        return a, T.rotary_append(q2, k2, v2, cos2, sin2, kc, vc, tables, later, starts), old
+
+    later = lens + np.array([2, 1], np.int32)  # (the second over part of the first's rows)
+    wide = P.batch(rng, [11, 31], [2, 4], 8)[0]
+    tables = np.arange(wide.size, dtype=np.int32).reshape(wide.shape)
+    caches = [draw(rng, (wide.size, 8, 2, 64), t) for _ in range(2)]
+    got = run(same, *x, *trig, *caches, tables, lens, later, starts)
+    one = P.append(*x[:3], *trig[:2], *caches, tables, lens, starts, t)
+    mid = [P.cast(a, t) for a in one[0][1:]]
+    two = P.append(*x[3:], *trig[2:], *mid, tables, later, starts, t)
+    for name, w, e in (("output0", one[0][0], one[1][0]), ("output1", two[0][0], two[1][0]), ("output2", one[0][1], one[1][1])):
+        close(got[name], w, e)
+    # (rows of the first call that stay are rounded already)
+    close(got["kc"], two[0][1], two[1][1] + one[1][1] * 2)
+    close(got["vc"], two[0][2], two[1][2])
 
 
 def test_append_many_sequences_strided():
