@@ -19,7 +19,8 @@ A query that sees no key, or only scores of -inf, gives zeros; so do rows of
 the packed batch outside every sequence.  What a query does not see has no
 part in its result, NaN and infinities included.
 
-The CPU forms are the definitions, evaluated in float64 and rounded once.
+The CPU forms are the definitions, evaluated in float64 and rounded once.  On
+the GPU scores are 32-bit sums: a row that sees one past their range is NaN.
 """
 
 from __future__ import annotations
@@ -113,8 +114,8 @@ def _scale(scale, dim):
     if scale is None:
         return 1.0 / math.sqrt(dim)
     scale = float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"scale must be a positive number, got {scale}")
+    if not 2.0**-64 <= scale <= 2.0**64:
+        raise ValueError(f"scale must be a positive number, of 2^-64 to 2^64, got {scale}")
     return scale
 
 

@@ -488,7 +488,9 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   for (int t2 = 0; t2 < D / 32; ++t2)
 #pragma unroll
     for (int r = 0; r < 16; ++r) z = __builtin_fmaf(acc[t2][r], 0.f, z);
-  uint64_t spoiled = __ballot(ok && z != 0.f);
+  // and those whose offset is too large to cancel: s c - m is then off by half a
+  // step of m
+  uint64_t spoiled = __ballot(ok && (z != 0.f || (fabsf(m_run) >= 0x1p24f && m_run > -1e29f)));
   spoiled = (spoiled | spoiled >> 32) & 0xffffffffull;
   const bool mine = spoiled >> l32 & 1;
   const bool put = row < rows && !mine;
@@ -629,7 +631,7 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   f32x4 acc[D / 16];
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -1e30f, l_run = 0.f;
+  float m_run = -1e30f, l_run = 0.f;  // (the offset of the scores themselves: large ones cancel exactly)
   const float sl2 = a.scale * 1.44269504088896340736f;
 
   // 16 rows of a transposing read, two chunks each, cover all banks
@@ -678,7 +680,7 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], sl2, -m_run));
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3] - m_run, sl2, Mat<T>::TOP));
         sum += x;
         pf[e] = (typename Mat<T>::E)x;
       }
@@ -691,8 +693,8 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
       for (int e = 1; e < 8; ++e) bm = fmaxf(bm, s[e >> 2][e & 3]);
       bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
       bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float m_new = fmaxf(m_run, bm * sl2 - Mat<T>::TOP);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      const float m_new = fmaxf(m_run, bm);
+      const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * sl2);
       m_run = m_new;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t)
@@ -731,7 +733,7 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   const float m = fmaxf(fmaxf(so[l16], so[16 + l16]), fmaxf(so[32 + l16], so[48 + l16]));
   __syncthreads();
   // (an infinite score's offset is infinite: its sums are NaN already)
-  const float f = m_run == m ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+  const float f = m_run == m ? 1.f : __builtin_amdgcn_exp2f((m_run - m) * sl2);
 #pragma unroll
   for (int t = 0; t < D / 16; ++t)
     *reinterpret_cast<float4 *>(so + (wave * 16 + l16) * D + t * 16 + grp * 4) =
@@ -753,7 +755,8 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   }
   if (pieces > 1 && wave == 0 && grp == 0 && h0 + l16 < rep) {
     float *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + r0 + l16) * 2;
-    wm[0] = m, wm[1] = (sm[l16] + sm[16 + l16]) + (sm[32 + l16] + sm[48 + l16]);
+    const float l = (sm[l16] + sm[16 + l16]) + (sm[32 + l16] + sm[48 + l16]);
+    wm[0] = l == 0.f ? -1e30f : m * sl2, wm[1] = l;
   }
 }
 #define NK_STEP(T, name, D)                                                                                 \

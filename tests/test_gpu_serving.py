@@ -378,6 +378,23 @@ def test_window_single_tokens(t, d):
             close(got, *P.dense(q, k, v, a, None if b is None else b.astype(np.int64), window, sinks, t))
 
 
+@pytest.mark.parametrize("t,d,big", [("bf16", 64, 1e12), ("bf16", 128, 1e17), ("f16", 64, 6e4), ("f16", 128, 3e4), ("f32", 48, 1e15)])
+@pytest.mark.parametrize("S", [1, 40, 130])
+@pytest.mark.parametrize("K", [130, 3000])
+def test_window_huge_scores(t, d, big, S, K):
+    """Scores far past where 32 bits hold their differences: the largest alone has
+    weight, equal ones share it."""
+    rng = np.random.default_rng(40)
+    v = P.cast(rng.integers(-8, 8, (2, K, 2, d)).astype(np.float32), t)
+    q, k = np.full((2, S, 4, d), big, np.float32), np.ones((2, K, 2, d), np.float32)
+    k[0, 70] = 2.0  # (every query sees it where S < 60)
+    q[:, :, 1] *= -1
+    k[1, :, 1] *= -1
+    want, tol = P.dense(*(P.cast(x, t) for x in (q, k)), v, None, None, 0, 0, t)
+    # among equal scores: at most 8, by the roundings of weights, sums and result
+    close(run(f_window, P.cast(q, t), P.cast(k, t), v)["output0"], want, np.minimum(tol, 8 * 4 * 2.0**-8))
+
+
 @pytest.mark.parametrize("S", [1, 50])
 def test_window_broadcast_keys(S):
     """Keys and values that all sequences share, and one row that is every key."""

@@ -260,3 +260,11 @@ def test_two_appends_keep_their_own_tables():
               f(4, 2, 2, 8), f(4, 2, 2, 8), i(2, 2), i(2))
     assert p.kernel_kinds == ["rotary_append", "rotary_append"]
     assert [sorted(s.desc.split(": ")[1].split(", ")) for s in p.steps] == [["k", "v"], ["k", "q", "v"]]
+
+
+def test_attention_refuses_scales_outside_32_bits():
+    q, k = np.zeros((1, 2, 2, 8), np.float32), np.zeros((1, 3, 2, 8), np.float32)
+    for scale in (2.0**65, 1e300, 2.0**-65, -1.0):
+        with pytest.raises(ValueError, match="scale"):
+            T.window_attention(q, k, k, scale=scale)
+    assert (T.window_attention(q, k, k, scale=2.0**-64) == 0).all()
