@@ -155,9 +155,9 @@ NK_APPEND(float, f32)
 //          that is up to LIST values, and the border and the draw are searched
 //          there; else that bin alone for the border, then the segment that holds
 //          uniform x the kept weight, by the segments' sums.
-// Rows of up to LIST tokens are one launch: the list is the row, cut down to the
-// bins that may be kept where those hold few (15 rows of 4546 with top_k and top_p:
-// 17 us, 29 without).
+// Rows of up to LIST tokens are one launch, read once: the list is the row, cut
+// down to the bins that may be kept where those hold few (15 rows of 4546 with
+// top_k and top_p 13 us, 29 with searches of the whole row).
 //
 // A list of up to FEW is ranked value against value.  Else a search (smp_select)
 // finds where the running count or weight, in descending order of a key, reaches
@@ -778,7 +778,25 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
   __shared__ SmpShared s;
   const int tid = threadIdx.x, r = blockIdx.x;
   const T *x = (const T *)a.x + r * a.ld;
-  const u64 top = SMALL ? smp_top<T, SMP_BLOCK>(x, 0, a.vocab, s.red, [](uint32_t) {}) : smp_row_top<SMP_BLOCK>(a, r, s.red);
+  constexpr int U = SMP_LIST / SMP_BLOCK;  // elements of a thread, all reads in flight
+  T held_row[U];                           // (SMALL: the row)
+  u64 top = 0;
+  if (SMALL) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = j * SMP_BLOCK + tid;
+      Elt<T>::store(&held_row[j], 0, -INFINITY);
+      if (i < a.vocab) held_row[j] = x[i];
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const float f = Elt<T>::load(&held_row[j], 0);
+      if (f > -INFINITY) top = max(top, (u64)SmpKey<T>::of(f) << 32 | (uint32_t)~(j * SMP_BLOCK + tid));
+    }
+    top = smp_max<SMP_BLOCK / 64>(top, s.red);
+  } else {
+    top = smp_row_top<SMP_BLOCK>(a, r, s.red);
+  }
   SmpRow row;
   if (!smp_settings<T>(a, r, top, row)) {
     if (tid == 0) a.out[r] = top ? (int32_t)~(uint32_t)top : -1;
@@ -825,7 +843,6 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     s.place[tid] = from;                       // and that in its order
     __syncthreads();
     n = min((int)all, SMP_LIST);
-    constexpr int U = SMP_LIST / SMP_BLOCK;  // all reads in flight
     uint32_t at[U];  // a segment, the last that begins by this place; then the token
     T v[U];
 #pragma unroll
@@ -898,9 +915,21 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
       total = smp_sum<SMP_BLOCK / 64>(total, s.red);
     }
   }
+  if (SMALL) {
+    n = a.vocab;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = j * SMP_BLOCK + tid;
+      if (i < n) {
+        const float f = Elt<T>::load(&held_row[j], 0);
+        const u64 w = smp_weight(row.depth(f));
+        s.key[i] = w ? SmpKey<T>::of(f) : 0, s.idx[i] = i, s.w[i] = w;  // (what weighs nothing, NaN too, comes last)
+      }
+    }
+    __syncthreads();
+  }
   // (a few listed values are ranked below, and need no bins)
-  const bool ranked = parts && whole && n <= SMP_FEW;
-  if (SMALL) n = smp_gather(s, x, 0, a.vocab, row.floor(), row.best, row);
+  const bool ranked = (SMALL || parts) && whole && n <= SMP_FEW;
   if (whole && !ranked) {
     if (cuts) {
       clear_bins();
@@ -1010,7 +1039,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     if (in) s.hsum[tid] = run;
     __syncthreads();
     if (p_cuts) {
-      const u64 goal = share(k_cuts ? s.hsum[keep - 1] : total);
+      const u64 goal = share(k_cuts || ranked ? s.hsum[keep - 1] : total);
       keep = min(keep, 1 + (uint32_t)smp_sum<SMP_BLOCK / 64>(in && run < goal, s.red));
     }
     if (by_m) keep = min(keep, (uint32_t)smp_sum<SMP_BLOCK / 64>(in && t >= tmin, s.red));
