@@ -616,7 +616,6 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   if (split >= pieces) return;
   const int p = sq.p0, klim = min(p, sq.cap - 1);
 
-  const bool head = h0 + l16 < rep;
   V8 qf[D / 32];
   {
     const uint16_t *q = (const uint16_t *)a.q + (PAGED ? (int64_t)b * a.q_ss : (int64_t)b * a.q_sb) +

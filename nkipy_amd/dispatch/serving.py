@@ -11,7 +11,7 @@ buffer, rows of other positions staying as they are.
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Tuple
 
 import numpy as np
 
