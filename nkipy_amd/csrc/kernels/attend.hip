@@ -1,5 +1,5 @@
 // Attention over a paged cache or plain tensors with a window and sinks
-// (attend.h holds the definition and the layout of the work).
+// (attend_index.h holds the definition and the layout of the work).
 
 #include "attend.h"
 
@@ -16,15 +16,12 @@ __device__ __forceinline__ void attend_rows_body(const AttendArgs &a) {
   const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (r >= (int64_t)a.N * a.Hq) return;
   const int t = (int)(r / a.Hq), h = (int)(r % a.Hq);
-  const int b = a.starts ? att_find(a.B, t, [&](int x) { return a.starts[x]; }) : t / a.S;
+  int b, i;
+  AttSeq sq;
   float m, l = 0.f, acc[4];
-  if (b >= 0) {
-    const AttSeq sq = att_seq(a, b);
-    const int i = t - sq.lo;
-    if (i < sq.n) {
-      const AttSpan sp = att_span(a, sq, (i * (a.Hq / a.Hkv) + h % (a.Hq / a.Hkv)) / ATT_ROWS);
-      att_row<T>(a, sq, sp, b, i, h, 0, sp.nb, m, l, acc);
-    }
+  if (att_query(a, t, b, sq, i)) {
+    const AttSpan sp = att_span(a, sq, (i * (a.Hq / a.Hkv) + h % (a.Hq / a.Hkv)) / ATT_ROWS);
+    att_row<T>(a, sq, sp, b, i, h, 0, sp.nb, m, l, acc);
   }
   T *o = (T *)a.o + r * a.D;
 #pragma unroll
@@ -116,33 +113,6 @@ NK_DEVICE void att_zero_rest(const AttendArgs &a, int wg, int nwg) {
   }
 }
 
-// Workgroups run round-robin over the eight XCDs: with the KV head fastest, the
-// tiles of one head (eight heads, or a multiple) share an XCD's cache.  The last
-// tiles of a sequence, the longest without a window, go first; splits that only
-// the longest sequences have come last, and so leave no CU with two workgroups
-// while others have none (256 tokens behind 4000: 70 us with the splits of a tile
-// side by side, 48 so).
-struct AttWork {
-  int g, split, b, tile;  // b < 0: nothing to do
-};
-template <bool PAGED>
-NK_DEVICE AttWork att_work(const AttendArgs &a, int w) {
-  AttWork k;
-  const int rep = a.Hq / a.Hkv;
-  k.g = w % a.Hkv;
-  w /= a.Hkv;
-  const int t = a.tiles - 1 - w % a.tiles;
-  k.split = w / a.tiles;
-  if (PAGED && a.starts) {
-    k.b = att_find(a.B, t, [&](int x) { return att_tile0(a, x); });
-    k.tile = k.b < 0 ? 0 : t - att_tile0(a, k.b);
-  } else {
-    const int per = (a.S * rep + ATT_ROWS - 1) / ATT_ROWS;
-    k.b = t / per, k.tile = t % per;
-  }
-  return k;
-}
-
 // FAR: keys or values over 4 GiB, or keys and values of different row strides in
 // one cache: 64-bit addresses, and a row of zeros for what has no use.  Else offsets
 // into a buffer resource, past whose end a move writes zeros.
@@ -163,11 +133,10 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   const int rep = a.Hq / a.Hkv;
 
   if (PAGED && a.starts) att_zero_rest<T>(a, blockIdx.x, a.tiles * a.Hkv * a.nsplit);
-  const AttWork wk = att_work<PAGED>(a, blockIdx.x);
+  AttWork wk;
+  AttSeq sq;
+  if (!att_tile<PAGED>(a, blockIdx.x, wk, sq)) return;
   const int g = wk.g, split = wk.split, b = wk.b, tile = wk.tile;
-  if (b < 0) return;
-  const AttSeq sq = att_seq(a, b);
-  if ((int64_t)tile * ATT_ROWS >= (int64_t)sq.n * rep) return;
   const AttSpan sp = att_span(a, sq, tile);
   int j0, j1;
   const int pieces = att_split(a, sp.nb, split, j0, j1);
@@ -784,11 +753,9 @@ __device__ __forceinline__ void attend_join_body(const AttendArgs &a) {
   const int64_t r = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x, nr = (int64_t)a.N * a.Hq;
   if (r >= nr) return;
   const int t = (int)(r / a.Hq), h = (int)(r % a.Hq), rep = a.Hq / a.Hkv;
-  const int b = a.starts ? att_find(a.B, t, [&](int x) { return a.starts[x]; }) : t / a.S;
-  if (b < 0) return;
-  const AttSeq sq = att_seq(a, b);
-  const int i = t - sq.lo;
-  if (i >= sq.n) return;
+  int b, i;
+  AttSeq sq;
+  if (!att_query(a, t, b, sq, i)) return;
   int j0, j1;
   const int pieces = att_split(a, att_span(a, sq, (i * rep + h % rep) / ATT_ROWS).nb, 0, j0, j1);
   if (pieces == 1) return;
