@@ -150,8 +150,12 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     if tables:
         if width < 1 or page < 1 or width * page >= 2**30 or pages * pitch >= 2**31:
             raise LaunchError("attention: cache too large, or no page")
+        if pitch < page:
+            raise LaunchError(f"attention: pages of {page} rows at a pitch of {pitch}")
     elif B * S != N or T >= 2**30 or S >= 2**30:
         raise LaunchError("attention: sequences too long")
+    if min(k_str[1], v_str[1]) < (1 if tables else 0):
+        raise LaunchError(f"attention: row strides {k_str[1]} and {v_str[1]} of keys and values")
     a = _fields(AttendArgs(), q=q, k=k, v=v, o=o, tables=tables, lens=lens, starts=starts, first=first,
                 q_sb=q_str[0], q_ss=q_str[1], q_sh=q_str[2], k_sb=k_str[0], k_ss=k_str[1], k_sh=k_str[2],
                 v_sb=v_str[0], v_ss=v_str[1], v_sh=v_str[2], B=B, S=S, N=N, T=T, Hq=Hq, Hkv=Hkv, D=D, page=page, pages=pages,
@@ -259,14 +263,15 @@ def _strided(v: Value) -> Tuple[View, List[int]]:
 
 def _cache_strided(v: Value):
     """A cache (pages, page, heads, dim) whose pages lie a whole number of rows
-    apart: (view, (0, row, head), rows from page to page)."""
+    apart, at least a page's own (the tiles' buffer resource ends behind the last
+    of them): (view, (0, row, head), rows from page to page)."""
     vw, st = _strided(v)
     pages, page = v.shape[:2]
     if page == 1:
         st[1] = st[0] if pages > 1 else max(st[0], 1)
     if pages == 1:
         st[0] = st[1] * page
-    if st[1] < 1 or st[0] % st[1] or st[0] // st[1] * pages >= 2**31:
+    if st[1] < 1 or st[0] < st[1] * page or st[0] % st[1] or st[0] // st[1] * pages >= 2**31:
         vw, st = _contiguous(v)
     return vw, (0, st[1], st[2]), st[0] // st[1]
 

@@ -26,3 +26,16 @@ def test_long_batches_of_unordered_starts(d):
         last = P.paged(q[700:], kc, vc, tables[3:], lens[3:], np.array([0, 300], np.int32), 40, 1, "bf16")
         if first[0] <= 700 and first[1] <= 700:  # (each tile behind row 700 finds its sequence)
             close(P.cast(got[700:], "f32"), *last)
+
+
+@pytest.mark.parametrize("new", [None, [9, 40]])
+def test_caches_whose_pages_are_one(new):
+    rng = np.random.default_rng(72)
+    tables, lens, starts, pages = P.batch(rng, [70, 45], new, 16)
+    q = draw(rng, (2 if new is None else sum(new), 4, 64), "bf16")
+    k, v = draw(rng, (1, 16, 2, 64), "bf16"), draw(rng, (1, 16, 2, 64), "bf16")
+    shape = (pages, 16, 2, 64)
+    f = lambda q, k, v, tables, lens, starts=None: T.paged_attention(  # noqa: E731
+        q, np.broadcast_to(k, shape), np.broadcast_to(v, shape), tables, lens, starts)
+    kc, vc = (np.ascontiguousarray(np.broadcast_to(x, shape)) for x in (k, v))
+    close(run(f, q, k, v, tables, lens, starts)["output0"], *P.paged(q, kc, vc, tables, lens, starts, 0, 0, "bf16"))
