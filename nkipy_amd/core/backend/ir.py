@@ -30,7 +30,7 @@ Op vocabulary (attributes in brackets):
   put_along_axis [axis] (operand, indices, values)
   scatter_strided [indices_per_dim] (operand, updates)
   rotate_rows [starts] (rows, cos, sin, lengths[, starts])
-  paged_write [rotary, starts] (cache, rows[, cos, sin], tables, lengths[, starts])
+  paged_write [rotary, starts, positions] (cache, rows[, cos, sin], tables, lengths[, starts])
   paged_attention [window, sinks, scale, starts] (q, keys, values, tables, lengths[, starts])
   window_attention [window, sinks, scale, lengths, positions] (q, k, v[, lengths][, positions])
   sample [temperature, top_k, top_p, min_p] (logits, uniform[, filters given per row])

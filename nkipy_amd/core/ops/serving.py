@@ -235,7 +235,7 @@ def _rotary_append_hip(q, k, v, cos, sin, key_cache, value_cache, block_tables, 
     rotated = cx.build_op("rotate_rows", [qv] + turn + where[1:] + starts, qv.shape, qv.dtype, {"starts": bool(starts)})
     for cache, cv, x, extra in ((key_cache, kc, kv, turn), (value_cache, vc, vv, [])):
         out = cx.build_op("paged_write", [cv, x] + extra + where + starts, cv.shape, cv.dtype,
-                          {"rotary": bool(extra), "starts": bool(starts)})
+                          {"rotary": bool(extra), "starts": bool(starts), "positions": int(cos.shape[0])})
         cache._is_mutated = True
         cache._rebind(wrap(out))
     return wrap(rotated)

@@ -323,7 +323,8 @@ class AppendMatch(Match):
         if "q" in parts:
             q = parts["q"].inputs[0]
             shape = {"page": 1, "pages": 0, "Hkv": 0, **shape, "Hq": q.shape[1], "D": q.shape[2]}
-        P, half = cos.shape if cos is not None else (2**30, 0)
+        # (values alone have no tables, and still drop what has no row in them)
+        P, half = cos.shape if cos is not None else (some.attrs["positions"], 0)
 
         def make(addr):
             kw = {}
@@ -368,6 +369,9 @@ class AppendPattern:
         if n.op == "rotate_rows" or n.attrs["rotary"]:
             at = 1 if n.op == "rotate_rows" else 2
             out["turn"] = [v.id for v in n.inputs[at:at + 2]]
+            out["positions"] = n.inputs[at].shape[0]
+        else:
+            out["positions"] = n.attrs["positions"]
         if n.op == "paged_write":
             out["cache"] = (n.inputs[0].shape, n.inputs[4 if n.attrs["rotary"] else 2].id)
         return out

@@ -8,6 +8,7 @@ from nkipy_amd.core import tensor_apis as T
 
 import serving_plain as P
 from test_gpu_serving import close, draw, f_paged, run
+from test_serving_layouts import values_alone
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,19 @@ def test_caches_whose_pages_are_one(new):
         q, np.broadcast_to(k, shape), np.broadcast_to(v, shape), tables, lens, starts)
     kc, vc = (np.ascontiguousarray(np.broadcast_to(x, shape)) for x in (k, v))
     close(run(f, q, k, v, tables, lens, starts)["output0"], *P.paged(q, kc, vc, tables, lens, starts, 0, 0, "bf16"))
+
+
+@pytest.mark.parametrize("new", [None, [3, 9, 1]])
+def test_values_written_alone(new):
+    """Tokens whose position has no row in the tables are dropped also where the
+    value cache is all that is written."""
+    rng = np.random.default_rng(73)
+    tables, lens, starts, pages = P.batch(rng, [12, 20, 14], new, 4)
+    n = 3 if new is None else sum(new)
+    q, k, v = (draw(rng, (n, h, 64), "f32") for h in (4, 2, 2))
+    vc = draw(rng, (pages, 4, 2, 64), "f32")
+    ang = np.arange(13 * 32, dtype=np.float32).reshape(13, 32)  # positions 0 to 12
+    cos, sin = np.cos(ang), np.sin(ang)
+    want = P.append(q, k, v, cos, sin, vc, vc, tables, lens, starts, "f32")[0][2]
+    got = run(values_alone, q, k, v, cos, sin, vc, tables, lens, starts)
+    assert (got["vc"] == want).all()

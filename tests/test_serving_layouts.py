@@ -58,3 +58,14 @@ def test_attention_refuses_overlapping_pages_and_rows_backwards():
             with pytest.raises(LaunchError, match="stride"):
                 S.attend(dt.bfloat16, 256, 256, 256, 256, **{**kw, name: (0, -128, 64)}, T=4, zeros=zeros, ws=256)
             S.attend(dt.bfloat16, 256, 256, 256, 256, **{**kw, name: (0, 0, 64)}, T=4, zeros=zeros, ws=256)  # (one row is every key)
+
+
+def values_alone(q, k, v, cos, sin, vc, tables, lens, starts=None):
+    """The rotated q and keys are used by nothing: one launch, of the values."""
+    T.rotary_append(q, k, v, cos, sin, vc * np.float32(2), vc, tables, lens, starts)
+
+
+def test_values_written_alone_know_the_positions():
+    p = plan(values_alone, f32(3, 4, 8), f32(3, 2, 8), f32(3, 2, 8), f32(7, 4), f32(7, 4), f32(5, 4, 2, 8), i32(3, 2), i32(3))
+    (x,) = launches(p, "rotary_append")
+    assert not x.args.oq and not x.args.ok and x.args.ov and x.args.P == 7
