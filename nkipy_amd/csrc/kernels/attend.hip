@@ -85,6 +85,7 @@ template <> struct Mat<f16> {
 template <bool B> struct Flag {
   static constexpr bool value = B;
 };
+#define ATT_LOWEST -3.40282347e38f  // the least finite offset
 template <int N> struct Slot {
   static constexpr int value = N;
 };
@@ -165,7 +166,7 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   for (int t2 = 0; t2 < D / 32; ++t2)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[t2][r] = 0.f;
-  float m_run = -1e30f, l_run = 0.f;  // (finite: a masked score gives p = 0)
+  float m_run = -1e30f, l_run = 0.f;  // (finite: a masked score gives p = 0; scores below it: see `sees`)
   const float sl2 = a.scale * 1.44269504088896340736f;
 
   // swizzles: 16-byte chunk c of row r stands at chunk c ^ kswz / vswz, so that
@@ -451,6 +452,15 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   float *wo = a.ws + (split * nr + orow) * D, *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + orow) * 2;
   uint16_t *o = (uint16_t *)a.o + orow * D;
 
+  // whether this row sees any key of these blocks, pages aside
+  bool sees = false;
+  auto part = [&](int a0, int a1) __attribute__((always_inline)) {  // (blocks that follow each other)
+    const int lo = sp.kb(a0) * ATT_KEYS, hi = min(sp.kb(a1 - 1) * ATT_KEYS + ATT_KEYS - 1, klim);
+    sees |= a0 < a1 && (max(lo, p - a.window + 1) <= hi || lo <= min(hi, a.sinks - 1));
+  };
+  part(j0, min(j1, sp.ns));
+  part(max(j0, sp.ns), j1);
+
   // rows that a value which is not finite may have spoiled
   float z = l_run * 0.f;
 #pragma unroll
@@ -458,8 +468,9 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) z = __builtin_fmaf(acc[t2][r], 0.f, z);
   // and those whose offset is too large to cancel: s c - m is then off by half a
-  // step of m
-  uint64_t spoiled = __ballot(ok && (z != 0.f || (fabsf(m_run) >= 0x1p24f && m_run > -1e29f)));
+  // step of m.  A row without weight still has the offset it began with: where it
+  // sees keys their scores are below that, or -inf.
+  uint64_t spoiled = __ballot(ok && (z != 0.f || (fabsf(m_run) >= 0x1p24f && (l_run != 0.f || sees))));
   spoiled = (spoiled | spoiled >> 32) & 0xffffffffull;
   const bool mine = spoiled >> l32 & 1;
   const bool put = row < rows && !mine;
@@ -491,7 +502,7 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
         x.w = ok ? acc[t2][gq * 4 + 3] : 0.f;
         *reinterpret_cast<float4 *>(wo + t2 * 32 + gq * 8 + lhi * 4) = x;
       }
-    if (lhi == 0) wm[0] = ok ? m_run : -1e30f, wm[1] = ok ? l_run : 0.f;
+    if (lhi == 0) wm[0] = m_run, wm[1] = ok ? l_run : 0.f;
   }
   // These again, reading only what they see.  (The arguments are read anew, so
   // that none of them takes a register through the loop above for this.)
@@ -521,7 +532,7 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
     }
     if (pieces2 > 1 && lane == 0) {
       float *q = a2.ws + (int64_t)a2.nsplit * nr2 * D + (wk2.split * nr2 + at) * 2;
-      q[0] = l == 0.f ? -1e30f : m * 1.44269504088896340736f;
+      q[0] = fmaxf(m * 1.44269504088896340736f, ATT_LOWEST);
       q[1] = l;
     }
   }
@@ -599,7 +610,7 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   f32x4 acc[D / 16];
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -1e30f, l_run = 0.f;  // (the offset of the scores themselves: large ones cancel exactly)
+  float m_run = ATT_LOWEST, l_run = 0.f;  // (the offset of the scores themselves: large ones cancel exactly)
   const float sl2 = a.scale * 1.44269504088896340736f;
 
   // 16 rows of a transposing read, two chunks each, cover all banks
@@ -724,7 +735,7 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   if (pieces > 1 && wave == 0 && grp == 0 && h0 + l16 < rep) {
     float *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + r0 + l16) * 2;
     const float l = (sm[l16] + sm[16 + l16]) + (sm[32 + l16] + sm[48 + l16]);
-    wm[0] = l == 0.f ? -1e30f : m * sl2, wm[1] = l;
+    wm[0] = fmaxf(m * sl2, ATT_LOWEST), wm[1] = l;
   }
 }
 #define NK_STEP(T, name, D)                                                                                 \
@@ -741,8 +752,8 @@ NK_STEP(f16, f16, 64)
 
 // ---------------------------------------------------------------------------
 // The splits of a row joined, in their order: o = sum 2^(m_s - M) o_s / sum
-// 2^(m_s - M) l_s.  Up to 64 splits, a lane each for their offsets; bound by the
-// latency of its reads.  One wave per row, or (W = 4) a workgroup, each wave a
+// 2^(m_s - M) l_s, over the splits with any weight.  Up to 64 splits, a lane each for
+// their offsets; bound by the latency of its reads.  One wave per row, or (W = 4) a workgroup, each wave a
 // quarter of the splits, all of its reads in flight at once.  Rows that one split
 // had are written already.
 // ---------------------------------------------------------------------------
@@ -771,13 +782,14 @@ __device__ __forceinline__ void attend_join_body(const AttendArgs &a) {
         x[s][e] = a.ws[((int64_t)min(s0 + s * W, pieces - 1) * nr + r) * D + lane + 64 * e];
   };
   fetch(w0);
-  float m = -1e30f, l = 0.f;
+  float m = -INFINITY, l = 0.f;
   if (lane < pieces) {
     const float2 v = *reinterpret_cast<const float2 *>(wm + (lane * nr + r) * 2);
-    m = v.x, l = v.y;
+    l = v.y;
+    if (l != 0.f) m = v.x;
   }
-  const float w = __builtin_amdgcn_exp2f(m - wave_max(m));
-  const float total = wave_sum(lane < pieces ? w * l : 0.f);
+  const float top = wave_max(m), w = l != 0.f ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+  const float total = wave_sum(w * l);
   const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) acc[e] = 0.f;
