@@ -17,7 +17,9 @@ Which keys the query at position p sees (the same in both attentions):
 
 A query that sees no key, or only scores of -inf, gives zeros; so do rows of
 the packed batch outside every sequence.  What a query does not see has no
-part in its result, NaN and infinities included.
+part in its result, NaN and infinities included; a value that is not finite
+reaches every query that sees its key with a score above -inf, however small
+the weight.
 
 The CPU forms are the definitions, evaluated in float64 and rounded once.  On
 the GPU scores are 32-bit sums: a row that sees one past their range is NaN.
@@ -379,6 +381,7 @@ def _attend(q, k, v, seen, scale):
                 if s.size == 0 or s.max() == -np.inf:
                     continue
                 e = np.exp(s - s.max())
+                e = np.where(s == -np.inf, 0.0, np.maximum(e, 5e-324))  # (no weight of a finite score is 0)
                 out[i, h] = (e @ vv[seen[i]]) / e.sum()
     return out
 

@@ -519,8 +519,8 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
     const int pieces2 = att_split(a2, sp2.nb, wk2.split, k0, k1);
     const int src = __builtin_ctzll(spoiled);
     spoiled &= spoiled - 1;
-    float m, l, x[4];
-    att_row<T>(a2, sq2, sp2, wk2.b, __shfl(qi, src, 64), __shfl(h, src, 64), k0, k1, m, l, x);
+    float m, l, x[D / 64];
+    att_row<T, D>(a2, sq2, sp2, wk2.b, __shfl(qi, src, 64), __shfl(h, src, 64), k0, k1, m, l, x);
     const int64_t at = __shfl((int)orow, src, 64);  // (rows are below 2^31)
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
@@ -567,7 +567,7 @@ NK_TILE(f16, f16, 64, 3, 4)
 // S^T = K Q^T and O^T = V^T P^T.  K fragments come straight from memory (16 bytes
 // of a row per lane); V goes to an LDS slot of the wave's own, from which
 // transposing reads take four keys of a column.  Every head sees the same keys.
-// 64 sequences of up to 8192 tokens, 32 / 8 heads of 128: 238 us, 4.7 TB/s.
+// 64 sequences of up to 8192 tokens, 32 / 8 heads of 128: 240 us, 4.6 TB/s.
 // ---------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 NK_DEVICE f32x4 mul16(Mat<bf16>::V a, Mat<bf16>::V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -706,6 +706,15 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
   float *so = reinterpret_cast<float *>(lds), *sm = so + NW * 16 * D;  // (NW, 16, D) sums; (NW, 16) weights, (16) in all
+  __shared__ uint32_t spoiled[NW];  // a bit for each row with a sum that is not finite
+  float z = l_run * 0.f;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z = __builtin_fmaf(acc[t][r], 0.f, z);
+  uint64_t bits = __ballot(z != 0.f);
+  bits |= bits >> 32;
+  if (lane == 0) spoiled[wave] = (uint32_t)(bits | bits >> 16) & 0xffffu;
   __syncthreads();
   if (grp == 0) so[wave * 16 + l16] = m_run;
   __syncthreads();
@@ -720,22 +729,41 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   if (grp == 0) sm[wave * 16 + l16] = l_run * f;
   __syncthreads();
   const int64_t nr = (int64_t)a.N * a.Hq, r0 = (int64_t)b * a.Hq + g * rep + h0;
+  auto weight = [&](int r) __attribute__((always_inline)) { return (sm[r] + sm[16 + r]) + (sm[32 + r] + sm[48 + r]); };
+  const uint32_t again = __builtin_amdgcn_readfirstlane(spoiled[0] | spoiled[1] | spoiled[2] | spoiled[3]);
 #pragma unroll
   for (int x = 0; x < 16 * D / 256; ++x) {
     const int e = x * 256 + tid, r = e / D;
     if (h0 + r >= rep) break;  // (rows rise)
-    const float o = (so[e] + so[16 * D + e]) + (so[2 * 16 * D + e] + so[3 * 16 * D + e]);
-    const float l = (sm[r] + sm[16 + r]) + (sm[32 + r] + sm[48 + r]);
+    if (again >> r & 1) continue;
+    const float o = (so[e] + so[16 * D + e]) + (so[2 * 16 * D + e] + so[3 * 16 * D + e]), l = weight(r);
     if (pieces == 1) {
       Elt<T>::store((T *)a.o + r0 * D, e, l == 0.f ? 0.f : o / l);
     } else {
       a.ws[(split * nr + r0) * D + e] = o;
     }
   }
-  if (pieces > 1 && wave == 0 && grp == 0 && h0 + l16 < rep) {
-    float *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + r0 + l16) * 2;
-    const float l = (sm[l16] + sm[16 + l16]) + (sm[32 + l16] + sm[48 + l16]);
-    wm[0] = fmaxf(m * sl2, ATT_LOWEST), wm[1] = l;
+  float *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + r0) * 2;
+  if (pieces > 1 && wave == 0 && grp == 0 && h0 + l16 < rep && !(again >> l16 & 1))
+    wm[2 * l16] = fmaxf(m * sl2, ATT_LOWEST), wm[2 * l16 + 1] = weight(l16);
+  // Values that are not finite under weights that rounded to 0: those rows again, a
+  // wave for each.
+  for (uint32_t left = again; left; left &= left - 1) {
+    const int r = __builtin_ctz(left);
+    if (h0 + r >= rep) break;
+    if (r % NW != wave) continue;
+    float mr, lr, x[D / 64];
+    att_row<T, D>(a, sq, sp, b, 0, g * rep + h0 + r, j0, j1, mr, lr, x);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      if (pieces == 1) {
+        Elt<T>::store((T *)a.o + (r0 + r) * D, lane + 64 * e, lr == 0.f ? 0.f : x[e] / lr);
+      } else {
+        a.ws[(split * nr + r0 + r) * D + lane + 64 * e] = x[e];
+      }
+    }
+    // (the step's weights are 2^TOP of these)
+    if (pieces > 1 && lane == 0) wm[2 * r] = fmaxf(mr * 1.44269504088896340736f, ATT_LOWEST) + Mat<T>::TOP, wm[2 * r + 1] = lr;
   }
 }
 #define NK_STEP(T, name, D)                                                                                 \
@@ -791,17 +819,27 @@ __device__ __forceinline__ void attend_join_body(const AttendArgs &a) {
   const float top = wave_max(m), w = l != 0.f ? __builtin_amdgcn_exp2f(m - top) : 0.f;
   const float total = wave_sum(w * l);
   const float inv = total == 0.f ? 0.f : 1.f / total;
+  auto add = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) acc[e] = 0.f;
-  for (int s0 = w0; s0 < pieces; s0 += U * W) {
-    if (s0 != w0) fetch(s0);
+    for (int e = 0; e < D / 64; ++e) acc[e] = 0.f;
+    for (int s0 = w0; s0 < pieces; s0 += U * W) {
+      if (s0 != w0) fetch(s0);
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      if (s0 + s * W >= pieces) break;
-      const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + s * W));
+      for (int s = 0; s < U; ++s) {
+        if (s0 + s * W >= pieces) break;
+        const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + s * W));
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(ws, x[s][e], acc[e]);
+        for (int e = 0; e < D / 64; ++e) acc[e] = f(ws, x[s][e], acc[e]);
+      }
     }
+  };
+  add([](float ws, float y, float c) { return fmaf(ws, y, c); });
+  bool whole = true;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) whole &= __builtin_isfinite(acc[e]);
+  if (__builtin_expect(__any(!whole), 0)) {  // (0 x inf: a split's sum is not finite, and its weight is nothing beside the others')
+    fetch(w0);
+    add(att_add);
   }
   if constexpr (W > 1) {
 #pragma unroll

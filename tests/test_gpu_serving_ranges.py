@@ -64,3 +64,48 @@ def test_only_scores_of_minus_infinity():
         assert (got[0] == 0).all()
         first = max(0, 11 - (K - S))  # (the query at position 11)
         assert (got[1, :first] == 0).all() and (got[1, first:] == np.repeat(P.up(v)[1, 11], 2, 0)).all()
+
+
+@pytest.mark.parametrize("t,d,far", [("bf16", 64, 60.0), ("bf16", 128, 95.0), ("f16", 64, 30.0), ("f16", 128, 60.0), ("f32", 48, 95.0)])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("S,K", [(1, 130), (1, 3000), (40, 300)])
+def test_infinite_values_of_small_weight(t, d, far, value, S, K):
+    """A value that is not finite reaches each query that sees its key, also where the
+    weight e^-far is nothing in the operands' type, and no other element."""
+    rng = np.random.default_rng(84)
+    q, k = np.zeros((2, S, 4, d), np.float32), np.zeros((2, K, 2, d), np.float32)
+    q[..., 0], k[..., 0] = 1.0, rng.random((2, K, 2)) * 0.5
+    at = K - S - 5  # (seen by all)
+    k[0, at, 1, 0] = -far
+    v = rng.standard_normal((2, K, 2, d)).astype(np.float32)
+    q, k, v = P.cast(q, t), P.cast(k, t), P.cast(v, t)
+    clean = v.copy()
+    clean[0, at, 1, 7] = P.cast(np.float32(0), t)
+    v[0, at, 1, 7] = P.cast(np.float32(value), t)
+    want, tol = P.dense(q, k, clean, None, None, 0, 0, t, 1.0)
+    got = P.up(run(f_window, q, k, v, scale=1.0)["output0"])
+    hit = np.zeros(got.shape, bool)
+    hit[0, :, 2:, 7] = True
+    assert np.isnan(got[hit]).all() if np.isnan(value) else (got[hit] == value).all()
+    assert (np.abs(got - want)[~hit] <= tol[~hit]).all()
+
+
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (40, 1)])
+def test_paged_infinite_values_of_small_weight(hq, hkv):
+    rng = np.random.default_rng(85)
+    tables, lens, _, pages = P.batch(rng, [2500, 40, 300], None, 16)
+    q, kc = np.zeros((3, hq, 64), np.float32), np.zeros((pages, 16, hkv, 64), np.float32)
+    q[..., 0], kc[..., 0] = 1.0, rng.random((pages, 16, hkv)) * 0.5
+    q[:, 0, 0] = 2.0
+    kc[tables[0, 70], 3, 0, 0] = -30.0
+    kc[tables[2, 18], 11, 0, 0] = -30.0
+    q, kc, vc = P.cast(q, "f16"), P.cast(kc, "f16"), draw(rng, kc.shape, "f16")
+    clean = vc.copy()
+    clean[tables[0, 70], 3, 0, 5] = clean[tables[2, 18], 11, 0, 60] = 0
+    vc[tables[0, 70], 3, 0, 5], vc[tables[2, 18], 11, 0, 60] = np.inf, -np.inf
+    want, tol = P.paged(q, kc, clean, tables, lens, None, 0, 0, "f16", 1.0)
+    got = P.up(run(f_paged, q, kc, vc, tables, lens, scale=1.0)["output0"])
+    hit = np.zeros(got.shape, bool)
+    hit[0, :hq // hkv, 5] = hit[2, :hq // hkv, 60] = True
+    assert (got[0, :hq // hkv, 5] == np.inf).all() and (got[2, :hq // hkv, 60] == -np.inf).all()
+    assert (np.abs(got - want)[~hit] <= tol[~hit]).all()
