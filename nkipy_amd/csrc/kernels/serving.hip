@@ -185,10 +185,11 @@ struct SampleArgs {
   uint16_t *places;      // (rows, nseg, BINS + 2): where each bin's begin, and the last one's end; or how many
   uint16_t *subs;        // (rows, nseg, sub): high halves of the keys of parts' largest values
   int64_t ld;            // elements from row to row
+  double c_topp;         // 1: all (64 bits: the share that was given, where ties hold it exactly)
   int32_t rows, vocab, seg, nseg, sub;  // seg: tokens of a segment; sub: parts of one, at most 64
   float c_temp;
   int32_t c_topk;        // below 1: all
-  float c_topp, c_minp;  // 1, 0: all
+  float c_minp;          // 0: all
 };
 
 #define SMP_BLOCK 1024
@@ -601,7 +602,7 @@ __device__ __forceinline__ void sample_hist_body(const SampleArgs &a) {
     const int c = smp_list<T, SMP_SEG_BLOCK, SMP_SEG_LIST>(&count, (uint32_t *)bins, x, 0, n, low, row.best);
     for (int i = tid; i < min(c, SMP_SEG_LIST); i += SMP_SEG_BLOCK) order[i] = ((uint32_t *)bins)[i];
     if (tid == 0) places[0] = c;
-  } else if (a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.f || a.c_minp > 0.f) {
+  } else if (a.topk || a.topp || a.minp || a.c_topk > 0 || a.c_topp < 1.0 || a.c_minp > 0.f) {
     smp_segment<T>(bins, ord, red, x, n, row, ho, order, places);
   } else {
     u64 all = 0;
@@ -803,8 +804,9 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     return;
   }
   const int topk = smp_topk(a, r);
-  const float topp = a.topp ? a.topp[r] : a.c_topp, minp = a.minp ? a.minp[r] : a.c_minp;
-  const bool by_k = topk > 0 && topk < a.vocab, by_p = topp < 1.f, by_m = minp > 0.f;
+  const double topp = a.topp ? (double)a.topp[r] : a.c_topp;
+  const float minp = a.minp ? a.minp[r] : a.c_minp;
+  const bool by_k = topk > 0 && topk < a.vocab, by_p = topp < 1.0, by_m = minp > 0.f;
   const float tmin = by_m ? log2f(fminf(minp, 1.f)) : -INFINITY;  // the least depth that min_p keeps
 
   const uint64_t *hist = a.hist + (int64_t)r * a.nseg * (SMP_BINS + 1);
@@ -965,7 +967,7 @@ __device__ __forceinline__ void sample_pick_body(const SampleArgs &a) {
     else smp_search<false>(s, c, w, 0, 0, need, goal);
   };
   auto share = [&](u64 of) {  // whole steps: at least topp of it, at least one
-    return min(max((u64)ceil((double)fmaxf(topp, 0.f) * (double)of), (u64)1), of);
+    return min(max((u64)ceil(fmax(topp, 0.0) * (double)of), (u64)1), of);
   };
   bool k_cuts = by_k, p_cuts = by_p;
   if (cuts && !ranked) {

@@ -47,9 +47,9 @@ class AttendArgs(ctypes.Structure):
 class SampleArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "u", "out", "temp", "topk", "topp", "minp", "tops", "hist",
                                                  "order", "places", "subs")]
-                + [("ld", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("rows", "vocab", "seg", "nseg", "sub")]
-                + [("c_temp", ctypes.c_float), ("c_topk", ctypes.c_int32), ("c_topp", ctypes.c_float),
-                   ("c_minp", ctypes.c_float)])
+                + [("ld", ctypes.c_int64), ("c_topp", ctypes.c_double)]
+                + [(n, ctypes.c_int32) for n in ("rows", "vocab", "seg", "nseg", "sub")]
+                + [("c_temp", ctypes.c_float), ("c_topk", ctypes.c_int32), ("c_minp", ctypes.c_float)])
 
 
 def _fields(args, **values):
