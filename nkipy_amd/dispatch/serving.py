@@ -222,7 +222,9 @@ def sample(dtype, x, u, out, rows, vocab, ld, *, temperature, top_k, top_p, min_
     row or 0, number).  ``ws``: ``sample_workspace_bytes``."""
     if rows < 1 or not 1 <= vocab <= 2**22:
         raise LaunchError(f"sample: {rows} rows of {vocab}")
-    a = _fields(SampleArgs(), x=x, u=u, out=out, ld=ld, rows=rows, vocab=vocab, temp=temperature[0], c_temp=temperature[1],
+    a = _fields(SampleArgs(), x=x, u=u, out=out, ld=ld, rows=rows, vocab=vocab, temp=temperature[0],
+                # (above 0 in 32 bits too: 0 is the largest logit's)
+                c_temp=max(temperature[1], 2.0**-149) if temperature[1] > 0 else 0.0,
                 topk=top_k[0], c_topk=top_k[1], topp=top_p[0], c_topp=top_p[1], minp=min_p[0], c_minp=min_p[1])
     tag, nbytes = dtype_tag(dtype), rows * (vocab * dt.itemsize(dtype) + 8)
     if vocab <= SMP_LIST:

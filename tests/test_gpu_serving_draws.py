@@ -27,6 +27,19 @@ def test_nucleus_that_ends_on_a_tie(t, vocab):
             assert run(f_sample, x, u, top_k=top_k, top_p=top_p)["output0"][0] == at[n - 1], (top_p, top_k)
 
 
+def test_temperatures_below_32_bits():
+    """The largest logits share the draw at any temperature above 0."""
+    x = np.zeros((2, 50), np.float32)
+    x[:, 10:20] = 1.0
+    u = np.array([0.05, 0.95], np.float32)
+    for temperature in (1e-3, 1e-38, 1e-45, 1e-60, 1e-300):
+        assert list(f_sample(x, u, temperature)) == [10, 19]
+        assert list(run(f_sample, x, u, temperature=temperature)["output0"]) == [10, 19], temperature
+    for temperature in (1e38, 1e60, np.inf):
+        assert list(f_sample(x, u, temperature)) == [2, 47]
+        assert list(run(f_sample, x, u, temperature=temperature)["output0"]) == [2, 47], temperature
+
+
 @pytest.mark.parametrize("vocab", [4000, 17001])
 def test_rows_without_temperature(vocab):
     """A temperature of 0, below it or NaN takes the largest logit, the first of equal
