@@ -216,6 +216,20 @@ def _int_value(x):
     return _index_value(ctx(), x)
 
 
+_LAYOUT_OPS = ("slice", "reshape", "transpose", "broadcast_in_dim")
+_WRITE_OPS = ("dynamic_update_slice", "scatter_along_axis", "put_along_axis", "scatter_strided", "paged_write")
+
+
+def _part_of(v):
+    """The argument that ``v`` is a part or another layout of, None for a whole
+    argument and for an array that the kernel makes."""
+    part = False
+    while v.node is not None and v.node.op in _LAYOUT_OPS + _WRITE_OPS:  # (written into: the same argument)
+        part = part or v.node.op in _LAYOUT_OPS
+        v = v.node.inputs[0]
+    return v if part and v.is_parameter else None
+
+
 rotary_append = Op("rotary_append")
 
 
@@ -227,6 +241,10 @@ def _rotary_append_hip(q, k, v, cos, sin, key_cache, value_cache, block_tables, 
     for c, name in ((key_cache, "key_cache"), (value_cache, "value_cache")):
         if not is_traced(c):
             raise TypeError(f"{name} is written in place: it must be an argument of the kernel or computed from one")
+        whole = _part_of(val(c))
+        if whole is not None:
+            raise ValueError(f"{name} is a part or another layout of the argument {whole.name!r}, which a write into it would not "
+                             "reach: pass each cache as an argument of its own")
     if key_cache is value_cache:
         raise ValueError("key_cache and value_cache are the same array")
     cx = ctx()
