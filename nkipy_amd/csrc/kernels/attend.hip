@@ -21,7 +21,11 @@ __device__ __forceinline__ void attend_rows_body(const AttendArgs &a) {
   float m, l = 0.f, acc[4];
   if (att_query(a, t, b, sq, i)) {
     const AttSpan sp = att_span(a, sq, (i * (a.Hq / a.Hkv) + h % (a.Hq / a.Hkv)) / ATT_ROWS);
-    att_row<T>(a, sq, sp, b, i, h, 0, sp.nb, m, l, acc);
+    att_row<T, false>(a, sq, sp, b, i, h, 0, sp.nb, m, l, acc);
+    float z = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z = fmaf(acc[e], 0.f, z);
+    if (__any(z != 0.f)) att_row<T, true>(a, sq, sp, b, i, h, 0, sp.nb, m, l, acc);
   }
   T *o = (T *)a.o + r * a.D;
 #pragma unroll
@@ -520,7 +524,7 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
     const int src = __builtin_ctzll(spoiled);
     spoiled &= spoiled - 1;
     float m, l, x[D / 64];
-    att_row<T, D>(a2, sq2, sp2, wk2.b, __shfl(qi, src, 64), __shfl(h, src, 64), k0, k1, m, l, x);
+    att_row<T, true, D>(a2, sq2, sp2, wk2.b, __shfl(qi, src, 64), __shfl(h, src, 64), k0, k1, m, l, x);
     const int64_t at = __shfl((int)orow, src, 64);  // (rows are below 2^31)
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
@@ -753,7 +757,7 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
     if (h0 + r >= rep) break;
     if (r % NW != wave) continue;
     float mr, lr, x[D / 64];
-    att_row<T, D>(a, sq, sp, b, 0, g * rep + h0 + r, j0, j1, mr, lr, x);
+    att_row<T, true, D>(a, sq, sp, b, 0, g * rep + h0 + r, j0, j1, mr, lr, x);
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
       if (pieces == 1) {
