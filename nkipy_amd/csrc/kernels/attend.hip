@@ -86,9 +86,6 @@ template <> struct Mat<f16> {
   static constexpr float LIMIT = 16384.f, TOP = 10.f;
   static NK_DEVICE f32x16 mul(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
-template <bool B> struct Flag {
-  static constexpr bool value = B;
-};
 #define ATT_LOWEST -3.40282347e38f  // the least finite offset
 template <int N> struct Slot {
   static constexpr int value = N;
@@ -456,14 +453,16 @@ __device__ __forceinline__ void attend_tile_body(const AttendArgs &a) {
   float *wo = a.ws + (split * nr + orow) * D, *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + orow) * 2;
   uint16_t *o = (uint16_t *)a.o + orow * D;
 
-  // whether this row sees any key of these blocks, pages aside
+  // whether this row, if it has no weight, sees any key of these blocks, pages aside
   bool sees = false;
-  auto part = [&](int a0, int a1) __attribute__((always_inline)) {  // (blocks that follow each other)
-    const int lo = sp.kb(a0) * ATT_KEYS, hi = min(sp.kb(a1 - 1) * ATT_KEYS + ATT_KEYS - 1, klim);
-    sees |= a0 < a1 && (max(lo, p - a.window + 1) <= hi || lo <= min(hi, a.sinks - 1));
-  };
-  part(j0, min(j1, sp.ns));
-  part(max(j0, sp.ns), j1);
+  if (__any(ok && l_run == 0.f)) {
+    auto part = [&](int a0, int a1) __attribute__((always_inline)) {  // (blocks that follow each other)
+      const int lo = sp.kb(a0) * ATT_KEYS, hi = min(sp.kb(a1 - 1) * ATT_KEYS + ATT_KEYS - 1, klim);
+      sees |= a0 < a1 && (max(lo, p - a.window + 1) <= hi || lo <= min(hi, a.sinks - 1));
+    };
+    part(j0, min(j1, sp.ns));
+    part(max(j0, sp.ns), j1);
+  }
 
   // rows that a value which is not finite may have spoiled
   float z = l_run * 0.f;
