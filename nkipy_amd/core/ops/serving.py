@@ -22,7 +22,10 @@ reaches every query that sees its key with a score above -inf, however small
 the weight.
 
 The CPU forms are the definitions, evaluated in float64 and rounded once.  On
-the GPU scores are 32-bit sums: a row that sees one past their range is NaN.
+the GPU scores and weighted values are 32-bit sums: a row that sees a score past
+their range is NaN.  Operands of 16 bits with a head_dim of 64 or 128 have their
+weights rounded to the operands' type before the values are summed, which adds
+up to half a step of that type to the result's own.
 """
 
 from __future__ import annotations
@@ -462,7 +465,11 @@ def _sample_cpu(logits, uniform, temperature=1.0, top_k=None, top_p=None, min_p=
     uniform times their sum.  A temperature of 0 takes the largest logit.
     Filters are numbers or one value per row; those of a row outside their
     range count as the nearest end.  NaN and -inf logits are never drawn; a
-    row without any other gives -1."""
+    row without any other gives -1.
+
+    On the GPU weights are whole steps of 2^-36 of the largest: tokens below
+    2^-37 of it (25.6 temperatures under the largest logit) are never drawn and
+    add nothing to a sum; a share is taken of those sums, exactly."""
     rows, vocab, temperature, top_k, top_p, min_p = _check_sample(logits, uniform, temperature, top_k, top_p, min_p)
     x = _to64(logits)
     row = lambda v, r: v if not hasattr(v, "shape") else v[r]  # noqa: E731

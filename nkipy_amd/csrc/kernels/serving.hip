@@ -16,7 +16,9 @@ using namespace nk;
 // read and written once.  One workgroup per token: its sequence, position and
 // page are found once and its heads share the tables' row.  A thread moves E
 // elements of each half of a pair (16 bytes with E = 8).  8000 tokens of 32 / 8
-// heads of 128, bf16: 40 us, 4.9 TB/s.
+// heads of 128, bf16: 40 us, 5.0 TB/s, over inputs that change from call to call; 31
+// over the same ones, which the last-level cache then holds in part.  In single
+// elements (20 of 128 rotated) 120.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   const void *q, *k, *v;
@@ -141,7 +143,7 @@ NK_APPEND(float, f32)
 // index) that stays, and the row is never sorted.
 //
 // Long rows take three launches, two of them over segments of the row, so that
-// a few rows fill the chip:
+// eight rows and more fill the chip (fewer stay on as many XCDs, one each: smp_place):
 //   top    each segment's largest value, and those of its parts, some lanes' each;
 //   hist   each segment's counts and weights over BINS equal steps of t, a bin's
 //          both in one word (14 bits count up to 8192 tokens, 50 the weight), so
@@ -169,8 +171,8 @@ NK_APPEND(float, f32)
 //
 // Bound by the latency of one CU's steps in pick, by about 30 instructions per
 // logit in hist, and by one read of the logits (top, hist, pick in us): 64 rows of
-// 151936 bf16 with every filter 6, 11, 16, by nucleus alone 7, 20, 40; 17 rows of
-// 128257 fp32 by nucleus 5, 12, 33; one row of 32000 with top_k 3, 8, 9.
+// 151936 bf16 with every filter 6, 12, 16, by nucleus alone 7, 20, 40; 17 rows of
+// 128257 fp32 by nucleus 5, 12, 34; one row of 32000 with top_k 3, 9, 9.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
   const void *x;

@@ -82,8 +82,8 @@ def rotary_append(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q=0, 
                   bytes=nbytes)
 
 
-ATT_ROWS, ATT_KEYS = 128, 32  # rows of a tile, keys of a block (attend.h)
-ATT_CUS, ATT_SLOTS = 256, 512  # CUs; workgroups that fill them, two each
+ATT_ROWS, ATT_KEYS = 128, 32  # rows of a tile, keys of a block (attend_index.h)
+ATT_CUS, ATT_SLOTS = 256, 512  # CUs; workgroups that a step is split into (two a CU; three or more would fit)
 ATT_STEP_GRID = 2048          # workgroups of a step, to even out lengths
 ATT_STEP_BLOCKS = 32          # blocks that a split of a step has at least past ATT_SLOTS
 ATT_MIN_BLOCKS = 4            # blocks that any split of a step has at least
@@ -106,15 +106,19 @@ def attend_work(B, S, N, Hq, Hkv, D, keys, window=0, sinks=0, starts=False) -> T
 
     A step's keys are split where the rest leaves CUs idle, and long ones
     further, so that sequences of many lengths end together (64 of up to 8192
-    keys: 260 us with one split, 238 with four; 64 with a window of 500: 27 us
-    with one, 45 with four).
+    keys: 263 us with one split, 242 with four; 64 with a window of 500: 27 us
+    with one, 33 with four).
 
-    Tiles take the splits of the least estimated time, in us: a block of keys is
-    0.75 for a CU's only workgroup and 0.52 for each of more; the sums of every
-    split are written and read at 4.5 TB/s, by a launch of 5.  (Measured: 1000
-    tokens of one prompt 27 us with one split, 42 with eight; 256 tokens behind
-    3744 cached 42 with seven, 44 with four, 104 with one; 40 tokens of eight
-    sequences of 8000 43 with seven, 60 with three.)"""
+    Tiles take the splits of the least estimate: a block of keys counts 0.75 for
+    a CU's only workgroup and 0.52 for each of more; the sums of every split are
+    written and read at 4.5 TB/s, by a launch of 5.  The constants were fitted, at
+    head dim 128, to which split wins below; they rank splits and are no times
+    (2100 tokens of 24 sequences in a window of 1024: 55 by the estimate, 82 us
+    measured, as two workgroups share a CU and the third waits).  Measured, whole
+    calls: 1000 tokens of one prompt 27 us with one split, 46 with eight; 256
+    tokens behind 3744 cached 42 with seven or four, 95 with one; 40 tokens of
+    eight sequences of 8000 44 with seven, 72 with three; the 2100 tokens 82 with
+    one, 115 with two."""
     rep = Hq // Hkv
     step = not starts and S == 1
     if step:
@@ -177,8 +181,8 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     far = not step and (reach >= 2**32 - 4096 or (tables and k_str[1] != v_str[1]))
     kind = f"{'step' if step else 'tile'}_{'paged' if tables else 'plain'}{'_far' if far else ''}"
     out = [Launch("attend", f"nk_attend_{kind}_{tag}_d{D}", (a.tiles * Hkv * a.nsplit, 1, 1), (256, 1, 1), a)]
-    # a workgroup a row, then a wave, us: 32 rows of 63 splits 14 and 29, 256 of 19
-    # 94 and 99, 1024 of 8 46.3 and 45.7, 8192 of 7 58 and 42
+    # whole calls with a workgroup a row and with a wave, us: 32 rows of 63 splits
+    # 14.4 and 31.5, of 12 10.2 and 10.5, 256 of 19 97 and 100, 1280 of 7 45.5 and 43.8
     if a.nsplit > ATT_JOIN_WIDE and N * Hq < ATT_JOIN_ROWS:
         out.append(Launch("attend", f"nk_attend_join4_{tag}_d{D}", (N * Hq, 1, 1), (256, 1, 1), a))
     elif a.nsplit > 1:
@@ -255,7 +259,8 @@ def _contiguous(v: Value) -> Tuple[View, List[int]]:
 
 def _strided(v: Value) -> Tuple[View, List[int]]:
     """``v`` as a view with one stride per dimension and a dense last one, or
-    ``v`` itself, materialised."""
+    ``v`` itself, materialised: a step of its own in the plan, which copies all of
+    it (a cache whose layout is no such view is better laid out once)."""
     vw = resolve(v, widen_ok=False)
     st = [vw.simple(d) for d in range(v.ndim)]
     if any(s is None for s in st) or (st[-1] != 1 and v.shape[-1] != 1) or vw.base.dtype != v.dtype:
