@@ -219,7 +219,12 @@ class Lowering:
             res = g.results[a.output_index]
             p = param_by_name[f"{a.param_name}.must_alias_input"]
             prod = res.node
-            late = prod is None or not self._reads_done_before(p, prod, order)
+            chain = self._write_chain(p, prod, order)
+            late = prod is None or not self._reads_done_before(p, (chain or [prod])[0], order)
+            if late and chain:
+                chain, late = [], not self._reads_done_before(p, prod, order)
+            for n in chain[:-1]:
+                slots[n.out.id] = slots[res.id]
             if late:
                 # the producer writes a staging temporary; a final copy moves
                 # it into the caller's (aliased) buffer
@@ -274,6 +279,20 @@ class Lowering:
             plan.steps.append(G.ProgramStep(f"write back {res.name}", G.flat_copy_program(res), outv))
         G.fuse_swiglu_planes(plan)
         return plan
+
+    def _write_chain(self, p: Value, last: Node, order: Dict[int, int]) -> List[Node]:
+        """Paged writes one after the other from parameter ``p`` to ``last``,
+        each done with by its readers when the next one's step begins: all of
+        them may write ``p``'s buffer.  Empty where ``last`` is the only one."""
+        chain = [last]
+        while chain[0] is not None and chain[0].op == "paged_write":
+            before = chain[0].inputs[0]
+            if before is p:
+                return chain if len(chain) > 1 else []
+            if before.id in self.result_ids or before.is_parameter or not self._reads_done_before(before, chain[0], order):
+                break
+            chain.insert(0, before.node)
+        return []
 
     _INPLACE_OPS = ("dynamic_update_slice", "scatter_along_axis", "put_along_axis", "scatter_strided", "paged_write")
 

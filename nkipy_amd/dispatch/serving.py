@@ -315,9 +315,10 @@ class AppendMatch(Match):
             n = parts[p]
             cache = n.inputs[0]
             shape = dict(page=cache.shape[1], pages=cache.shape[0], Hkv=cache.shape[2], D=cache.shape[3])
-            # the caller's buffer, or a copy of the cache where that is still read
+            # the caller's buffer (behind an earlier write, too), or a copy of the cache
+            # where that is still read
             src, dst = plan.buffers[plan.slot(cache).buffer], plan.buffers[plan.slot(n.out).buffer]
-            own = dst.kind == "output" and src.kind == "input" and plan.alias_outputs.get(dst.name) == src.name
+            own = src is dst or dst.kind == "output" and src.kind == "input" and plan.alias_outputs.get(dst.name) == src.name
             if not own:
                 steps.append(G.ProgramStep(f"copy {cache!r}", G.flat_copy_program(cache), n.out))
         some = next(iter(parts.values()))
