@@ -89,13 +89,15 @@ def qwen3_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, norm_eps
 
 def qwen3_paged_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, norm_eps, n_heads, head_dim, n_kv_heads,
                                  key_cache, value_cache, block_tables, context_lens, query_starts, o_weight,
-                                 rope_base=1000000, window=None, sinks=0):
+                                 rope_base=1000000, window=None, sinks=0, cos=None, sin=None):
     """x (tokens, hidden), the new tokens of all sequences one after another ->
     (tokens, hidden); key_cache / value_cache (pages, page_size, n_kv_heads,
     head_dim) take their keys and values in place.  Sequence b's tokens are
     query_starts[b] .. query_starts[b + 1] - 1, the last of its
     context_lens[b] (``query_starts=None``: one token each), on the pages of
-    block_tables[b]; a window with its sinks narrows what each sees."""
+    block_tables[b]; a window with its sinks narrows what each sees.  cos / sin
+    (positions, head_dim / 2): rotary tables that the layers share; without
+    them each kernel holds its own, as long as block_tables is wide."""
     n = x.shape[0]
     q_end = n_heads * head_dim
     k_end = q_end + n_kv_heads * head_dim
@@ -103,9 +105,12 @@ def qwen3_paged_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, no
     xq = rmsnorm_kernel(xq.reshape(n, n_heads, head_dim), q_norm_weight, norm_eps)
     xk = rmsnorm_kernel(xk.reshape(n, n_kv_heads, head_dim), k_norm_weight, norm_eps)
     xv = xv.reshape(n, n_kv_heads, head_dim)
-    cos, sin = compute_cos_sin_cache(head_dim, block_tables.shape[1] * key_cache.shape[1], base=rope_base)
-    xq = tensor_apis.rotary_append(xq, xk, xv, tensor_apis.constant(cos), tensor_apis.constant(sin), key_cache, value_cache,
-                                   block_tables, context_lens, query_starts)
+    if (cos is None) != (sin is None):
+        raise ValueError("give both of cos and sin, or neither")
+    if cos is None:
+        cos, sin = (tensor_apis.constant(x) for x in compute_cos_sin_cache(
+            head_dim, block_tables.shape[1] * key_cache.shape[1], base=rope_base))
+    xq = tensor_apis.rotary_append(xq, xk, xv, cos, sin, key_cache, value_cache, block_tables, context_lens, query_starts)
     out = tensor_apis.paged_attention(xq, key_cache, value_cache, block_tables, context_lens, query_starts,
                                       window=window, sinks=sinks)
     return np.matmul(out.reshape(n, q_end), o_weight)
