@@ -713,13 +713,15 @@ __device__ __forceinline__ void attend_step_body(const AttendArgs &a) {
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
   float *so = reinterpret_cast<float *>(lds), *sm = so + NW * 16 * D;  // (NW, 16, D) sums; (NW, 16) weights, (16) in all
-  __shared__ uint32_t spoiled[NW];  // a bit for each row with a sum that is not finite
-  float z = l_run * 0.f;
+  // a bit for each row with a sum that is not finite under weights that are (those of
+  // a NaN score are NaN, and so is all of the row)
+  __shared__ uint32_t spoiled[NW];
+  float z = 0.f;
 #pragma unroll
   for (int t = 0; t < D / 16; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) z = __builtin_fmaf(acc[t][r], 0.f, z);
-  uint64_t bits = __ballot(z != 0.f);
+  uint64_t bits = __ballot(z != 0.f && l_run == l_run);
   bits |= bits >> 32;
   if (lane == 0) spoiled[wave] = (uint32_t)(bits | bits >> 16) & 0xffffu;
   __syncthreads();

@@ -109,3 +109,24 @@ def test_paged_infinite_values_of_small_weight(hq, hkv):
     hit[0, :hq // hkv, 5] = hit[2, :hq // hkv, 60] = True
     assert (got[0, :hq // hkv, 5] == np.inf).all() and (got[2, :hq // hkv, 60] == -np.inf).all()
     assert (np.abs(got - want)[~hit] <= tol[~hit]).all()
+
+
+@pytest.mark.parametrize("S,K", [(1, 130), (1, 3000), (40, 300)])
+@pytest.mark.parametrize("t,d", [("bf16", 64), ("f16", 128), ("f32", 48)])
+def test_scores_that_are_no_number(t, d, S, K):
+    """A NaN query, and a NaN key, make the rows that meet them NaN, whole, and no other."""
+    rng = np.random.default_rng(86)
+    q, k, v = draw(rng, (3, S, 4, d), t), draw(rng, (3, K, 2, d), t), draw(rng, (3, K, 2, d), t)
+    want, tol = P.dense(q, k, v, None, None, 0, 0, t)
+    q[0, S - 1, 2, 3] = P.cast(np.float32(np.nan), t)
+    k[1, K - 1, 0, 5] = P.cast(np.float32(np.nan), t)
+    v[0, 2, 1, 9] = P.cast(np.float32(np.inf), t)  # (seen by the NaN query as well)
+    hit = np.zeros(want.shape, bool)
+    hit[0, S - 1, 2] = hit[1, S - 1, :2] = True
+    got = P.up(run(f_window, q, k, v)["output0"])
+    assert np.isnan(got[hit]).all()
+    inf = np.zeros(want.shape, bool)
+    inf[0, :, 2:, 9] = True
+    inf &= ~hit
+    assert (got[inf] == np.inf).all()
+    assert (np.abs(got - want)[~hit & ~inf] <= tol[~hit & ~inf]).all()
