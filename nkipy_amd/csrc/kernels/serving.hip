@@ -171,8 +171,8 @@ NK_APPEND(float, f32)
 //
 // Bound by the latency of one CU's steps in pick, by about 30 instructions per
 // logit in hist, and by one read of the logits (top, hist, pick in us): 64 rows of
-// 151936 bf16 with every filter 6, 12, 16, by nucleus alone 7, 20, 40; 17 rows of
-// 128257 fp32 by nucleus 5, 12, 34; one row of 32000 with top_k 3, 9, 9.
+// 151936 bf16 with every filter 6, 11, 16, by nucleus alone 7, 20, 40; 17 rows of
+// 128257 fp32 by nucleus 5, 12, 34; one row of 32000 with top_k 3, 8, 9.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
   const void *x;
