@@ -34,6 +34,12 @@ Op vocabulary (attributes in brackets):
   paged_attention [window, sinks, scale, starts] (q, keys, values, tables, lengths[, starts])
   window_attention [window, sinks, scale, lengths, positions] (q, k, v[, lengths][, positions])
   sample [temperature, top_k, top_p, min_p] (logits, uniform[, filters given per row])
+  paged_attention_fp8 [window, sinks, scale, starts] (q, keys, values, key exps, value exps, tables, lengths[, starts])
+  and, one node for each result or updated operand (attributes part, and target: which operand) over the same operands:
+  append_fp8 [starts] (q, k, v, cos, sin, keys, values, key exps, value exps, tables, lengths[, starts])
+  assign_pages [pages, page, tokens] (tables, lengths, new lengths)
+  beam_select [end] (logits, scores, ended)
+  beam_reorder (parents, lengths, tables, keys, values[, key exps, value exps])
 """
 
 from __future__ import annotations

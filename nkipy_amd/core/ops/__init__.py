@@ -2,6 +2,7 @@
 
 from nkipy_amd.core.backend import get_backend, set_source_location
 from nkipy_amd.core.ops._registry import Op
+from nkipy_amd.core.ops.beams import assign_pages, beam_reorder, beam_select
 from nkipy_amd.core.ops.creation import (
     constant, diag, empty_like, full, full_like, ones_like, tril, triu, zeros, zeros_like,
 )
@@ -23,6 +24,7 @@ from nkipy_amd.core.ops.reduce import (
     all, any, argmax, argmin, count_nonzero, cumsum, max, mean, min, prod, std, sum, var,
 )
 from nkipy_amd.core.ops.serving import paged_attention, rotary_append, sample, window_attention
+from nkipy_amd.core.ops.serving_fp8 import paged_attention_fp8, rotary_append_fp8
 from nkipy_amd.core.ops.transform import (
     astype, broadcast_to, concatenate, copy, copyto, diff, expand_dims, flip, pad, repeat,
     reshape, roll, split, squeeze, stack, swapaxes, tile, transpose,

@@ -1,0 +1,213 @@
+// Keys and values rotated and quantised into a paged cache of e4m3 codes.
+
+#include "cache8.h"
+
+using namespace nk;
+
+// ---------------------------------------------------------------------------
+// With row p of the tables for the token at position p, and one exponent e for
+// the rows of a page and head:
+//
+//   y_i = x_i c_i - x_{i+r/2} s_i,  y_{i+r/2} = x_i s_i + x_{i+r/2} c_i,   i < r/2
+//   code = e4m3(y 2^-e),  e the least with max |y| <= 448 2^e (and none below the
+//   page's where rows written earlier stay)
+//
+// in fp32, every product and sum rounded by itself, so that the largest magnitude,
+// and with it e, is what the same steps give anywhere.  Workgroups: one for each
+// token's queries; one for each (page that a sequence writes, keys or values, some
+// heads), which reads its rows twice: for the largest magnitude, then, mostly from
+// cache, for the codes.  Maxima are of whole numbers (bits), so no order changes
+// them.  Bound by memory, single tokens by latency.
+// ---------------------------------------------------------------------------
+struct Append8Args {
+  const void *q, *k, *v;
+  void *oq;                // (N, Hq, D); null: left out
+  uint8_t *kc, *vc;        // (pages, page, Hkv, D)
+  int32_t *ke, *ve;        // (pages, Hkv)
+  const float *cos, *sin;  // (P, half)
+  const int32_t *tables, *lens, *starts;
+  int64_t q_ss, q_sh, k_ss, k_sh, v_ss, v_sh;  // element strides of rows and heads
+  int32_t B, N, Hq, Hkv, D, half, P;
+  int32_t page, pages, width;
+  int32_t heads;  // of a workgroup, up to A8_HEADS
+};
+#define A8_HEADS 64
+
+// the sequence of token or tile t, by its first one: the last that begins at or before
+template <typename F>
+NK_DEVICE int a8_find(int n, int t, F f) {
+  const int lane = threadIdx.x & 63;
+  int c = 0;
+  for (int b0 = 0; b0 < n; b0 += 64) c += __popcll(__ballot(b0 + lane < n && f(min(b0 + lane, n - 1)) <= t));
+  return c - 1;
+}
+struct A8Seq {
+  int lo, n, len;
+};
+NK_DEVICE A8Seq a8_seq(const Append8Args &a, int b) {
+  A8Seq s;
+  s.lo = b, s.n = 1;
+  if (a.starts) {
+    s.lo = min(max(a.starts[b], 0), a.N);
+    s.n = min(max(a.starts[b + 1], s.lo), a.N) - s.lo;
+  }
+  s.len = min(max(a.lens[b], 0), 1 << 30);
+  return s;
+}
+// Pages that a sequence writes are tiles floor(start / page) + 2 b ...: room for
+// the n / page + 2 that n tokens may touch.
+NK_DEVICE int a8_tile0(const Append8Args &a, int b) { return min(max(a.starts[b], 0), a.N) / a.page + 2 * b; }
+
+// E elements of both halves of a rotated piece, or of a piece that is copied
+template <typename T, int E>
+NK_DEVICE void a8_turn(const T *x, const float *cr, const float *sr, int half, float (&y0)[E], float (&y1)[E]) {
+#pragma clang fp contract(off)
+  float x0[E], x1[E], c[E], s[E];
+  Piece<T, E>::load(x, x0);
+  Piece<T, E>::load(x + half, x1);
+  Piece<float, E>::load(cr, c);
+  Piece<float, E>::load(sr, s);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float p0 = x0[e] * c[e], p1 = x1[e] * s[e], p2 = x0[e] * s[e], p3 = x1[e] * c[e];
+    y0[e] = p0 - p1;
+    y1[e] = p2 + p3;
+  }
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void append8_queries(const Append8Args &a, int t) {
+  int b = t;
+  if (a.starts) b = a8_find(a.B, t, [&](int x) { return a.starts[x]; });
+  int p = -1;
+  if (b >= 0) {
+    const A8Seq s = a8_seq(a, b);
+    if (t - s.lo < s.n) p = s.len - s.n + (t - s.lo);
+  }
+  const bool in = p >= 0 && p < a.P;
+  const int turns = a.half / E, per = turns + (a.D - 2 * a.half) / E;
+  const float *cr = a.cos + (int64_t)(in ? p : 0) * a.half, *sr = a.sin + (int64_t)(in ? p : 0) * a.half;
+  for (int x = threadIdx.x; x < a.Hq * per; x += 256) {
+    const int h = x / per, c = x % per;
+    const T *src = (const T *)a.q + t * a.q_ss + h * a.q_sh;
+    T *dst = (T *)a.oq + ((int64_t)t * a.Hq + h) * a.D;
+    if (!in) {
+      const float z[E] = {};
+      const int d = c < turns ? c * E : 2 * a.half + (c - turns) * E;
+      Piece<T, E>::store(dst + d, z);
+      if (c < turns) Piece<T, E>::store(dst + a.half + d, z);
+    } else if (c >= turns) {
+      copy_piece<T, E>(src + 2 * a.half + (c - turns) * E, dst + 2 * a.half + (c - turns) * E);
+    } else {
+      float y0[E], y1[E];
+      a8_turn<T, E>(src + c * E, cr + c * E, sr + c * E, a.half, y0, y1);
+      Piece<T, E>::store(dst + c * E, y0);
+      Piece<T, E>::store(dst + a.half + c * E, y1);
+    }
+  }
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void append8_body(const Append8Args &a) {
+  __shared__ uint32_t top[A8_HEADS];
+  __shared__ int32_t now[A8_HEADS], old[A8_HEADS];
+  const int tid = threadIdx.x, nq = a.oq ? a.N : 0;
+  if ((int)blockIdx.x < nq) {
+    append8_queries<T, E>(a, blockIdx.x);
+    return;
+  }
+  const int parts = (a.Hkv + a.heads - 1) / a.heads;
+  int w = blockIdx.x - nq;
+  const int h0 = w % parts * a.heads, hn = min(a.heads, a.Hkv - h0);
+  w /= parts;
+  const bool values = w & 1;
+  const int t = w >> 1;
+  int b = t, i = 0;
+  if (a.starts) {
+    b = a8_find(a.B, t, [&](int x) { return a8_tile0(a, x); });
+    if (b < 0) return;
+    i = t - a8_tile0(a, b);
+  }
+  const A8Seq s = a8_seq(a, b);
+  const int p0 = s.len - s.n;              // of the first new token
+  const int g = max(p0, 0) / a.page + i;   // page of the sequence
+  if (i < 0 || g >= a.width) return;
+  const int lo = max(g * a.page, max(p0, 0)), hi = min(min(g * a.page + a.page, s.len), a.P);  // positions written
+  if (lo >= hi) return;
+  const int pg = a.tables[(int64_t)b * a.width + g];
+  if (pg < 0 || pg >= a.pages) return;
+  const int first = lo - g * a.page, n = hi - lo;
+  int32_t *const exps = (values ? a.ve : a.ke) + (int64_t)pg * a.Hkv + h0;
+  uint8_t *const codes = (values ? a.vc : a.kc) + ((int64_t)pg * a.page * a.Hkv + h0) * a.D;
+  const T *const src = values ? (const T *)a.v + (int64_t)(s.lo + lo - p0) * a.v_ss + h0 * a.v_sh
+                              : (const T *)a.k + (int64_t)(s.lo + lo - p0) * a.k_ss + h0 * a.k_sh;
+  const int64_t ss = values ? a.v_ss : a.k_ss, sh = values ? a.v_sh : a.k_sh;
+  const int half = values ? 0 : a.half;
+  const int turns = half / E, per = turns + (a.D - 2 * half) / E;
+
+  if (tid < hn) top[tid] = 0, old[tid] = first ? c8_clip(exps[tid]) : C8_MIN;
+  __syncthreads();
+  // every piece of these rows: f(row, head, first element, whether it is a pair, its values)
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    for (int x = tid; x < n * hn * per; x += 256) {
+      const int r = x / (hn * per), y = x % (hn * per), h = y / per, c = y % per;
+      const T *from = src + r * ss + h * sh;
+      float y0[E], y1[E];
+      if (c < turns) {
+        const int64_t at = (int64_t)(lo + r) * half + c * E;
+        a8_turn<T, E>(from + c * E, a.cos + at, a.sin + at, half, y0, y1);
+        f(r, h, c * E, true, y0, y1);
+      } else {
+        const int d = 2 * half + (c - turns) * E;
+        Piece<T, E>::load(from + d, y0);
+        f(r, h, d, false, y0, y0);
+      }
+    }
+  };
+  int mine = -1;
+  uint32_t most = 0;
+  each([&](int, int h, int, bool pair, const float (&y0)[E], const float (&y1)[E]) __attribute__((always_inline)) {
+    if (h != mine) {
+      if (most) atomicMax(&top[mine], most);
+      mine = h, most = 0;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t u = __float_as_uint(y0[e]) & 0x7fffffffu, v = __float_as_uint(y1[e]) & 0x7fffffffu;
+      if (u < 0x7f800000u) most = max(most, u);
+      if (pair && v < 0x7f800000u) most = max(most, v);
+    }
+  });
+  if (most) atomicMax(&top[mine], most);
+  __syncthreads();
+  if (tid < hn) {
+    const int e = max(c8_exponent(__uint_as_float(top[tid])), old[tid]);
+    now[tid] = e;
+    exps[tid] = e;
+  }
+  __syncthreads();
+  each([&](int r, int h, int d, bool pair, const float (&y0)[E], const float (&y1)[E]) __attribute__((always_inline)) {
+    const float scale = c8_power(-now[h]);
+    uint8_t *to = codes + ((int64_t)(first + r) * a.Hkv + h) * a.D + d;
+    c8_store<E>(to, y0, scale);
+    if (pair) c8_store<E>(to + half, y1, scale);
+  });
+  // the rows before, where the scale grew
+  for (int h = 0; h < hn && first; ++h) {
+    const int by = old[h] - now[h];
+    if (by == 0) continue;
+    const float scale = c8_power(max(by, -126));
+    for (int x = tid; x < first * (a.D / E); x += 256) {
+      uint8_t *at = codes + ((int64_t)(x / (a.D / E)) * a.Hkv + h) * a.D + x % (a.D / E) * E;
+      float y[E];
+      c8_load<E>(at, y);
+      c8_store<E>(at, y, scale);
+    }
+  }
+}
+#define NK_APPEND8(T, name)                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void nk_append8_##name(Append8Args a) { append8_body<T, 8>(a); }   \
+  extern "C" __global__ __launch_bounds__(256) void nk_append81_##name(Append8Args a) { append8_body<T, 1>(a); }
+NK_APPEND8(bf16, bf16)
+NK_APPEND8(f16, f16)
+NK_APPEND8(float, f32)

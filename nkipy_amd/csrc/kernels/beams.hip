@@ -1,0 +1,524 @@
+// A generation loop around its kernels: block tables and slots from lengths, the
+// choice of a beam search's beams, and the paged caches that follow them.
+
+#include "common.h"
+
+using namespace nk;
+
+typedef unsigned long long u64;
+
+// running sums over the lanes of a wave, this one's included
+template <typename T>
+NK_DEVICE T running(T v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const T u = __shfl_up(v, o, 64);
+    v += lane >= o ? u : 0;
+  }
+  return v;
+}
+// and over a workgroup of W waves; `all`: the whole sum
+template <int W, typename T>
+NK_DEVICE T running_block(T v, T *red, T &all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  v = running(v);
+  __syncthreads();
+  if (lane == 63) red[wave] = v;
+  __syncthreads();
+  // (the waves' sums again by a running sum: W registers less)
+  const T w = running(lane < W ? red[lane] : 0);
+  all = __shfl(w, W - 1, 64);
+  if (wave) v += __shfl(w, wave - 1, 64);
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// Block tables.
+//
+// Row b holds ceil((len - new) / page) pages; those of all rows are marked in a
+// bitmap in LDS.  What is not marked is free, and the r-th free page goes to the
+// r-th entry that wants one: r by running sums over the rows, the page by running
+// counts over the bitmap.  Marks are ORs and sums are whole numbers, so no order
+// changes a result.  Bound by latency: one workgroup, a few dependent reads.
+// ---------------------------------------------------------------------------
+struct AssignArgs {
+  int32_t *tables;  // (rows, width)
+  const int32_t *lens, *news;
+  int32_t *starts, *slots, *free;
+  int32_t *wants;  // (rows) pages wanted by the rows before
+  int32_t rows, width, page, pages, tokens;
+  int32_t small;  // the slots are this launch's too
+};
+#define ASG_BLOCK 1024
+#define ASG_WORDS 32768  // of 32 pages
+
+struct AsgRow {
+  int len, fresh, held, need;
+};
+NK_DEVICE AsgRow asg_row(const AssignArgs &a, int b) {
+  AsgRow r;
+  r.len = min(max(a.lens[b], 0), 1 << 30);
+  r.fresh = min(max(a.news[b], 0), 1 << 30);
+  // (sums below 2^31: page is at most 2^30)
+  r.held = min((int)(((uint32_t)max(r.len - r.fresh, 0) + (uint32_t)a.page - 1) / (uint32_t)a.page), a.width);
+  r.need = min((int)(((uint32_t)r.len + (uint32_t)a.page - 1) / (uint32_t)a.page), a.width);
+  return r;
+}
+
+// Slots of 64 tokens t0 ..: the rows that begin among them are read side by side.
+NK_DEVICE void asg_slots(const AssignArgs &a, int t0) {
+  const int lane = threadIdx.x & 63, t = t0 + lane;
+  int b0 = 0;  // rows that begin at or before t0
+  for (int b = 0; b < a.rows; b += 64) b0 += __popcll(__ballot(b + lane < a.rows && a.starts[min(b + lane, a.rows - 1)] <= t0));
+  int b = b0 - 1;
+  for (int x = b0;; x += 64) {
+    const int s = x + lane < a.rows ? a.starts[x + lane] : 0x7fffffff;
+    int more = 0;
+#pragma unroll 8
+    for (int k = 0; k < 64; ++k) more += __builtin_amdgcn_readlane(s, k) <= t ? 1 : 0;
+    b += more;
+    if (!__any(more == 64)) break;
+  }
+  if (t >= a.tokens) return;
+  int slot = -1;
+  if (b >= 0 && t < a.starts[b + 1]) {
+    const int p = min(max(a.lens[b], 0), 1 << 30) - min(max(a.news[b], 0), 1 << 30) + (t - a.starts[b]);
+    if (p >= 0 && p / a.page < a.width) {
+      const int pg = a.tables[(int64_t)b * a.width + p / a.page];
+      if (pg >= 0 && pg < a.pages) slot = pg * a.page + p % a.page;
+    }
+  }
+  a.slots[t] = slot;
+}
+
+extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_pages(AssignArgs a) {
+  __shared__ uint32_t used[ASG_WORDS];
+  __shared__ int32_t before[ASG_BLOCK];  // free pages before a thread's words
+  __shared__ int64_t red[ASG_BLOCK / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int words = (a.pages + 31) / 32;
+  for (int i = tid; i < words; i += ASG_BLOCK) used[i] = 0;
+  __syncthreads();
+  for (int b = wave; b < a.rows; b += ASG_BLOCK / 64) {
+    const int held = asg_row(a, b).held;
+    for (int i = lane; i < held; i += 64) {
+      const int pg = a.tables[(int64_t)b * a.width + i];
+      if (pg >= 0 && pg < a.pages) atomicOr(&used[pg >> 5], 1u << (pg & 31));
+    }
+  }
+  int64_t starts = 0, wants = 0, all;
+  for (int b0 = 0; b0 < a.rows; b0 += ASG_BLOCK) {
+    const int b = b0 + tid;
+    int64_t n = 0, w = 0;
+    if (b < a.rows) {
+      const AsgRow r = asg_row(a, b);
+      n = r.fresh, w = max(r.need - r.held, 0);
+    }
+    const int64_t ns = running_block<ASG_BLOCK / 64>(n, red, all) + starts;
+    starts += all;
+    const int64_t ws = running_block<ASG_BLOCK / 64>(w, red, all) + wants;
+    wants += all;
+    if (b < a.rows) {
+      a.starts[b] = (int32_t)min(ns - n, (int64_t)0x7fffffff);
+      a.wants[b] = (int32_t)min(ws - w, (int64_t)a.pages);
+    }
+  }
+  const int per = (words + ASG_BLOCK - 1) / ASG_BLOCK, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+  __syncthreads();
+  if (tid == 0 && (a.pages & 31)) used[words - 1] |= ~0u << (a.pages & 31);  // (no pages)
+  __syncthreads();
+  int64_t n = 0;
+  for (int i = w0; i < w1; ++i) n += __popc(~used[i]);
+  const int64_t upto = running_block<ASG_BLOCK / 64>(n, red, all);
+  before[tid] = (int32_t)(upto - n);
+  if (tid == 0) {
+    a.starts[a.rows] = (int32_t)min(starts, (int64_t)0x7fffffff);
+    a.free[0] = (int32_t)max(all - wants, (int64_t)-0x7fffffff);
+  }
+  __syncthreads();
+  const int free = (int)all;
+  for (int b = wave; b < a.rows; b += ASG_BLOCK / 64) {
+    const AsgRow r = asg_row(a, b);
+    const int first = a.wants[b];
+    for (int i = r.held + lane; i < a.width; i += 64) {
+      int pg = -1;
+      const int k = first + (i - r.held);
+      if (i < r.need && k < free) {
+        // the last thread with so many free pages before its words, then its words
+        int lo = 0, hi = ASG_BLOCK - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (before[mid] <= k) lo = mid; else hi = mid - 1;
+        }
+        int left = k - before[lo], w = lo * per;
+        uint32_t bits = ~used[w];
+        while (left >= __popc(bits)) left -= __popc(bits), bits = ~used[++w];
+        for (; left; --left) bits &= bits - 1;
+        pg = w * 32 + __builtin_ctz(bits);
+      }
+      a.tables[(int64_t)b * a.width + i] = pg;
+    }
+  }
+  if (a.small) {
+    __threadfence_block();
+    __syncthreads();
+    for (int t = wave * 64; t < a.tokens; t += ASG_BLOCK) asg_slots(a, t);
+  }
+}
+extern "C" __global__ __launch_bounds__(256) void nk_assign_slots(AssignArgs a) {
+  const int t = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+  if (t < a.tokens) asg_slots(a, t);
+}
+
+// ---------------------------------------------------------------------------
+// The choice of beams.
+//
+// Two launches.  The first reads the logits once: a wave has 2048 of a row in
+// registers, their largest value m, sum of 2^((x - m) log2 e) and the K best (K:
+// beams); a workgroup joins its waves' lists.  The K best of a wave: the K-th
+// largest of the lanes' largest values bounds them from below, what is not below
+// it (a few more than K) is listed in LDS and ranked one against the other; more
+// than LIST of them (ties) are taken in K rounds.
+//
+// The second, a workgroup per group, ranks the segments' best by score, value and
+// place; an entry with j before it in a list whose best has rank r has r + j
+// better ones, so K (K + 1) / 2 entries are left to rank.
+// ---------------------------------------------------------------------------
+struct SelectArgs {
+  const void *x;
+  const float *scores;
+  const int32_t *ended;
+  int32_t *tokens, *parents;
+  float *out;
+  int32_t *ends;
+  float2 *sums;   // (rows, nseg): largest value, sum
+  float2 *best;   // (rows, nseg, K): value, token (as bits); tokens of -1: no more
+  int64_t ld;
+  int32_t groups, beams, vocab, nseg, end;
+};
+#define SEL_WAVE 2048
+#define SEL_LIST 128
+#define SEL_BEAMS 32
+
+// a before b: the larger value, or the lower place
+NK_DEVICE bool sel_before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
+
+template <typename T>
+__device__ __forceinline__ void select_top_body(const SelectArgs &a) {
+  constexpr int E = 16 / sizeof(T), U = 32 / E;  // elements of a piece, pieces of a lane
+  __shared__ float lv[4][SEL_LIST];
+  __shared__ int32_t li[4][SEL_LIST];
+  __shared__ float bv[4][SEL_BEAMS];
+  __shared__ int32_t bi[4][SEL_BEAMS];
+  __shared__ float2 ms[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = blockIdx.x / a.nseg, seg = blockIdx.x % a.nseg, K = a.beams;
+  if (a.ended[r] != 0) return;  // (not read)
+  const T *x = (const T *)a.x + r * a.ld;
+  const int off = (int)(((uintptr_t)x & 15) / sizeof(T));  // elements of the first piece before the row
+  const int i0 = (seg * 4 + wave) * SEL_WAVE - off + lane * E;
+  float v[32];
+  float top = -INFINITY;
+  {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 64 * E;
+      if (i >= 0 && i + E <= a.vocab) w[u] = *reinterpret_cast<const uint4 *>(x + i);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 64 * E;
+      if (i >= 0 && i + E <= a.vocab) {
+        T y[E];
+        __builtin_memcpy(y, &w[u], 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u * E + e] = Elt<T>::load(y, e);
+      } else {  // an end
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u * E + e] = i + e >= 0 && i + e < a.vocab ? Elt<T>::load(x, i + e) : -INFINITY;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 32; ++e) top = fmaxf(top, v[e]);  // (fmaxf drops NaN)
+  const float m = wave_max(top);
+  float sum = 0.f;
+  if (fabsf(m) < INFINITY) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const float p = __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896340736f);
+      sum += p == p ? p : 0.f;
+    }
+  } else if (m > 0.f) {  // infinite logits share the weight
+#pragma unroll
+    for (int e = 0; e < 32; ++e) sum += v[e] == m ? 1.f : 0.f;
+  }
+  sum = wave_sum(sum);
+  // rank of this lane's largest among the lanes'
+  int rank = 0;
+#pragma unroll 8
+  for (int k = 0; k < 64; ++k) {
+    const float y = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(top), k));
+    rank += y > top || (y == top && k < lane) ? 1 : 0;
+  }
+  const uint64_t kth = __ballot(rank == K - 1);
+  const float low = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(top), __builtin_ctzll(kth)));
+  uint32_t in = 0;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) in |= v[e] >= low && v[e] > -INFINITY ? 1u << e : 0;
+  const int mine = __popc(in), upto = running(mine), total = __builtin_amdgcn_readlane(upto, 63);
+  int count = min(total, K);
+  if (total <= SEL_LIST) {
+    int at = upto - mine;
+    for (uint32_t left = in; left; left &= left - 1, ++at) {
+      const int e = __builtin_ctz(left), i = i0 + e / E * 64 * E + e % E;
+      lv[wave][at] = Elt<T>::load(x, i);
+      li[wave][at] = i;
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own list
+    asm volatile("" ::: "memory");
+    for (int k = lane; k < total; k += 64) {
+      const float y = lv[wave][k];
+      const int i = li[wave][k];
+      int before = 0;
+      for (int q = 0; q < total; ++q) before += sel_before(lv[wave][q], li[wave][q], y, i) ? 1 : 0;
+      if (before < K) bv[wave][before] = y, bi[wave][before] = i;
+    }
+  } else {
+    float ly = INFINITY;
+    int lj = -1;  // the last one taken
+    for (int k = 0; k < count; ++k) {
+      float y = -INFINITY;
+      int j = 0x7fffffff;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int i = i0 + e / E * 64 * E + e % E;
+        if (v[e] > -INFINITY && sel_before(ly, lj, v[e], i) && sel_before(v[e], i, y, j)) y = v[e], j = i;
+      }
+#pragma unroll
+      for (int o = 32; o; o >>= 1) {
+        const float oy = __shfl_xor(y, o, 64);
+        const int oj = __shfl_xor(j, o, 64);
+        if (sel_before(oy, oj, y, j)) y = oy, j = oj;
+      }
+      if (lane == 0) bv[wave][k] = y, bi[wave][k] = j;
+      ly = y, lj = j;
+    }
+  }
+  if (lane >= count && lane < K) bv[wave][lane] = -INFINITY, bi[wave][lane] = 0x7fffffff;
+  if (lane == 0) ms[wave] = make_float2(m, sum);
+  __syncthreads();
+  const int64_t at = (int64_t)r * a.nseg + seg;
+  if (threadIdx.x < 4 * K) {
+    const int w = threadIdx.x / K, k = threadIdx.x % K, i = bi[w][k];
+    const float y = bv[w][k];
+    int before = k;
+#pragma unroll
+    for (int o = 1; o < 4; ++o)
+      for (int q = 0; q < K; ++q) {
+        const float z = bv[(w + o) & 3][q];
+        const int j = bi[(w + o) & 3][q];
+        // (places that hold nothing are equal: those of the lower waves first)
+        before += sel_before(z, j, y, i) || (z == y && i == j && ((w + o) & 3) < w) ? 1 : 0;
+      }
+    if (before < K) a.best[at * K + before] = make_float2(y, __int_as_float(i == 0x7fffffff ? -1 : i));
+  }
+  if (threadIdx.x == 0) {
+    const float t = fmaxf(fmaxf(ms[0].x, ms[1].x), fmaxf(ms[2].x, ms[3].x));
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) s += ms[w].x == t ? ms[w].y : ms[w].x == -INFINITY ? 0.f : ms[w].y * exp_acc(ms[w].x - t);
+    a.sums[at] = make_float2(t, s);
+  }
+}
+extern "C" __global__ __launch_bounds__(256) void nk_select_top_bf16(SelectArgs a) { select_top_body<bf16>(a); }
+extern "C" __global__ __launch_bounds__(256) void nk_select_top_f16(SelectArgs a) { select_top_body<f16>(a); }
+extern "C" __global__ __launch_bounds__(256) void nk_select_top_f32(SelectArgs a) { select_top_body<float>(a); }
+
+#define SEL_BLOCK 1024
+#define SEL_HEADS 2048  // beams x segments at most
+#define SEL_LEFT (SEL_BEAMS * (SEL_BEAMS + 1) / 2)
+#define SEL_NONE 0xffffffffu
+
+// a score in its order among all, places packed as beam * 2^22 + token
+NK_DEVICE bool sel_better(double s, uint32_t p, double t, uint32_t q) { return s > t || (s == t && p < q); }
+
+extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArgs a) {
+  __shared__ double hs[SEL_HEADS];
+  __shared__ uint32_t hp[SEL_HEADS];
+  __shared__ double cs[SEL_LEFT];
+  __shared__ uint32_t cp[SEL_LEFT];
+  __shared__ double base[SEL_BEAMS];
+  __shared__ float largest[SEL_BEAMS];
+  __shared__ int32_t kind[SEL_BEAMS];  // 0: nothing, 1: its logits, 2: ended
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = blockIdx.x, K = a.beams, heads = K * a.nseg;
+  for (int b = wave; b < K; b += SEL_BLOCK / 64) {
+    const int r = g * K + b;
+    const float s = a.scores[r];
+    const bool over = a.ended[r] != 0;
+    int what = s == s && s > -INFINITY ? (over ? 2 : 1) : 0;
+    double z = (double)s;
+    float m = -INFINITY;
+    if (what == 1) {
+      for (int i = lane; i < a.nseg; i += 64) m = fmaxf(m, a.sums[(int64_t)r * a.nseg + i].x);
+      m = wave_max(m);
+      if (m == -INFINITY) what = 0;
+      double sum = 0.0;
+      for (int i = lane; i < a.nseg; i += 64) {
+        const float2 y = a.sums[(int64_t)r * a.nseg + i];
+        sum += y.x == m ? (double)y.y : y.x == -INFINITY ? 0.0 : (double)y.y * exp((double)y.x - (double)m);
+      }
+#pragma unroll
+      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      z -= log(sum);
+    }
+    if (lane == 0) base[b] = z, largest[b] = m, kind[b] = what;
+  }
+  for (int i = tid; i < K * (K + 1) / 2; i += SEL_BLOCK) cp[i] = SEL_NONE;
+  __syncthreads();
+  // entry j of a list: false where there is none
+  auto entry = [&](int h, int j, double &s, uint32_t &p) {
+    const int b = h / a.nseg, i = h % a.nseg;
+    if (kind[b] == 0 || (kind[b] == 2 && (i || j))) return false;
+    if (kind[b] == 2) {
+      s = base[b], p = (uint32_t)b << 22 | (uint32_t)max(a.end, 0);
+      return true;
+    }
+    const float2 y = a.best[(((int64_t)g * K + b) * a.nseg + i) * K + j];
+    const int t = __float_as_int(y.y);
+    if (t < 0 || (y.x != largest[b] && largest[b] == INFINITY)) return false;
+    s = base[b] + (y.x == largest[b] ? 0.0 : (double)y.x - (double)largest[b]), p = (uint32_t)b << 22 | (uint32_t)t;
+    return true;
+  };
+  for (int h = tid; h < heads; h += SEL_BLOCK) {
+    double s;
+    uint32_t p;
+    const bool is = entry(h, 0, s, p);
+    hs[h] = is ? s : 0.0;
+    hp[h] = is ? p : SEL_NONE;
+  }
+  __syncthreads();
+  for (int h = tid; h < heads; h += SEL_BLOCK) {
+    const double s = hs[h];
+    const uint32_t p = hp[h];
+    if (p == SEL_NONE) continue;
+    int rank = 0;
+    for (int q = 0; q < heads; ++q) rank += hp[q] != SEL_NONE && sel_better(hs[q], hp[q], s, p) ? 1 : 0;
+    if (rank >= K) continue;
+    const int to = rank * K - rank * (rank - 1) / 2;
+    for (int j = 0; j < K - rank; ++j) {
+      double t;
+      uint32_t q;
+      if (!entry(h, j, t, q)) break;
+      cs[to + j] = t, cp[to + j] = q;
+    }
+  }
+  __syncthreads();
+  const int n = K * (K + 1) / 2;
+  int taken = 0;
+  for (int c = tid; c < n; c += SEL_BLOCK) {
+    const double s = cs[c];
+    const uint32_t p = cp[c];
+    if (p == SEL_NONE) continue;
+    int rank = 0;
+    for (int q = 0; q < n; ++q) rank += cp[q] != SEL_NONE && sel_better(cs[q], cp[q], s, p) ? 1 : 0;
+    if (rank >= K) continue;
+    const int b = p >> 22, t = kind[b] == 2 ? a.end : (int)(p & 0x3fffff), to = g * K + rank;
+    a.tokens[to] = t;
+    a.parents[to] = b;
+    a.out[to] = (float)s;
+    a.ends[to] = kind[b] == 2 || t == a.end ? 1 : 0;
+  }
+  // the places left
+  for (int i = lane; i < n; i += 64) taken += cp[i] != SEL_NONE ? 1 : 0;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) taken += __shfl_xor(taken, o, 64);
+  if (tid >= taken && tid < K) {
+    a.tokens[g * K + tid] = -1;
+    a.parents[g * K + tid] = tid;
+    a.out[g * K + tid] = -INFINITY;
+    a.ends[g * K + tid] = a.ended[g * K + tid] != 0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Caches behind their parents.
+//
+// A thread has one place (an entry of the tables, 16 bytes of a page) of every
+// beam of a group: it reads what all of them come from, then writes, so no
+// thread reads what another has written.  Beams that are their own parents move
+// nothing.  Bound by memory, small ones by two dependent reads.
+// ---------------------------------------------------------------------------
+struct ReorderArgs {
+  const int32_t *parents, *lens;
+  int32_t *tables;
+  void *k, *v;
+  int32_t *ke, *ve;   // null: none
+  int64_t row;        // bytes of a cache row
+  int32_t groups, beams, width, page, pages, hkv;
+  int32_t tblocks, kblocks;  // workgroups of a group for the tables and for each cache
+};
+
+template <int K, typename U>
+__device__ __forceinline__ void reorder_body(const ReorderArgs &a) {
+  __shared__ int32_t up[K], from[K], to[K];  // a beam's parent; pages, -1 where nothing moves
+  const int per = a.tblocks + 2 * a.kblocks + (a.ke ? 1 : 0), tid = threadIdx.x;
+  const int g = blockIdx.x / per, part = blockIdx.x % per;
+  const int len = (int)min((int64_t)max(a.lens[(int64_t)g * a.beams], 0), (int64_t)a.width * a.page);
+  const int full = len / a.page, tail = len % a.page;
+  int32_t *table = a.tables + (int64_t)g * a.beams * a.width;
+  if (part < a.tblocks ? part * 256 >= full : tail == 0) return;
+  if (tid < K) {
+    const int b = min(tid, a.beams - 1), p = a.parents[(int64_t)g * a.beams + b];
+    const bool moves = tid < a.beams && p >= 0 && p < a.beams && p != b;
+    up[tid] = moves ? p : tid;
+    int x = -1, y = -1;
+    if (moves && part >= a.tblocks) {  // (full is below width: the length leaves a page in part filled)
+      x = table[(int64_t)p * a.width + full], y = table[(int64_t)b * a.width + full];
+      if (x < 0 || x >= a.pages || y >= a.pages) y = -1;
+    }
+    from[tid] = x, to[tid] = y;
+  }
+  __syncthreads();
+  if (part < a.tblocks) {
+    const int j = part * 256 + tid;
+    if (j >= full) return;
+    int32_t x[K];
+#pragma unroll
+    for (int b = 0; b < K; ++b) {
+      const int p = __builtin_amdgcn_readfirstlane(up[b]);
+      if (p != b) x[b] = table[(int64_t)p * a.width + j];
+    }
+#pragma unroll
+    for (int b = 0; b < K; ++b)
+      if (__builtin_amdgcn_readfirstlane(up[b]) != b) table[(int64_t)b * a.width + j] = x[b];
+    return;
+  }
+  const int which = (part - a.tblocks) / a.kblocks;  // 0: keys, 1: values, 2: exponents
+  auto move = [&](auto *x, int64_t pitch, int64_t at) __attribute__((always_inline)) {
+    typename std::remove_reference<decltype(*x)>::type y[K];
+#pragma unroll
+    for (int b = 0; b < K; ++b)
+      if (__builtin_amdgcn_readfirstlane(to[b]) >= 0) y[b] = x[__builtin_amdgcn_readfirstlane(from[b]) * pitch + at];
+#pragma unroll
+    for (int b = 0; b < K; ++b) {
+      const int p = __builtin_amdgcn_readfirstlane(to[b]);
+      if (p >= 0) x[p * pitch + at] = y[b];
+    }
+  };
+  if (which < 2) {
+    const int64_t at = (int64_t)((part - a.tblocks) % a.kblocks) * 256 + tid, units = a.row / (int64_t)sizeof(U);  // (of a row)
+    if (at < tail * units) move((U *)(which ? a.v : a.k), a.page * units, at);
+  } else {
+    for (int h = tid; h < 2 * a.hkv; h += 256) move(h < a.hkv ? a.ke : a.ve, a.hkv, h < a.hkv ? h : h - a.hkv);
+  }
+}
+#define NK_REORDER(K)                                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void nk_beam_reorder16_k##K(ReorderArgs a) { reorder_body<K, u32x4>(a); }  \
+  extern "C" __global__ __launch_bounds__(256) void nk_beam_reorder1_k##K(ReorderArgs a) { reorder_body<K, uint8_t>(a); }
+NK_REORDER(4)
+NK_REORDER(8)
+NK_REORDER(32)

@@ -359,6 +359,38 @@ NK_DEVICE void encode8(const float v[8], Raw8<f16> &r) {
   r.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// E consecutive elements, one by one or (8) in 16-byte accesses
+template <typename T, int E> struct Piece {
+  static NK_DEVICE void load(const T *p, float (&x)[E]) {
+    if constexpr (E == 8) {
+      Vec8<T>::load(p, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = Elt<T>::load(p, e);
+    }
+  }
+  static NK_DEVICE void store(T *p, const float (&x)[E]) {
+    if constexpr (E == 8) {
+      Vec8<T>::store(p, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) Elt<T>::store(p, e, x[e]);
+    }
+  }
+};
+// bits unchanged, signalling NaN included
+template <typename T, int E>
+NK_DEVICE void copy_piece(const T *x, T *y) {
+  if constexpr (E == 8) {
+    Raw8<T> r;
+    r.template load<false>(x);
+    r.template store<false>(y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = x[e];
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Workgroup barrier for LDS hand-offs.  __syncthreads() carries a release
 // fence, which also waits for every outstanding global load (vmcnt(0)) and

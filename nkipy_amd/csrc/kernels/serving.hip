@@ -30,37 +30,6 @@ struct AppendArgs {
   int32_t page, pages, width;
 };
 
-template <typename T, int E> struct Piece {  // E consecutive elements
-  static NK_DEVICE void load(const T *p, float (&x)[E]) {
-    if constexpr (E == 8) {
-      Vec8<T>::load(p, x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = Elt<T>::load(p, e);
-    }
-  }
-  static NK_DEVICE void store(T *p, const float (&x)[E]) {
-    if constexpr (E == 8) {
-      Vec8<T>::store(p, x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) Elt<T>::store(p, e, x[e]);
-    }
-  }
-};
-// bits unchanged, signalling NaN included
-template <typename T, int E>
-NK_DEVICE void copy_piece(const T *x, T *y) {
-  if constexpr (E == 8) {
-    Raw8<T> r;
-    r.template load<false>(x);
-    r.template store<false>(y);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = x[e];
-  }
-}
-
 template <typename T, int E>
 __device__ __forceinline__ void rotary_append_body(const AppendArgs &a) {
   const int t = blockIdx.x, lane = threadIdx.x & 63;

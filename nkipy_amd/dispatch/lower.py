@@ -285,8 +285,8 @@ class Lowering:
         each done with by its readers when the next one's step begins: all of
         them may write ``p``'s buffer.  Empty where ``last`` is the only one."""
         chain = [last]
-        while chain[0] is not None and chain[0].op == "paged_write":
-            before = chain[0].inputs[0]
+        while chain[0] is not None and (chain[0].op == "paged_write" or "target" in chain[0].attrs):
+            before = chain[0].inputs[chain[0].attrs.get("target", 0)]
             if before is p:
                 return chain if len(chain) > 1 else []
             if before.id in self.result_ids or before.is_parameter or not self._reads_done_before(before, chain[0], order):
@@ -304,12 +304,17 @@ class Lowering:
         fused elementwise / layout node, or a reshape sharing ``p``'s
         storage): it happens inside the step of a later consumer, so the
         consumers are followed transitively.  ``prod`` itself may read ``p``
-        only as the operand it updates in place."""
+        only as the operand it updates in place, and so may the nodes of a
+        match that updates several (``Match.updated``)."""
         limit = order[id(prod)]
+        whole = self.covered.get(id(prod))
+        together = whole.nodes if whole is not None and p.id in whole.updated else ()
         work, seen = [p], {p.id}
         while work:
             x = work.pop()
             for u in self.users.get(x.id, ()):
+                if x is p and id(u) in together:
+                    continue
                 if u is prod:
                     in_place_target = (x is p and prod.op in self._INPLACE_OPS and prod.inputs[0] is p
                                        and not any(y is p for y in prod.inputs[1:]))

@@ -99,6 +99,7 @@ class Match:
     """A claimed subgraph and the step(s) that replace it."""
 
     name = "match"
+    updated: frozenset = frozenset()  # ids of the values that its launch reads and updates in place
 
     def __init__(self, nodes: Iterable[Node], inputs: List[Value], outputs: List[Value]):
         self.node_list = list(dict.fromkeys(nodes))
@@ -496,13 +497,15 @@ def _build_default_patterns():
     )
     from nkipy_amd.dispatch.patterns_gemm import GemmPattern, SwigluPattern
     from nkipy_amd.dispatch.patterns_linattn import LinearAttentionPattern
+    from nkipy_amd.dispatch.beams import BeamPattern
     from nkipy_amd.dispatch.serving import AppendPattern, ServingPattern
+    from nkipy_amd.dispatch.serving_fp8 import Fp8CachePattern
 
     # larger structures first: they contain matmuls / softmaxes that smaller
     # patterns would claim; GEMMs before RMSNorm so that a residual add
     # after a projection goes into the GEMM epilogue; the RoPE of q / k then
     # folds into its QKV projection
-    return [AppendPattern(), ServingPattern(), LinearAttentionPattern(), DecodeAttentionPattern(), AttentionPattern(),
-            RopePattern(), HeadRopePattern(), SwigluPattern(), GemmPattern(), SoftmaxPattern(), RmsNormPattern(),
+    return [AppendPattern(), ServingPattern(), Fp8CachePattern(), BeamPattern(), LinearAttentionPattern(),
+            DecodeAttentionPattern(), AttentionPattern(), RopePattern(), HeadRopePattern(), SwigluPattern(), GemmPattern(), SoftmaxPattern(), RmsNormPattern(),
             QkvRopeFusion(), ProjectionPlanesFusion()]
 

@@ -140,6 +140,16 @@ def attend_work(B, S, N, Hq, Hkv, D, keys, window=0, sinks=0, starts=False) -> T
     return step, units, max(1, min(splits, ATT_MAX_SPLIT))
 
 
+def attend_join(dtype, a: AttendArgs) -> Launch:
+    """The launch that joins the splits of ``a``.  Whole calls with a workgroup
+    a row and with a wave, us: 32 rows of 63 splits 14.4 and 31.5, of 12 10.2
+    and 10.5, 256 of 19 97 and 100, 1280 of 7 45.5 and 43.8."""
+    rows, tag = a.N * a.Hq, f"{dtype_tag(dtype)}_d{a.D}"
+    if a.nsplit > ATT_JOIN_WIDE and rows < ATT_JOIN_ROWS:
+        return Launch("attend", f"nk_attend_join4_{tag}", (rows, 1, 1), (256, 1, 1), a)
+    return Launch("attend", f"nk_attend_join_{tag}", (-(-rows // 4), 1, 1), (256, 1, 1), a)
+
+
 def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S=1, T=0, tables=0, lens=0, starts=0, first=0,
            page=1, pages=0, width=0, pitch=0, window=0, sinks=0, ws=0, zeros=0) -> List[Launch]:
     """Attention over a paged cache (``tables``; strides of q are (0, row,
@@ -181,12 +191,8 @@ def attend(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, S
     far = not step and (reach >= 2**32 - 4096 or (tables and k_str[1] != v_str[1]))
     kind = f"{'step' if step else 'tile'}_{'paged' if tables else 'plain'}{'_far' if far else ''}"
     out = [Launch("attend", f"nk_attend_{kind}_{tag}_d{D}", (a.tiles * Hkv * a.nsplit, 1, 1), (256, 1, 1), a)]
-    # whole calls with a workgroup a row and with a wave, us: 32 rows of 63 splits
-    # 14.4 and 31.5, of 12 10.2 and 10.5, 256 of 19 97 and 100, 1280 of 7 45.5 and 43.8
-    if a.nsplit > ATT_JOIN_WIDE and N * Hq < ATT_JOIN_ROWS:
-        out.append(Launch("attend", f"nk_attend_join4_{tag}_d{D}", (N * Hq, 1, 1), (256, 1, 1), a))
-    elif a.nsplit > 1:
-        out.append(Launch("attend", f"nk_attend_join_{tag}_d{D}", (-(-N * Hq // 4), 1, 1), (256, 1, 1), a))
+    if a.nsplit > 1:
+        out.append(attend_join(dtype, a))
     return out
 
 
