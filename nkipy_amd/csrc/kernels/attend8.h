@@ -14,23 +14,24 @@ struct Attend8Args : AttendArgs {  // k, v: codes; strides in bytes
 // One query row by one wave, over blocks j0 .. j1-1 of its tile's span: eight lanes
 // share a key's product, 64 keys a step; then the lanes share the head's elements,
 // d = lane + 64 e.  Only the keys that the row sees are read; 32-bit weights of at
-// most 1.
-template <typename T>
+// most 1.  DIM: the head dim where it is known, which saves registers.
+template <typename T, int DIM = 0>
 NK_DEVICE void att8_row(const Attend8Args &a, const AttSeq &sq, const AttSpan &sp, int b, int i, int h, int j0, int j1,
-                        float &m, float &l, float (&acc)[4]) {
+                        float &m, float &l, float (&acc)[DIM ? (DIM + 63) / 64 : 4]) {
   const int lane = threadIdx.x & 63, c = lane & 7;
-  const int g = h / (a.Hq / a.Hkv), p = sq.p0 + i, D = a.D, per = (D + 7) / 8;
+  const int g = h / (a.Hq / a.Hkv), p = sq.p0 + i, D = DIM ? DIM : a.D, per = (D + 7) / 8;
+  constexpr int C = DIM ? (DIM + 7) / 8 : 32, V = DIM ? (DIM + 63) / 64 : 4;
   const T *q = (const T *)a.q + (int64_t)(sq.lo + i) * a.q_ss + (int64_t)h * a.q_sh;
   const uint8_t *k = (const uint8_t *)a.k + (int64_t)g * a.k_sh, *v = (const uint8_t *)a.v + (int64_t)g * a.v_sh;
-  float qc[32];
+  float qc[C];
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
+  for (int e = 0; e < C; ++e) {
     const int d = c * per + e;
     qc[e] = e < per && d < D ? Elt<T>::load(q, d) * a.scale : 0.f;
   }
   m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] = 0.f;
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
   for (int x0 = j0 * ATT_KEYS; x0 < j1 * ATT_KEYS; x0 += 64) {
     const int x = x0 + lane;
     const int key = sp.kb(x / ATT_KEYS) * ATT_KEYS + x % ATT_KEYS;
@@ -53,7 +54,7 @@ NK_DEVICE void att8_row(const Attend8Args &a, const AttSeq &sq, const AttSpan &s
       if (r >= 0) {
         const uint8_t *kr = k + (int64_t)r * a.k_ss;
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
+        for (int e = 0; e < C; ++e)
           if (e < per && c * per + e < D) d = fmaf(qc[e], __builtin_amdgcn_cvt_f32_fp8((int)kr[c * per + e], 0), d);
       }
       d += __shfl_xor(d, 1, 64);
@@ -67,7 +68,7 @@ NK_DEVICE void att8_row(const Attend8Args &a, const AttSeq &sq, const AttSpan &s
     m = mn;
     l = l * alpha + wave_sum(w);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= alpha;
+    for (int e = 0; e < V; ++e) acc[e] *= alpha;
     while (todo) {
       const int n = __builtin_ctzll(todo);
       todo &= todo - 1;
@@ -75,7 +76,7 @@ NK_DEVICE void att8_row(const Attend8Args &a, const AttSeq &sq, const AttSpan &s
       const float vn = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), n));
       const uint8_t *vr = v + (int64_t)__builtin_amdgcn_readlane(row, n) * a.v_ss;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < V; ++e)
         if (lane + 64 * e < D) acc[e] = fmaf(wn, __builtin_amdgcn_cvt_f32_fp8((int)vr[lane + 64 * e], 0) * vn, acc[e]);
     }
   }

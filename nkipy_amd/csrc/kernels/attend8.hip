@@ -83,8 +83,11 @@ NK_DEVICE B8 codes8(uint32_t lo, uint32_t hi, float scale) {
 
 // ---------------------------------------------------------------------------
 // One new token per sequence (16-bit queries, head dim 64 or 128): bound by the read
-// of the codes, so the waves of a workgroup take blocks of 32 keys of their own, no
-// barrier between them, and meet at the end.
+// of the codes.  A wave takes one piece of one sequence's blocks of 32 keys for one
+// KV head, by itself: no LDS and no barrier.  Waves that run side by side take
+// neighbouring heads of the same keys, whose rows lie next to each other in memory
+// (64 contexts of up to 8192, 8 heads of 128: 142 us where the four waves of a
+// workgroup take blocks of one head, XXX so).
 //
 // A wave has up to 16 heads of the group as the columns of 16x16x32 products,
 // S^T = K Q^T and O^T = V^T P^T.  Everything stays in registers: which element of
@@ -92,29 +95,22 @@ NK_DEVICE B8 codes8(uint32_t lo, uint32_t hi, float scale) {
 // long as both factors agree.  So a lane takes 16 bytes of a key as they lie in
 // memory; and of the values it takes D / 16 columns of the eight keys whose weights
 // it holds, pairs of which v_perm puts side by side after conversion.  The next
-// block's reads are under way while one is worked on.
+// block's keys are read as soon as this one's scores stand, its values behind this
+// one's products.
 // ---------------------------------------------------------------------------
-template <int D> struct Block8 {
-  uint4 k[2][D / 64];         // tile, piece
-  uint32_t v[8][D / 64];      // key, four columns
-  float scale;                // of key lane % 32: lanes below 32 keys', above values'
-  uint32_t seen;              // a bit for each key
-};
-
 template <typename T, int D>
 __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
-  constexpr int NP = Parts<T>::N, NW = 4, VW = D / 64;
-  constexpr int SUM = NW * 16 * (D + 2) * 4;  // the waves' sums
-  __shared__ __attribute__((aligned(16))) uint8_t lds[SUM];
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int NP = Parts<T>::N, VW = D / 64;
+  const int lane = threadIdx.x & 63;
   const int l16 = lane & 15, grp = lane >> 4;
-  const int rep = a.Hq / a.Hkv, per = (rep + 15) / 16;
-  int w = blockIdx.x;
-  const int g = w % a.Hkv;
-  w /= a.Hkv;
-  const int split = w / a.tiles, h0 = w % a.tiles % per * 16, b = w % a.tiles / per;  // (h0: first head of the group's)
+  const int rep = a.Hq / a.Hkv, per = (rep + 15) / 16, units = a.Hkv * per;
+  int w = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = w % units / per, h0 = w % units % per * 16;  // (h0: first head of the group's)
+  w /= units;
+  // (nsplit is a multiple of eight: the first pieces, which all sequences have, come
+  // to all XCDs by turns)
+  const int b = w / a.nsplit, split = (w % a.nsplit + b) % a.nsplit;
+  if (b >= a.B) return;
   const AttSeq sq = att_seq(a, b);
   const AttSpan sp = att_span(a, sq, 0);
   int j0, j1;
@@ -148,36 +144,51 @@ __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
     in = key - x * a.page;
     return pg >= 0 && pg < a.pages ? pg : -1;
   };
-  auto fetch = [&](Block8<D> &x, int pg, int in) __attribute__((always_inline)) {
-    const int at = max(pg, 0) * a.pitch + in;  // (a key that is not seen: some row, unused)
-    x.seen = (uint32_t)__ballot(pg >= 0);
-    x.scale = c8_power(c8_clip(ex[(int64_t)max(pg, 0) * a.Hkv]));
+  int at;                  // the next block's rows: this lane's key's, some row (unused) where it is not seen
+  uint32_t seen, seen_next;
+  float scale, scale_next;  // of key lane % 32: lanes below 32 keys', above values'
+  uint4 kr[2][D / 64];
+  uint32_t vr[8][VW];
+  auto fetch_k = [&](int pg, int in) __attribute__((always_inline)) {
+    at = max(pg, 0) * a.pitch + in;
+    seen_next = (uint32_t)__ballot(pg >= 0);
+    scale_next = c8_power(c8_clip(ex[(int64_t)max(pg, 0) * a.Hkv]));
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       const uint8_t *k = kp + (int64_t)__shfl(at, kt * 16 + l16, 64) * a.k_ss;
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) x.k[kt][i] = *reinterpret_cast<const uint4 *>(k + i * 64);
+      for (int i = 0; i < D / 64; ++i) kr[kt][i] = *reinterpret_cast<const uint4 *>(k + i * 64);
     }
+  };
+  auto fetch_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const uint8_t *v = vp + (int64_t)__shfl(at, (r >> 2) * 16 + 4 * grp + (r & 3), 64) * a.v_ss;
       if constexpr (VW == 2) {
         const uint2 y = *reinterpret_cast<const uint2 *>(v);
-        x.v[r][0] = y.x, x.v[r][1] = y.y;
+        vr[r][0] = y.x, vr[r][1] = y.y;
       } else {
-        x.v[r][0] = *reinterpret_cast<const uint32_t *>(v);
+        vr[r][0] = *reinterpret_cast<const uint32_t *>(v);
       }
     }
   };
-  auto work = [&](Block8<D> &x) __attribute__((always_inline)) {
+
+  int in, pg = page_of(j0, in);
+  if (j0 < j1) {
+    fetch_k(pg, in);
+    fetch_v();
+    pg = page_of(j0 + 1, in);
+  }
+  for (int j = j0; j < j1; ++j) {
+    seen = seen_next, scale = scale_next;
     f32x4 s[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const float ks = __shfl(x.scale, kt * 16 + l16, 64);
+      const float ks = __shfl(scale, kt * 16 + l16, 64);
       s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
-        const uint4 k = x.k[kt][i];
+        const uint4 k = kr[kt][i];
         const B8 f0 = codes8(k.x, k.y, ks), f1 = codes8(k.z, k.w, ks);
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
@@ -186,15 +197,17 @@ __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
         }
       }
     }
+    const bool more = j + 1 < j1;
+    if (more) fetch_k(pg, in);
     // element r of tile kt is key 16 kt + 4 grp + r
-    if (x.seen != 0xffffffffu) {
-      const uint32_t mine = x.seen >> (grp * 4);
+    if (seen != 0xffffffffu) {
+      const uint32_t mine = seen >> (grp * 4);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bool in = mine >> ((e >> 2) * 16 + (e & 3)) & 1;
-        s[e >> 2][e & 3] = in ? s[e >> 2][e & 3] : -INFINITY;
+        const bool is = mine >> ((e >> 2) * 16 + (e & 3)) & 1;
+        s[e >> 2][e & 3] = is ? s[e >> 2][e & 3] : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < VW; ++i) x.v[e][i] = in ? x.v[e][i] : 0;
+        for (int i = 0; i < VW; ++i) vr[e][i] = is ? vr[e][i] : 0;
       }
     }
     B8 pf[NP];
@@ -228,7 +241,7 @@ __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
     l_run += ls;
     float vs[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) vs[r] = __shfl(x.scale, 32 + (r >> 2) * 16 + 4 * grp + (r & 3), 64);
+    for (int r = 0; r < 8; ++r) vs[r] = __shfl(scale, 32 + (r >> 2) * 16 + 4 * grp + (r & 3), 64);
 #pragma unroll
     for (int i = 0; i < VW; ++i)
 #pragma unroll
@@ -236,8 +249,8 @@ __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
         uint32_t c[8];  // columns 4 i + 2 h and the next, of each key
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          c[r] = bf16x2_bits(h ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.v[r][i], vs[r], true)
-                               : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.v[r][i], vs[r], false));
+          c[r] = bf16x2_bits(h ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vr[r][i], vs[r], true)
+                               : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vr[r][i], vs[r], false));
         u32x4_t lo, hi;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -251,102 +264,157 @@ __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
           acc[t + 1] = mul16(__builtin_bit_cast(B8, hi), pf[n], acc[t + 1]);
         }
       }
-  };
-
-  Block8<D> x0, x1;
-  int in, pg = page_of(j0 + wave, in);
-  if (j0 + wave < j1) {
-    fetch(x0, pg, in);
-    pg = page_of(j0 + wave + NW, in);
-  }
-  for (int j = j0 + wave; j < j1; j += 2 * NW) {
-    if (j + NW < j1) {
-      fetch(x1, pg, in);
-      pg = page_of(j + 2 * NW, in);
+    if (more) {
+      fetch_v();
+      pg = page_of(j + 2, in);
     }
-    work(x0);
-    if (j + NW >= j1) break;
-    if (j + 2 * NW < j1) {
-      fetch(x0, pg, in);
-      pg = page_of(j + 3 * NW, in);
-    }
-    work(x1);
   }
 
-  // The waves' sums: their offsets meet, then each row's sums are added in the
-  // waves' order.  acc[t][r] is column (4 grp + r) D / 16 + t.
+  // acc[t][r] is column (4 grp + r) D / 16 + t of row l16
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
-  float *so = reinterpret_cast<float *>(lds), *sm = so + NW * 16 * D;  // (NW, 16, D) sums; (NW, 16) weights
-  // a bit for each row with a sum that is not finite under weights that are
-  __shared__ uint32_t spoiled[NW];
   float z = 0.f;
 #pragma unroll
   for (int t = 0; t < D / 16; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) z = __builtin_fmaf(acc[t][r], 0.f, z);
-  uint64_t bits = __ballot(z != 0.f && l_run == l_run);
+  // a bit for each row with a sum that is not finite under weights that are
+  uint64_t bits = __ballot(z != 0.f && l_run == l_run && h0 + l16 < rep);
   bits |= bits >> 32;
-  if (lane == 0) spoiled[wave] = (uint32_t)(bits | bits >> 16) & 0xffffu;
-  if (grp == 0) so[wave * 16 + l16] = m_run;
-  __syncthreads();
-  const float m = fmaxf(fmaxf(so[l16], so[16 + l16]), fmaxf(so[32 + l16], so[48 + l16]));
-  __syncthreads();
-  // (an infinite score's offset is infinite: its sums are NaN already)
-  const float f = m_run == m ? 1.f : __builtin_amdgcn_exp2f((m_run - m) * sl2);
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int t = 0; t < D / 16; t += 4)
-      *reinterpret_cast<float4 *>(so + (wave * 16 + l16) * D + (4 * grp + r) * (D / 16) + t) =
-          make_float4(acc[t][r] * f, acc[t + 1][r] * f, acc[t + 2][r] * f, acc[t + 3][r] * f);
-  if (grp == 0) sm[wave * 16 + l16] = l_run * f;
-  __syncthreads();
+  uint32_t again = (uint32_t)(bits | bits >> 16) & 0xffffu;
   const int64_t nr = (int64_t)a.N * a.Hq, r0 = (int64_t)b * a.Hq + g * rep + h0;
-  auto weight = [&](int r) __attribute__((always_inline)) { return (sm[r] + sm[16 + r]) + (sm[32 + r] + sm[48 + r]); };
-  const uint32_t again = __builtin_amdgcn_readfirstlane(spoiled[0] | spoiled[1] | spoiled[2] | spoiled[3]);
-#pragma unroll
-  for (int x = 0; x < 16 * D / 256; ++x) {
-    const int e = x * 256 + tid, r = e / D;
-    if (h0 + r >= rep) break;  // (rows rise)
-    if (again >> r & 1) continue;
-    const float o = (so[e] + so[16 * D + e]) + (so[2 * 16 * D + e] + so[3 * 16 * D + e]), l = weight(r);
+  float *const wo = a.ws + (split * nr + r0) * D, *const wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + r0) * 2;
+  if (h0 + l16 < rep && !(again >> l16 & 1)) {
     if (pieces == 1) {
-      Elt<T>::store((T *)a.o + r0 * D, e, l == 0.f ? 0.f : o / l);
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float y[8];
+        T *o = (T *)a.o + (r0 + l16) * D + (4 * grp + r) * (D / 16);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) y[t] = l_run == 0.f ? 0.f : acc[t][r] * inv;
+        if constexpr (D == 128) {
+          Vec8<T>::store(o, y);
+        } else {
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t) Elt<T>::store(o, t, y[t]);
+        }
+      }
     } else {
-      a.ws[(split * nr + r0) * D + e] = o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = 0; t < D / 16; t += 4)
+          *reinterpret_cast<float4 *>(wo + l16 * D + (4 * grp + r) * (D / 16) + t) =
+              make_float4(acc[t][r], acc[t + 1][r], acc[t + 2][r], acc[t + 3][r]);
+      if (grp == 0) wm[2 * l16] = fmaxf(m_run * sl2, ATT8_LOWEST), wm[2 * l16 + 1] = l_run;
     }
   }
-  float *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + r0) * 2;
-  if (pieces > 1 && wave == 0 && grp == 0 && h0 + l16 < rep && !(again >> l16 & 1))
-    wm[2 * l16] = fmaxf(m * sl2, ATT8_LOWEST), wm[2 * l16 + 1] = weight(l16);
   // Sums that are not finite (NaN values, or large ones under weights past 1): those
-  // rows again, a wave for each.
-  for (uint32_t left = again; left; left &= left - 1) {
-    const int r = __builtin_ctz(left);
-    if (h0 + r >= rep) break;
-    if (r % NW != wave) continue;
-    float mr, lr, y[4];
-    att8_row<T>(a, sq, sp, b, 0, g * rep + h0 + r, j0, j1, mr, lr, y);
+  // rows again.
+  for (; again; again &= again - 1) {
+    const int r = __builtin_ctz(again);
+    float mr, lr, y[D / 64];
+    att8_row<T, D>(a, sq, sp, b, 0, g * rep + h0 + r, j0, j1, mr, lr, y);
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
       if (pieces == 1) {
         Elt<T>::store((T *)a.o + (r0 + r) * D, lane + 64 * e, lr == 0.f ? 0.f : y[e] / lr);
       } else {
-        a.ws[(split * nr + r0 + r) * D + lane + 64 * e] = y[e];
+        wo[r * D + lane + 64 * e] = y[e];
       }
     }
     if (pieces > 1 && lane == 0) wm[2 * r] = fmaxf(mr * LOG2E, ATT8_LOWEST), wm[2 * r + 1] = lr;
   }
 }
-#define NK_STEP8(T, name, D)                                                                             \
-  extern "C" __global__ __launch_bounds__(256, 2) void nk_attend8_step_##name##_d##D(Attend8Args a) {    \
-    attend8_step_body<T, D>(a);                                                                          \
+#define NK_STEP8(T, name, D, OCC)                                                                          \
+  extern "C" __global__ __launch_bounds__(256, OCC) void nk_attend8_step_##name##_d##D(Attend8Args a) {    \
+    attend8_step_body<T, D>(a);                                                                            \
   }
-NK_STEP8(bf16, bf16, 128)
-NK_STEP8(f16, f16, 128)
-NK_STEP8(bf16, bf16, 64)
-NK_STEP8(f16, f16, 64)
+NK_STEP8(bf16, bf16, 128, 3)
+NK_STEP8(f16, f16, 128, 3)
+NK_STEP8(bf16, bf16, 64, 4)
+NK_STEP8(f16, f16, 64, 4)
+
+// ---------------------------------------------------------------------------
+// The pieces of a step's row joined: o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s,
+// over the pieces with any weight, up to JOIN of them.  One workgroup per row: D / 4
+// threads side by side for a piece's sums, the pieces shared out over the rest and
+// added in a fixed order.  Bound by the latency of its two dependent reads.
+// ---------------------------------------------------------------------------
+#define ATT8_JOIN 256
+template <typename T, int D>
+__device__ __forceinline__ void attend8_join_body(const Attend8Args &a) {
+  constexpr int DL = D / 4, PL = 256 / DL;  // threads of a piece, pieces side by side
+  __shared__ float weight[ATT8_JOIN];
+  __shared__ __attribute__((aligned(16))) float part[PL][D];
+  __shared__ float total;
+  const int tid = threadIdx.x, lane = tid & 63, d = tid % DL * 4, s0 = tid / DL;
+  const int64_t r = blockIdx.x, nr = (int64_t)a.N * a.Hq;
+  const int b = (int)(r / a.Hq);
+  const AttSeq sq = att_seq(a, b);
+  int j0, j1;
+  const int pieces = att_split(a, att_span(a, sq, 0).nb, 0, j0, j1);
+  if (pieces == 1) return;
+  const float *ws = a.ws + r * D + d, *wm = a.ws + (int64_t)a.nsplit * nr * D;
+  constexpr int U = 8;
+  float4 x[U];
+  auto fetch = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)  // (past the last piece: the last again, unused)
+      x[u] = *reinterpret_cast<const float4 *>(ws + (int64_t)min(s + u * PL, pieces - 1) * nr * D);
+  };
+  fetch(s0);
+  if (tid < 64) {
+    float m[ATT8_JOIN / 64], l[ATT8_JOIN / 64], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < ATT8_JOIN / 64; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f;
+      if (lane + 64 * i < pieces) {
+        const float2 v = *reinterpret_cast<const float2 *>(wm + ((lane + 64 * i) * nr + r) * 2);
+        l[i] = v.y;
+        if (l[i] != 0.f) m[i] = v.x;
+      }
+      top = fmaxf(top, m[i]);
+    }
+    top = wave_max(top);
+#pragma unroll
+    for (int i = 0; i < ATT8_JOIN / 64; ++i) {
+      const float w = l[i] != 0.f ? __builtin_amdgcn_exp2f(m[i] - top) : 0.f;
+      if (lane + 64 * i < pieces) weight[lane + 64 * i] = w;
+      sum += w * l[i];
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) total = sum;
+  }
+  __syncthreads();
+  float acc[4] = {};
+  for (int s = s0; s < pieces; s += U * PL) {
+    if (s != s0) fetch(s);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u * PL >= pieces) break;
+      const float w = weight[s + u * PL];
+      acc[0] = fmaf(w, x[u].x, acc[0]), acc[1] = fmaf(w, x[u].y, acc[1]);
+      acc[2] = fmaf(w, x[u].z, acc[2]), acc[3] = fmaf(w, x[u].w, acc[3]);
+    }
+  }
+  *reinterpret_cast<float4 *>(&part[s0][d]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (tid >= D) return;
+  float y = 0.f;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) y += part[i][tid];
+  Elt<T>::store((T *)a.o + r * D, tid, total == 0.f ? 0.f : y / total);
+}
+#define NK_JOIN8(T, name, D)                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void nk_attend8_join_##name##_d##D(Attend8Args a) {    \
+    attend8_join_body<T, D>(a);                                                                       \
+  }
+NK_JOIN8(bf16, bf16, 128)
+NK_JOIN8(f16, f16, 128)
+NK_JOIN8(bf16, bf16, 64)
+NK_JOIN8(f16, f16, 64)
 
 // ---------------------------------------------------------------------------
 // Packed queries (16-bit, head dim 64 or 128): the tiles of attend.hip.  One
@@ -703,8 +771,8 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   while (spoiled) {
     const int src = __builtin_ctzll(spoiled);
     spoiled &= spoiled - 1;
-    float m, l, x[4];
-    att8_row<T>(a, sq, sp, b, __shfl(qi, src, 64), __shfl(h, src, 64), j0, j1, m, l, x);
+    float m, l, x[D / 64];
+    att8_row<T, D>(a, sq, sp, b, __shfl(qi, src, 64), __shfl(h, src, 64), j0, j1, m, l, x);
     const int64_t at = __shfl((int)orow, src, 64);  // (rows are below 2^31)
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
