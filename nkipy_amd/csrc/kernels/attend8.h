@@ -82,4 +82,57 @@ NK_DEVICE void att8_row(const Attend8Args &a, const AttSeq &sq, const AttSpan &s
   }
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 B8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+NK_DEVICE f32x4 mul16(B8 a, B8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+NK_DEVICE f32x16 mul32(B8 a, B8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// Codes enter the products as bf16: code 2^e is exact there (4 significant bits,
+// fp32's exponents).  fp16 queries and weights, which bf16 does not hold, enter as
+// two bf16 numbers each, x = RN(x) + RN(x - RN(x)): exact for a query's 11 bits, a
+// weight keeps 16.
+template <int N> struct Count {
+  static constexpr int value = N;
+};
+template <typename T> struct Parts;
+template <> struct Parts<bf16> { static constexpr int N = 1; };
+template <> struct Parts<f16> { static constexpr int N = 2; };
+#define ATT8_LIMIT 65536.f
+#define ATT8_LOWEST -3.40282347e38f  // the least finite offset
+#define LOG2E 1.44269504088896340736f
+
+template <typename T, int NP>
+NK_DEVICE void load_q(const T *q, B8 (&f)[NP]) {
+  if constexpr (NP == 1) {
+    f[0] = *reinterpret_cast<const B8 *>(q);
+  } else {
+    float x[8];
+    Vec8<T>::load(q, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[0][e] = (__bf16)x[e];
+      f[1][e] = (__bf16)(x[e] - (float)f[0][e]);
+    }
+  }
+}
+template <int NP>
+NK_DEVICE void put_weight(B8 *f, int e, float x) {
+  f[0][e] = (__bf16)x;
+  if constexpr (NP == 2) f[1][e] = (__bf16)(x - (float)f[0][e]);
+}
+// eight codes times a power of two
+NK_DEVICE B8 codes8(uint32_t lo, uint32_t hi, float scale) {
+  u32x4_t w;
+  w[0] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+  w[1] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+  w[2] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+  w[3] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+  return __builtin_bit_cast(B8, w);
+}
+
 }  // namespace nk

@@ -31,63 +31,13 @@ extern "C" __global__ __launch_bounds__(256) void nk_attend8_rows_bf16(Attend8Ar
 extern "C" __global__ __launch_bounds__(256) void nk_attend8_rows_f16(Attend8Args a) { attend8_rows_body<f16>(a); }
 extern "C" __global__ __launch_bounds__(256) void nk_attend8_rows_f32(Attend8Args a) { attend8_rows_body<float>(a); }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 B8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-NK_DEVICE f32x4 mul16(B8 a, B8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-NK_DEVICE f32x16 mul32(B8 a, B8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-
-// Codes enter the products as bf16: code 2^e is exact there (4 significant bits,
-// fp32's exponents).  fp16 queries and weights, which bf16 does not hold, enter as
-// two bf16 numbers each, x = RN(x) + RN(x - RN(x)): exact for a query's 11 bits, a
-// weight keeps 16.
-template <typename T> struct Parts;
-template <> struct Parts<bf16> { static constexpr int N = 1; };
-template <> struct Parts<f16> { static constexpr int N = 2; };
-#define ATT8_LIMIT 65536.f
-#define ATT8_LOWEST -3.40282347e38f  // the least finite offset
-#define LOG2E 1.44269504088896340736f
-
-template <typename T, int NP>
-NK_DEVICE void load_q(const T *q, B8 (&f)[NP]) {
-  if constexpr (NP == 1) {
-    f[0] = *reinterpret_cast<const B8 *>(q);
-  } else {
-    float x[8];
-    Vec8<T>::load(q, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f[0][e] = (__bf16)x[e];
-      f[1][e] = (__bf16)(x[e] - (float)f[0][e]);
-    }
-  }
-}
-template <int NP>
-NK_DEVICE void put_weight(B8 *f, int e, float x) {
-  f[0][e] = (__bf16)x;
-  if constexpr (NP == 2) f[1][e] = (__bf16)(x - (float)f[0][e]);
-}
-// eight codes times a power of two
-NK_DEVICE B8 codes8(uint32_t lo, uint32_t hi, float scale) {
-  u32x4_t w;
-  w[0] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
-  w[1] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
-  w[2] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
-  w[3] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
-  return __builtin_bit_cast(B8, w);
-}
-
 // ---------------------------------------------------------------------------
 // One new token per sequence (16-bit queries, head dim 64 or 128): bound by the read
 // of the codes.  A wave takes one piece of one sequence's blocks of 32 keys for one
 // KV head, by itself: no LDS and no barrier.  Waves that run side by side take
 // neighbouring heads of the same keys, whose rows lie next to each other in memory
-// (64 contexts of up to 8192, 8 heads of 128: 142 us where the four waves of a
-// workgroup take blocks of one head, XXX so).
+// (64 contexts of up to 8192, 8 heads of 128, without the sums of what was read: 145 us
+// where the four waves of a workgroup take blocks of one head, 120 so).
 //
 // A wave has up to 16 heads of the group as the columns of 16x16x32 products,
 // S^T = K Q^T and O^T = V^T P^T.  Everything stays in registers: which element of
@@ -415,385 +365,3 @@ NK_JOIN8(bf16, bf16, 128)
 NK_JOIN8(f16, f16, 128)
 NK_JOIN8(bf16, bf16, 64)
 NK_JOIN8(f16, f16, 64)
-
-// ---------------------------------------------------------------------------
-// Packed queries (16-bit, head dim 64 or 128): the tiles of attend.hip.  One
-// workgroup of four waves per (tile of 128 rows, KV head, split); a wave owns 32
-// rows.  S^T = K Q^T and O^T = V^T P^T by 32x32x16 products, so that a lane owns one
-// row and the weights leave the first product in the order the second one takes
-// them.
-//
-// The codes of a block of 32 keys go through registers, where a thread converts the
-// 16 it read into bf16 values once for all four waves, into two LDS slots each for K
-// and V: iteration j has the scores of block j + 1, the values of block j - 1 and
-// the softmax of block j, then stores K of block j + 2 and V of block j, read an
-// iteration ago, and reads the next: one barrier per block.  A key's row and its
-// scales are looked up once per workgroup, 32 blocks ahead.
-//
-// Softmax, masks and what is computed again at the end are those of attend.hip: the
-// offset of a row is raised when a lane's 16 weights of a block exceed LIMIT, masks
-// are applied only to blocks that some row does not see whole, and rows whose sums
-// are not finite (a NaN value that other rows of the tile see), or whose offset is
-// too large to cancel, are computed again, a wave each.
-// ---------------------------------------------------------------------------
-#define ATT8_AHEAD 32  // blocks whose rows are looked up at once
-// rows outside every sequence: zeros, shared out over the grid
-template <typename T>
-NK_DEVICE void att8_zero_rest(const Attend8Args &a, int wg, int nwg) {
-  const int s0 = min(max(a.starts[0], 0), a.N), s1 = min(max(a.starts[a.B], s0), a.N);
-  const int n = a.Hq * a.D;
-  for (int x = wg; x < s0 + a.N - s1; x += nwg) {
-    T *o = (T *)a.o + (int64_t)(x < s0 ? x : x - s0 + s1) * n;
-    for (int e = threadIdx.x; e < n; e += 256) o[e] = T{};
-  }
-}
-
-template <typename T, int D>
-__device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
-  constexpr int NP = Parts<T>::N;
-  constexpr int RB = D * 2, TB = ATT_KEYS * RB;      // bytes of a row, of a block, as bf16
-  constexpr int LPR = D / 16;                        // threads that read a key's codes
-  constexpr bool BOTH = ATT_KEYS * LPR == 256;       // every thread reads keys and values (else half of them each)
-  __shared__ __attribute__((aligned(1024))) uint8_t KR[2 * TB];
-  __shared__ __attribute__((aligned(1024))) uint8_t VR[2 * TB];
-  __shared__ __attribute__((aligned(16))) int32_t ent[2 * ATT8_AHEAD * ATT_KEYS];   // rows, -1: none
-  __shared__ uint16_t exps[2 * ATT8_AHEAD * ATT_KEYS];  // exponents + 127, keys' below values'
-  __shared__ int32_t lost[8];  // per half of ent and wave: some key has no page
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, lhi = lane >> 5;
-  const int rep = a.Hq / a.Hkv;
-
-  if (a.starts) att8_zero_rest<T>(a, blockIdx.x, a.tiles * a.Hkv * a.nsplit);
-  AttWork wk;
-  AttSeq sq;
-  if (!att_tile<true>(a, blockIdx.x, wk, sq)) return;
-  const int g = wk.g, split = wk.split, b = wk.b, tile = wk.tile;
-  const AttSpan sp = att_span(a, sq, tile);
-  int j0, j1;
-  const int pieces = att_split(a, sp.nb, split, j0, j1);
-  if (split >= pieces) return;
-  const int n = j1 - j0;  // blocks of this workgroup
-
-  // this lane's row
-  const int row0 = tile * ATT_ROWS + wave * 32, rows = sq.n * rep;
-  const bool active = row0 < rows;
-  B8 qf[D / 16][NP];
-  int p, klim;  // its position and last key
-  {
-    const int rld = min(row0 + l32, rows - 1), qi = rld / rep, h = g * rep + rld % rep;
-    p = sq.p0 + qi;
-    klim = row0 + l32 < rows && p >= 0 && p < sq.len ? min(p, sq.cap - 1) : -1;
-    const T *q = (const T *)a.q + (int64_t)(sq.lo + qi) * a.q_ss + (int64_t)h * a.q_sh;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) load_q<T, NP>(q + kk * 16 + lhi * 8, qf[kk]);
-  }
-
-  f32x16 acc[D / 32];
-#pragma unroll
-  for (int t2 = 0; t2 < D / 32; ++t2)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[t2][r] = 0.f;
-  float m_run = -1e30f, l_run = 0.f;  // (finite: a masked score gives p = 0; scores below it: see `sees`)
-  const float sl2 = a.scale * LOG2E;
-
-  // swizzles: 16-byte chunk c of row r stands at chunk c ^ kswz / vswz, so that
-  // 16 rows of a K fragment, and the four rows of a transposing V read, cover
-  // all banks
-  auto kswz = [](int r) __attribute__((always_inline)) { return D == 128 ? r & 15 : (r >> 1) & 7; };
-  auto vswz = [](int r) __attribute__((always_inline)) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; };
-
-  // look up the rows of blocks 32 c .. 32 c + 31 of this workgroup
-  auto look_up = [&](int c) __attribute__((always_inline)) {
-    bool miss = false;
-#pragma unroll 1
-    for (int x = tid; x < ATT8_AHEAD * ATT_KEYS; x += 256) {
-      const int j = j0 + c * ATT8_AHEAD + x / ATT_KEYS;
-      const int key = sp.kb(j) * ATT_KEYS + x % ATT_KEYS;
-      int at = -1, ex = 0;
-      if (j < j1 && key < sp.hi && (key >= sp.lo || key < a.sinks)) {
-        const int pg = a.tables[(int64_t)b * a.width + key / a.page];
-        if (pg >= 0 && pg < a.pages) {
-          at = pg * a.pitch + key % a.page;
-          ex = (c8_clip(a.ke[(int64_t)pg * a.Hkv + g]) + 127) | (c8_clip(a.ve[(int64_t)pg * a.Hkv + g]) + 127) << 8;
-        }
-        miss |= at < 0;
-      }
-      ent[(c & 1) * ATT8_AHEAD * ATT_KEYS + x] = at;
-      exps[(c & 1) * ATT8_AHEAD * ATT_KEYS + x] = (uint16_t)ex;
-    }
-    const bool any = __ballot(miss) != 0;
-    if (lane == 0) lost[(c & 1) * 4 + wave] = any;
-  };
-
-  // a thread's codes of a block: row rr, elements 16 cc ... ; `mine`: whether it reads this array
-  const int rr = (BOTH ? tid : tid & 127) / LPR, cc = tid % LPR;
-  const uint8_t *kp = (const uint8_t *)a.k + (int64_t)g * a.k_sh + cc * 16;
-  const uint8_t *vp = (const uint8_t *)a.v + (int64_t)g * a.v_sh + cc * 16;
-  struct Codes {
-    uint4 w;
-    float scale;
-  };
-  Codes ck, cv;
-  auto load = [&](Codes &x, const uint8_t *base, int64_t ss, int jr, bool mine, int shift) __attribute__((always_inline)) {
-    const int at = jr >= 0 && jr < n && mine ? ent[(jr & (2 * ATT8_AHEAD - 1)) * ATT_KEYS + rr] : -1;
-    const int ex = at >= 0 ? exps[(jr & (2 * ATT8_AHEAD - 1)) * ATT_KEYS + rr] : 0;
-    x.scale = __uint_as_float((uint32_t)(ex >> shift & 0xff) << 23);
-    x.w = make_uint4(0, 0, 0, 0);
-    if (at >= 0) x.w = *reinterpret_cast<const uint4 *>(base + at * ss);
-  };
-  const bool kmine = BOTH || tid < 128, vmine = BOTH || tid >= 128;
-  auto load_k = [&](int jr) __attribute__((always_inline)) { load(ck, kp, a.k_ss, jr, kmine, 0); };
-  auto load_v = [&](int jr) __attribute__((always_inline)) { load(cv, vp, a.v_ss, jr, vmine, 8); };
-  auto store = [&](const Codes &x, uint8_t *to, int swz) __attribute__((always_inline)) {
-    *reinterpret_cast<B8 *>(to + rr * RB + (((2 * cc) ^ swz) << 4)) = codes8(x.w.x, x.w.y, x.scale);
-    *reinterpret_cast<B8 *>(to + rr * RB + (((2 * cc + 1) ^ swz) << 4)) = codes8(x.w.z, x.w.w, x.scale);
-  };
-  auto store_k = [&](int jr) __attribute__((always_inline)) { if (kmine) store(ck, KR + (jr & 1) * TB, kswz(rr)); };
-  auto store_v = [&](int jr) __attribute__((always_inline)) { if (vmine) store(cv, VR + (jr & 1) * TB, vswz(rr)); };
-
-  // K fragment kk: row l32, chunk 2 kk + lhi
-  const int kbase = l32 * RB + ((lhi ^ (kswz(l32) & 1)) << 4), kx = (kswz(l32) & ~1) << 4;
-  // transposing V read (group lane / 16, i = lane % 16): row 16 j + 8 si + 4 (group / 2) + i / 4,
-  // columns 32 dt + 16 (group % 2) + 4 (i % 4)
-  int vbase, vx;
-  {
-    const int grp = lane >> 4, gi = lane & 15, r = 4 * (grp >> 1) + (gi >> 2);
-    vbase = r * RB + (((grp & 1) * 2 + ((gi & 3) >> 1)) << 4) + (gi & 1) * 8;
-    vx = vswz(r) << 4;
-  }
-  auto qk1 = [&](const uint8_t *K, f32x16 &s, int kk) __attribute__((always_inline)) {
-    const B8 f = *reinterpret_cast<const B8 *>(K + kbase + ((kk << 5) ^ kx));
-#pragma unroll
-    for (int i = 0; i < NP; ++i) s = mul32(f, qf[kk][i], s);
-  };
-  auto pv1 = [&](const uint8_t *Vt, const B8 (&pf)[2][NP], int j, int dt) __attribute__((always_inline)) {
-    s16x4 v[2];
-#pragma unroll
-    for (int si = 0; si < 2; ++si)
-      v[si] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_s16x4 *)(Vt + (16 * j + 8 * si) * RB + vbase + ((dt << 6) ^ vx)));
-    const s16x8 vf = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) acc[dt] = mul32(__builtin_bit_cast(B8, vf), pf[j][i], acc[dt]);
-  };
-  // The scores of one block and the values of another, in turns: each product of
-  // the scores waits for the one before it, the values' are apart.
-  auto qk_pv = [&](const uint8_t *K, f32x16 &s, const uint8_t *Vt, const B8 (&pf)[2][NP]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      qk1(K, s, i);
-      pv1(Vt, pf, i / (D / 32), i % (D / 32));
-    }
-  };
-  auto expblock = [&](const f32x16 &s, B8 (&pf)[2][NP]) __attribute__((always_inline)) {
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * j + e], sl2, -m_run));
-        if (e & 1) s1 += x; else s0 += x;
-        put_weight<NP>(pf[j], e, x);
-      }
-    return s0 + s1;
-  };
-  int missing = 0;  // the blocks being worked on have keys without a page
-  // What no row sees of block jr out of its scores; past the last block, all of it.
-  // Element r of a lane is key 32 kb + 8 (r / 4) + 4 lhi + r % 4.
-  auto mask = [&](f32x16 &s, int jr) __attribute__((always_inline)) {
-    const int k0 = sp.kb(j0 + jr) * ATT_KEYS + lhi * 4;
-    const int t0 = jr < n ? klim - k0 : -1, w0 = p - a.window - k0, s0 = a.sinks - k0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int x = (r >> 2) * 8 + (r & 3);
-      s[r] = x > t0 || (x <= w0 && x >= s0) ? -INFINITY : s[r];
-    }
-    if (missing) {
-      const int32_t *en = ent + (jr & (2 * ATT8_AHEAD - 1)) * ATT_KEYS + lhi * 4;
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int4 e = *reinterpret_cast<const int4 *>(en + r * 2);
-        s[r] = e.x < 0 ? -INFINITY : s[r];
-        s[r + 1] = e.y < 0 ? -INFINITY : s[r + 1];
-        s[r + 2] = e.z < 0 ? -INFINITY : s[r + 2];
-        s[r + 3] = e.w < 0 ? -INFINITY : s[r + 3];
-      }
-    }
-  };
-  auto raise = [&](f32x16 &s, B8 (&pf)[2][NP], float ls) __attribute__((always_inline)) {
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ls <= ATT8_LIMIT)) != 0, 0)) {
-      float bm = s[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) bm = fmaxf(bm, s[r]);
-      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float m_new = fmaxf(m_run, bm * sl2);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-      m_run = m_new;
-#pragma unroll
-      for (int t2 = 0; t2 < D / 32; ++t2)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[t2][r] *= alpha;
-      l_run *= alpha;
-      ls = expblock(s, pf);
-    }
-    l_run += ls;
-  };
-  auto whole = [&](int jr) __attribute__((always_inline)) {  // every row sees the whole block
-    const int k0 = sp.kb(j0 + jr) * ATT_KEYS;
-    return jr < n && k0 + ATT_KEYS - 1 <= sp.pa && k0 + ATT_KEYS <= sp.hi && (k0 > sp.pb - a.window || k0 + ATT_KEYS <= a.sinks) && !missing;
-  };
-
-  f32x16 sA, sB;
-  B8 pA[2][NP], pB[2][NP];
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) put_weight<NP>(pB[j], e, 0.f);
-  // the end of an iteration: what was read is stored, the next is read
-  auto move_on = [&](int jr) __attribute__((always_inline)) {
-    store_k(jr + 2);
-    store_v(jr);
-    lds_barrier();
-    load_k(jr + 3);
-    load_v(jr + 1);
-  };
-  // Iteration jr, one body for all: the values of the block before (of zeros before
-  // the first), the scores of the one behind (of zeros past the last), the softmax of
-  // this one.  The last, jr = n, adds the last block's values.
-  auto step = [&](int jr, f32x16 &cur, f32x16 &nxt, B8 (&prev)[2][NP], B8 (&now)[2][NP]) __attribute__((always_inline)) {
-    if (!whole(jr)) mask(cur, jr);
-    qk_pv(KR + ((jr + 1) & 1) * TB, nxt, VR + ((jr + 1) & 1) * TB, prev);
-    const float ls = expblock(cur, now);
-    raise(cur, now, ls);
-    move_on(jr);
-  };
-
-  if (n > 0) {
-    look_up(0);
-    __syncthreads();
-    load_k(0);
-    load_v(-1);  // (zeros)
-    store_k(0);
-    store_v(1);
-    load_k(1);
-    store_k(1);
-    load_k(2);
-    load_v(0);
-    lds_barrier();
-    if (active) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sA[r] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) qk1(KR, sA, kk);
-    }
-    lds_barrier();  // (block 0 is read before its slot is refilled)
-    auto ahead = [&](int jr) __attribute__((always_inline)) {
-      if (jr % ATT8_AHEAD == 0) {
-        const int32_t *f = lost + (jr / ATT8_AHEAD & 1) * 4;
-        missing = __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]);
-        // (the other half was last read an iteration, and a barrier, ago)
-        if (jr + ATT8_AHEAD < n) look_up(jr / ATT8_AHEAD + 1);
-      }
-    };
-    if (active) {
-      for (int jr = 0;; jr += 2) {
-        ahead(jr);
-        step(jr, sA, sB, pB, pA);
-        if (jr + 1 > n) break;
-        step(jr + 1, sB, sA, pA, pB);
-        if (jr + 2 > n) break;
-      }
-    } else {  // rows past the sequence's: the moves only
-      for (int jr = 0; jr <= n; ++jr) {
-        ahead(jr);
-        move_on(jr);
-      }
-    }
-  }
-
-  const int row = row0 + l32, rld = min(row, rows - 1), qi = rld / rep, h = g * rep + rld % rep;
-  const bool ok = klim >= 0;
-  l_run += __shfl_xor(l_run, 32, 64);
-  const int64_t nr = (int64_t)a.N * a.Hq;
-  const int64_t orow = ((int64_t)(sq.lo + qi)) * a.Hq + h;
-  float *wo = a.ws + (split * nr + orow) * D, *wm = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + orow) * 2;
-  uint16_t *o = (uint16_t *)a.o + orow * D;
-
-  // whether this row, if it has no weight, sees any key of these blocks, pages aside
-  bool sees = false;
-  if (__any(ok && l_run == 0.f)) {
-    auto part = [&](int a0, int a1) __attribute__((always_inline)) {  // (blocks that follow each other)
-      const int lo = sp.kb(a0) * ATT_KEYS, hi = min(sp.kb(a1 - 1) * ATT_KEYS + ATT_KEYS - 1, klim);
-      sees |= a0 < a1 && (max(lo, p - a.window + 1) <= hi || lo <= min(hi, a.sinks - 1));
-    };
-    part(j0, min(j1, sp.ns));
-    part(max(j0, sp.ns), j1);
-  }
-
-  // rows that a NaN value may have spoiled, and those whose offset is too large to
-  // cancel: s c - m is then off by half a step of m.  A row without weight still has
-  // the offset it began with: where it sees keys their scores are below that, or -inf.
-  float z = l_run * 0.f;
-#pragma unroll
-  for (int t2 = 0; t2 < D / 32; ++t2)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) z = __builtin_fmaf(acc[t2][r], 0.f, z);
-  uint64_t spoiled = __ballot(ok && (z != 0.f || (fabsf(m_run) >= 0x1p24f && (l_run != 0.f || sees))));
-  spoiled = (spoiled | spoiled >> 32) & 0xffffffffull;
-  const bool put = row < rows && !(spoiled >> l32 & 1);
-  if (put && pieces == 1) {
-    const float inv = ok && l_run != 0.f ? 1.0f / l_run : 0.f;
-#pragma unroll
-    for (int t2 = 0; t2 < D / 32; ++t2)
-#pragma unroll
-      for (int gq = 0; gq < 4; ++gq) {
-        T y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) Elt<T>::store(y, e, inv == 0.f ? 0.f : acc[t2][gq * 4 + e] * inv);
-        uint2 u;
-        __builtin_memcpy(&u, y, 8);
-        *reinterpret_cast<uint2 *>(o + t2 * 32 + gq * 8 + lhi * 4) = u;
-      }
-  } else if (put) {
-#pragma unroll
-    for (int t2 = 0; t2 < D / 32; ++t2)
-#pragma unroll
-      for (int gq = 0; gq < 4; ++gq)
-        *reinterpret_cast<float4 *>(wo + t2 * 32 + gq * 8 + lhi * 4) =
-            ok ? make_float4(acc[t2][gq * 4], acc[t2][gq * 4 + 1], acc[t2][gq * 4 + 2], acc[t2][gq * 4 + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (lhi == 0) wm[0] = m_run, wm[1] = ok ? l_run : 0.f;
-  }
-  // these again, reading only what they see
-  while (spoiled) {
-    const int src = __builtin_ctzll(spoiled);
-    spoiled &= spoiled - 1;
-    float m, l, x[D / 64];
-    att8_row<T, D>(a, sq, sp, b, __shfl(qi, src, 64), __shfl(h, src, 64), j0, j1, m, l, x);
-    const int64_t at = __shfl((int)orow, src, 64);  // (rows are below 2^31)
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      if (pieces == 1) {
-        Elt<T>::store((T *)a.o + at * D, lane + 64 * e, l == 0.f ? 0.f : x[e] / l);
-      } else {
-        a.ws[(split * nr + at) * D + lane + 64 * e] = x[e];
-      }
-    }
-    if (pieces > 1 && lane == 0) {
-      float *y = a.ws + (int64_t)a.nsplit * nr * D + (split * nr + at) * 2;
-      y[0] = fmaxf(m * LOG2E, ATT8_LOWEST);
-      y[1] = l;
-    }
-  }
-}
-#define NK_TILE8(T, name, D, OCC)                                                                          \
-  extern "C" __global__ __launch_bounds__(256, OCC) void nk_attend8_tile_##name##_d##D(Attend8Args a) {    \
-    attend8_tile_body<T, D>(a);                                                                            \
-  }
-NK_TILE8(bf16, bf16, 128, 2)
-NK_TILE8(f16, f16, 128, 1)  // (under a bound of two, registers in memory)
-NK_TILE8(bf16, bf16, 64, 2)
-NK_TILE8(f16, f16, 64, 2)

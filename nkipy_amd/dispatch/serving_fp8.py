@@ -117,7 +117,8 @@ def attend8(dtype, q, k, v, o, *, B, N, Hq, Hkv, D, q_str, k_str, v_str, scale, 
     n = -(-units * a.nsplit // 4) if step else units * Hkv * a.nsplit
     if n >= 2**29:
         raise LaunchError("attention: too many tiles for one launch")
-    out = [Launch("attend8", f"nk_attend8_{'step' if step else 'tile'}_{tag}_d{D}", (n, 1, 1), (256, 1, 1), a)]
+    out = [Launch("attend8", f"nk_attend8_step_{tag}_d{D}", (n, 1, 1), (256, 1, 1), a) if step else
+           Launch("attend8_tile", f"nk_attend8_tile_{tag}_d{D}", (n, 1, 1), (256, 1, 1), a)]
     if a.nsplit > 1 and step:
         out.append(Launch("attend8", f"nk_attend8_join_{tag}_d{D}", (N * Hq, 1, 1), (256, 1, 1), a))
     elif a.nsplit > 1:
