@@ -15,9 +15,10 @@ using namespace nk;
 // in fp32, every product and sum rounded by itself, so that the largest magnitude,
 // and with it e, is what the same steps give anywhere.  Workgroups: one for each
 // token's queries; one for each (page that a sequence writes, keys or values, some
-// heads), which reads its rows twice: for the largest magnitude, then, mostly from
-// cache, for the codes.  Maxima are of whole numbers (bits), so no order changes
-// them.  Bound by memory, single tokens by latency.
+// heads), as many as its threads can keep between the largest magnitude and the codes
+// (large pages, odd sizes and heads rotated in part: read again, mostly from cache).
+// Maxima are of whole numbers (bits), so no order changes them.  Bound by memory,
+// single tokens by latency.
 // ---------------------------------------------------------------------------
 struct Append8Args {
   const void *q, *k, *v;
@@ -30,8 +31,10 @@ struct Append8Args {
   int32_t B, N, Hq, Hkv, D, half, P;
   int32_t page, pages, width;
   int32_t heads;  // of a workgroup, up to A8_HEADS
+  int32_t blocks;  // workgroups of keys and values
 };
 #define A8_HEADS 64
+#define A8_ITEMS 4  // pairs of pieces that a thread keeps
 
 // the sequence of token or tile t, by its first one: the last that begins at or before
 template <typename F>
@@ -111,13 +114,14 @@ template <typename T, int E>
 __device__ __forceinline__ void append8_body(const Append8Args &a) {
   __shared__ uint32_t top[A8_HEADS];
   __shared__ int32_t now[A8_HEADS], old[A8_HEADS];
-  const int tid = threadIdx.x, nq = a.oq ? a.N : 0;
-  if ((int)blockIdx.x < nq) {
-    append8_queries<T, E>(a, blockIdx.x);
+  const int tid = threadIdx.x;
+  // (keys and values first: they take longer)
+  if ((int)blockIdx.x >= a.blocks) {
+    append8_queries<T, E>(a, blockIdx.x - a.blocks);
     return;
   }
   const int parts = (a.Hkv + a.heads - 1) / a.heads;
-  int w = blockIdx.x - nq;
+  int w = blockIdx.x;
   const int h0 = w % parts * a.heads, hn = min(a.heads, a.Hkv - h0);
   w /= parts;
   const bool values = w & 1;
@@ -147,51 +151,85 @@ __device__ __forceinline__ void append8_body(const Append8Args &a) {
 
   if (tid < hn) top[tid] = 0, old[tid] = first ? c8_clip(exps[tid]) : C8_MIN;
   __syncthreads();
-  // every piece of these rows: f(row, head, first element, whether it is a pair, its values)
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    for (int x = tid; x < n * hn * per; x += 256) {
-      const int r = x / (hn * per), y = x % (hn * per), h = y / per, c = y % per;
-      const T *from = src + r * ss + h * sh;
-      float y0[E], y1[E];
-      if (c < turns) {
-        const int64_t at = (int64_t)(lo + r) * half + c * E;
-        a8_turn<T, E>(from + c * E, a.cos + at, a.sin + at, half, y0, y1);
-        f(r, h, c * E, true, y0, y1);
-      } else {
-        const int d = 2 * half + (c - turns) * E;
-        Piece<T, E>::load(from + d, y0);
-        f(r, h, d, false, y0, y0);
-      }
-    }
-  };
-  int mine = -1;
-  uint32_t most = 0;
-  each([&](int, int h, int, bool pair, const float (&y0)[E], const float (&y1)[E]) __attribute__((always_inline)) {
-    if (h != mine) {
-      if (most) atomicMax(&top[mine], most);
-      mine = h, most = 0;
-    }
+  auto larger = [&](uint32_t most, const float (&y)[E]) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const uint32_t u = __float_as_uint(y0[e]) & 0x7fffffffu, v = __float_as_uint(y1[e]) & 0x7fffffffu;
-      if (u < 0x7f800000u) most = max(most, u);
-      if (pair && v < 0x7f800000u) most = max(most, v);
+      const uint32_t u = __float_as_uint(y[e]) & 0x7fffffffu;
+      most = u < 0x7f800000u ? max(most, u) : most;
     }
-  });
-  if (most) atomicMax(&top[mine], most);
-  __syncthreads();
-  if (tid < hn) {
-    const int e = max(c8_exponent(__uint_as_float(top[tid])), old[tid]);
-    now[tid] = e;
-    exps[tid] = e;
+    return most;
+  };
+  auto settle = [&]() __attribute__((always_inline)) {  // the heads' exponents
+    __syncthreads();
+    if (tid < hn) {
+      const int e = max(c8_exponent(__uint_as_float(top[tid])), old[tid]);
+      now[tid] = e;
+      exps[tid] = e;
+    }
+    __syncthreads();
+  };
+  if (E == 8 && n * hn * a.D <= 1024 * A8_ITEMS * 4 && a.D % 16 == 0 && (values || 2 * half == a.D)) {
+    // read once: a thread's pairs of pieces, the same place of both halves of a head
+    const int pc = a.D / 16, total = n * hn * pc;
+    float y[A8_ITEMS][2][E];
+    int at[A8_ITEMS], head[A8_ITEMS];
+#pragma unroll
+    for (int i = 0; i < A8_ITEMS; ++i) {
+      const int x = min(tid + 256 * i, total - 1), r = x / (hn * pc), z = x % (hn * pc), h = z / pc, c = z % pc;
+      const T *from = src + r * ss + h * sh + c * E;
+      head[i] = h, at[i] = ((first + r) * a.Hkv + h) * a.D + c * E;
+      if (values) {
+        Piece<T, E>::load(from, y[i][0]);
+        Piece<T, E>::load(from + a.D / 2, y[i][1]);
+      } else {
+        const int64_t turn = (int64_t)(lo + r) * half + c * E;
+        a8_turn<T, E>(from, a.cos + turn, a.sin + turn, half, y[i][0], y[i][1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < A8_ITEMS; ++i) {
+      // (past the last item: that one again)
+      const uint32_t most = larger(larger(0, y[i][0]), y[i][1]);
+      if (most) atomicMax(&top[head[i]], most);
+    }
+    settle();
+#pragma unroll
+    for (int i = 0; i < A8_ITEMS; ++i) {
+      if (tid + 256 * i >= total) break;
+      const float scale = c8_power(-now[head[i]]);
+      c8_store<E>(codes + at[i], y[i][0], scale);
+      c8_store<E>(codes + at[i] + a.D / 2, y[i][1], scale);
+    }
+  } else {
+    // every piece of these rows: f(row, head, first element, whether it is a pair, its values)
+    auto each = [&](auto f) __attribute__((always_inline)) {
+      for (int x = tid; x < n * hn * per; x += 256) {
+        const int r = x / (hn * per), y = x % (hn * per), h = y / per, c = y % per;
+        const T *from = src + r * ss + h * sh;
+        float y0[E], y1[E];
+        if (c < turns) {
+          const int64_t at = (int64_t)(lo + r) * half + c * E;
+          a8_turn<T, E>(from + c * E, a.cos + at, a.sin + at, half, y0, y1);
+          f(r, h, c * E, true, y0, y1);
+        } else {
+          const int d = 2 * half + (c - turns) * E;
+          Piece<T, E>::load(from + d, y0);
+          f(r, h, d, false, y0, y0);
+        }
+      }
+    };
+    each([&](int, int h, int, bool, const float (&y0)[E], const float (&y1)[E]) __attribute__((always_inline)) {
+      const uint32_t most = larger(larger(0, y0), y1);
+      if (most) atomicMax(&top[h], most);
+    });
+    settle();
+    each([&](int r, int h, int d, bool pair, const float (&y0)[E], const float (&y1)[E]) __attribute__((always_inline)) {
+      const float scale = c8_power(-now[h]);
+      uint8_t *to = codes + ((int64_t)(first + r) * a.Hkv + h) * a.D + d;
+      c8_store<E>(to, y0, scale);
+      if (pair) c8_store<E>(to + half, y1, scale);
+    });
   }
-  __syncthreads();
-  each([&](int r, int h, int d, bool pair, const float (&y0)[E], const float (&y1)[E]) __attribute__((always_inline)) {
-    const float scale = c8_power(-now[h]);
-    uint8_t *to = codes + ((int64_t)(first + r) * a.Hkv + h) * a.D + d;
-    c8_store<E>(to, y0, scale);
-    if (pair) c8_store<E>(to + half, y1, scale);
-  });
   // the rows before, where the scale grew
   for (int h = 0; h < hn && first; ++h) {
     const int by = old[h] - now[h];

@@ -40,15 +40,22 @@ NK_DEVICE T running_block(T v, T *red, T &all) {
 // bitmap in LDS.  What is not marked is free, and the r-th free page goes to the
 // r-th entry that wants one: r by running sums over the rows, the page by running
 // counts over the bitmap.  Marks are ORs and sums are whole numbers, so no order
-// changes a result.  Bound by latency: one workgroup, a few dependent reads.
+// changes a result.
+//
+// Bound by latency.  Small batches are one launch of one workgroup; larger ones
+// three: workgroups that mark some rows each, into bitmaps of their own; one that
+// joins the bitmaps, sums up and lists the free pages that are wanted; and as many as
+// there are rows and tokens for the entries and slots (500 rows of up to 375 pages,
+// 20000 tokens: 83 us by the one workgroup, XXX so).
 // ---------------------------------------------------------------------------
 struct AssignArgs {
   int32_t *tables;  // (rows, width)
   const int32_t *lens, *news;
   int32_t *starts, *slots, *free;
-  int32_t *wants;  // (rows) pages wanted by the rows before
-  int32_t rows, width, page, pages, tokens;
-  int32_t small;  // the slots are this launch's too
+  int32_t *wants;   // (rows) pages wanted by the rows before
+  int32_t *list;    // the free pages that are wanted, in order; -1 behind the last
+  uint32_t *marks;  // (parts, words) bitmaps of some rows each
+  int32_t rows, width, page, pages, tokens, parts;
 };
 #define ASG_BLOCK 1024
 #define ASG_WORDS 32768  // of 32 pages
@@ -56,57 +63,51 @@ struct AssignArgs {
 struct AsgRow {
   int len, fresh, held, need;
 };
-NK_DEVICE AsgRow asg_row(const AssignArgs &a, int b) {
+NK_DEVICE AsgRow asg_row(const AssignArgs &a, int len, int fresh) {
   AsgRow r;
-  r.len = min(max(a.lens[b], 0), 1 << 30);
-  r.fresh = min(max(a.news[b], 0), 1 << 30);
+  r.len = min(max(len, 0), 1 << 30);
+  r.fresh = min(max(fresh, 0), 1 << 30);
   // (sums below 2^31: page is at most 2^30)
   r.held = min((int)(((uint32_t)max(r.len - r.fresh, 0) + (uint32_t)a.page - 1) / (uint32_t)a.page), a.width);
   r.need = min((int)(((uint32_t)r.len + (uint32_t)a.page - 1) / (uint32_t)a.page), a.width);
   return r;
 }
+NK_DEVICE AsgRow asg_row(const AssignArgs &a, int b) { return asg_row(a, a.lens[b], a.news[b]); }
 
-// Slots of 64 tokens t0 ..: the rows that begin among them are read side by side.
-NK_DEVICE void asg_slots(const AssignArgs &a, int t0) {
-  const int lane = threadIdx.x & 63, t = t0 + lane;
-  int b0 = 0;  // rows that begin at or before t0
-  for (int b = 0; b < a.rows; b += 64) b0 += __popcll(__ballot(b + lane < a.rows && a.starts[min(b + lane, a.rows - 1)] <= t0));
-  int b = b0 - 1;
-  for (int x = b0;; x += 64) {
-    const int s = x + lane < a.rows ? a.starts[x + lane] : 0x7fffffff;
-    int more = 0;
-#pragma unroll 8
-    for (int k = 0; k < 64; ++k) more += __builtin_amdgcn_readlane(s, k) <= t ? 1 : 0;
-    b += more;
-    if (!__any(more == 64)) break;
-  }
-  if (t >= a.tokens) return;
-  int slot = -1;
-  if (b >= 0 && t < a.starts[b + 1]) {
-    const int p = min(max(a.lens[b], 0), 1 << 30) - min(max(a.news[b], 0), 1 << 30) + (t - a.starts[b]);
-    if (p >= 0 && p / a.page < a.width) {
-      const int pg = a.tables[(int64_t)b * a.width + p / a.page];
-      if (pg >= 0 && pg < a.pages) slot = pg * a.page + p % a.page;
+// The pages that rows b0, b0 + step, ... hold, marked by a wave: four rows' entries
+// on their way at once.
+NK_DEVICE void asg_mark(const AssignArgs &a, uint32_t *used, int b0, int step) {
+  const int lane = threadIdx.x & 63;
+  auto mark = [&](int pg) __attribute__((always_inline)) {
+    if (pg >= 0 && pg < a.pages) atomicOr(&used[pg >> 5], 1u << (pg & 31));
+  };
+  for (int c0 = b0; c0 < a.rows; c0 += 64 * step) {
+    const int64_t b = c0 + (int64_t)lane * step;  // (a lane's row of the next 64)
+    const int held = b < a.rows ? asg_row(a, (int)b).held : 0;
+    for (int r = 0; r < 64 && c0 + (int64_t)r * step < a.rows; r += 4) {
+      int pg[4][4], n[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        n[u] = __builtin_amdgcn_readlane(held, r + u);
+        const int32_t *t = a.tables + min(c0 + (int64_t)(r + u) * step, (int64_t)a.rows - 1) * a.width;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pg[u][k] = k * 64 + lane < n[u] ? t[k * 64 + lane] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mark(pg[u][k]);
+        const int32_t *t = a.tables + min(c0 + (int64_t)(r + u) * step, (int64_t)a.rows - 1) * a.width;
+        for (int i = 256 + lane; i < n[u]; i += 64) mark(t[i]);
+      }
     }
   }
-  a.slots[t] = slot;
 }
 
-extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_pages(AssignArgs a) {
-  __shared__ uint32_t used[ASG_WORDS];
-  __shared__ int32_t before[ASG_BLOCK];  // free pages before a thread's words
-  __shared__ int64_t red[ASG_BLOCK / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int words = (a.pages + 31) / 32;
-  for (int i = tid; i < words; i += ASG_BLOCK) used[i] = 0;
-  __syncthreads();
-  for (int b = wave; b < a.rows; b += ASG_BLOCK / 64) {
-    const int held = asg_row(a, b).held;
-    for (int i = lane; i < held; i += 64) {
-      const int pg = a.tables[(int64_t)b * a.width + i];
-      if (pg >= 0 && pg < a.pages) atomicOr(&used[pg >> 5], 1u << (pg & 31));
-    }
-  }
+// Starts and wanted pages of the rows, and from the bitmap the free pages before each
+// thread's words; returns (pages wanted, pages free).
+NK_DEVICE void asg_sums(const AssignArgs &a, const uint32_t *used, int32_t *before, int64_t *red, int64_t &wanted, int64_t &free) {
+  const int tid = threadIdx.x;
   int64_t starts = 0, wants = 0, all;
   for (int b0 = 0; b0 < a.rows; b0 += ASG_BLOCK) {
     const int b = b0 + tid;
@@ -124,10 +125,8 @@ extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_pages(AssignAr
       a.wants[b] = (int32_t)min(ws - w, (int64_t)a.pages);
     }
   }
+  const int words = (a.pages + 31) / 32;
   const int per = (words + ASG_BLOCK - 1) / ASG_BLOCK, w0 = min(tid * per, words), w1 = min(w0 + per, words);
-  __syncthreads();
-  if (tid == 0 && (a.pages & 31)) used[words - 1] |= ~0u << (a.pages & 31);  // (no pages)
-  __syncthreads();
   int64_t n = 0;
   for (int i = w0; i < w1; ++i) n += __popc(~used[i]);
   const int64_t upto = running_block<ASG_BLOCK / 64>(n, red, all);
@@ -136,39 +135,109 @@ extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_pages(AssignAr
     a.starts[a.rows] = (int32_t)min(starts, (int64_t)0x7fffffff);
     a.free[0] = (int32_t)max(all - wants, (int64_t)-0x7fffffff);
   }
-  __syncthreads();
-  const int free = (int)all;
-  for (int b = wave; b < a.rows; b += ASG_BLOCK / 64) {
+  wanted = wants, free = all;
+}
+// the wanted free pages of a thread's words
+NK_DEVICE void asg_list(const AssignArgs &a, const uint32_t *used, int before, int64_t wanted, int64_t free) {
+  const int words = (a.pages + 31) / 32;
+  const int per = (words + ASG_BLOCK - 1) / ASG_BLOCK, w0 = min((int)threadIdx.x * per, words), w1 = min(w0 + per, words);
+  const int most = (int)min(wanted, (int64_t)a.pages);
+  for (int i = w0, k = before; i < w1 && k < most; ++i)
+    for (uint32_t bits = ~used[i]; bits && k < most; bits &= bits - 1, ++k) a.list[k] = i * 32 + __builtin_ctz(bits);
+  for (int k = (int)free + threadIdx.x; k < most; k += ASG_BLOCK) a.list[k] = -1;
+}
+// the page of entry i of a row
+NK_DEVICE int asg_entry(const AssignArgs &a, int64_t b, const AsgRow &r, int first, int i) {
+  if (i < r.held) return a.tables[b * a.width + i];
+  const int k = first + (i - r.held);
+  return i < r.need && k < a.pages ? a.list[k] : -1;
+}
+// the entries of row b that it does not hold, by `threads` from t on
+NK_DEVICE void asg_fill(const AssignArgs &a, int b, int t, int threads) {
+  const AsgRow r = asg_row(a, b);
+  const int first = a.wants[b];
+  for (int i = r.held + t; i < a.width; i += threads) a.tables[(int64_t)b * a.width + i] = asg_entry(a, b, r, first, i);
+}
+
+// Slots of 64 tokens t0 ..: the rows that begin among them are read side by side.
+NK_DEVICE void asg_slots(const AssignArgs &a, int t0) {
+  const int lane = threadIdx.x & 63, t = t0 + lane;
+  int b0 = 0;  // rows that begin at or before t0
+#pragma unroll 4
+  for (int b = 0; b < a.rows; b += 64) b0 += __popcll(__ballot(b + lane < a.rows && a.starts[min(b + lane, a.rows - 1)] <= t0));
+  int b = b0 - 1;
+  for (int x = b0;; x += 64) {
+    const int s = x + lane < a.rows ? a.starts[x + lane] : 0x7fffffff;
+    int more = 0;
+#pragma unroll 8
+    for (int k = 0; k < 64; ++k) more += __builtin_amdgcn_readlane(s, k) <= t ? 1 : 0;
+    b += more;
+    if (!__any(more == 64)) break;
+  }
+  if (t >= a.tokens) return;
+  int slot = -1;
+  if (b >= 0 && t < a.starts[b + 1]) {
     const AsgRow r = asg_row(a, b);
-    const int first = a.wants[b];
-    for (int i = r.held + lane; i < a.width; i += 64) {
-      int pg = -1;
-      const int k = first + (i - r.held);
-      if (i < r.need && k < free) {
-        // the last thread with so many free pages before its words, then its words
-        int lo = 0, hi = ASG_BLOCK - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (before[mid] <= k) lo = mid; else hi = mid - 1;
-        }
-        int left = k - before[lo], w = lo * per;
-        uint32_t bits = ~used[w];
-        while (left >= __popc(bits)) left -= __popc(bits), bits = ~used[++w];
-        for (; left; --left) bits &= bits - 1;
-        pg = w * 32 + __builtin_ctz(bits);
-      }
-      a.tables[(int64_t)b * a.width + i] = pg;
+    const int p = r.len - r.fresh + (t - a.starts[b]);
+    if (p >= 0 && p / a.page < a.width) {
+      const int pg = asg_entry(a, b, r, a.wants[b], p / a.page);
+      if (pg >= 0 && pg < a.pages) slot = pg * a.page + p % a.page;
     }
   }
-  if (a.small) {
-    __threadfence_block();
-    __syncthreads();
-    for (int t = wave * 64; t < a.tokens; t += ASG_BLOCK) asg_slots(a, t);
-  }
+  a.slots[t] = slot;
 }
-extern "C" __global__ __launch_bounds__(256) void nk_assign_slots(AssignArgs a) {
-  const int t = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
-  if (t < a.tokens) asg_slots(a, t);
+
+extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_pages(AssignArgs a) {
+  __shared__ uint32_t used[ASG_WORDS];
+  __shared__ int32_t before[ASG_BLOCK];
+  __shared__ int64_t red[ASG_BLOCK / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, words = (a.pages + 31) / 32;
+  for (int i = tid; i < words; i += ASG_BLOCK) used[i] = i == words - 1 && (a.pages & 31) ? ~0u << (a.pages & 31) : 0;  // (no pages)
+  __syncthreads();
+  asg_mark(a, used, wave, ASG_BLOCK / 64);
+  __syncthreads();
+  int64_t wanted, free;
+  asg_sums(a, used, before, red, wanted, free);
+  asg_list(a, used, before[tid], wanted, free);
+  __threadfence_block();
+  __syncthreads();
+  for (int t = wave * 64; t < a.tokens; t += ASG_BLOCK) asg_slots(a, t);
+  for (int b = wave; b < a.rows; b += ASG_BLOCK / 64) asg_fill(a, b, lane, 64);
+}
+// the bitmap of a share of the rows
+extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_mark(AssignArgs a) {
+  __shared__ uint32_t used[ASG_WORDS];
+  const int tid = threadIdx.x, wave = tid >> 6, words = (a.pages + 31) / 32;
+  for (int i = tid; i < words; i += ASG_BLOCK) used[i] = i == words - 1 && (a.pages & 31) ? ~0u << (a.pages & 31) : 0;
+  __syncthreads();
+  asg_mark(a, used, blockIdx.x * (ASG_BLOCK / 64) + wave, a.parts * (ASG_BLOCK / 64));
+  __syncthreads();
+  for (int i = tid; i < words; i += ASG_BLOCK) a.marks[(int64_t)blockIdx.x * words + i] = used[i];
+}
+extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_plan(AssignArgs a) {
+  __shared__ uint32_t used[ASG_WORDS];
+  __shared__ int32_t before[ASG_BLOCK];
+  __shared__ int64_t red[ASG_BLOCK / 64];
+  const int tid = threadIdx.x, words = (a.pages + 31) / 32;
+  for (int i = tid; i < words; i += ASG_BLOCK) {
+    uint32_t u = 0;
+#pragma unroll 8
+    for (int p = 0; p < a.parts; ++p) u |= a.marks[(int64_t)p * words + i];
+    used[i] = u;
+  }
+  __syncthreads();
+  int64_t wanted, free;
+  asg_sums(a, used, before, red, wanted, free);
+  asg_list(a, used, before[tid], wanted, free);
+}
+// a workgroup for each row's entries, then for 256 tokens each
+extern "C" __global__ __launch_bounds__(256) void nk_assign_fill(AssignArgs a) {
+  if ((int)blockIdx.x < a.rows) {
+    asg_fill(a, blockIdx.x, threadIdx.x, 256);
+  } else {
+    const int t = ((blockIdx.x - a.rows) * 4 + (threadIdx.x >> 6)) * 64;
+    if (t < a.tokens) asg_slots(a, t);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -176,10 +245,11 @@ extern "C" __global__ __launch_bounds__(256) void nk_assign_slots(AssignArgs a) 
 //
 // Two launches.  The first reads the logits once: a wave has 2048 of a row in
 // registers, their largest value m, sum of 2^((x - m) log2 e) and the K best (K:
-// beams); a workgroup joins its waves' lists.  The K best of a wave: the K-th
-// largest of the lanes' largest values bounds them from below, what is not below
-// it (a few more than K) is listed in LDS and ranked one against the other; more
-// than LIST of them (ties) are taken in K rounds.
+// beams); a workgroup joins its waves' lists.  The K best of a wave: K groups of its
+// lanes or more have their largest value at or above the least of these, which bounds
+// the K best from below; what is not below it (about K (1 + 1/2 + ... + 1/K)) is
+// listed in LDS and ranked one against the other; more than LIST of them (ties) are
+// taken in K rounds.
 //
 // The second, a workgroup per group, ranks the segments' best by score, value and
 // place; an entry with j before it in a list whose best has rank r has r + j
@@ -198,7 +268,7 @@ struct SelectArgs {
   int32_t groups, beams, vocab, nseg, end;
 };
 #define SEL_WAVE 2048
-#define SEL_LIST 128
+#define SEL_LIST 256
 #define SEL_BEAMS 32
 
 // a before b: the larger value, or the lower place
@@ -246,34 +316,34 @@ __device__ __forceinline__ void select_top_body(const SelectArgs &a) {
   const float m = wave_max(top);
   float sum = 0.f;
   if (fabsf(m) < INFINITY) {
+    // (the difference first: x log2(e) alone would lose the last places of large logits)
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      const float p = __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896340736f);
-      sum += p == p ? p : 0.f;
+    for (int e = 0; e < 32; ++e) sum += __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896340736f);
+    if (__any(sum != sum)) {  // (NaN logits)
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sum += v[e] == v[e] ? __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896340736f) : 0.f;
     }
   } else if (m > 0.f) {  // infinite logits share the weight
 #pragma unroll
     for (int e = 0; e < 32; ++e) sum += v[e] == m ? 1.f : 0.f;
   }
   sum = wave_sum(sum);
-  // rank of this lane's largest among the lanes'
-  int rank = 0;
-#pragma unroll 8
-  for (int k = 0; k < 64; ++k) {
-    const float y = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(top), k));
-    rank += y > top || (y == top && k < lane) ? 1 : 0;
-  }
-  const uint64_t kth = __ballot(rank == K - 1);
-  const float low = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(top), __builtin_ctzll(kth)));
-  uint32_t in = 0;
+  // K groups of lanes or more have their largest values at or above the least of them
+  float low = top;
+  int o = 32;
+  for (; o >= K; o >>= 1) low = fmaxf(low, __shfl_xor(low, o, 64));  // (lanes far apart: a row's last wave has few)
+  for (; o; o >>= 1) low = fminf(low, __shfl_xor(low, o, 64));
+  low = fmaxf(low, -3.40282347e38f);  // (-inf is listed nowhere)
+  uint32_t in = 0;  // a bit for each element, the first the highest
 #pragma unroll
-  for (int e = 0; e < 32; ++e) in |= v[e] >= low && v[e] > -INFINITY ? 1u << e : 0;
+  for (int e = 0; e < 32; ++e) in += in + (v[e] >= low ? 1 : 0);
   const int mine = __popc(in), upto = running(mine), total = __builtin_amdgcn_readlane(upto, 63);
   int count = min(total, K);
   if (total <= SEL_LIST) {
     int at = upto - mine;
     for (uint32_t left = in; left; left &= left - 1, ++at) {
-      const int e = __builtin_ctz(left), i = i0 + e / E * 64 * E + e % E;
+      const int e = 31 - __builtin_ctz(left), i = i0 + e / E * 64 * E + e % E;
       lv[wave][at] = Elt<T>::load(x, i);
       li[wave][at] = i;
     }
@@ -352,6 +422,7 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
   __shared__ uint32_t cp[SEL_LEFT];
   __shared__ double base[SEL_BEAMS];
   __shared__ float largest[SEL_BEAMS];
+  __shared__ int32_t order[SEL_BEAMS];  // the lists of the K best heads; -1: none
   __shared__ int32_t kind[SEL_BEAMS];  // 0: nothing, 1: its logits, 2: ended
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = blockIdx.x, K = a.beams, heads = K * a.nseg;
@@ -378,6 +449,7 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
     if (lane == 0) base[b] = z, largest[b] = m, kind[b] = what;
   }
   for (int i = tid; i < K * (K + 1) / 2; i += SEL_BLOCK) cp[i] = SEL_NONE;
+  if (tid < K) order[tid] = -1;
   __syncthreads();
   // entry j of a list: false where there is none
   auto entry = [&](int h, int j, double &s, uint32_t &p) {
@@ -401,20 +473,29 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
     hp[h] = is ? p : SEL_NONE;
   }
   __syncthreads();
-  for (int h = tid; h < heads; h += SEL_BLOCK) {
+  // a head's rank, by S threads side by side
+  int S = 1;
+  while (S < 64 && heads * S * 2 <= SEL_BLOCK) S *= 2;
+  for (int x = tid; x < (heads * S + 63) / 64 * 64; x += SEL_BLOCK) {
+    const int h = min(x / S, heads - 1);
     const double s = hs[h];
     const uint32_t p = hp[h];
-    if (p == SEL_NONE) continue;
     int rank = 0;
-    for (int q = 0; q < heads; ++q) rank += hp[q] != SEL_NONE && sel_better(hs[q], hp[q], s, p) ? 1 : 0;
-    if (rank >= K) continue;
-    const int to = rank * K - rank * (rank - 1) / 2;
-    for (int j = 0; j < K - rank; ++j) {
-      double t;
-      uint32_t q;
-      if (!entry(h, j, t, q)) break;
-      cs[to + j] = t, cp[to + j] = q;
-    }
+#pragma unroll 4
+    for (int q = x % S; q < heads; q += S) rank += hp[q] != SEL_NONE && sel_better(hs[q], hp[q], s, p) ? 1 : 0;
+    for (int o = 1; o < S; o <<= 1) rank += __shfl_xor(rank, o, 64);
+    if (x % S == 0 && x / S < heads && p != SEL_NONE && rank < K) order[rank] = h;
+  }
+  __syncthreads();
+  // entry j of the list whose best has rank r: a thread for each r + j < K
+  for (int c = tid; c < K * K; c += SEL_BLOCK) {
+    const int r = c / K, j = c % K;
+    if (r + j >= K || order[r] < 0) continue;
+    double t;
+    uint32_t q;
+    if (!entry(order[r], j, t, q)) continue;
+    const int to = r * K - r * (r - 1) / 2 + j;
+    cs[to] = t, cp[to] = q;
   }
   __syncthreads();
   const int n = K * (K + 1) / 2;
@@ -424,6 +505,7 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
     const uint32_t p = cp[c];
     if (p == SEL_NONE) continue;
     int rank = 0;
+#pragma unroll 4
     for (int q = 0; q < n; ++q) rank += cp[q] != SEL_NONE && sel_better(cs[q], cp[q], s, p) ? 1 : 0;
     if (rank >= K) continue;
     const int b = p >> 22, t = kind[b] == 2 ? a.end : (int)(p & 0x3fffff), to = g * K + rank;
@@ -489,8 +571,7 @@ __device__ __forceinline__ void reorder_body(const ReorderArgs &a) {
     int32_t x[K];
 #pragma unroll
     for (int b = 0; b < K; ++b) {
-      const int p = __builtin_amdgcn_readfirstlane(up[b]);
-      if (p != b) x[b] = table[(int64_t)p * a.width + j];
+      x[b] = table[(int64_t)min(__builtin_amdgcn_readfirstlane(up[b]), a.beams - 1) * a.width + j];
     }
 #pragma unroll
     for (int b = 0; b < K; ++b)
@@ -498,20 +579,25 @@ __device__ __forceinline__ void reorder_body(const ReorderArgs &a) {
     return;
   }
   const int which = (part - a.tblocks) / a.kblocks;  // 0: keys, 1: values, 2: exponents
-  auto move = [&](auto *x, int64_t pitch, int64_t at) __attribute__((always_inline)) {
+  // (a page's address is uniform, the place in it 32 bits of a lane; what moves
+  // nothing reads page 0, since a read in a branch would be waited for at its end)
+  auto move = [&](auto *x, int64_t pitch, uint32_t at) __attribute__((always_inline)) {
     typename std::remove_reference<decltype(*x)>::type y[K];
 #pragma unroll
-    for (int b = 0; b < K; ++b)
-      if (__builtin_amdgcn_readfirstlane(to[b]) >= 0) y[b] = x[__builtin_amdgcn_readfirstlane(from[b]) * pitch + at];
+    for (int b = 0; b < K; ++b) {
+      const auto *src = x + __builtin_amdgcn_readfirstlane(max(from[b], 0)) * pitch;
+      y[b] = src[at];
+    }
 #pragma unroll
     for (int b = 0; b < K; ++b) {
       const int p = __builtin_amdgcn_readfirstlane(to[b]);
-      if (p >= 0) x[p * pitch + at] = y[b];
+      auto *dst = x + p * pitch;
+      if (p >= 0) dst[at] = y[b];
     }
   };
   if (which < 2) {
     const int64_t at = (int64_t)((part - a.tblocks) % a.kblocks) * 256 + tid, units = a.row / (int64_t)sizeof(U);  // (of a row)
-    if (at < tail * units) move((U *)(which ? a.v : a.k), a.page * units, at);
+    if (at < tail * units) move((U *)(which ? a.v : a.k), a.page * units, (uint32_t)at);
   } else {
     for (int h = tid; h < 2 * a.hkv; h += 256) move(h < a.hkv ? a.ke : a.ve, a.hkv, h < a.hkv ? h : h - a.hkv);
   }

@@ -28,8 +28,8 @@ MAX_BEAMS = 32
 # Launch helpers
 # ---------------------------------------------------------------------------
 class AssignArgs(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("tables", "lens", "news", "starts", "slots", "free", "wants")]
-                + [(n, ctypes.c_int32) for n in ("rows", "width", "page", "pages", "tokens", "small")])
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("tables", "lens", "news", "starts", "slots", "free", "wants", "list", "marks")]
+                + [(n, ctypes.c_int32) for n in ("rows", "width", "page", "pages", "tokens", "parts")])
 
 
 class SelectArgs(ctypes.Structure):
@@ -45,21 +45,40 @@ class ReorderArgs(ctypes.Structure):
 
 
 ASSIGN_PAGES = 2**20  # bits of a workgroup's LDS
-ASSIGN_SMALL = 1024   # tokens whose slots the one workgroup writes
+ASSIGN_SMALL = 1024   # tokens, and
+ASSIGN_ROWS = 128     # rows of
+ASSIGN_WIDTH = 512    # entries, that one workgroup deals with
+ASSIGN_WAVES = 16     # rows that a workgroup marks at once
+ASSIGN_WORDS = 2**18  # words of bitmaps that one workgroup joins, about
+
+
+def assign_parts(rows, width, pages, tokens) -> int:
+    """Workgroups that mark the pages held, 0 where one does everything."""
+    if tokens <= ASSIGN_SMALL and rows <= ASSIGN_ROWS and width <= ASSIGN_WIDTH:
+        return 0
+    return max(1, min(-(-rows // ASSIGN_WAVES), ASSIGN_WORDS // -(-pages // 32)))
+
+
+def assign_workspace_bytes(rows, width, pages, tokens) -> int:
+    words = -(-pages // 32)
+    return 4 * (-(-rows // 4) * 4 + -(-pages // 4) * 4 + assign_parts(rows, width, pages, tokens) * words)
 
 
 def assign_pages(rows, width, page, pages, tokens, *, tables, lens, news, starts, slots, free, ws) -> List[Launch]:
     """Tables updated in place, starts (rows + 1), slots (tokens) and the
-    number of pages left; ``ws``: 4 bytes for each row."""
+    number of pages left; ``ws``: ``assign_workspace_bytes``."""
     if not (1 <= rows <= 2**16 and width >= 1 and 1 <= pages <= ASSIGN_PAGES and page >= 1 and 0 <= tokens <= 2**30
             and width * page < 2**30 and pages * page < 2**31):
         raise LaunchError(f"assign_pages: {tokens} tokens of {rows} rows of {width}, {pages} pages of {page}")
-    a = _fields(AssignArgs(), tables=tables, lens=lens, news=news, starts=starts, slots=slots, free=free, wants=ws, rows=rows,
-                width=width, page=page, pages=pages, tokens=tokens, small=int(tokens <= ASSIGN_SMALL))
-    out = [Launch("beams", "nk_assign_pages", (1, 1, 1), (1024, 1, 1), a)]
-    if not a.small:
-        out.append(Launch("beams", "nk_assign_slots", (-(-tokens // 256), 1, 1), (256, 1, 1), a))
-    return out
+    parts = assign_parts(rows, width, pages, tokens)
+    taken = ws + 16 * -(-rows // 4)
+    a = _fields(AssignArgs(), tables=tables, lens=lens, news=news, starts=starts, slots=slots, free=free, wants=ws, list=taken,
+                marks=taken + 16 * -(-pages // 4), rows=rows, width=width, page=page, pages=pages, tokens=tokens, parts=parts)
+    if not parts:
+        return [Launch("beams", "nk_assign_pages", (1, 1, 1), (1024, 1, 1), a)]
+    return [Launch("beams", "nk_assign_mark", (parts, 1, 1), (1024, 1, 1), a),
+            Launch("beams", "nk_assign_plan", (1, 1, 1), (1024, 1, 1), a),
+            Launch("beams", "nk_assign_fill", (rows + -(-tokens // 256), 1, 1), (256, 1, 1), a)]
 
 
 SELECT_SEG, SELECT_HEADS = 8192, 2048  # logits of a workgroup, lists of a group at most (beams.hip)
@@ -151,7 +170,7 @@ class AssignMatch(UpdateMatch):
         rows, width = tables.shape
         at = self.at
         steps, to = self.begin(plan, {"starts": 4 * rows + 4, "slots": 4 * at["tokens"], "free": 4})
-        ws = Slot(plan.add_buffer(4 * rows, "temp", "assign_pages.wants"))
+        ws = Slot(plan.add_buffer(assign_workspace_bytes(rows, width, at["pages"], at["tokens"]), "temp", "assign_pages.plan"))
 
         def make(addr):
             return assign_pages(rows, width, at["page"], at["pages"], at["tokens"], lens=addr(lens), news=addr(news), ws=addr(ws),

@@ -29,7 +29,8 @@ class Append8Args(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "oq", "kc", "vc", "ke", "ve", "cos", "sin", "tables", "lens",
                                                  "starts")]
                 + [(n, ctypes.c_int64) for n in ("q_ss", "q_sh", "k_ss", "k_sh", "v_ss", "v_sh")]
-                + [(n, ctypes.c_int32) for n in ("B", "N", "Hq", "Hkv", "D", "half", "P", "page", "pages", "width", "heads")])
+                + [(n, ctypes.c_int32) for n in ("B", "N", "Hq", "Hkv", "D", "half", "P", "page", "pages", "width", "heads",
+                                              "blocks")])
 
 
 class Attend8Args(S.AttendArgs):
@@ -54,8 +55,8 @@ def rotary_append_fp8(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q
     a = _fields(Append8Args(), q=q, k=k, v=v, oq=oq, kc=kc, vc=vc, ke=ke, ve=ve, cos=cos, sin=sin, tables=tables, lens=lens,
                 starts=starts, q_ss=q_str[0], q_sh=q_str[1], k_ss=k_str[0], k_sh=k_str[1], v_ss=v_str[0], v_sh=v_str[1],
                 B=B, N=N, Hq=Hq, Hkv=Hkv, D=D, half=half, P=P, page=page, pages=pages, width=width, heads=heads)
-    tiles = N // page + 2 * B if starts else B
-    n = (N if oq else 0) + tiles * 2 * -(-Hkv // heads)
+    a.blocks = (N // page + 2 * B if starts else B) * 2 * -(-Hkv // heads)
+    n = (N if oq else 0) + a.blocks
     if n >= 2**31:
         raise LaunchError("rotary_append_fp8: too many workgroups for one launch")
     size = dt.itemsize(dtype)
