@@ -171,34 +171,48 @@ __device__ __forceinline__ void append8_body(const Append8Args &a) {
   if (E == 8 && n * hn * a.D <= 1024 * A8_ITEMS * 4 && a.D % 16 == 0 && (values || 2 * half == a.D)) {
     // read once: a thread's pairs of pieces, the same place of both halves of a head
     const int pc = a.D / 16, total = n * hn * pc;
-    float y[A8_ITEMS][2][E];
-    int at[A8_ITEMS], head[A8_ITEMS];
+    const bool side = (pc & (pc - 1)) == 0 && pc <= 64;  // a head's pieces lie with neighbouring lanes
+    auto once = [&](auto count) __attribute__((always_inline)) {
+      constexpr int I = decltype(count)::value;
+      float y[I][2][E];
+      int at[I], head[I];
 #pragma unroll
-    for (int i = 0; i < A8_ITEMS; ++i) {
-      const int x = min(tid + 256 * i, total - 1), r = x / (hn * pc), z = x % (hn * pc), h = z / pc, c = z % pc;
-      const T *from = src + r * ss + h * sh + c * E;
-      head[i] = h, at[i] = ((first + r) * a.Hkv + h) * a.D + c * E;
-      if (values) {
-        Piece<T, E>::load(from, y[i][0]);
-        Piece<T, E>::load(from + a.D / 2, y[i][1]);
-      } else {
-        const int64_t turn = (int64_t)(lo + r) * half + c * E;
-        a8_turn<T, E>(from, a.cos + turn, a.sin + turn, half, y[i][0], y[i][1]);
+      for (int i = 0; i < I; ++i) {
+        const int x = min(tid + 256 * i, total - 1), r = x / (hn * pc), z = x % (hn * pc), h = z / pc, c = z % pc;
+        const T *from = src + r * ss + h * sh + c * E;
+        head[i] = h, at[i] = ((first + r) * a.Hkv + h) * a.D + c * E;
+        if (values) {
+          Piece<T, E>::load(from, y[i][0]);
+          Piece<T, E>::load(from + a.D / 2, y[i][1]);
+        } else {
+          const int64_t turn = (int64_t)(lo + r) * half + c * E;
+          a8_turn<T, E>(from, a.cos + turn, a.sin + turn, half, y[i][0], y[i][1]);
+        }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < A8_ITEMS; ++i) {
-      // (past the last item: that one again)
-      const uint32_t most = larger(larger(0, y[i][0]), y[i][1]);
-      if (most) atomicMax(&top[head[i]], most);
-    }
-    settle();
+      for (int i = 0; i < I; ++i) {
+        const bool is = tid + 256 * i < total;
+        uint32_t most = is ? larger(larger(0, y[i][0]), y[i][1]) : 0;
+        if (side) {
+          for (int o = 1; o < pc; o <<= 1) most = max(most, (uint32_t)__shfl_xor(most, o, 64));
+          if (tid % pc == 0 && most) atomicMax(&top[head[i]], most);
+        } else if (most) {
+          atomicMax(&top[head[i]], most);
+        }
+      }
+      settle();
 #pragma unroll
-    for (int i = 0; i < A8_ITEMS; ++i) {
-      if (tid + 256 * i >= total) break;
-      const float scale = c8_power(-now[head[i]]);
-      c8_store<E>(codes + at[i], y[i][0], scale);
-      c8_store<E>(codes + at[i] + a.D / 2, y[i][1], scale);
+      for (int i = 0; i < I; ++i) {
+        if (tid + 256 * i >= total) break;
+        const float scale = c8_power(-now[head[i]]);
+        c8_store<E>(codes + at[i], y[i][0], scale);
+        c8_store<E>(codes + at[i] + a.D / 2, y[i][1], scale);
+      }
+    };
+    if (total <= 256) {
+      once(Count<1>{});
+    } else {
+      once(Count<A8_ITEMS>{});
     }
   } else {
     // every piece of these rows: f(row, head, first element, whether it is a pair, its values)

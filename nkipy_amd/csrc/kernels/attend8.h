@@ -96,9 +96,6 @@ NK_DEVICE f32x16 mul32(B8 a, B8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_
 // fp32's exponents).  fp16 queries and weights, which bf16 does not hold, enter as
 // two bf16 numbers each, x = RN(x) + RN(x - RN(x)): exact for a query's 11 bits, a
 // weight keeps 16.
-template <int N> struct Count {
-  static constexpr int value = N;
-};
 template <typename T> struct Parts;
 template <> struct Parts<bf16> { static constexpr int N = 1; };
 template <> struct Parts<f16> { static constexpr int N = 2; };

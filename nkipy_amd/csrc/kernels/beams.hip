@@ -54,7 +54,7 @@ struct AssignArgs {
   int32_t *starts, *slots, *free;
   int32_t *wants;   // (rows) pages wanted by the rows before
   int32_t *list;    // the free pages that are wanted, in order; -1 behind the last
-  uint32_t *marks;  // (parts, words) bitmaps of some rows each
+  uint32_t *marks;  // (parts, words in fours) bitmaps of some rows each
   int32_t rows, width, page, pages, tokens, parts;
 };
 #define ASG_BLOCK 1024
@@ -212,18 +212,18 @@ extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_mark(AssignArg
   __syncthreads();
   asg_mark(a, used, blockIdx.x * (ASG_BLOCK / 64) + wave, a.parts * (ASG_BLOCK / 64));
   __syncthreads();
-  for (int i = tid; i < words; i += ASG_BLOCK) a.marks[(int64_t)blockIdx.x * words + i] = used[i];
+  for (int i = tid; i < words; i += ASG_BLOCK) a.marks[(int64_t)blockIdx.x * ((words + 3) & ~3) + i] = used[i];
 }
 extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_plan(AssignArgs a) {
-  __shared__ uint32_t used[ASG_WORDS];
+  __shared__ __attribute__((aligned(16))) uint32_t used[ASG_WORDS];
   __shared__ int32_t before[ASG_BLOCK];
   __shared__ int64_t red[ASG_BLOCK / 64];
-  const int tid = threadIdx.x, words = (a.pages + 31) / 32;
-  for (int i = tid; i < words; i += ASG_BLOCK) {
-    uint32_t u = 0;
+  const int tid = threadIdx.x, words = (a.pages + 31) / 32, pitch = (words + 3) & ~3;
+  for (int i = tid * 4; i < words; i += ASG_BLOCK * 4) {
+    u32x4 u = {0, 0, 0, 0};
 #pragma unroll 8
-    for (int p = 0; p < a.parts; ++p) u |= a.marks[(int64_t)p * words + i];
-    used[i] = u;
+    for (int p = 0; p < a.parts; ++p) u |= *reinterpret_cast<const u32x4 *>(a.marks + (int64_t)p * pitch + i);
+    *reinterpret_cast<u32x4 *>(used + i) = u;
   }
   __syncthreads();
   int64_t wanted, free;
@@ -245,11 +245,10 @@ extern "C" __global__ __launch_bounds__(256) void nk_assign_fill(AssignArgs a) {
 //
 // Two launches.  The first reads the logits once: a wave has 2048 of a row in
 // registers, their largest value m, sum of 2^((x - m) log2 e) and the K best (K:
-// beams); a workgroup joins its waves' lists.  The K best of a wave: K groups of its
-// lanes or more have their largest value at or above the least of these, which bounds
-// the K best from below; what is not below it (about K (1 + 1/2 + ... + 1/K)) is
-// listed in LDS and ranked one against the other; more than LIST of them (ties) are
-// taken in K rounds.
+// beams); a workgroup joins its waves' lists.  The K best of a wave: the K-th largest
+// of its lanes' largest values bounds them from below; what is not below it (a few more
+// than K) is listed in LDS and ranked one against the other; more than LIST of them
+// (ties) are taken in K rounds.
 //
 // The second, a workgroup per group, ranks the segments' best by score, value and
 // place; an entry with j before it in a list whose best has rank r has r + j
@@ -316,25 +315,30 @@ __device__ __forceinline__ void select_top_body(const SelectArgs &a) {
   const float m = wave_max(top);
   float sum = 0.f;
   if (fabsf(m) < INFINITY) {
-    // (the difference first: x log2(e) alone would lose the last places of large logits)
+    // 2^(x L - c), with c = RN(m L): what c is off by, d = m L - c, is a factor 2^-d of all
+    const float L = 1.44269504088896340736f, c = m * L, d = __builtin_fmaf(m, L, -c);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) sum += __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896340736f);
-    if (__any(sum != sum)) {  // (NaN logits)
+    for (int e = 0; e < 32; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], L, -c));
+    sum *= __builtin_amdgcn_exp2f(-d);
+    if (__any(sum != sum) || !(fabsf(c) < INFINITY)) {  // NaN logits, or ones past fp32's range times L
       sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) sum += v[e] == v[e] ? __builtin_amdgcn_exp2f((v[e] - m) * 1.44269504088896340736f) : 0.f;
+      for (int e = 0; e < 32; ++e) sum += v[e] == v[e] ? __builtin_amdgcn_exp2f((v[e] - m) * L) : 0.f;
     }
   } else if (m > 0.f) {  // infinite logits share the weight
 #pragma unroll
     for (int e = 0; e < 32; ++e) sum += v[e] == m ? 1.f : 0.f;
   }
   sum = wave_sum(sum);
-  // K groups of lanes or more have their largest values at or above the least of them
-  float low = top;
-  int o = 32;
-  for (; o >= K; o >>= 1) low = fmaxf(low, __shfl_xor(low, o, 64));  // (lanes far apart: a row's last wave has few)
-  for (; o; o >>= 1) low = fminf(low, __shfl_xor(low, o, 64));
-  low = fmaxf(low, -3.40282347e38f);  // (-inf is listed nowhere)
+  // the K-th largest of the lanes' largest values, its key's high half: as many values
+  // are not below it
+  const uint32_t bits = __float_as_uint(top + 0.f), key = (bits & 0x80000000u ? ~bits : bits | 0x80000000u) >> 16;
+  uint32_t kth = 0;
+#pragma unroll
+  for (uint32_t bit = 0x8000; bit; bit >>= 1) kth |= __popcll(__ballot(key >= (kth | bit))) >= K ? bit : 0;
+  kth <<= 16;
+  float low = __uint_as_float(kth & 0x80000000u ? kth & 0x7fffffffu : ~kth);
+  low = low > -3.40282347e38f ? low : -3.40282347e38f;  // (-inf, or what is no number, is listed nowhere)
   uint32_t in = 0;  // a bit for each element, the first the highest
 #pragma unroll
   for (int e = 0; e < 32; ++e) in += in + (v[e] >= low ? 1 : 0);

@@ -6,6 +6,10 @@
 
 namespace nk {
 
+template <int N> struct Count {  // a number as a type
+  static constexpr int value = N;
+};
+
 // exponents outside this range count as the nearest end: 2^e and 2^-e are normal
 // fp32 numbers, and 448 2^120 is past fp32's largest
 #define C8_MIN -120

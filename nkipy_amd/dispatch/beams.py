@@ -48,7 +48,7 @@ ASSIGN_PAGES = 2**20  # bits of a workgroup's LDS
 ASSIGN_SMALL = 1024   # tokens, and
 ASSIGN_ROWS = 128     # rows of
 ASSIGN_WIDTH = 512    # entries, that one workgroup deals with
-ASSIGN_WAVES = 16     # rows that a workgroup marks at once
+ASSIGN_MARKS = 64     # rows that a workgroup marks at once, four a wave
 ASSIGN_WORDS = 2**18  # words of bitmaps that one workgroup joins, about
 
 
@@ -56,12 +56,11 @@ def assign_parts(rows, width, pages, tokens) -> int:
     """Workgroups that mark the pages held, 0 where one does everything."""
     if tokens <= ASSIGN_SMALL and rows <= ASSIGN_ROWS and width <= ASSIGN_WIDTH:
         return 0
-    return max(1, min(-(-rows // ASSIGN_WAVES), ASSIGN_WORDS // -(-pages // 32)))
+    return max(1, min(-(-rows // ASSIGN_MARKS), ASSIGN_WORDS // -(-pages // 32)))
 
 
 def assign_workspace_bytes(rows, width, pages, tokens) -> int:
-    words = -(-pages // 32)
-    return 4 * (-(-rows // 4) * 4 + -(-pages // 4) * 4 + assign_parts(rows, width, pages, tokens) * words)
+    return 16 * (-(-rows // 4) + -(-pages // 4) + assign_parts(rows, width, pages, tokens) * -(-pages // 128))
 
 
 def assign_pages(rows, width, page, pages, tokens, *, tables, lens, news, starts, slots, free, ws) -> List[Launch]:
