@@ -430,6 +430,11 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
   __shared__ int32_t kind[SEL_BEAMS];  // 0: nothing, 1: its logits, 2: ended
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = blockIdx.x, K = a.beams, heads = K * a.nseg;
+  // the lists' best are on their way meanwhile
+  float2 mine[SEL_HEADS / SEL_BLOCK];
+#pragma unroll
+  for (int i = 0; i < SEL_HEADS / SEL_BLOCK; ++i)
+    mine[i] = a.best[((int64_t)g * heads + min(tid + i * SEL_BLOCK, heads - 1)) * K];
   for (int b = wave; b < K; b += SEL_BLOCK / 64) {
     const int r = g * K + b;
     const float s = a.scores[r];
@@ -444,7 +449,7 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
       double sum = 0.0;
       for (int i = lane; i < a.nseg; i += 64) {
         const float2 y = a.sums[(int64_t)r * a.nseg + i];
-        sum += y.x == m ? (double)y.y : y.x == -INFINITY ? 0.0 : (double)y.y * exp((double)y.x - (double)m);
+        sum += y.x == m ? (double)y.y : y.x == -INFINITY ? 0.0 : (double)y.y * exp_acc(y.x - m);
       }
 #pragma unroll
       for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -455,24 +460,26 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
   for (int i = tid; i < K * (K + 1) / 2; i += SEL_BLOCK) cp[i] = SEL_NONE;
   if (tid < K) order[tid] = -1;
   __syncthreads();
-  // entry j of a list: false where there is none
-  auto entry = [&](int h, int j, double &s, uint32_t &p) {
+  // entry y, j-th of list h: false where there is none
+  auto entry = [&](int h, int j, float2 y, double &s, uint32_t &p) {
     const int b = h / a.nseg, i = h % a.nseg;
     if (kind[b] == 0 || (kind[b] == 2 && (i || j))) return false;
     if (kind[b] == 2) {
       s = base[b], p = (uint32_t)b << 22 | (uint32_t)max(a.end, 0);
       return true;
     }
-    const float2 y = a.best[(((int64_t)g * K + b) * a.nseg + i) * K + j];
     const int t = __float_as_int(y.y);
     if (t < 0 || (y.x != largest[b] && largest[b] == INFINITY)) return false;
     s = base[b] + (y.x == largest[b] ? 0.0 : (double)y.x - (double)largest[b]), p = (uint32_t)b << 22 | (uint32_t)t;
     return true;
   };
-  for (int h = tid; h < heads; h += SEL_BLOCK) {
+#pragma unroll
+  for (int i = 0; i < SEL_HEADS / SEL_BLOCK; ++i) {
+    const int h = tid + i * SEL_BLOCK;
     double s;
     uint32_t p;
-    const bool is = entry(h, 0, s, p);
+    if (h >= heads) break;
+    const bool is = entry(h, 0, mine[i], s, p);
     hs[h] = is ? s : 0.0;
     hp[h] = is ? p : SEL_NONE;
   }
@@ -497,7 +504,7 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
     if (r + j >= K || order[r] < 0) continue;
     double t;
     uint32_t q;
-    if (!entry(order[r], j, t, q)) continue;
+    if (!entry(order[r], j, a.best[((int64_t)g * heads + order[r]) * K + j], t, q)) continue;
     const int to = r * K - r * (r - 1) / 2 + j;
     cs[to] = t, cp[to] = q;
   }
