@@ -12,11 +12,13 @@ the diagonal), softmax, weighted values and the output projection.
 
 ``qwen3_paged_attention_kernel`` is the same layer for a batch of sequences
 of their own lengths, packed without padding, over a paged cache: prompts,
-pieces of prompts and single tokens alike.
+pieces of prompts and single tokens alike; with the exponents of its pages the
+cache holds 8-bit codes.
 
 ``greedy_sampling`` follows kernels/sampling.py:113-148 on one device: the
 final RMSNorm, logits of the last position and the index of the largest
-logit by ``topk(k=1)``.  ``sampling`` draws from the same logits instead.
+logit by ``topk(k=1)``.  ``sampling`` draws from the same logits instead, and
+``beam_step`` chooses a beam search's continuations from them.
 """
 
 import numpy as np
@@ -89,7 +91,7 @@ def qwen3_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, norm_eps
 
 def qwen3_paged_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, norm_eps, n_heads, head_dim, n_kv_heads,
                                  key_cache, value_cache, block_tables, context_lens, query_starts, o_weight,
-                                 rope_base=1000000, window=None, sinks=0, cos=None, sin=None):
+                                 rope_base=1000000, window=None, sinks=0, cos=None, sin=None, key_exps=None, value_exps=None):
     """x (tokens, hidden), the new tokens of all sequences one after another ->
     (tokens, hidden); key_cache / value_cache (pages, page_size, n_kv_heads,
     head_dim) take their keys and values in place.  Sequence b's tokens are
@@ -97,7 +99,9 @@ def qwen3_paged_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, no
     context_lens[b] (``query_starts=None``: one token each), on the pages of
     block_tables[b]; a window with its sinks narrows what each sees.  cos / sin
     (positions, head_dim / 2): rotary tables that the layers share; without
-    them each kernel holds its own, as long as block_tables is wide."""
+    them each kernel holds its own, as long as block_tables is wide.  key_exps /
+    value_exps (pages, n_kv_heads) int32: the caches hold float8_e4m3fn codes with
+    these exponents, which take the new tokens' in place as well."""
     n = x.shape[0]
     q_end = n_heads * head_dim
     k_end = q_end + n_kv_heads * head_dim
@@ -107,12 +111,19 @@ def qwen3_paged_attention_kernel(x, qkv_weight, q_norm_weight, k_norm_weight, no
     xv = xv.reshape(n, n_kv_heads, head_dim)
     if (cos is None) != (sin is None):
         raise ValueError("give both of cos and sin, or neither")
+    if (key_exps is None) != (value_exps is None):
+        raise ValueError("give both of key_exps and value_exps, or neither")
     if cos is None:
         cos, sin = (tensor_apis.constant(x) for x in compute_cos_sin_cache(
             head_dim, block_tables.shape[1] * key_cache.shape[1], base=rope_base))
-    xq = tensor_apis.rotary_append(xq, xk, xv, cos, sin, key_cache, value_cache, block_tables, context_lens, query_starts)
-    out = tensor_apis.paged_attention(xq, key_cache, value_cache, block_tables, context_lens, query_starts,
-                                      window=window, sinks=sinks)
+    where = (block_tables, context_lens, query_starts)
+    if key_exps is None:
+        xq = tensor_apis.rotary_append(xq, xk, xv, cos, sin, key_cache, value_cache, *where)
+        out = tensor_apis.paged_attention(xq, key_cache, value_cache, *where, window=window, sinks=sinks)
+    else:
+        cache = (key_cache, value_cache, key_exps, value_exps)
+        xq = tensor_apis.rotary_append_fp8(xq, xk, xv, cos, sin, *cache, *where)
+        out = tensor_apis.paged_attention_fp8(xq, *cache, *where, window=window, sinks=sinks)
     return np.matmul(out.reshape(n, q_end), o_weight)
 
 
@@ -163,3 +174,12 @@ def sampling(h, norm_weight, lm_head_weight, norm_eps, uniform, temperature=1.0,
     h = rmsnorm_kernel(h, norm_weight, norm_eps)
     logits = h[:, -1, :] @ lm_head_weight
     return tensor_apis.sample(logits, uniform, temperature, top_k, top_p, min_p)
+
+
+def beam_step(h, norm_weight, lm_head_weight, norm_eps, scores, ended, end_token):
+    """A beam search's continuations by the last position's token: h (groups *
+    beams, S, H), scores / ended (groups, beams) -> (tokens, parents, scores,
+    ended), as ``tensor_apis.beam_select`` gives them."""
+    h = rmsnorm_kernel(h, norm_weight, norm_eps)
+    logits = h[:, -1, :] @ lm_head_weight
+    return tensor_apis.beam_select(logits, scores, ended, end_token=end_token)
