@@ -322,6 +322,8 @@ class DeviceKernel:
                     shape, dtype = self._out_specs[on]
                     st = self._staging[on] = DeviceTensor.empty(shape, dtype, name=on)
                 run_outputs[on] = st
+                if on in self.plan.alias_outputs:  # updated where it stands
+                    get_runtime().d2d(st.ptr, outputs[on].ptr, outputs[on].nbytes)
             self._execute(self._io_ptrs(inputs, run_outputs), save_trace, ntff_name, graph)
             rt = get_runtime()
             for on in staged:

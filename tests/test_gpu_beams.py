@@ -97,7 +97,8 @@ def check_select(x, scores, ended, end):
 
 @pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("g,k,vocab", [(1, 1, 1), (1, 4, 3), (3, 4, 50), (2, 32, 40), (1, 4, 32000), (2, 3, 2047), (5, 8, 8193),
-                                       (2, 5, 8191), (1, 2, 16385), (3, 16, 50257), (1, 32, 20000), (33, 2, 1000)])
+                                       (2, 5, 8191), (1, 2, 16385), (3, 16, 50257), (1, 32, 20000), (33, 2, 1000), (2, 25, 90000),
+                                       (1, 7, 300000)])
 def test_select(t, g, k, vocab):
     rng = np.random.default_rng(vocab)
     x, scores = B.logits(rng, g * k, vocab, t), (-5 - 3 * rng.random((g, k))).astype(np.float32)
@@ -127,7 +128,7 @@ def test_select_special_values():
         assert (got["output0"] == -1).all() and (got["output1"] == [0, 1, 2, 3]).all() and (got["output2"] == -np.inf).all()
 
 
-@pytest.mark.parametrize("k,vocab", [(4, 20), (8, 9000), (32, 40000), (1, 2500)])
+@pytest.mark.parametrize("k,vocab", [(4, 20), (8, 9000), (32, 40000), (32, 70000), (1, 2500)])
 def test_select_ties(k, vocab):
     """Equal logits, whole rows of them: the lower beam, then the lower token."""
     x = np.zeros((2 * k, vocab), np.float32)
@@ -202,3 +203,22 @@ def test_reorder_long_tables_and_large_pages():
     check_reorder(rng, "fp8", 2, 4, 1, 1, 16, [700, 531], 701)
     check_reorder(rng, "bf16", 2, 4, 200, 2, 128, [399, 1], 2)
     check_reorder(rng, "fp8", 1, 7, 64, 300, 16, [63], 1)
+
+
+def test_reorder_of_one_array_as_both_caches():
+    """Keys and values in the same memory: both results are the same."""
+    from nkipy_amd.runtime import DeviceTensor
+
+    rng = np.random.default_rng(9)
+    tables = rng.permutation(12).reshape(6, 2).astype(np.int32)
+    parents, lens = np.array([[2, 0, 0], [1, 1, 2]], np.int32), np.full(6, 21, np.int32)
+    cache = B.logits(rng, 12 * 16, 64, "bf16").reshape(12, 16, 1, 64)
+    t, (want, _) = B.reorder(parents, tables, lens, [cache, cache])
+    both = DeviceTensor.from_numpy(cache)
+    dk, ins, outs = load(f_reorder, parents, tables, lens, both, both)
+    for graph in (False, True, True):
+        both.write_from_numpy(cache)
+        outs["block_tables"].write_from_numpy(tables)
+        dk(ins, outs, graph=graph)
+        assert (outs["block_tables"].numpy() == t).all()
+        assert both.numpy().tobytes() == want.tobytes()
