@@ -226,8 +226,8 @@ def _beam_select_cpu(logits, scores, ended, *, end_token):
     token -1, the parent at their own place, score -inf and that parent's
     ``ended``.  Logits of +inf share the weight of their row.
 
-    On the GPU the row's sum has 32-bit terms, added up in 64 bits behind the
-    first few hundred, and sums of scores are compared in 64 bits."""
+    On the GPU a row's sum has 32-bit terms, added up in 32 bits over up to
+    8192 logits and in 64 over those sums; scores are compared in 64 bits."""
     groups, beams, vocab, end = _check_select(logits, scores, ended, end_token)
     x = _to64(logits).reshape(groups, beams, vocab)
     out = [np.zeros((groups, beams), d) for d in (np.int32, np.int32, np.float32, np.int32)]

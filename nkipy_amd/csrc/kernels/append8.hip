@@ -175,12 +175,13 @@ __device__ __forceinline__ void append8_body(const Append8Args &a) {
     auto once = [&](auto count) __attribute__((always_inline)) {
       constexpr int I = decltype(count)::value;
       float y[I][2][E];
-      int at[I], head[I];
+      int64_t at[I];
+      int head[I];
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const int x = min(tid + 256 * i, total - 1), r = x / (hn * pc), z = x % (hn * pc), h = z / pc, c = z % pc;
         const T *from = src + r * ss + h * sh + c * E;
-        head[i] = h, at[i] = ((first + r) * a.Hkv + h) * a.D + c * E;
+        head[i] = h, at[i] = ((int64_t)(first + r) * a.Hkv + h) * a.D + c * E;
         if (values) {
           Piece<T, E>::load(from, y[i][0]);
           Piece<T, E>::load(from + a.D / 2, y[i][1]);

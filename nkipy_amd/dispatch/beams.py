@@ -109,9 +109,10 @@ def beam_select(dtype, groups, beams, vocab, ld, end, *, x, scores, ended, token
 
 def beam_reorder(groups, beams, width, page, pages, hkv, row, *, parents, lens, tables, k, v, ke=0, ve=0) -> Launch:
     """Tables, caches (rows of ``row`` bytes) and exponents updated in place."""
-    if not (groups >= 1 and 1 <= beams <= MAX_BEAMS and width >= 1 and page >= 1 and row >= 1 and width * page < 2**30):
-        raise LaunchError(f"beam_reorder: {groups} groups of {beams} beams, pages of {page} rows")
     unit = 16 if not any(p % 16 for p in (k, v, row)) else 1
+    if not (groups >= 1 and 1 <= beams <= MAX_BEAMS and width >= 1 and pages >= 1 and page >= 1 and row >= 1
+            and width * page < 2**30 and page * row // unit < 2**31):
+        raise LaunchError(f"beam_reorder: {groups} groups of {beams} beams, pages of {page} rows")
     # (a page in part filled has a row less)
     a = _fields(ReorderArgs(), parents=parents, lens=lens, tables=tables, k=k, v=v, ke=ke, ve=ve, row=row, groups=groups,
                 beams=beams, width=width, page=page, pages=pages, hkv=hkv, tblocks=-(-width // 256),

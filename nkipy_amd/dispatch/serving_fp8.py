@@ -48,17 +48,18 @@ def rotary_append_fp8(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q
     if N < 1 or B < 1 or N >= 2**31 or B >= 2**30:
         raise LaunchError(f"rotary_append_fp8: {N} tokens of {B} sequences")
     if not (0 < 2 * half <= D and Hkv >= 1 and page >= 1 and pages >= 1 and width >= 1 and pages * page < 2**31
-            and width * page < 2**30):
+            and width * page < 2**30 and page * D < 2**31):
         raise LaunchError(f"rotary_append_fp8: {2 * half} rotated elements of {D}, {pages} pages of {page}")
     rows = min(page, N) if starts else 1
     heads = max(1, min(Hkv, APPEND_HEADS, APPEND_ELEMENTS // (rows * D)))
     a = _fields(Append8Args(), q=q, k=k, v=v, oq=oq, kc=kc, vc=vc, ke=ke, ve=ve, cos=cos, sin=sin, tables=tables, lens=lens,
                 starts=starts, q_ss=q_str[0], q_sh=q_str[1], k_ss=k_str[0], k_sh=k_str[1], v_ss=v_str[0], v_sh=v_str[1],
                 B=B, N=N, Hq=Hq, Hkv=Hkv, D=D, half=half, P=P, page=page, pages=pages, width=width, heads=heads)
-    a.blocks = (N // page + 2 * B if starts else B) * 2 * -(-Hkv // heads)
-    n = (N if oq else 0) + a.blocks
+    blocks = (N // page + 2 * B if starts else B) * 2 * -(-Hkv // heads)
+    n = (N if oq else 0) + blocks
     if n >= 2**31:
         raise LaunchError("rotary_append_fp8: too many workgroups for one launch")
+    a.blocks = blocks
     size = dt.itemsize(dtype)
     # pieces of eight elements: whole, and at 16-byte addresses (codes: 8)
     whole = half % 8 == 0 and D % 8 == 0 and not any(x % 16 for x in (q, k, v, oq, kc, vc, cos, sin)) \

@@ -200,6 +200,7 @@ def test_launch_helpers_refuse():
     ptr = dict(parents=16, lens=16, tables=16, k=16, v=16)
     assert D.beam_reorder(2, 3, 4, 16, 9, 2, 1024, **ptr).symbol == "nk_beam_reorder16_k4"
     assert D.beam_reorder(2, 9, 4, 16, 9, 2, 24, **ptr).symbol == "nk_beam_reorder1_k32"
-    for args in [(0, 3, 4, 16, 9, 2, 64), (2, 33, 4, 16, 9, 2, 64), (2, 3, 4, 0, 9, 2, 64)]:
+    for args in [(0, 3, 4, 16, 9, 2, 64), (2, 33, 4, 16, 9, 2, 64), (2, 3, 4, 0, 9, 2, 64), (2, 3, 4, 16, 0, 2, 64),
+                 (2, 3, 4, 2**20, 9, 2, 2**15 + 1)]:
         with pytest.raises(LaunchError):
             D.beam_reorder(*args, **ptr)

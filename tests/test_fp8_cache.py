@@ -230,7 +230,8 @@ def test_launch_helpers_refuse():
     ok = dict(q=0, k=0, v=0, oq=0, kc=0, vc=0, ke=0, ve=0, cos=0, sin=0, tables=0, lens=0)
     F.rotary_append_fp8(dt.bfloat16, 2, 4, 4, 2, 128, 64, 10, 16, 5, 3, **ok, starts=16)
     for args in [(0, 4, 4, 2, 128, 64, 10, 16, 5, 3), (2, 0, 4, 2, 128, 64, 10, 16, 5, 3), (2, 4, 4, 2, 128, 65, 10, 16, 5, 3),
-                 (2, 4, 4, 2, 128, 64, 10, 0, 5, 3), (2, 4, 4, 2, 128, 64, 10, 16, 2**28, 3)]:
+                 (2, 4, 4, 2, 128, 64, 10, 0, 5, 3), (2, 4, 4, 2, 128, 64, 10, 16, 2**28, 3), (2**30 - 1, 4, 4, 512, 128, 64, 10, 16, 5, 3),
+                 (2, 4, 4, 2, 256, 64, 10, 2**23, 5, 3)]:
         with pytest.raises(LaunchError):
             F.rotary_append_fp8(dt.bfloat16, *args, **ok)
     kw = dict(B=1, N=1, Hq=4, Hkv=2, D=128, q_str=(0, 512, 128), k_str=(0, 256, 128), v_str=(0, 256, 128), scale=1.0, tables=16,

@@ -102,7 +102,7 @@ def test_append_grows_and_keeps_scales(t):
         ke[:] = np.array([-30, 10])[None]
         ve[tables[0, 0]] = [-500, 500]
         ve[tables[1, 0]] = [-120, 120]
-        k[0], v[1] = k[0] if t == "f32" else k[0], P.cast(np.zeros(v[1].shape), t)
+        v[1] = P.cast(np.zeros(v[1].shape), t)
 
     check_append(np.random.default_rng(26), t, 4, 2, 64, 32, 16, [5, 9, 16, 17], None, spoil=spoil)
     check_append(np.random.default_rng(27), t, 4, 2, 64, 32, 16, [12, 15, 18, 40], [4, 9, 2, 7], std=1e-30)
@@ -315,6 +315,14 @@ def test_attend_many_sequences():
     check_attend(rng, "bf16", 4, 2, 64, 16, [max(x, 1) for x in lens], None, 40, 2)
 
 
+@pytest.mark.parametrize("n", [256, 257, 700])
+def test_attend_sequences_in_order_of_length_and_not(n):
+    """As many sequences as a workgroup sorts, and more."""
+    rng = np.random.default_rng(57)
+    new = [int(x) for x in rng.integers(0, 3, n)]
+    check_attend(rng, "bf16", 4, 2, 128, 16, [x + int(rng.integers(0, 60)) for x in new], new, 0, 0)
+
+
 def test_attend_layouts():
     """A layer of one big cache, heads before rows, queries out of a projection."""
     rng = np.random.default_rng(55)
@@ -359,3 +367,42 @@ def test_steps_queue_and_repeat():
         dk(ins, outs, graph=graph)
         for n, x in first.items():
             assert outs[n].numpy().tobytes() == x.tobytes()
+
+
+@pytest.mark.parametrize("new", [None, [3, 60]])
+def test_attend_heads_at_odd_addresses(new):
+    """Caches whose heads are parts of longer ones: rows that fit no 16 bytes."""
+    rng = np.random.default_rng(58)
+    tables, lens, starts, pages = P.batch(rng, [50, 70], new, 16)
+    q = draw(rng, (63 if new else 2, 4, 64), "bf16")
+    (kc, ke), (vc, ve) = Q.random_cache(rng, pages, 16, 2, 72), Q.random_cache(rng, pages, 16, 2, 72)
+
+    def f(q, kc, vc, ke, ve, tables, lens, starts=None):
+        return T.paged_attention_fp8(q, kc[:, :, :, 8:], vc[:, :, :, :64], ke, ve, tables, lens, starts)
+
+    got = run(f, q, kc, vc, ke, ve, tables, lens, starts)["output0"]
+    close(got, *Q.paged(q, kc[..., 8:], vc[..., :64], ke, ve, tables, lens, starts, 0, 0, "bf16"))
+
+
+@pytest.mark.parametrize("half", [64, 32])
+def test_append_behind_2_31_codes_of_a_page(half):
+    """Rows of a page whose places pass 32 bits."""
+    rng = np.random.default_rng(59)
+    hkv, d, page = 128, 128, 2**17 + 24
+    row = page - 9  # (131087 rows of 16384 codes before it)
+    k, v = draw(rng, (1, hkv, d), "bf16"), draw(rng, (1, hkv, d), "bf16")
+    kc, vc = (np.zeros((1, page, hkv, d), dt.float8_e4m3fn) for _ in range(2))
+    ke, ve = (np.full((1, hkv), -5, np.int32) for _ in range(2))
+    cos, sin = np.ones((page, half), np.float32), np.zeros((page, half), np.float32)
+    dk, ins, outs = load(f_append, k, k, v, cos, sin, kc, vc, ke, ve, np.zeros((1, 1), np.int32),
+                         np.array([row + 1], np.int32))
+    dk(ins, outs)
+    for name, x in (("key", k), ("value", v)):
+        assert (outs[name + "_exps"].numpy() == -5).all()  # (up to 14 in magnitude)
+        got = outs[name + "_cache"].numpy()
+        y = P.up(x)[0]
+        close(Q.values(got[:, row:row + 1], np.full((1, hkv), -5))[0, 0], y, np.maximum(np.abs(y) * 2.0**-4, 2.0**-15))
+        z = Q.bits(got)
+        assert z[0, row].any()
+        z[0, row] = 0
+        assert not z.any()
