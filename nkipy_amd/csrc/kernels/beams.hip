@@ -46,7 +46,7 @@ NK_DEVICE T running_block(T v, T *red, T &all) {
 // three: workgroups that mark some rows each, into bitmaps of their own; one that
 // joins the bitmaps, sums up and lists the free pages that are wanted; and as many as
 // there are rows and tokens for the entries and slots (500 rows of up to 375 pages,
-// 20000 tokens: 83 us by the one workgroup, XXX so).
+// 20000 tokens: 83 us by the one workgroup, 23 so).
 // ---------------------------------------------------------------------------
 struct AssignArgs {
   int32_t *tables;  // (rows, width)
@@ -357,6 +357,7 @@ __device__ __forceinline__ void select_top_body(const SelectArgs &a) {
       const float y = lv[wave][k];
       const int i = li[wave][k];
       int before = 0;
+#pragma unroll 4
       for (int q = 0; q < total; ++q) before += sel_before(lv[wave][q], li[wave][q], y, i) ? 1 : 0;
       if (before < K) bv[wave][before] = y, bi[wave][before] = i;
     }
@@ -389,14 +390,20 @@ __device__ __forceinline__ void select_top_body(const SelectArgs &a) {
     const int w = threadIdx.x / K, k = threadIdx.x % K, i = bi[w][k];
     const float y = bv[w][k];
     int before = k;
+    // (in another list: the first entry that is not before this one; places that hold
+    // nothing are equal, those of the lower waves first)
 #pragma unroll
-    for (int o = 1; o < 4; ++o)
-      for (int q = 0; q < K; ++q) {
-        const float z = bv[(w + o) & 3][q];
-        const int j = bi[(w + o) & 3][q];
-        // (places that hold nothing are equal: those of the lower waves first)
-        before += sel_before(z, j, y, i) || (z == y && i == j && ((w + o) & 3) < w) ? 1 : 0;
+    for (int o = 1; o < 4; ++o) {
+      const int u = (w + o) & 3;
+      int lo = 0, hi = K;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const float z = bv[u][mid];
+        const int j = bi[u][mid];
+        if (sel_before(z, j, y, i) || (z == y && i == j && u < w)) lo = mid + 1; else hi = mid;
       }
+      before += lo;
+    }
     if (before < K) a.best[at * K + before] = make_float2(y, __int_as_float(i == 0x7fffffff ? -1 : i));
   }
   if (threadIdx.x == 0) {
@@ -419,7 +426,68 @@ extern "C" __global__ __launch_bounds__(256) void nk_select_top_f32(SelectArgs a
 // a score in its order among all, places packed as beam * 2^22 + token
 NK_DEVICE bool sel_better(double s, uint32_t p, double t, uint32_t q) { return s > t || (s == t && p < q); }
 
+// order[r]: the entry of rank r < K of n (those with a place), by a workgroup.  Up to
+// DIRECT are ranked each against all, some threads side by side; of more, a search bit
+// by bit for the K-th largest's upper half leaves few more than K of them (992 lists of
+// 32 beams, then 528 entries: 153 us without, 25 so).
+#define SEL_DIRECT 256
+struct SelFew {
+  uint16_t list[SEL_HEADS];
+  uint32_t count[2][SEL_BLOCK / 64], n;
+};
+NK_DEVICE void sel_rank(const double *s, const uint32_t *p, int n, int K, int32_t *order, SelFew &few) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool all = n <= SEL_DIRECT;
+  int c = n;
+  if (!all) {
+    constexpr int E = SEL_HEADS / SEL_BLOCK;
+    uint32_t key[E], low = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = tid + e * SEL_BLOCK;
+      key[e] = 0;
+      if (i < n && p[i] != SEL_NONE) {
+        const uint32_t u = (uint32_t)__double2hiint(s[i] + 0.0);
+        key[e] = max(u & 0x80000000u ? ~u : u | 0x80000000u, 1u);
+      }
+    }
+    if (tid == 0) few.n = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t at = low | 1u << bit;
+      int m = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) m += __popcll(__ballot(key[e] >= at));
+      if (lane == 0) few.count[bit & 1][wave] = m;
+      __syncthreads();
+      m = 0;
+#pragma unroll
+      for (int w = 0; w < SEL_BLOCK / 64; ++w) m += few.count[bit & 1][w];
+      if (m >= K) low = at;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (key[e] && key[e] >= low) few.list[atomicAdd(&few.n, 1u)] = (uint16_t)(tid + e * SEL_BLOCK);
+    __syncthreads();
+    c = few.n;
+  }
+  auto id = [&](int x) { return all ? x : (int)few.list[x]; };
+  int S = 1;
+  while (S < 64 && c * S * 2 <= SEL_BLOCK) S *= 2;
+  for (int x = tid; x < (c * S + 63) / 64 * 64; x += SEL_BLOCK) {
+    const int i = id(min(x / S, c - 1));
+    const double y = s[i];
+    const uint32_t z = p[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int q = x % S; q < c; q += S) rank += p[id(q)] != SEL_NONE && sel_better(s[id(q)], p[id(q)], y, z) ? 1 : 0;
+    for (int o = 1; o < S; o <<= 1) rank += __shfl_xor(rank, o, 64);
+    if (x % S == 0 && x / S < c && z != SEL_NONE && rank < K) order[rank] = i;
+  }
+  __syncthreads();
+}
+
 extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArgs a) {
+  __shared__ SelFew few;
   __shared__ double hs[SEL_HEADS];
   __shared__ uint32_t hp[SEL_HEADS];
   __shared__ double cs[SEL_LEFT];
@@ -484,20 +552,7 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
     hp[h] = is ? p : SEL_NONE;
   }
   __syncthreads();
-  // a head's rank, by S threads side by side
-  int S = 1;
-  while (S < 64 && heads * S * 2 <= SEL_BLOCK) S *= 2;
-  for (int x = tid; x < (heads * S + 63) / 64 * 64; x += SEL_BLOCK) {
-    const int h = min(x / S, heads - 1);
-    const double s = hs[h];
-    const uint32_t p = hp[h];
-    int rank = 0;
-#pragma unroll 4
-    for (int q = x % S; q < heads; q += S) rank += hp[q] != SEL_NONE && sel_better(hs[q], hp[q], s, p) ? 1 : 0;
-    for (int o = 1; o < S; o <<= 1) rank += __shfl_xor(rank, o, 64);
-    if (x % S == 0 && x / S < heads && p != SEL_NONE && rank < K) order[rank] = h;
-  }
-  __syncthreads();
+  sel_rank(hs, hp, heads, K, order, few);
   // entry j of the list whose best has rank r: a thread for each r + j < K
   for (int c = tid; c < K * K; c += SEL_BLOCK) {
     const int r = c / K, j = c % K;
@@ -510,26 +565,18 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
   }
   __syncthreads();
   const int n = K * (K + 1) / 2;
-  int taken = 0;
-  for (int c = tid; c < n; c += SEL_BLOCK) {
-    const double s = cs[c];
-    const uint32_t p = cp[c];
-    if (p == SEL_NONE) continue;
-    int rank = 0;
-#pragma unroll 4
-    for (int q = 0; q < n; ++q) rank += cp[q] != SEL_NONE && sel_better(cs[q], cp[q], s, p) ? 1 : 0;
-    if (rank >= K) continue;
-    const int b = p >> 22, t = kind[b] == 2 ? a.end : (int)(p & 0x3fffff), to = g * K + rank;
+  if (tid < K) order[tid] = -1;
+  __syncthreads();
+  sel_rank(cs, cp, n, K, order, few);
+  if (tid < K && order[tid] >= 0) {
+    const double s = cs[order[tid]];
+    const uint32_t p = cp[order[tid]];
+    const int b = p >> 22, t = kind[b] == 2 ? a.end : (int)(p & 0x3fffff), to = g * K + tid;
     a.tokens[to] = t;
     a.parents[to] = b;
     a.out[to] = (float)s;
     a.ends[to] = kind[b] == 2 || t == a.end ? 1 : 0;
-  }
-  // the places left
-  for (int i = lane; i < n; i += 64) taken += cp[i] != SEL_NONE ? 1 : 0;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) taken += __shfl_xor(taken, o, 64);
-  if (tid >= taken && tid < K) {
+  } else if (tid < K) {  // too few continuations
     a.tokens[g * K + tid] = -1;
     a.parents[g * K + tid] = tid;
     a.out[g * K + tid] = -INFINITY;
