@@ -427,46 +427,40 @@ extern "C" __global__ __launch_bounds__(256) void nk_select_top_f32(SelectArgs a
 NK_DEVICE bool sel_better(double s, uint32_t p, double t, uint32_t q) { return s > t || (s == t && p < q); }
 
 // order[r]: the entry of rank r < K of n (those with a place), by a workgroup.  Up to
-// DIRECT are ranked each against all, some threads side by side; of more, a search bit
-// by bit for the K-th largest's upper half leaves few more than K of them (992 lists of
-// 32 beams, then 528 entries: 153 us without, 25 so).
-#define SEL_DIRECT 256
+// DIRECT are ranked each against all, some threads side by side.  Of more, the first
+// wave lists those that can count, as above: what is not below the K-th largest of its
+// lanes' largest, by the upper halves.
+#define SEL_DIRECT 64
 struct SelFew {
   uint16_t list[SEL_HEADS];
-  uint32_t count[2][SEL_BLOCK / 64], n;
+  uint32_t n;
 };
 NK_DEVICE void sel_rank(const double *s, const uint32_t *p, int n, int K, int32_t *order, SelFew &few) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
   const bool all = n <= SEL_DIRECT;
   int c = n;
   if (!all) {
-    constexpr int E = SEL_HEADS / SEL_BLOCK;
-    uint32_t key[E], low = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = tid + e * SEL_BLOCK;
-      key[e] = 0;
-      if (i < n && p[i] != SEL_NONE) {
+    if (tid < 64) {
+      auto key = [&](int i) __attribute__((always_inline)) {
         const uint32_t u = (uint32_t)__double2hiint(s[i] + 0.0);
-        key[e] = max(u & 0x80000000u ? ~u : u | 0x80000000u, 1u);
+        return p[i] != SEL_NONE ? max(u & 0x80000000u ? ~u : u | 0x80000000u, 1u) : 0u;
+      };
+      uint32_t top = 0, low = 0;
+#pragma unroll 4
+      for (int i = lane; i < n; i += 64) top = max(top, key(i));
+#pragma unroll
+      for (uint32_t bit = 0x80000000u; bit; bit >>= 1) low |= __popcll(__ballot(top >= (low | bit))) >= K ? bit : 0;
+      low = max(low, 1u);
+      uint32_t at = 0;
+#pragma unroll 4
+      for (int i0 = 0; i0 < n; i0 += 64) {
+        const bool in = i0 + lane < n && key(min(i0 + lane, n - 1)) >= low;
+        const u64 those = __ballot(in);
+        if (in) few.list[at + __popcll(those & ((1ull << lane) - 1))] = (uint16_t)(i0 + lane);
+        at += __popcll(those);
       }
+      if (lane == 0) few.n = at;
     }
-    if (tid == 0) few.n = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t at = low | 1u << bit;
-      int m = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) m += __popcll(__ballot(key[e] >= at));
-      if (lane == 0) few.count[bit & 1][wave] = m;
-      __syncthreads();
-      m = 0;
-#pragma unroll
-      for (int w = 0; w < SEL_BLOCK / 64; ++w) m += few.count[bit & 1][w];
-      if (m >= K) low = at;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (key[e] && key[e] >= low) few.list[atomicAdd(&few.n, 1u)] = (uint16_t)(tid + e * SEL_BLOCK);
     __syncthreads();
     c = few.n;
   }
