@@ -270,16 +270,20 @@ struct SelectArgs {
 #define SEL_LIST 256
 #define SEL_BEAMS 32
 
-// a before b: the larger value, or the lower place
-NK_DEVICE bool sel_before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
+// A value and its place as one number: the larger value first, then the lower place.
+// (No number, and infinitely little, are below SEL_LEAST.)
+#define SEL_LEAST ((u64)0x00800000u << 32)
+NK_DEVICE uint32_t sel_order(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);  // (one zero)
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+NK_DEVICE u64 sel_key(float v, int i) { return (u64)sel_order(v) << 32 | (uint32_t)~i; }
 
 template <typename T>
 __device__ __forceinline__ void select_top_body(const SelectArgs &a) {
   constexpr int E = 16 / sizeof(T), U = 32 / E;  // elements of a piece, pieces of a lane
-  __shared__ float lv[4][SEL_LIST];
-  __shared__ int32_t li[4][SEL_LIST];
-  __shared__ float bv[4][SEL_BEAMS];
-  __shared__ int32_t bi[4][SEL_BEAMS];
+  __shared__ u64 list[4][SEL_LIST];
+  __shared__ u64 best[4][SEL_BEAMS];
   __shared__ float2 ms[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = blockIdx.x / a.nseg, seg = blockIdx.x % a.nseg, K = a.beams;
@@ -332,79 +336,74 @@ __device__ __forceinline__ void select_top_body(const SelectArgs &a) {
   sum = wave_sum(sum);
   // the K-th largest of the lanes' largest values, its key's high half: as many values
   // are not below it
-  const uint32_t bits = __float_as_uint(top + 0.f), key = (bits & 0x80000000u ? ~bits : bits | 0x80000000u) >> 16;
+  const uint32_t key = sel_order(top) >> 16;
   uint32_t kth = 0;
 #pragma unroll
   for (uint32_t bit = 0x8000; bit; bit >>= 1) kth |= __popcll(__ballot(key >= (kth | bit))) >= K ? bit : 0;
   kth <<= 16;
   float low = __uint_as_float(kth & 0x80000000u ? kth & 0x7fffffffu : ~kth);
   low = low > -3.40282347e38f ? low : -3.40282347e38f;  // (-inf, or what is no number, is listed nowhere)
-  uint32_t in = 0;  // a bit for each element, the first the highest
+  int total = 0;
 #pragma unroll
-  for (int e = 0; e < 32; ++e) in += in + (v[e] >= low ? 1 : 0);
-  const int mine = __popc(in), upto = running(mine), total = __builtin_amdgcn_readlane(upto, 63);
-  int count = min(total, K);
+  for (int e = 0; e < 32; ++e) {
+    const bool in = v[e] >= low;
+    const u64 those = __ballot(in);
+    if (those == 0) continue;
+    const int at = total + __builtin_amdgcn_mbcnt_hi((uint32_t)(those >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)those, 0));
+    if (in && at < SEL_LIST) list[wave][at] = sel_key(v[e], i0 + e / E * 64 * E + e % E);
+    total += __popcll(those);
+  }
+  const int count = min(total, K);
   if (total <= SEL_LIST) {
-    int at = upto - mine;
-    for (uint32_t left = in; left; left &= left - 1, ++at) {
-      const int e = 31 - __builtin_ctz(left), i = i0 + e / E * 64 * E + e % E;
-      lv[wave][at] = Elt<T>::load(x, i);
-      li[wave][at] = i;
-    }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own list
     asm volatile("" ::: "memory");
     for (int k = lane; k < total; k += 64) {
-      const float y = lv[wave][k];
-      const int i = li[wave][k];
+      const u64 y = list[wave][k];
       int before = 0;
-#pragma unroll 4
-      for (int q = 0; q < total; ++q) before += sel_before(lv[wave][q], li[wave][q], y, i) ? 1 : 0;
-      if (before < K) bv[wave][before] = y, bi[wave][before] = i;
+#pragma unroll 8
+      for (int q = 0; q < total; ++q) before += list[wave][q] > y ? 1 : 0;
+      if (before < K) best[wave][before] = y;
     }
   } else {
-    float ly = INFINITY;
-    int lj = -1;  // the last one taken
+    u64 last = ~0ull;  // taken
     for (int k = 0; k < count; ++k) {
-      float y = -INFINITY;
-      int j = 0x7fffffff;
+      u64 y = 0;
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        const int i = i0 + e / E * 64 * E + e % E;
-        if (v[e] > -INFINITY && sel_before(ly, lj, v[e], i) && sel_before(v[e], i, y, j)) y = v[e], j = i;
+        const u64 z = v[e] >= low ? sel_key(v[e], i0 + e / E * 64 * E + e % E) : 0;
+        y = z < last && z > y ? z : y;
       }
 #pragma unroll
-      for (int o = 32; o; o >>= 1) {
-        const float oy = __shfl_xor(y, o, 64);
-        const int oj = __shfl_xor(j, o, 64);
-        if (sel_before(oy, oj, y, j)) y = oy, j = oj;
-      }
-      if (lane == 0) bv[wave][k] = y, bi[wave][k] = j;
-      ly = y, lj = j;
+      for (int o = 32; o; o >>= 1) y = max(y, (u64)__shfl_xor(y, o, 64));
+      if (lane == 0) best[wave][k] = y;
+      last = y;
     }
   }
-  if (lane >= count && lane < K) bv[wave][lane] = -INFINITY, bi[wave][lane] = 0x7fffffff;
+  if (lane >= count && lane < K) best[wave][lane] = (u64)(4 * SEL_BEAMS - wave * SEL_BEAMS - lane);  // (nothing, in order)
   if (lane == 0) ms[wave] = make_float2(m, sum);
   __syncthreads();
   const int64_t at = (int64_t)r * a.nseg + seg;
   if (threadIdx.x < 4 * K) {
-    const int w = threadIdx.x / K, k = threadIdx.x % K, i = bi[w][k];
-    const float y = bv[w][k];
+    const int w = threadIdx.x / K, k = threadIdx.x % K;
+    const u64 y = best[w][k];
     int before = k;
-    // (in another list: the first entry that is not before this one; places that hold
-    // nothing are equal, those of the lower waves first)
+    // (of another list as many as are before this one)
 #pragma unroll
     for (int o = 1; o < 4; ++o) {
       const int u = (w + o) & 3;
       int lo = 0, hi = K;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        const float z = bv[u][mid];
-        const int j = bi[u][mid];
-        if (sel_before(z, j, y, i) || (z == y && i == j && u < w)) lo = mid + 1; else hi = mid;
+        if (best[u][mid] > y) lo = mid + 1; else hi = mid;
       }
       before += lo;
     }
-    if (before < K) a.best[at * K + before] = make_float2(y, __int_as_float(i == 0x7fffffff ? -1 : i));
+    if (before < K) {
+      const uint32_t u = (uint32_t)(y >> 32);
+      const bool is = y >= SEL_LEAST;
+      a.best[at * K + before] = make_float2(is ? __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u) : -INFINITY,
+                                            __int_as_float(is ? (int)~(uint32_t)y : -1));
+    }
   }
   if (threadIdx.x == 0) {
     const float t = fmaxf(fmaxf(ms[0].x, ms[1].x), fmaxf(ms[2].x, ms[3].x));
@@ -424,7 +423,7 @@ extern "C" __global__ __launch_bounds__(256) void nk_select_top_f32(SelectArgs a
 #define SEL_NONE 0xffffffffu
 
 // a score in its order among all, places packed as beam * 2^22 + token
-NK_DEVICE bool sel_better(double s, uint32_t p, double t, uint32_t q) { return s > t || (s == t && p < q); }
+NK_DEVICE bool sel_better(double s, uint32_t p, double t, uint32_t q) { return (s > t) | ((s == t) & (p < q)); }
 
 // order[r]: the entry of rank r < K of n (those with a place), by a workgroup.  Up to
 // DIRECT are ranked each against all, some threads side by side.  Of more, the first
@@ -473,7 +472,7 @@ NK_DEVICE void sel_rank(const double *s, const uint32_t *p, int n, int K, int32_
     const uint32_t z = p[i];
     int rank = 0;
 #pragma unroll 4
-    for (int q = x % S; q < c; q += S) rank += p[id(q)] != SEL_NONE && sel_better(s[id(q)], p[id(q)], y, z) ? 1 : 0;
+    for (int q = x % S; q < c; q += S) rank += (p[id(q)] != SEL_NONE) & sel_better(s[id(q)], p[id(q)], y, z) ? 1 : 0;
     for (int o = 1; o < S; o <<= 1) rank += __shfl_xor(rank, o, 64);
     if (x % S == 0 && x / S < c && z != SEL_NONE && rank < K) order[rank] = i;
   }
