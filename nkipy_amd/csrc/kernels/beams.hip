@@ -7,30 +7,42 @@ using namespace nk;
 
 typedef unsigned long long u64;
 
-// running sums over the lanes of a wave, this one's included
-template <typename T>
-NK_DEVICE T running(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T u = __shfl_up(v, o, 64);
-    v += lane >= o ? u : 0;
-  }
+// running sums over the lanes of a wave, this one's included: within rows of 16 lanes,
+// then from the rows before
+template <int CTRL, int ROWS>
+NK_DEVICE int64_t lanes_before(int64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)((u64)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+NK_DEVICE int64_t running(int64_t v) {
+  v += lanes_before<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += lanes_before<0x112, 0xf>(v);
+  v += lanes_before<0x114, 0xf>(v);
+  v += lanes_before<0x118, 0xf>(v);
+  v += lanes_before<0x142, 0xa>(v);  // row_bcast 15: lane 15 of rows 0 and 2
+  v += lanes_before<0x143, 0xc>(v);  // row_bcast 31: lane 31
   return v;
 }
-// and over a workgroup of W waves; `all`: the whole sum
-template <int W, typename T>
-NK_DEVICE T running_block(T v, T *red, T &all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  v = running(v);
+NK_DEVICE int64_t lane_of(int64_t v, int lane) {
+  return (int64_t)((u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32
+                   | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+// and of two numbers over a workgroup of W waves; `all`: the whole sums
+template <int W>
+NK_DEVICE void running_block(int64_t (&v)[2], int64_t (*red)[W], int64_t (&all)[2]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  v[0] = running(v[0]), v[1] = running(v[1]);
   __syncthreads();
-  if (lane == 63) red[wave] = v;
+  if (lane == 63) red[0][wave] = v[0], red[1][wave] = v[1];
   __syncthreads();
-  // (the waves' sums again by a running sum: W registers less)
-  const T w = running(lane < W ? red[lane] : 0);
-  all = __shfl(w, W - 1, 64);
-  if (wave) v += __shfl(w, wave - 1, 64);
-  return v;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    // (the waves' sums again by a running sum: W registers less)
+    const int64_t w = running(lane < W ? red[k][lane] : 0);
+    all[k] = lane_of(w, W - 1);
+    if (wave) v[k] += lane_of(w, wave - 1);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -106,36 +118,36 @@ NK_DEVICE void asg_mark(const AssignArgs &a, uint32_t *used, int b0, int step) {
 
 // Starts and wanted pages of the rows, and from the bitmap the free pages before each
 // thread's words; returns (pages wanted, pages free).
-NK_DEVICE void asg_sums(const AssignArgs &a, const uint32_t *used, int32_t *before, int64_t *red, int64_t &wanted, int64_t &free) {
+NK_DEVICE void asg_sums(const AssignArgs &a, const uint32_t *used, int32_t *before, int64_t (*red)[ASG_BLOCK / 64],
+                        int64_t &wanted, int64_t &free) {
   const int tid = threadIdx.x;
-  int64_t starts = 0, wants = 0, all;
+  const int words = (a.pages + 31) / 32;
+  const int per = (words + ASG_BLOCK - 1) / ASG_BLOCK, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+  int count = 0;
+  for (int i = w0; i < w1; ++i) count += __popc(~used[i]);
+  int64_t starts = 0, wants = 0, v[2], all[2];
   for (int b0 = 0; b0 < a.rows; b0 += ASG_BLOCK) {
     const int b = b0 + tid;
-    int64_t n = 0, w = 0;
+    int n = 0, w = 0;
     if (b < a.rows) {
       const AsgRow r = asg_row(a, b);
       n = r.fresh, w = max(r.need - r.held, 0);
     }
-    const int64_t ns = running_block<ASG_BLOCK / 64>(n, red, all) + starts;
-    starts += all;
-    const int64_t ws = running_block<ASG_BLOCK / 64>(w, red, all) + wants;
-    wants += all;
+    // (what is wanted in the upper bits: below 2^40 in all; free pages: up to 2^20)
+    v[0] = n, v[1] = (int64_t)w << 21 | (b0 ? 0 : count);
+    running_block(v, red, all);
+    if (b0 == 0) before[tid] = (int)(v[1] & 0x1fffff) - count, free = all[1] & 0x1fffff;
     if (b < a.rows) {
-      a.starts[b] = (int32_t)min(ns - n, (int64_t)0x7fffffff);
-      a.wants[b] = (int32_t)min(ws - w, (int64_t)a.pages);
+      a.starts[b] = (int32_t)min(starts + v[0] - n, (int64_t)0x7fffffff);
+      a.wants[b] = (int32_t)min(wants + (v[1] >> 21) - w, (int64_t)a.pages);
     }
+    starts += all[0], wants += all[1] >> 21;
   }
-  const int words = (a.pages + 31) / 32;
-  const int per = (words + ASG_BLOCK - 1) / ASG_BLOCK, w0 = min(tid * per, words), w1 = min(w0 + per, words);
-  int64_t n = 0;
-  for (int i = w0; i < w1; ++i) n += __popc(~used[i]);
-  const int64_t upto = running_block<ASG_BLOCK / 64>(n, red, all);
-  before[tid] = (int32_t)(upto - n);
   if (tid == 0) {
     a.starts[a.rows] = (int32_t)min(starts, (int64_t)0x7fffffff);
-    a.free[0] = (int32_t)max(all - wants, (int64_t)-0x7fffffff);
+    a.free[0] = (int32_t)max(free - wants, (int64_t)-0x7fffffff);
   }
-  wanted = wants, free = all;
+  wanted = wants;
 }
 // the wanted free pages of a thread's words
 NK_DEVICE void asg_list(const AssignArgs &a, const uint32_t *used, int before, int64_t wanted, int64_t free) {
@@ -190,7 +202,7 @@ NK_DEVICE void asg_slots(const AssignArgs &a, int t0) {
 extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_pages(AssignArgs a) {
   __shared__ uint32_t used[ASG_WORDS];
   __shared__ int32_t before[ASG_BLOCK];
-  __shared__ int64_t red[ASG_BLOCK / 64];
+  __shared__ int64_t red[2][ASG_BLOCK / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, words = (a.pages + 31) / 32;
   for (int i = tid; i < words; i += ASG_BLOCK) used[i] = i == words - 1 && (a.pages & 31) ? ~0u << (a.pages & 31) : 0;  // (no pages)
   __syncthreads();
@@ -217,7 +229,7 @@ extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_mark(AssignArg
 extern "C" __global__ __launch_bounds__(ASG_BLOCK) void nk_assign_plan(AssignArgs a) {
   __shared__ __attribute__((aligned(16))) uint32_t used[ASG_WORDS];
   __shared__ int32_t before[ASG_BLOCK];
-  __shared__ int64_t red[ASG_BLOCK / 64];
+  __shared__ int64_t red[2][ASG_BLOCK / 64];
   const int tid = threadIdx.x, words = (a.pages + 31) / 32, pitch = (words + 3) & ~3;
   for (int i = tid * 4; i < words; i += ASG_BLOCK * 4) {
     u32x4 u = {0, 0, 0, 0};
