@@ -13,8 +13,8 @@ using namespace nk;
 //   page's where rows written earlier stay)
 //
 // in fp32, every product and sum rounded by itself, so that the largest magnitude,
-// and with it e, is what the same steps give anywhere.  Workgroups: one for each
-// token's queries; one for each (page that a sequence writes, keys or values, some
+// and with it e, is what the same steps give anywhere.  Workgroups: one for the queries
+// of a token or of four; one for each (page that a sequence writes, keys or values, some
 // heads), as many as its threads can keep between the largest magnitude and the codes
 // (large pages, odd sizes and heads rotated in part: read again, mostly from cache).
 // Maxima are of whole numbers (bits), so no order changes them.  Bound by memory,
@@ -32,6 +32,7 @@ struct Append8Args {
   int32_t page, pages, width;
   int32_t heads;  // of a workgroup, up to A8_HEADS
   int32_t blocks;  // workgroups of keys and values
+  int32_t qwaves;  // waves of a token's queries: 1 or 4
 };
 #define A8_HEADS 64
 #define A8_ITEMS 4  // pairs of pieces that a thread keeps
@@ -61,15 +62,11 @@ NK_DEVICE A8Seq a8_seq(const Append8Args &a, int b) {
 // the n / page + 2 that n tokens may touch.
 NK_DEVICE int a8_tile0(const Append8Args &a, int b) { return min(max(a.starts[b], 0), a.N) / a.page + 2 * b; }
 
-// E elements of both halves of a rotated piece, or of a piece that is copied
-template <typename T, int E>
-NK_DEVICE void a8_turn(const T *x, const float *cr, const float *sr, int half, float (&y0)[E], float (&y1)[E]) {
+// E elements of both halves of a piece, rotated
+template <int E>
+NK_DEVICE void a8_turn(const float (&x0)[E], const float (&x1)[E], const float (&c)[E], const float (&s)[E], float (&y0)[E],
+                       float (&y1)[E]) {
 #pragma clang fp contract(off)
-  float x0[E], x1[E], c[E], s[E];
-  Piece<T, E>::load(x, x0);
-  Piece<T, E>::load(x + half, x1);
-  Piece<float, E>::load(cr, c);
-  Piece<float, E>::load(sr, s);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const float p0 = x0[e] * c[e], p1 = x1[e] * s[e], p2 = x0[e] * s[e], p3 = x1[e] * c[e];
@@ -77,9 +74,25 @@ NK_DEVICE void a8_turn(const T *x, const float *cr, const float *sr, int half, f
     y1[e] = p2 + p3;
   }
 }
-
 template <typename T, int E>
-__device__ __forceinline__ void append8_queries(const Append8Args &a, int t) {
+NK_DEVICE void a8_turn(const T *x, const float *cr, const float *sr, int half, float (&y0)[E], float (&y1)[E]) {
+  float x0[E], x1[E], c[E], s[E];
+  Piece<T, E>::load(x, x0);
+  Piece<T, E>::load(x + half, x1);
+  Piece<float, E>::load(cr, c);
+  Piece<float, E>::load(sr, s);
+  a8_turn<E>(x0, x1, c, s, y0, y1);
+}
+
+// The queries of a token, by `qwaves` waves; 4 / qwaves tokens to a workgroup.  Heads
+// rotated as a whole, of a power of two of pieces: a lane keeps its place in the head
+// and its angles, with A8_ITEMS heads on their way at once (8000 tokens of 32 heads of
+// 128: 42 us with a head at a time, XXX so).
+template <typename T, int E>
+__device__ __forceinline__ void append8_queries(const Append8Args &a, int blk) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blk * (4 / a.qwaves) + wave / a.qwaves, place = wave % a.qwaves * 64 + lane, step = 64 * a.qwaves;
+  if (t >= a.N) return;
   int b = t;
   if (a.starts) b = a8_find(a.B, t, [&](int x) { return a.starts[x]; });
   int p = -1;
@@ -90,10 +103,37 @@ __device__ __forceinline__ void append8_queries(const Append8Args &a, int t) {
   const bool in = p >= 0 && p < a.P;
   const int turns = a.half / E, per = turns + (a.D - 2 * a.half) / E;
   const float *cr = a.cos + (int64_t)(in ? p : 0) * a.half, *sr = a.sin + (int64_t)(in ? p : 0) * a.half;
-  for (int x = threadIdx.x; x < a.Hq * per; x += 256) {
+  const T *const q = (const T *)a.q + t * a.q_ss;
+  T *const o = (T *)a.oq + (int64_t)t * a.Hq * a.D;
+  if (E == 8 && in && per == turns && (turns & (turns - 1)) == 0 && turns <= 64) {
+    const int d = place % turns * E, hs = step / turns;
+    float c[E], s[E];
+    Piece<float, E>::load(cr + d, c);
+    Piece<float, E>::load(sr + d, s);
+    for (int h0 = place / turns; h0 < a.Hq; h0 += A8_ITEMS * hs) {
+      float x[A8_ITEMS][2][E];
+#pragma unroll
+      for (int i = 0; i < A8_ITEMS; ++i) {
+        const T *src = q + min(h0 + i * hs, a.Hq - 1) * a.q_sh + d;
+        Piece<T, E>::load(src, x[i][0]);
+        Piece<T, E>::load(src + a.half, x[i][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < A8_ITEMS; ++i) {
+        float y0[E], y1[E];
+        if (h0 + i * hs >= a.Hq) break;
+        a8_turn<E>(x[i][0], x[i][1], c, s, y0, y1);
+        T *dst = o + (int64_t)(h0 + i * hs) * a.D + d;
+        Piece<T, E>::store(dst, y0);
+        Piece<T, E>::store(dst + a.half, y1);
+      }
+    }
+    return;
+  }
+  for (int x = place; x < a.Hq * per; x += step) {
     const int h = x / per, c = x % per;
-    const T *src = (const T *)a.q + t * a.q_ss + h * a.q_sh;
-    T *dst = (T *)a.oq + ((int64_t)t * a.Hq + h) * a.D;
+    const T *src = q + h * a.q_sh;
+    T *dst = o + (int64_t)h * a.D;
     if (!in) {
       const float z[E] = {};
       const int d = c < turns ? c * E : 2 * a.half + (c - turns) * E;

@@ -30,7 +30,7 @@ class Append8Args(ctypes.Structure):
                                                  "starts")]
                 + [(n, ctypes.c_int64) for n in ("q_ss", "q_sh", "k_ss", "k_sh", "v_ss", "v_sh")]
                 + [(n, ctypes.c_int32) for n in ("B", "N", "Hq", "Hkv", "D", "half", "P", "page", "pages", "width", "heads",
-                                              "blocks")])
+                                              "blocks", "qwaves")])
 
 
 class Attend8Args(S.AttendArgs):
@@ -39,6 +39,7 @@ class Attend8Args(S.AttendArgs):
 
 APPEND_HEADS = 64      # heads of a workgroup at most (append8.hip)
 APPEND_ELEMENTS = 2**14  # elements that a workgroup quantises, about
+APPEND_TOKENS = 1024   # tokens that are a wave's work each
 
 
 def rotary_append_fp8(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q, k, v, oq, kc, vc, ke, ve, cos, sin, tables, lens,
@@ -56,7 +57,8 @@ def rotary_append_fp8(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q
                 starts=starts, q_ss=q_str[0], q_sh=q_str[1], k_ss=k_str[0], k_sh=k_str[1], v_ss=v_str[0], v_sh=v_str[1],
                 B=B, N=N, Hq=Hq, Hkv=Hkv, D=D, half=half, P=P, page=page, pages=pages, width=width, heads=heads)
     blocks = (N // page + 2 * B if starts else B) * 2 * -(-Hkv // heads)
-    n = (N if oq else 0) + blocks
+    a.qwaves = 1 if N >= APPEND_TOKENS else 4
+    n = (-(-N * a.qwaves // 4) if oq else 0) + blocks
     if n >= 2**31:
         raise LaunchError("rotary_append_fp8: too many workgroups for one launch")
     a.blocks = blocks
