@@ -187,9 +187,9 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
 
   // a thread's codes of a block: row rr, elements 16 cc ..., of K and V or of one of them
   const int rr = (BOTH ? tid : tid & 127) / LPR, cc = tid % LPR;
-  const bool keys = BOTH || tid < 128;
-  const uint8_t *const kp = (keys ? (const uint8_t *)a.k + (int64_t)g * a.k_sh : (const uint8_t *)a.v + (int64_t)g * a.v_sh) + cc * 16;
-  const uint8_t *const vp = (const uint8_t *)a.v + (int64_t)g * a.v_sh + cc * 16;
+  const bool keys = BOTH || wave < 2;
+  const uint8_t *const kp = (keys ? (const uint8_t *)a.k + (int64_t)g * a.k_sh : (const uint8_t *)a.v + (int64_t)g * a.v_sh);
+  const uint8_t *const vp = (const uint8_t *)a.v + (int64_t)g * a.v_sh;
   const int64_t kss = keys ? a.k_ss : a.v_ss;
   struct Codes {
     uint4 w;
@@ -209,10 +209,10 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   };
   auto fetch = [&]() __attribute__((always_inline)) {
     ck.scale = __uint_as_float((keys ? kex & 0xff : kex >> 8) << 23);
-    ck.w = *reinterpret_cast<const uint4 *>(kp + max(kat, 0) * kss);
+    ck.w = *reinterpret_cast<const uint4 *>(kp + (max(kat, 0) * kss + cc * 16));
     if constexpr (BOTH) {
       cv.scale = __uint_as_float((vex >> 8) << 23);
-      cv.w = *reinterpret_cast<const uint4 *>(vp + max(vat, 0) * a.v_ss);
+      cv.w = *reinterpret_cast<const uint4 *>(vp + (max(vat, 0) * a.v_ss + cc * 16));
     }
   };
   auto put = [&](const Codes &x, uint8_t *to, int swz) __attribute__((always_inline)) {
@@ -240,26 +240,48 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) s = mul32(f, qf[kk][i], s);
   };
-  auto pv1 = [&](const uint8_t *Vt, const B8 (&pf)[2][NP], int j, int dt) __attribute__((always_inline)) {
+  auto read_k = [&](const uint8_t *K, int kk) __attribute__((always_inline)) {
+    return *reinterpret_cast<const B8 *>(K + kbase + ((kk << 5) ^ kx));
+  };
+  auto read_v = [&](const uint8_t *Vt, int j, int dt) __attribute__((always_inline)) {
     s16x4 v[2];
 #pragma unroll
     for (int si = 0; si < 2; ++si)
       v[si] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (lds_s16x4 *)(Vt + (16 * j + 8 * si) * RB + vbase + ((dt << 6) ^ vx)));
-    const s16x8 vf = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) acc[dt] = mul32(__builtin_bit_cast(B8, vf), pf[j][i], acc[dt]);
+    return __builtin_bit_cast(B8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  // The scores of one block and the values of another, in turns: each product of
-  // the scores waits for the one before it, the values' are apart.
-  auto qk_pv = [&](const uint8_t *K, f32x16 &s, const uint8_t *Vt, const B8 (&pf)[2][NP]) __attribute__((always_inline)) {
+  // The scores of one block, the values of another and the weights of a third, in turns
+  // (each product of the scores waits for the one before it; the weights go on beside the
+  // products), with what a step reads on its way a step before.  Returns the sum of the
+  // weights 2^(s c - m).  (2100 tokens of 24 sequences: 265 us with the weights behind all
+  // products, 246 so at a raised priority, 240 in turns; 1.24 and 1.13 a block where a CU
+  // has one workgroup, 1.75 and 1.62 where it has two.  With the codes' stores among the
+  // products as well 290: they wait for their reads.)
+  auto work = [&](const uint8_t *K, f32x16 &nxt, const uint8_t *Vt, const B8 (&prev)[2][NP], const f32x16 &cur,
+                  B8 (&now)[2][NP]) __attribute__((always_inline)) {
+    constexpr int STEPS = D / 16, W = 16 / STEPS;
+    float s0 = 0.f, s1 = 0.f;
+    B8 kf[2], vf[2];
+    kf[0] = read_k(K, 0), vf[0] = read_v(Vt, 0, 0);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    for (int r = 0; r < 16; ++r) nxt[r] = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      qk1(K, s, i);
-      pv1(Vt, pf, i / (D / 32), i % (D / 32));
+    for (int i = 0; i < STEPS; ++i) {
+      if (i + 1 < STEPS) kf[(i + 1) & 1] = read_k(K, i + 1), vf[(i + 1) & 1] = read_v(Vt, (i + 1) / (D / 32), (i + 1) % (D / 32));
+#pragma unroll
+      for (int u = 0; u < NP; ++u) nxt = mul32(kf[i & 1], qf[i][u], nxt);
+#pragma unroll
+      for (int u = 0; u < NP; ++u) acc[i % (D / 32)] = mul32(vf[i & 1], prev[i / (D / 32)][u], acc[i % (D / 32)]);
+#pragma unroll
+      for (int e = i * W; e < i * W + W; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[e], sl2, -m_run));
+        if (e & 1) s1 += x; else s0 += x;
+        put_weight<NP>(now[e / 8], e % 8, x);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    return s0 + s1;
   };
   auto expblock = [&](const f32x16 &s, B8 (&pf)[2][NP]) __attribute__((always_inline)) {
     float s0 = 0.f, s1 = 0.f;
@@ -332,8 +354,7 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
       const int k0 = sp.kb(j0 + jr) * ATT_KEYS;
       if (!(jr < n && k0 + ATT_KEYS - 1 <= sp.pa && k0 + ATT_KEYS <= sp.hi && (k0 > sp.pb - a.window || k0 + ATT_KEYS <= a.sinks) && !missing))
         mask(cur, jr, missing);  // (else every row sees the whole block)
-      qk_pv(KR + (I ^ 1) * TB, nxt, VR + (I ^ 1) * TB, prev);
-      const float ls = expblock(cur, now);
+      const float ls = work(KR + (I ^ 1) * TB, nxt, VR + (I ^ 1) * TB, prev, cur, now);
       raise(cur, now, ls);
     }
     store(I);
