@@ -46,7 +46,8 @@ extern "C" __global__ __launch_bounds__(256) void nk_attend8_rows_f32(Attend8Arg
 // memory; and of the values it takes D / 16 columns of the eight keys whose weights
 // it holds, pairs of which v_perm puts side by side after conversion.  The next
 // block's keys are read as soon as this one's scores stand, its values behind this
-// one's products.
+// one's products.  (Those 64 contexts: 113 us for 556 MB, 4.9 TB/s; one of 1500 keys:
+// 5.6 us.)
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
@@ -290,7 +291,8 @@ NK_STEP8(f16, f16, 64, 4)
 // The pieces of a step's row joined: o = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s,
 // over the pieces with any weight, up to JOIN of them.  One workgroup per row: D / 4
 // threads side by side for a piece's sums, the pieces shared out over the rest and
-// added in a fixed order.  Bound by the latency of its two dependent reads.
+// added in a fixed order.  Bound by the latency of its two dependent reads (32 rows: 3.6
+// us, 2048 rows of up to 10 pieces: 6.0).
 // ---------------------------------------------------------------------------
 #define ATT8_JOIN 256
 template <typename T, int D>

@@ -46,15 +46,20 @@ class ReorderArgs(ctypes.Structure):
 
 ASSIGN_PAGES = 2**20  # bits of a workgroup's LDS
 ASSIGN_SMALL = 1024   # tokens, and
-ASSIGN_ROWS = 128     # rows of
-ASSIGN_WIDTH = 512    # entries, that one workgroup deals with
+ASSIGN_ROWS = 64      # rows, of
+ASSIGN_WIDTH = 2048   # entries each, and
+ASSIGN_ENTRIES = 2**15  # in all, that one workgroup deals with
 ASSIGN_MARKS = 64     # rows that a workgroup marks at once, four a wave
 ASSIGN_WORDS = 2**18  # words of bitmaps that one workgroup joins, about
 
 
 def assign_parts(rows, width, pages, tokens) -> int:
-    """Workgroups that mark the pages held, 0 where one does everything."""
-    if tokens <= ASSIGN_SMALL and rows <= ASSIGN_ROWS and width <= ASSIGN_WIDTH:
+    """Workgroups that mark the pages held, 0 where one does everything (by one
+    workgroup and by three launches, us: 64 rows of 250 entries 11.6 and 13.2, of
+    512 14.7 and 15.2; 8 of 2048 14.4 and 16.1; 1 of 250 with 1000 tokens 11.6 and
+    14.8; 96 of 256 15.3 and 14.1; 1 of 6250 20.8 and 17.7; 16 of 250 with 2048
+    tokens 16.3 and 15.0)."""
+    if tokens <= ASSIGN_SMALL and rows <= ASSIGN_ROWS and width <= ASSIGN_WIDTH and rows * width <= ASSIGN_ENTRIES:
         return 0
     return max(1, min(-(-rows // ASSIGN_MARKS), ASSIGN_WORDS // -(-pages // 32)))
 

@@ -39,7 +39,10 @@ class Attend8Args(S.AttendArgs):
 
 APPEND_HEADS = 64      # heads of a workgroup at most (append8.hip)
 APPEND_ELEMENTS = 2**14  # elements that a workgroup quantises, about
-APPEND_TOKENS = 1024   # tokens that are a wave's work each
+# Tokens from which on a token's queries are one wave's work, not four's (us: 8 tokens of
+# 128 heads of 256 10.9 by one wave and 7.0 by four, of 32 of 128 7.3 and 7.1; 2048 of 32
+# 23.3 and 25.7, of 64 29.1 and 28.8).
+APPEND_TOKENS = 1024
 
 
 def rotary_append_fp8(dtype, B, N, Hq, Hkv, D, half, P, page, pages, width, *, q, k, v, oq, kc, vc, ke, ve, cos, sin, tables, lens,
