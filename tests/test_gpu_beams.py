@@ -55,7 +55,8 @@ def test_assign_small():
 
 @pytest.mark.parametrize("rows,page,pages,most,new", [(64, 16, 5000, 1000, 1), (1, 16, 200, 3000, 2900), (200, 1, 9000, 40, 3),
                                                       (1500, 8, 40000, 150, 2), (30, 24, 900, 600, 300), (70, 128, 2**20, 4000, 0),
-                                                      (3000, 16, 3000, 30, 1)])
+                                                      (3000, 16, 3000, 30, 1), (2**16, 16, 2**20, 40, 1), (64, 16, 40000, 8000, 3),
+                                                      (65, 16, 40000, 8000, 3), (7, 16, 20000, 40000, 100)])
 def test_assign_batches(rows, page, pages, most, new):
     """Rows of many lengths, some ended, some without new tokens; more pages
     wanted than there are."""
@@ -98,7 +99,7 @@ def check_select(x, scores, ended, end):
 @pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("g,k,vocab", [(1, 1, 1), (1, 4, 3), (3, 4, 50), (2, 32, 40), (1, 4, 32000), (2, 3, 2047), (5, 8, 8193),
                                        (2, 5, 8191), (1, 2, 16385), (3, 16, 50257), (1, 32, 20000), (33, 2, 1000), (2, 25, 90000),
-                                       (1, 7, 300000)])
+                                       (1, 7, 300000), (1, 2, 2**22), (1, 32, 2**18), (4000, 2, 5)])
 def test_select(t, g, k, vocab):
     rng = np.random.default_rng(vocab)
     x, scores = B.logits(rng, g * k, vocab, t), (-5 - 3 * rng.random((g, k))).astype(np.float32)
@@ -222,3 +223,20 @@ def test_reorder_of_one_array_as_both_caches():
         dk(ins, outs, graph=graph)
         assert (outs["block_tables"].numpy() == t).all()
         assert both.numpy().tobytes() == want.tobytes()
+
+
+def test_two_sets_of_tensors_replayed_in_turns():
+    """Two graphs of one kernel share its workspace."""
+    rng = np.random.default_rng(10)
+    dk, sets = None, []
+    for _ in range(2):
+        x = B.logits(rng, 12, 20000, "bf16")
+        scores, ended = -rng.random((3, 4)).astype(np.float32), (rng.random((3, 4)) < 0.2).astype(np.int32)
+        one, ins, outs = load(f_select, x, scores, ended, end_token=2)
+        dk = dk or one
+        sets.append((ins, outs, (x, scores, ended)))
+    for _ in range(3):
+        for ins, outs, _ in sets:
+            dk(ins, outs, graph=True, sync=False)
+        for ins, outs, (x, scores, ended) in sets:
+            B.check_select([outs[f"output{j}"].numpy() for j in range(4)], x, scores, ended, 2, select_tolerance(x, 20000))

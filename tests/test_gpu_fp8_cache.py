@@ -406,3 +406,107 @@ def test_append_behind_2_31_codes_of_a_page(half):
         assert z[0, row].any()
         z[0, row] = 0
         assert not z.any()
+
+
+def test_caches_past_2_31_bytes():
+    """Pages whose places pass 32 bits: appended to, then read by single tokens
+    and by a prompt."""
+    rng = np.random.default_rng(60)
+    hkv, d, page, few = 8, 128, 16, 64
+    pages = 2**17 + few
+    small = [Q.random_cache(rng, few, page, hkv, d) for _ in range(2)]
+    caches, exps = [], []
+    for codes, e in small:
+        big = np.zeros((pages, page, hkv, d), codes.dtype)
+        big[-few:] = codes
+        caches.append(big)
+        exps.append(np.concatenate([np.full((pages - few, hkv), 9, np.int32), e]))
+    ang = rng.standard_normal((600, 64)).astype(np.float32)
+
+    def f(q, k, v, cos, sin, key_cache, value_cache, key_exps, value_exps, tables, lens, starts=None):
+        y = T.rotary_append_fp8(q, k, v, cos, sin, key_cache, value_cache, key_exps, value_exps, tables, lens, starts)
+        return y, T.paged_attention_fp8(y, key_cache, value_cache, key_exps, value_exps, tables, lens, starts)
+
+    for new in (None, [140, 3]):
+        tables, lens, starts, n = P.batch(rng, [500, 200], new, page)
+        assert n <= few
+        t = 143 if new else 2
+        q, k, v = draw(rng, (t, 16, d), "bf16"), draw(rng, (t, hkv, d), "bf16"), draw(rng, (t, hkv, d), "bf16")
+        (kc, ke), (vc, ve) = small
+        (rq, tq), parts = Q.append(q, k, v, np.cos(ang), np.sin(ang), kc, vc, ke, ve, tables, lens, starts, "bf16")
+        got = run(f, q, k, v, np.cos(ang), np.sin(ang), *caches, *exps, np.where(tables < 0, -1, tables + pages - few).astype(np.int32),
+                  lens, starts)
+        close(got["output0"], rq, tq)
+        for name, (e, val, tol, _) in (("key", parts[0]), ("value", parts[1])):
+            assert (got[name + "_exps"][-few:] == e).all() and (got[name + "_exps"][:-few] == 9).all()
+            close(Q.values(got[name + "_cache"][-few:], got[name + "_exps"][-few:]), val, tol)
+            assert not Q.bits(got[name + "_cache"][:-few]).any()
+        close(got["output1"], *Q.paged(got["output0"], got["key_cache"][-few:], got["value_cache"][-few:],
+                                       got["key_exps"][-few:], got["value_exps"][-few:], tables, lens, starts, 0, 0, "bf16"))
+
+
+def test_starts_in_no_order():
+    """Query starts that decrease or lie outside the tokens change nothing else:
+    the call behind gives what it always does."""
+    rng = np.random.default_rng(61)
+    tables, lens, starts, pages = P.batch(rng, [50, 70, 20], [3, 4, 5], 16)
+    q, k, v = (draw(rng, (12, h, 64), "bf16") for h in (4, 2, 2))
+    (kc, ke), (vc, ve) = Q.random_cache(rng, pages, 16, 2, 64), Q.random_cache(rng, pages, 16, 2, 64)
+    ang = rng.standard_normal((100, 32)).astype(np.float32)
+
+    def f(q, k, v, cos, sin, kc, vc, ke, ve, tables, lens, starts):
+        y = T.rotary_append_fp8(q, k, v, cos, sin, kc, vc, ke, ve, tables, lens, starts)
+        return T.paged_attention_fp8(y, kc, vc, ke, ve, tables, lens, starts)
+
+    args = (q, k, v, np.cos(ang), np.sin(ang), kc, vc, ke, ve, tables)
+    first = run(f, *args, lens, starts)
+    far = [2**31 - 1, -2**31]
+    for s in ([0, 9, 3, 12], [-5, far[0], 0, far[0]], [7, 7, 7, 7], [12, 0, 0, 0], [far[0], far[1], far[0], 3]):
+        for n in (lens, np.array([far[0], far[1], 7], np.int32)):
+            got = run(f, *args, n, np.array(s, np.int32))
+            held = np.unique(tables[tables >= 0])
+            others = np.setdiff1d(np.arange(pages), held)
+            for name, x in (("kc", kc), ("vc", vc)):  # (pages of nobody)
+                assert (Q.bits(got[name])[others] == Q.bits(x)[others]).all()
+    again = run(f, *args, lens, starts)
+    assert all(again[n].tobytes() == first[n].tobytes() for n in first)
+
+
+def test_two_sets_of_tensors_replayed_in_turns():
+    """Two graphs of one kernel share its workspace (the splits of a step)."""
+    rng = np.random.default_rng(62)
+    sets = []
+    dk = None
+    for _ in range(2):
+        tables, lens, _, pages = P.batch(rng, [700, 90, 1500], None, 16)
+        q = draw(rng, (3, 8, 128), "bf16")
+        (kc, ke), (vc, ve) = Q.random_cache(rng, 160, 16, 2, 128), Q.random_cache(rng, 160, 16, 2, 128)
+        tables = np.pad(tables, ((0, 0), (0, 100 - tables.shape[1])), constant_values=-1)
+        one, ins, outs = load(f_attend, q, kc, vc, ke, ve, tables, lens)
+        dk = dk or one
+        sets.append((ins, outs, Q.paged(q, kc, vc, ke, ve, tables, lens, None, 0, 0, "bf16")))
+    for _ in range(3):
+        for ins, outs, want in sets:
+            dk(ins, outs, graph=True, sync=False)
+        for ins, outs, want in sets:
+            close(outs["output0"].numpy(), *want)
+
+
+def test_exponents_overwritten_behind_an_append():
+    """An array that the kernel writes again: the append updates a copy of it."""
+    rng = np.random.default_rng(63)
+    tables, lens, starts, pages = P.batch(rng, [30, 20], [7, 20], 16)
+    q, k, v = (draw(rng, (27, h, 64), "bf16") for h in (4, 2, 2))
+    (kc, ke), (vc, ve) = Q.random_cache(rng, pages, 16, 2, 64), Q.random_cache(rng, pages, 16, 2, 64)
+    ang = rng.standard_normal((30, 32)).astype(np.float32)
+
+    def f(q, k, v, cos, sin, kc, vc, ke, ve, tables, lens, starts):
+        T.rotary_append_fp8(q, k, v, cos, sin, kc, vc, ke, ve, tables, lens, starts)
+        seen = ke + 1
+        ke[:] = 7
+        return seen
+
+    _, parts = Q.append(q, k, v, np.cos(ang), np.sin(ang), kc, vc, ke, ve, tables, lens, starts, "bf16")
+    got = run(f, q, k, v, np.cos(ang), np.sin(ang), kc, vc, ke, ve, tables, lens, starts)
+    assert (got["output0"] == parts[0][0] + 1).all() and (got["ke"] == 7).all() and (got["ve"] == parts[1][0]).all()
+    close(Q.values(got["kc"], parts[0][0]), parts[0][1], parts[0][2])
