@@ -115,7 +115,10 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   AttWork wk;
   AttSeq sq;
   if (!att8_tile(a, blockIdx.x, reinterpret_cast<int32_t *>(KR), wk, sq)) return;
-  const int g = wk.g, split = wk.split, b = wk.b, tile = wk.tile;
+  // (one for the workgroup, in scalar registers: read behind stores, they came to vector ones)
+  auto uniform = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
+  sq.lo = uniform(sq.lo), sq.n = uniform(sq.n), sq.len = uniform(sq.len), sq.p0 = uniform(sq.p0), sq.cap = uniform(sq.cap);
+  const int g = wk.g, split = wk.split, b = uniform(wk.b), tile = uniform(wk.tile);
   const AttSpan sp = att_span(a, sq, tile);
   int j0, j1;
   const int pieces = att_split(a, sp.nb, split, j0, j1);
