@@ -202,6 +202,7 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   // K of block jr + 2 and V of block jr: where they lie, then their codes
   int kat, vat;
   uint32_t kex, vex;
+  int gone;  // whether some key of block jr has no page
   auto look = [&](int jr) __attribute__((always_inline)) {
     const int e = ((keys ? jr + 2 : jr) & (2 * ATT8_AHEAD - 1)) * ATT_KEYS + rr;
     kat = ent[e], kex = exps[e];
@@ -209,6 +210,7 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
       const int f = (jr & (2 * ATT8_AHEAD - 1)) * ATT_KEYS + rr;
       vat = ent[f], vex = exps[f];
     }
+    gone = lost[jr & (2 * ATT8_AHEAD - 1)];
   };
   auto fetch = [&]() __attribute__((always_inline)) {
     ck.scale = __uint_as_float((keys ? kex & 0xff : kex >> 8) << 23);
@@ -261,12 +263,12 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   // products, 246 so at a raised priority, 240 in turns; 1.24 and 1.13 a block where a CU
   // has one workgroup, 1.75 and 1.62 where it has two.  With the codes' stores among the
   // products as well 290: they wait for their reads.)
-  auto work = [&](const uint8_t *K, f32x16 &nxt, const uint8_t *Vt, const B8 (&prev)[2][NP], const f32x16 &cur,
-                  B8 (&now)[2][NP]) __attribute__((always_inline)) {
+  auto work = [&](const uint8_t *K, B8 k0, f32x16 &nxt, const uint8_t *Vt, B8 v0, const B8 (&prev)[2][NP],
+                  const f32x16 &cur, B8 (&now)[2][NP]) __attribute__((always_inline)) {
     constexpr int STEPS = D / 16, W = 16 / STEPS;
     float s0 = 0.f, s1 = 0.f;
     B8 kf[2], vf[2];
-    kf[0] = read_k(K, 0), vf[0] = read_v(Vt, 0, 0);
+    kf[0] = k0, vf[0] = v0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) nxt[r] = 0.f;
 #pragma unroll
@@ -350,14 +352,17 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   // the softmax of this one.  The last, jr = n, adds the last block's values.
   auto step = [&](auto slot, int jr, f32x16 &cur, f32x16 &nxt, B8 (&prev)[2][NP], B8 (&now)[2][NP]) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
+    // (the first products' factors before all else: what they wait for)
+    const uint8_t *const K = KR + (I ^ 1) * TB, *const Vt = VR + (I ^ 1) * TB;
+    const B8 k0 = read_k(K, 0), v0 = read_v(Vt, 0, 0);
+    const bool missing = __builtin_amdgcn_readfirstlane(gone) != 0;
     fetch();
     look(jr + 1);
     if (active) {
-      const bool missing = __builtin_amdgcn_readfirstlane(lost[jr & (2 * ATT8_AHEAD - 1)]) != 0;
-      const int k0 = sp.kb(j0 + jr) * ATT_KEYS;
-      if (!(jr < n && k0 + ATT_KEYS - 1 <= sp.pa && k0 + ATT_KEYS <= sp.hi && (k0 > sp.pb - a.window || k0 + ATT_KEYS <= a.sinks) && !missing))
+      const int key = sp.kb(j0 + jr) * ATT_KEYS;
+      if (!(jr < n && key + ATT_KEYS - 1 <= sp.pa && key + ATT_KEYS <= sp.hi && (key > sp.pb - a.window || key + ATT_KEYS <= a.sinks) && !missing))
         mask(cur, jr, missing);  // (else every row sees the whole block)
-      const float ls = work(KR + (I ^ 1) * TB, nxt, VR + (I ^ 1) * TB, prev, cur, now);
+      const float ls = work(K, k0, nxt, Vt, v0, prev, cur, now);
       raise(cur, now, ls);
     }
     store(I);
