@@ -14,8 +14,8 @@ using namespace nk;
 // The codes of a block of 32 keys go through registers, where a thread converts what
 // it read into bf16 values once for all four waves, into two LDS slots each for K and
 // V: iteration j has the scores of block j + 1, the values of block j - 1 and the
-// softmax of block j, then stores K of block j + 2 and V of block j, with one barrier;
-// what it stores was read an iteration before.  The rows and scales of 16 blocks are
+// softmax of block j, and stores K of block j + 2 and V of block j, with one barrier;
+// what it stores was read in the iteration before.  The rows and scales of 16 blocks are
 // looked up while the 16 before are worked on, in three steps four iterations apart,
 // so that no read of them is waited for (each block's by one wave as it came: 326 us
 // for 2100 tokens of 24 sequences of up to 6000, 263 so).  A key that is not seen by
@@ -225,8 +225,8 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
     *reinterpret_cast<B8 *>(to + rr * RB + (((2 * cc + 1) ^ swz) << 4)) = codes8(x.w.z, x.w.w, x.scale);
   };
   // both go to slot jr & 1
-  auto store = [&](int slot) __attribute__((always_inline)) {
-    put(ck, (keys ? KR : VR) + slot * TB, keys ? kswz(rr) : vswz(rr));
+  auto store_k = [&](int slot) __attribute__((always_inline)) { put(ck, (keys ? KR : VR) + slot * TB, keys ? kswz(rr) : vswz(rr)); };
+  auto store_v = [&](int slot) __attribute__((always_inline)) {
     if constexpr (BOTH) put(cv, VR + slot * TB, vswz(rr));
   };
 
@@ -257,33 +257,37 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
     return __builtin_bit_cast(B8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
   // The scores of one block, the values of another and the weights of a third, in turns
-  // (each product of the scores waits for the one before it; the weights go on beside the
-  // products), with what a step reads on its way a step before.  Returns the sum of the
-  // weights 2^(s c - m).  (2100 tokens of 24 sequences: 265 us with the weights behind all
-  // products, 246 so at a raised priority, 240 in turns; 1.24 and 1.13 a block where a CU
-  // has one workgroup, 1.75 and 1.62 where it has two.  With the codes' stores among the
-  // products as well 290: they wait for their reads.)
+  // (each product of the scores waits for the one before it; the weights, and what
+  // `between` does, go on beside the products), with what a step reads on its way two
+  // steps before.  Returns the sum of the weights 2^(s c - m).  2100 tokens of 24
+  // sequences, us: 265 with the weights behind all products and the codes stored behind
+  // those, 240 with the weights in turns, 227 with the sequence's numbers in scalar
+  // registers, 217 with the codes' stores and reads in turns as well, 208 at a raised
+  // priority (of two workgroups' waves one is at its products then; a block's time 1.75
+  // to 1.45, where a CU has one workgroup 1.24 to 1.03).
   auto work = [&](const uint8_t *K, B8 k0, f32x16 &nxt, const uint8_t *Vt, B8 v0, const B8 (&prev)[2][NP],
-                  const f32x16 &cur, B8 (&now)[2][NP]) __attribute__((always_inline)) {
+                  const f32x16 &cur, B8 (&now)[2][NP], auto between) __attribute__((always_inline)) {
     constexpr int STEPS = D / 16, W = 16 / STEPS;
     float s0 = 0.f, s1 = 0.f;
-    B8 kf[2], vf[2];
-    kf[0] = k0, vf[0] = v0;
+    constexpr int DI = 2;
+    B8 kf[DI + 1], vf[DI + 1];
+    kf[0] = k0, vf[0] = v0, kf[1] = read_k(K, 1), vf[1] = read_v(Vt, 1 / (D / 32), 1 % (D / 32));
 #pragma unroll
     for (int r = 0; r < 16; ++r) nxt[r] = 0.f;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      if (i + 1 < STEPS) kf[(i + 1) & 1] = read_k(K, i + 1), vf[(i + 1) & 1] = read_v(Vt, (i + 1) / (D / 32), (i + 1) % (D / 32));
+      if (i + DI < STEPS) kf[(i + DI) % (DI + 1)] = read_k(K, i + DI), vf[(i + DI) % (DI + 1)] = read_v(Vt, (i + DI) / (D / 32), (i + DI) % (D / 32));
 #pragma unroll
-      for (int u = 0; u < NP; ++u) nxt = mul32(kf[i & 1], qf[i][u], nxt);
+      for (int u = 0; u < NP; ++u) nxt = mul32(kf[i % (DI + 1)], qf[i][u], nxt);
 #pragma unroll
-      for (int u = 0; u < NP; ++u) acc[i % (D / 32)] = mul32(vf[i & 1], prev[i / (D / 32)][u], acc[i % (D / 32)]);
+      for (int u = 0; u < NP; ++u) acc[i % (D / 32)] = mul32(vf[i % (DI + 1)], prev[i / (D / 32)][u], acc[i % (D / 32)]);
 #pragma unroll
       for (int e = i * W; e < i * W + W; ++e) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[e], sl2, -m_run));
         if (e & 1) s1 += x; else s0 += x;
         put_weight<NP>(now[e / 8], e % 8, x);
       }
+      between(i);
       __builtin_amdgcn_sched_barrier(0);
     }
     return s0 + s1;
@@ -350,22 +354,35 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   // Iteration jr, in slot i = jr & 1, one body for all: the values of the block before
   // (of zeros before the first), the scores of the one behind (of zeros past the last),
   // the softmax of this one.  The last, jr = n, adds the last block's values.
-  auto step = [&](auto slot, int jr, f32x16 &cur, f32x16 &nxt, B8 (&prev)[2][NP], B8 (&now)[2][NP]) __attribute__((always_inline)) {
+  // (waves without rows have a loop of their own, with the same barriers: one body would
+  // branch around the products, and what is read in a branch is waited for at its end)
+  auto step = [&](auto act, auto slot, int jr, f32x16 &cur, f32x16 &nxt, B8 (&prev)[2][NP],
+                  B8 (&now)[2][NP]) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
-    // (the first products' factors before all else: what they wait for)
-    const uint8_t *const K = KR + (I ^ 1) * TB, *const Vt = VR + (I ^ 1) * TB;
-    const B8 k0 = read_k(K, 0), v0 = read_v(Vt, 0, 0);
-    const bool missing = __builtin_amdgcn_readfirstlane(gone) != 0;
-    fetch();
-    look(jr + 1);
-    if (active) {
+    if constexpr (decltype(act)::value) {
+      // (the first products' factors before all else: what they wait for)
+      const uint8_t *const K = KR + (I ^ 1) * TB, *const Vt = VR + (I ^ 1) * TB;
+      const B8 k0 = read_k(K, 0), v0 = read_v(Vt, 0, 0);
+      const bool missing = __builtin_amdgcn_readfirstlane(gone) != 0;
+      look(jr + 1);
       const int key = sp.kb(j0 + jr) * ATT_KEYS;
       if (!(jr < n && key + ATT_KEYS - 1 <= sp.pa && key + ATT_KEYS <= sp.hi && (key > sp.pb - a.window || key + ATT_KEYS <= a.sinks) && !missing))
         mask(cur, jr, missing);  // (else every row sees the whole block)
-      const float ls = work(K, k0, nxt, Vt, v0, prev, cur, now);
+      __builtin_amdgcn_s_setprio(1);
+      const float ls = work(K, k0, nxt, Vt, v0, prev, cur, now, [&](int i) __attribute__((always_inline)) {
+        constexpr int AT = D / 16 / 4;
+        if (i == AT) store_k(I);
+        if (i == AT + 1) store_v(I);
+        if (i == AT + 1 + (D == 128)) fetch();
+      });
+      __builtin_amdgcn_s_setprio(0);
       raise(cur, now, ls);
+    } else {
+      look(jr + 1);
+      store_k(I);
+      store_v(I);
+      fetch();
     }
-    store(I);
     lds_barrier();
   };
 
@@ -388,6 +405,7 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
       put(none, VR + TB, vswz(rr));
     }
     look(0);
+    fetch();
     lds_barrier();
     if (active) {
 #pragma unroll
@@ -396,20 +414,24 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
       for (int kk = 0; kk < D / 16; ++kk) qk1(KR, sA, kk);
     }
     lds_barrier();  // (block 0 is read before its slot is refilled)
-    for (int jr = 0;; jr += 2) {
-      // (the other half was last read an iteration, and a barrier, ago)
-      if (jr % ATT8_AHEAD == 0) {
-        find_pages(jr / ATT8_AHEAD + 1);
-      } else if (jr % ATT8_AHEAD == 4) {
-        find_exps();
-      } else if (jr % ATT8_AHEAD == 8) {
-        put_rows(jr / ATT8_AHEAD + 1);
+    auto run = [&](auto act) __attribute__((always_inline)) {
+      for (int jr = 0;; jr += 2) {
+        // (the other half was last read an iteration, and a barrier, ago)
+        if (jr % ATT8_AHEAD == 0) {
+          find_pages(jr / ATT8_AHEAD + 1);
+        } else if (jr % ATT8_AHEAD == 4) {
+          find_exps();
+        } else if (jr % ATT8_AHEAD == 8) {
+          put_rows(jr / ATT8_AHEAD + 1);
+        }
+        step(act, Count<0>{}, jr, sA, sB, pB, pA);
+        if (jr + 1 > n) break;
+        step(act, Count<1>{}, jr + 1, sB, sA, pA, pB);
+        if (jr + 2 > n) break;
       }
-      step(Count<0>{}, jr, sA, sB, pB, pA);
-      if (jr + 1 > n) break;
-      step(Count<1>{}, jr + 1, sB, sA, pA, pB);
-      if (jr + 2 > n) break;
-    }
+    };
+    if (active) run(Count<1>{});
+    else run(Count<0>{});
   }
 
   const int row = row0 + l32, rld = min(row, rows - 1), qi = rld / rep, h = g * rep + rld % rep;
