@@ -266,8 +266,8 @@ extern "C" __global__ __launch_bounds__(256) void nk_assign_fill(AssignArgs a) {
 // place; an entry with j before it in a list whose best has rank r has r + j
 // better ones, so K (K + 1) / 2 entries are left to rank.
 //
-// 16 groups of 8 beams of 151936 logits (bf16): 16 and 8 us; one of 4 of 32000 (fp32): 6
-// and 6.5.  The first is bound by the instructions of a wave's 2048 logits (2.4 TB/s; 64
+// 16 groups of 8 beams of 151936 logits (bf16): 16 and 7.6 us; one of 4 of 32000 (fp32): 6
+// and 4.6.  The first is bound by the instructions of a wave's 2048 logits (2.4 TB/s; 64
 // groups of 32 of 30000 in fp32 4.3), the second by its chain: two reads, two rankings.
 // ---------------------------------------------------------------------------
 struct SelectArgs {
@@ -441,10 +441,33 @@ extern "C" __global__ __launch_bounds__(256) void nk_select_top_f32(SelectArgs a
 // a score in its order among all, places packed as beam * 2^22 + token
 NK_DEVICE bool sel_better(double s, uint32_t p, double t, uint32_t q) { return (s > t) | ((s == t) & (p < q)); }
 
+// sums over 2, 4, 8 and 16 neighbouring lanes by lane moves, one after the other: with the
+// neighbour, the other pair, and mirrored in halves of a row and in a row
+template <int CTRL>
+NK_DEVICE int lanes_swapped(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false); }
+template <int CTRL>
+NK_DEVICE double lanes_swapped(double v) {
+  const u64 u = __double_as_longlong(v);
+  const uint32_t lo = lanes_swapped<CTRL>((int)(uint32_t)u), hi = lanes_swapped<CTRL>((int)(uint32_t)(u >> 32));
+  return __longlong_as_double((u64)hi << 32 | lo);
+}
+NK_DEVICE double sel_wave_sum(double v) {
+  v += lanes_swapped<0xB1>(v);   // quad_perm 1 0 3 2
+  v += lanes_swapped<0x4E>(v);   // quad_perm 2 3 0 1
+  v += lanes_swapped<0x141>(v);  // row_half_mirror
+  v += lanes_swapped<0x140>(v);  // row_mirror
+  const int64_t u = __double_as_longlong(v);
+  return (__longlong_as_double(lane_of(u, 0)) + __longlong_as_double(lane_of(u, 16))) +
+         (__longlong_as_double(lane_of(u, 32)) + __longlong_as_double(lane_of(u, 48)));
+}
+
 // order[r]: the entry of rank r < K of n (those with a place), by a workgroup.  Up to
 // DIRECT are ranked each against all, some threads side by side.  Of more, the first
 // wave lists those that can count, as above: what is not below the K-th largest of its
-// lanes' largest, by the upper halves.
+// lanes' largest, by the upper halves (152 lists of 8 beams: 13 us for the launch with
+// each against all, 8.7 so, of 36 entries or 64 lists no less; 992 lists of 32 beams: 153
+// and 16).  S threads rank an entry; 16 at most, as their sums are a chain (4 beams: 6.3 us
+// with 64, 4.6 so).
 #define SEL_DIRECT 64
 struct SelFew {
   uint16_t list[SEL_HEADS];
@@ -481,7 +504,7 @@ NK_DEVICE void sel_rank(const double *s, const uint32_t *p, int n, int K, int32_
   }
   auto id = [&](int x) { return all ? x : (int)few.list[x]; };
   int S = 1;
-  while (S < 64 && c * S * 2 <= SEL_BLOCK) S *= 2;
+  while (S < 16 && c * S * 2 <= SEL_BLOCK) S *= 2;
   for (int x = tid; x < (c * S + 63) / 64 * 64; x += SEL_BLOCK) {
     const int i = id(min(x / S, c - 1));
     const double y = s[i];
@@ -489,7 +512,10 @@ NK_DEVICE void sel_rank(const double *s, const uint32_t *p, int n, int K, int32_
     int rank = 0;
 #pragma unroll 4
     for (int q = x % S; q < c; q += S) rank += (p[id(q)] != SEL_NONE) & sel_better(s[id(q)], p[id(q)], y, z) ? 1 : 0;
-    for (int o = 1; o < S; o <<= 1) rank += __shfl_xor(rank, o, 64);
+    if (S > 1) rank += lanes_swapped<0xB1>(rank);
+    if (S > 2) rank += lanes_swapped<0x4E>(rank);
+    if (S > 4) rank += lanes_swapped<0x141>(rank);
+    if (S > 8) rank += lanes_swapped<0x140>(rank);
     if (x % S == 0 && x / S < c && z != SEL_NONE && rank < K) order[rank] = i;
   }
   __syncthreads();
@@ -528,9 +554,7 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
         const float2 y = a.sums[(int64_t)r * a.nseg + i];
         sum += y.x == m ? (double)y.y : y.x == -INFINITY ? 0.0 : (double)y.y * exp_acc(y.x - m);
       }
-#pragma unroll
-      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-      z -= log(sum);
+      z -= log(sel_wave_sum(sum));
     }
     if (lane == 0) base[b] = z, largest[b] = m, kind[b] = what;
   }
