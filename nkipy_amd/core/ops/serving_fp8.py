@@ -267,9 +267,9 @@ def _paged_attention_fp8_cpu(q, key_cache, value_cache, key_exps, value_exps, bl
     ``paged_attention``.
 
     On the GPU keys and values enter as exactly what they stand for.  Weights
-    are rounded to bfloat16 before the values are summed where q is bfloat16 of
-    head dim 64 or 128, kept to 2^-16 of themselves where it is float16 of those,
-    and have 32 bits otherwise."""
+    have 32 bits, but where q has 16 bits and a head dim of 64 or 128: there
+    they keep 2^-16 of themselves before the values are summed, and with
+    ``query_starts`` and a bfloat16 q are rounded to bfloat16."""
     window, sinks, scale = _check_attention(q, key_cache, value_cache, key_exps, value_exps, block_tables, context_lens,
                                             query_starts, window, sinks, scale)
     pages, page = key_cache.shape[:2]

@@ -93,9 +93,9 @@ NK_DEVICE f32x4 mul16(B8 a, B8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16
 NK_DEVICE f32x16 mul32(B8 a, B8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 // Codes enter the products as bf16: code 2^e is exact there (4 significant bits,
-// fp32's exponents).  fp16 queries and weights, which bf16 does not hold, enter as
-// two bf16 numbers each, x = RN(x) + RN(x - RN(x)): exact for a query's 11 bits, a
-// weight keeps 16.
+// fp32's exponents).  fp16 queries and the weights over them, which bf16 does not hold,
+// enter as two bf16 numbers each, x = RN(x) + RN(x - RN(x)): exact for a query's 11 bits,
+// a weight keeps 16.  (Weights of single tokens do so always.)
 template <typename T> struct Parts;
 template <> struct Parts<bf16> { static constexpr int N = 1; };
 template <> struct Parts<f16> { static constexpr int N = 2; };

@@ -44,14 +44,16 @@ extern "C" __global__ __launch_bounds__(256) void nk_attend8_rows_f32(Attend8Arg
 // a head, and which key of a block, has which place in a product's sum is free as
 // long as both factors agree.  So a lane takes 16 bytes of a key as they lie in
 // memory; and of the values it takes D / 16 columns of the eight keys whose weights
-// it holds, pairs of which v_perm puts side by side after conversion.  The next
-// block's keys are read as soon as this one's scores stand, its values behind this
-// one's products.  (Those 64 contexts: 113 us for 556 MB, 4.9 TB/s; one of 1500 keys:
-// 5.6 us.)
+// it holds, pairs of which v_perm puts side by side after conversion.  A weight is two
+// bf16 numbers, so that it keeps 2^-16 of itself: the products are not what bounds this
+// (118 us a call with one number and with two; results off by 2.33e-3 and by 1.66e-3 of
+// their norm, the latter their own rounding).  The next block's keys are read as soon as
+// this one's scores stand, its values behind this one's products.  (Those 64 contexts:
+// 113 us for 556 MB, 4.9 TB/s; one of 1500 keys: 5.6 us.)
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
-  constexpr int NP = Parts<T>::N, VW = D / 64;
+  constexpr int NP = Parts<T>::N, WP = 2, VW = D / 64;
   const int lane = threadIdx.x & 63;
   const int l16 = lane & 15, grp = lane >> 4;
   const int rep = a.Hq / a.Hkv, per = (rep + 15) / 16, units = a.Hkv * per;
@@ -161,14 +163,14 @@ __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
         for (int i = 0; i < VW; ++i) vr[e][i] = is ? vr[e][i] : 0;
       }
     }
-    B8 pf[NP];
+    B8 pf[WP];
     auto weigh = [&]() __attribute__((always_inline)) {
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float y = __builtin_amdgcn_exp2f((s[e >> 2][e & 3] - m_run) * sl2);
         sum += y;
-        put_weight<NP>(pf, e, y);
+        put_weight<WP>(pf, e, y);
       }
       return sum;
     };
@@ -210,7 +212,7 @@ __device__ __forceinline__ void attend8_step_body(const Attend8Args &a) {
         }
         const int t = 4 * i + 2 * h;
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
+        for (int n = 0; n < WP; ++n) {
           acc[t] = mul16(__builtin_bit_cast(B8, lo), pf[n], acc[t]);
           acc[t + 1] = mul16(__builtin_bit_cast(B8, hi), pf[n], acc[t + 1]);
         }
