@@ -652,7 +652,7 @@ __device__ __forceinline__ void reorder_body(const ReorderArgs &a) {
     int x = -1, y = -1;
     if (moves && part >= a.tblocks) {  // (full is below width: the length leaves a page in part filled)
       x = table[(int64_t)p * a.width + full], y = table[(int64_t)b * a.width + full];
-      if (x < 0 || x >= a.pages || y >= a.pages) y = -1;
+      if (x < 0 || x >= a.pages || y < 0 || y >= a.pages) x = y = -1;  // (no page, on either side)
     }
     from[tid] = x, to[tid] = y;
   }
