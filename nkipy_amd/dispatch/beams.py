@@ -229,11 +229,15 @@ class ReorderMatch(UpdateMatch):
 
 def calls(L, kinds):
     """The live nodes of ``kinds``, those of one call together: they follow
-    each other in the trace, over the same operands."""
+    each other in the trace, over the same operands and with the same
+    attributes (two such calls, of which one is read for what the other is
+    not, are one)."""
+    def call(n):
+        return n.op, [v.id for v in n.inputs], {k: x for k, x in n.attrs.items() if k not in ("part", "target")}
+
     group: List[Node] = []
     for n in L.live + [None]:
-        if group and (n is None or n.op != group[0].op or [v.id for v in n.inputs] != [v.id for v in group[0].inputs]
-                      or any(m.attrs["part"] == n.attrs["part"] for m in group)):
+        if group and (n is None or call(n) != call(group[0]) or any(m.attrs["part"] == n.attrs["part"] for m in group)):
             yield group
             group = []
         if n is not None and n.op in kinds:
