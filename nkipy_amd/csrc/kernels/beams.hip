@@ -335,12 +335,14 @@ __device__ __forceinline__ void select_top_body(const SelectArgs &a) {
   const float m = wave_max(top);
   float sum = 0.f;
   if (fabsf(m) < INFINITY) {
-    // 2^(x L - c), with c = RN(m L): what c is off by, d = m L - c, is a factor 2^-d of all
+    // 2^(x L - c), with c = RN(m L): what c is off by, d = m L - c, is a factor 2^-d of all.
+    // From |c| = 2^24 on d may be 1 and more, and later so large that the terms overflow
+    // or vanish: the differences there, as with NaN logits and ones past fp32's range times L.
     const float L = 1.44269504088896340736f, c = m * L, d = __builtin_fmaf(m, L, -c);
 #pragma unroll
     for (int e = 0; e < 32; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], L, -c));
     sum *= __builtin_amdgcn_exp2f(-d);
-    if (__any(sum != sum) || !(fabsf(c) < INFINITY)) {  // NaN logits, or ones past fp32's range times L
+    if (__any(sum != sum) || !(fabsf(d) < 1.f)) {
       sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 32; ++e) sum += v[e] == v[e] ? __builtin_amdgcn_exp2f((v[e] - m) * L) : 0.f;
