@@ -121,6 +121,9 @@ def updated_argument(x, name):
     if part:
         raise ValueError(f"{name} is a part or another layout of the argument {v.name!r}, which a write into it would not "
                          "reach: pass each array as an argument of its own")
+    if x._original_parameter is None:  # (a slice or reshape that changes nothing: the argument's value, not itself)
+        raise ValueError(f"{name} is a view of the argument {v.name!r}, which a write into it would not reach: "
+                         "pass the argument itself")
     return here
 
 
