@@ -19,7 +19,8 @@ using namespace nk;
 // (large pages, odd sizes and heads rotated in part: read again, mostly from cache).
 // Maxima are of whole numbers (bits), so no order changes them.  Bound by memory (8000
 // tokens of 32 / 8 heads of 128, 184 MB: 40 us, 4.6 TB/s; the queries alone take 27, keys
-// and values 16), single tokens by latency (8 of them: 4.5 us).
+// and values 16; in fp32, 344 MB, 70; with 64 of the 128 elements rotated, keys read
+// twice, 63), single tokens by latency (8 of them: 4.5 us).
 // ---------------------------------------------------------------------------
 struct Append8Args {
   const void *q, *k, *v;

@@ -14,7 +14,9 @@ struct Attend8Args : AttendArgs {  // k, v: codes; strides in bytes
 // One query row by one wave, over blocks j0 .. j1-1 of its tile's span: eight lanes
 // share a key's product, 64 keys a step; then the lanes share the head's elements,
 // d = lane + 64 e.  Only the keys that the row sees are read; 32-bit weights of at
-// most 1.  DIM: the head dim where it is known, which saves registers.
+// most 1.  A code is finite or NaN, and NaN reaches the sum under any weight, 0
+// included: no rule for values that are infinite, as those over 16-bit caches need.
+// DIM: the head dim where it is known, which saves registers.
 template <typename T, int DIM = 0>
 NK_DEVICE void att8_row(const Attend8Args &a, const AttSeq &sq, const AttSpan &sp, int b, int i, int h, int j0, int j1,
                         float &m, float &l, float (&acc)[DIM ? (DIM + 63) / 64 : 4]) {

@@ -267,11 +267,11 @@ __device__ __forceinline__ void attend8_tile_body(const Attend8Args &a) {
   // (each product of the scores waits for the one before it; the weights, and what
   // `between` does, go on beside the products), with what a step reads on its way two
   // steps before.  Returns the sum of the weights 2^(s c - m).  2100 tokens of 24
-  // sequences, us: 265 with the weights behind all products and the codes stored behind
-  // those, 240 with the weights in turns, 227 with the sequence's numbers in scalar
-  // registers, 217 with the codes' stores and reads in turns as well, 208 at a raised
-  // priority (of two workgroups' waves one is at its products then; a block's time 1.75
-  // to 1.45, where a CU has one workgroup 1.24 to 1.03).
+  // sequences, us as traced: 265 with the weights behind all products and the codes
+  // stored behind those, 240 with the weights in turns, 227 with the sequence's numbers
+  // in scalar registers.  The codes' stores and reads in turns as well, at a raised
+  // priority (of two workgroups' waves one is at its products then), took queued calls
+  // from 198 to 173 .. 181; traced, launches of 199 to 228 (median 221).
   auto work = [&](const uint8_t *K, B8 k0, f32x16 &nxt, const uint8_t *Vt, B8 v0, const B8 (&prev)[2][NP],
                   const f32x16 &cur, B8 (&now)[2][NP], auto between) __attribute__((always_inline)) {
     constexpr int STEPS = D / 16, W = 16 / STEPS;

@@ -267,8 +267,9 @@ extern "C" __global__ __launch_bounds__(256) void nk_assign_fill(AssignArgs a) {
 // better ones, so K (K + 1) / 2 entries are left to rank.
 //
 // 16 groups of 8 beams of 151936 logits (bf16): 16 and 7.6 us; one of 4 of 32000 (fp32): 6
-// and 4.6.  The first is bound by the instructions of a wave's 2048 logits (2.4 TB/s; 64
-// groups of 32 of 30000 in fp32 4.3), the second by its chain: two reads, two rankings.
+// and 4.6.  The first is bound by the instructions of a wave's 2048 logits (a quarter of
+// those beams have ended and are not read: 29 MB, 1.8 TB/s; 64 groups of 32 of 30000 in
+// fp32, none ended, 4.3), the second by its chain: two reads, two rankings.
 // ---------------------------------------------------------------------------
 struct SelectArgs {
   const void *x;
@@ -625,8 +626,9 @@ extern "C" __global__ __launch_bounds__(SEL_BLOCK) void nk_select_pick(SelectArg
 // A thread has one place (an entry of the tables, 16 bytes of a page) of every
 // beam of a group: it reads what all of them come from, then writes, so no
 // thread reads what another has written.  Beams that are their own parents move
-// nothing.  Bound by memory (32 groups of 8 beams, pages of 128 rows of 1024 codes, 75 MB:
-// 12 us, 6.2 TB/s), small ones by two dependent reads (4 beams: 3.6 us).
+// nothing.  Bound by memory (32 groups of 8 beams with parents at random, pages of 128
+// rows of 1024 codes: each parent read once and each beam with another parent written,
+// 56 MB in 12 us, 4.7 TB/s), small ones by two dependent reads (4 beams: 3.6 us).
 // ---------------------------------------------------------------------------
 struct ReorderArgs {
   const int32_t *parents, *lens;

@@ -82,10 +82,18 @@ def attend8_work(B, N, Hq, Hkv, D, keys, window=0, sinks=0, starts=False) -> Tup
     the keys, blocks that a split has at least).
 
     The pieces of a step have a length, not a number, so that short sequences
-    have few and all waves end together; their number is a multiple of eight, with
-    which the pieces of every sequence come to all XCDs (64 sequences of 400 to
-    8192 keys, whose sums differ by 13% over the XCDs otherwise: 145 us in
-    turns of sequences, 121 so)."""
+    have few and, where the tables are about as wide as the longest sequence, all
+    waves end together; their number is a multiple of eight, with which the
+    pieces of every sequence come to all XCDs (64 sequences of 400 to 8192 keys,
+    whose sums differ by 13% over the XCDs otherwise: 145 us in turns of
+    sequences, 121 so).
+
+    The lengths are not known here: pieces and splits follow the tables' width.
+    Wider tables have longer pieces (those 64 sequences in tables of 8192, 32768
+    and 131072 keys: 119, 288 and 495 us) and more splits of the tiles (2100 tokens
+    of 24 sequences of up to 6000, in tables of 6000, 32768 and 131072: 181, 257
+    and 257).  The splits of the tiles are weighed by ``attend_work``'s costs of a
+    block, which are those of the tiles over 16-bit caches."""
     if starts:
         return S.attend_work(B, 1, N, Hq, Hkv, D, keys, window, sinks, True) + (S.ATT_TILE_BLOCKS,)
     units = B * Hkv * -(-(Hq // Hkv) // S.ATT_STEP_HEADS)
