@@ -11,7 +11,8 @@ from test_gpu_serving import run
 
 pytestmark = pytest.mark.gpu
 
-# exact in bf16; times log2(e) in 32 bits off by 124, -7, ... from the product
+# exact in bf16 up to 2^40; the first two times log2(e), rounded to 32 bits, are off by
+# 124 and 126, their negatives by -124 and -126
 LARGE = [1509949440.0, 3439329280.0, -1509949440.0, -3439329280.0, 2.0**40, -(2.0**40), 1e30, -1e30, 2.0**126, 3e38, -3e38]
 
 
